@@ -1,0 +1,197 @@
+"""Attention of decoder tokens to the encoder's states (csrc/xattn.hip, csrc/xattn_step.hip): the operators an attention decoder needs beside
+the CTC branch (model.py:117-119).  cross_attention / cross_attention_grad are the training pair, cross_attention with one row per utterance
+is the single-token form, EncoderCache8 holds an utterance's keys and values in 8 bits and attends to them.
+
+Everything runs on the current HIP stream of the tensors' device, allocates through torch (so calls can be captured into a HIP graph) and
+raises ValueError for arguments it does not take.  layers.CrossAttention is the Layer over the same calls."""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+_SFX = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}
+_P, _L, _I = ctypes.c_void_p, ctypes.c_long, ctypes.c_int
+
+
+class Xattn(ctypes.Structure):
+    """include/sarnet.h: sarXattn."""
+    _fields_ = [(n, _P) for n in ("q", "k", "v", "dout", "out", "lse", "dq", "dk", "dv", "k_lens", "q_lens", "ws")] + [("ws_bytes", _L)] + \
+               [(n, _L) for n in ("q_sb", "q_st", "q_sh", "k_sb", "k_st", "k_sh", "v_sb", "v_st", "v_sh", "o_sb", "o_st", "o_sh", "g_sb", "g_st", "g_sh")] + \
+               [(n, _I) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "D")] + [("scale", ctypes.c_float), ("pad_", _I)]
+
+
+def _rows(name, x, like=None):
+    """x as the kernels take it: 4-D, last axis contiguous, rows on 16-byte boundaries -- a view that is not is copied."""
+    if x.dim() != 4:
+        raise ValueError("%s has to be (batch, time, heads, dim), got shape %r" % (name, tuple(x.shape)))
+    if x.dtype not in _SFX:
+        raise ValueError("%s has to be float32, bfloat16 or float16, got %s" % (name, x.dtype))
+    if like is not None and (x.dtype != like.dtype or x.device != like.device):
+        raise ValueError("%s is %s on %s, the queries are %s on %s" % (name, x.dtype, x.device, like.dtype, like.device))
+    if like is None and not x.is_cuda:
+        raise ValueError("%s is on %s: the kernels need a HIP device, there is no CPU fallback" % (name, x.device))
+    sb, st, sh, sd = x.stride()
+    if sd != 1 and x.shape[3] != 1 or (sb | st | sh) * x.element_size() % 16 or x.data_ptr() % 16:
+        return x.clone(memory_format=torch.contiguous_format)          # (a fresh allocation is aligned; contiguous() may hand x back)
+    return x
+
+
+def _lens(name, lens, B, device):
+    if lens is None:
+        return None
+    if lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != B or lens.device != device or not lens.is_contiguous():
+        raise ValueError("%s has to be a contiguous int32 tensor of %d lengths on %s" % (name, B, device))
+    return lens.data_ptr()
+
+
+def _heads(Hq, Hkv, D):
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError("%d query heads are not a multiple of %d key heads" % (Hq, Hkv))
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError("the head width has to be a multiple of 8 from 8 to 128, got %d" % D)
+
+
+def _launch(name, device, *args):
+    L = _lib.lib()
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            rc = L.fn[name](*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        rc = L.fn[name](*args, torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        raise RuntimeError("%s failed with status %d" % (name, rc))
+
+
+def _workspace(query, a, device):
+    n = _lib.lib().fn[query](ctypes.byref(a))
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        a.ws, a.ws_bytes = ws.data_ptr(), n
+        return ws
+
+
+def _result(name, t, shape, dtype, device):
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device or not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError("%s has to be a contiguous, 16-byte aligned %s tensor of shape %r on %s" % (name, dtype, tuple(shape), device))
+    return t
+
+
+def _check_kv(q, k, v):
+    k, v = _rows("k", k, q), _rows("v", v, q)
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError("q %r, k %r and v %r do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    _heads(q.shape[2], k.shape[2], q.shape[3])
+    return k, v
+
+
+def cross_attention(q, k, v, k_lens=None, q_lens=None, scale=None, return_lse=False, out=None, lse=None):
+    """softmax(scale q k^T) v over each utterance's first k_lens frames.
+
+    q (B, Tq, Hq, D), k, v (B, Tk, Hkv, D), Hq a multiple of Hkv (query head h reads key head h // (Hq // Hkv)); fp32, bf16 or fp16; any
+    strides whose last is 1.  k_lens, q_lens: int32 (B,) or None.  scale: 1 / sqrt(D) if None.  -> out (B, Tq, Hq, D), and with return_lse the rows'
+    log-sum-exp (B, Hq, Tq) fp32 that cross_attention_grad needs.  Rows from q_lens on and rows of an utterance without frames are
+    zeros (lse -inf); frames from k_lens on are not looked at.  `out`, `lse`: buffers to write into."""
+    q = _rows("q", q)
+    k, v = _check_kv(q, k, v)
+    B, Tq, Hq, D = q.shape
+    Tk, Hkv = k.shape[1], k.shape[2]
+    out = _result("out", out, (B, Tq, Hq, D), q.dtype, q.device)
+    if return_lse or lse is not None:
+        lse = _result("lse", lse, (B, Hq, Tq), torch.float32, q.device)
+    kl, ql = _lens("k_lens", k_lens, B, q.device), _lens("q_lens", q_lens, B, q.device)
+    if out.numel():
+        kv = (k.data_ptr(), v.data_ptr()) if Tk else (q.data_ptr(), q.data_ptr())                # (no frames: never read)
+        a = Xattn(q.data_ptr(), kv[0], kv[1], None, out.data_ptr(), None if lse is None else lse.data_ptr(), None, None, None, kl, ql, None, 0,
+                  *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], 0, 0, 0, B, Tq, Tk, Hq, Hkv, D,
+                  1.0 / math.sqrt(D) if scale is None else float(scale), 0)
+        ws = _workspace("sar_xattn_fwd_workspace_bytes", a, q.device)                            # noqa: F841  (alive until launched)
+        _launch("sar_xattn_fwd_" + _SFX[q.dtype], q.device, ctypes.byref(a))
+    return (out, lse) if return_lse else out
+
+
+def cross_attention_grad(dout, q, k, v, out, lse, k_lens=None, q_lens=None, scale=None, dq=None, dk=None, dv=None):
+    """Gradients of cross_attention: dout as out, the other arguments as the forward took and gave them -> (dq, dk, dv), contiguous, of the
+    inputs' type (each element rounded once from an fp32 sum; the gradient of a key head is the sum over its query heads).  No atomics: the
+    same inputs give the same bits.  `dq`, `dk`, `dv`: buffers to write into."""
+    q = _rows("q", q)
+    k, v = _check_kv(q, k, v)
+    dout, out = _rows("dout", dout, q), _rows("out", out, q)
+    B, Tq, Hq, D = q.shape
+    Tk, Hkv = k.shape[1], k.shape[2]
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise ValueError("dout %r and out %r have to have the shape of q %r" % (tuple(dout.shape), tuple(out.shape), tuple(q.shape)))
+    lse = _result("lse", lse, (B, Hq, Tq), torch.float32, q.device)
+    dq = _result("dq", dq, q.shape, q.dtype, q.device)
+    dk, dv = _result("dk", dk, k.shape, q.dtype, q.device), _result("dv", dv, v.shape, q.dtype, q.device)
+    kl, ql = _lens("k_lens", k_lens, B, q.device), _lens("q_lens", q_lens, B, q.device)
+    if Tq == 0:
+        dk.zero_(); dv.zero_()
+    elif q.numel():
+        kv = (k.data_ptr(), v.data_ptr(), dk.data_ptr(), dv.data_ptr()) if Tk else (q.data_ptr(),) * 4                # (no frames: never read or written)
+        a = Xattn(q.data_ptr(), kv[0], kv[1], dout.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), kv[2], kv[3], kl, ql, None, 0,
+                  *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *dout.stride()[:3], B, Tq, Tk, Hq, Hkv, D,
+                  1.0 / math.sqrt(D) if scale is None else float(scale), 0)
+        ws = _workspace("sar_xattn_bwd_workspace_bytes", a, q.device)                            # noqa: F841
+        _launch("sar_xattn_bwd_" + _SFX[q.dtype], q.device, ctypes.byref(a))
+    return dq, dk, dv
+
+
+class EncoderCache8:
+    """An utterance batch's keys and values in 8 bits for decoding token by token: half (a quarter) of the bytes of 16-bit (fp32) ones, and every
+    token reads all of them.
+
+    k8, v8 (batch, heads, frames rounded up to 64, dim) float8_e4m3fn; k_scale, v_scale (batch, heads, blocks of 64 frames) fp32 powers of two,
+    value = e4m3 * scale; lens (batch,) int32.  The buffers keep their addresses for the cache's life, so a captured step stays valid over store()."""
+
+    BLOCK = 64
+
+    def __init__(self, batch, frames, heads, dim, device="cuda"):
+        batch, frames, heads, dim = int(batch), int(frames), int(heads), int(dim)
+        _heads(heads, heads, dim)
+        if batch < 1 or frames < 1:
+            raise ValueError("a cache needs at least one utterance and one frame, got %d and %d" % (batch, frames))
+        self.batch, self.frames, self.heads, self.dim = batch, frames, heads, dim
+        n = -(-frames // self.BLOCK)
+        self.k8, self.v8 = (torch.zeros(batch, heads, n * self.BLOCK, dim, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
+        self.k_scale, self.v_scale = (torch.ones(batch, heads, n, dtype=torch.float32, device=device) for _ in range(2))
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.device = self.k8.device
+
+    def store(self, k, v, k_lens=None, first=0):
+        """Write frames [first, first + T) of every utterance from k, v (batch, T, heads, dim) (fp32, bf16 or fp16); `first` is a multiple of 64:
+        a streaming encoder appends whole blocks.  k_lens: how many of these T frames each utterance has (int32 (batch,); None: all) -- the
+        rest is stored as zeros.  The cache's lens become first + k_lens; with first > 0 an utterance without new frames keeps its length."""
+        k, v = _rows("k", k), _rows("v", v, k)
+        B, T, H, D = k.shape
+        if k.shape != v.shape or B != self.batch or H != self.heads or D != self.dim or k.device != self.device:
+            raise ValueError("k %r and v %r on %s do not fit a cache of %d utterances, %d heads of %d on %s" %
+                             (tuple(k.shape), tuple(v.shape), k.device, self.batch, self.heads, self.dim, self.device))
+        first = int(first)
+        if first < 0 or first % self.BLOCK or T < 1 or first + T > self.frames:
+            raise ValueError("frames [%d, %d) do not fit: first has to be a multiple of %d, the cache has %d frames" % (first, first + T, self.BLOCK, self.frames))
+        kl = _lens("k_lens", k_lens, B, k.device)
+        _launch("sar_kv8_store_" + _SFX[k.dtype], k.device, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], kl, self.k8.data_ptr(), self.k_scale.data_ptr(),
+                self.v8.data_ptr(), self.v_scale.data_ptr(), self.lens.data_ptr(), B, T, H, D, self.k8.shape[2], first)
+
+    def attend(self, q, q_lens=None, scale=None, out=None):
+        """cross_attention(q, held k, held v, k_lens=lens): q (batch, Tq, Hq, dim) of any of the three types, Hq a multiple of the cache's heads
+        -> out of q's type.  Made for a few rows (Tq Hq / heads); each 32 of them read the cache once."""
+        q = _rows("q", q)
+        B, Tq, Hq, D = q.shape
+        if B != self.batch or D != self.dim or q.device != self.device:
+            raise ValueError("q %r on %s does not fit a cache of %d utterances, %d heads of %d on %s" % (tuple(q.shape), q.device, self.batch, self.heads, self.dim, self.device))
+        _heads(Hq, self.heads, D)
+        out = _result("out", out, q.shape, q.dtype, q.device)
+        if out.numel():
+            a = Xattn(q.data_ptr(), None, None, None, out.data_ptr(), None, None, None, None, self.lens.data_ptr(), _lens("q_lens", q_lens, B, q.device), None, 0,
+                      *q.stride()[:3], 0, 0, 0, 0, 0, 0, *out.stride()[:3], 0, 0, 0, B, Tq, self.frames, Hq, self.heads, D,
+                      1.0 / math.sqrt(D) if scale is None else float(scale), 0)
+            ws = _workspace("sar_kv8_attend_workspace_bytes", a, q.device)                       # noqa: F841
+            _launch("sar_kv8_attend_" + _SFX[q.dtype], q.device, ctypes.byref(a), self.k8.data_ptr(), self.k_scale.data_ptr(), self.v8.data_ptr(),
+                    self.v_scale.data_ptr(), self.k8.shape[2])
+        return out

@@ -1,0 +1,141 @@
+// What the attention kernels share: 16-byte fragments, MFMA tiles of 32 x 32, the LDS layout of a (rows, D) tile.
+//
+// Every product here keeps one side in registers (32 columns n per wave) and streams the other through LDS (32 rows m per step), and is
+// written so that its 32 x 32 result can be the next product's operand WITHOUT leaving the registers:
+//   * a 32 x 32 result holds column n = lane % 32, rows m = 8 a + 4 h + c (h = lane / 32; a, c = 0..3): sixteen values of ONE column.
+//   * as the B operand of the next product (n = lane % 32, contraction index over those rows), the k-th slot of half h may be ANY row as
+//     long as the A operand names the same one: with 16-bit types step s takes rows 16 s + {4 h + c, 8 + 4 h + c}, in fp32 step (a, c)
+//     takes row 8 a + 4 h + c.  The A operand of that product is the streamed tile read "down its columns": ds_read_b64_tr_b16 hands
+//     a lane four consecutive rows of one column (16-bit), plain 4-byte reads do it in fp32.
+// A "fragment" is 16 bytes of a row: bytes [32 c + 16 h, +16) of chunk c -- eight 16-bit values (one 32x32x16 MFMA) or four fp32 values
+// (four 32x32x2 MFMAs whose k-th pair of dims is {8 c + k, 8 c + 4 + k}).
+#pragma once
+#include "common.h"
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(4))) short i16x4;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
+
+namespace attn {
+
+template <typename T> struct Num;
+template <> struct Num<float> { typedef f32x4 x16; typedef f32x4 x4; static constexpr int PER = 4; };
+template <> struct Num<__bf16> { typedef bf16x8 x16; typedef bf16x4 x4; static constexpr int PER = 8; };
+template <> struct Num<_Float16> { typedef f16x8 x16; typedef f16x4 x4; static constexpr int PER = 8; };
+
+template <typename T> __device__ __forceinline__ typename Num<T>::x16 as16(u32x4 v) { return __builtin_bit_cast(typename Num<T>::x16, v); }
+
+// acc += A B over one 32-byte chunk
+template <typename T> __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 acc) {
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 x = as16<float>(a), y = as16<float>(b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], acc, 0, 0, 0);
+        return acc;
+    } else if constexpr (__is_same(T, __bf16)) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as16<__bf16>(a), as16<__bf16>(b), acc, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(as16<_Float16>(a), as16<_Float16>(b), acc, 0, 0, 0);
+    }
+}
+
+// bytes between two rows of a tile in LDS: a power of two, so that the swizzle below stays inside the row
+template <typename T, int DP> constexpr int pitch() {
+    constexpr int b = DP * (int)sizeof(T);
+    return b <= 64 ? 64 : b <= 128 ? 128 : b <= 256 ? 256 : 512;
+}
+// 16-byte chunk `ch` of row `row`: eight consecutive rows put one chunk into eight different bank groups of 16 bytes (row-wise 16-byte
+// reads), four consecutive rows put a PAIR of chunks into four different ones (the transposing reads)
+template <int PITCH> __device__ __forceinline__ int chunk_at(int row, int ch) {
+    const int f = PITCH == 64 ? (row & 2) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1);
+    return row * PITCH + ((ch ^ f) << 4);
+}
+// fragment of chunk c: row `row`
+template <int PITCH> __device__ __forceinline__ u32x4 frag(const char* tile, int row, int c, int h) {
+    return *reinterpret_cast<const u32x4*>(tile + chunk_at<PITCH>(row, 2 * c + h));
+}
+__device__ __forceinline__ u32x2 tr16(const char* p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)p));
+}
+
+// acc (32 columns-of-the-tile x 32 n) += tile^T P for 32 tile rows starting at row0; dims [32 dt, +32); p: a 32 x 32 result (see above)
+// P's planes: 16-bit operands in groups of two fragments (steps s = 0, 1)
+template <typename T, int PITCH> __device__ __forceinline__ f32x16 mma_down(const char* tile, int row0, int dt, const u32x4* p, f32x16 acc, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+        const int d = 32 * dt + (lane & 31);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const f32x4 x = as16<float>(p[a]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int r = row0 + 8 * a + 4 * h + c;
+                const float v = *reinterpret_cast<const float*>(tile + chunk_at<PITCH>(r, d >> 2) + ((d & 3) << 2));
+                acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v, x[c], acc, 0, 0, 0);
+            }
+        }
+    } else {
+        // lane i of a group of 16 reads 8 bytes of row (i / 4), columns 4 (i % 4) ..; it receives column i of those four rows
+        const int i = lane & 15, g = (lane >> 4) & 1;
+        const int ch = 4 * dt + 2 * g + ((i >> 1) & 1), off = (i & 1) * 8;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int r = row0 + 16 * s + 4 * h + (i >> 2);
+            const u32x2 lo = tr16(tile + chunk_at<PITCH>(r, ch) + off), hi = tr16(tile + chunk_at<PITCH>(r + 8, ch) + off);
+            acc = mma<T>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[s], acc);
+        }
+    }
+    return acc;
+}
+
+// a 32 x 32 result as the B operand of mma_down: fp32 as it is (four fragments), 16-bit rounded to nearest even (two)
+template <typename T> __device__ __forceinline__ void pack(const f32x16& s, u32x4* p) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int a = 0; a < 4; ++a) p[a] = __builtin_bit_cast(u32x4, f32x4{s[4 * a], s[4 * a + 1], s[4 * a + 2], s[4 * a + 3]});
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            typename Num<T>::x16 v;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = (T)s[8 * k + j];
+            p[k] = __builtin_bit_cast(u32x4, v);
+        }
+    }
+}
+
+// the fragments of one row (a wave's column n), zero past D and for rows that do not exist
+template <typename T, int DP> __device__ __forceinline__ void load_row(const T* p, bool ok, int D, int h, u32x4* f) {
+    constexpr int NC = DP * (int)sizeof(T) / 32;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = (2 * c + h) * Num<T>::PER;
+        f[c] = u32x4{0, 0, 0, 0};
+        if (ok && d < D) f[c] = *reinterpret_cast<const u32x4*>(p + d);
+    }
+}
+
+// v of the lower and of the upper half of a column (lanes l and l ^ 32), to both.  (Written out: hipcc 7.2 takes the two results of its builtin for
+// one.  The wait states are those it puts between a VALU write of an operand and the swap.)
+__device__ __forceinline__ void halves(float v, float& lo, float& hi) {
+    lo = v; hi = v;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(lo), "+v"(hi));
+}
+__device__ __forceinline__ float half_max(float v) { float a, b; halves(v, a, b); return fmaxf(a, b); }
+__device__ __forceinline__ float half_sum(float v) { float a, b; halves(v, a, b); return a + b; }
+
+// blockIdx -> work item such that consecutive items (which share keys and values) land on ONE of the eight XCDs, whose L2 then holds them;
+// the grid is rounded up to a multiple of 8, surplus blocks get -1
+__device__ __forceinline__ long xcd_item(long n) {
+    const long per = (n + 7) >> 3, i = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    return (long)(blockIdx.x >> 3) < per && i < n ? i : -1;
+}
+static inline long xcd_grid(long n) { return ((n + 7) >> 3) << 3; }
+
+}  // namespace attn

@@ -1,0 +1,74 @@
+// Arguments and row folding shared by the cross-attention kernels (xattn.hip, xattn_step.hip).
+#pragma once
+#include "attn_tiles.h"
+
+// include/sarnet.h: sarXattn (kept field for field)
+struct sarXattn {
+    const void *q, *k, *v, *dout;
+    void* out;
+    float* lse;
+    void *dq, *dk, *dv;
+    const int *k_lens, *q_lens;
+    void* ws;
+    long ws_bytes;
+    long q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, o_sb, o_st, o_sh, g_sb, g_st, g_sh;
+    int B, Tq, Tk, Hq, Hkv, D;
+    float scale;
+    int pad_;
+};
+
+namespace attn {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float NO_MAX = -1e30f;        // the running maximum before any key: finite, so that exp2(x - NO_MAX) needs no special case
+
+// The query heads of one key head are folded into the rows: row r = t G + g is token t of query head hkv G + g, so a key / value tile is
+// fetched once for all of them, and G tokens of a single-token step share one MFMA tile.
+__device__ __forceinline__ int live_keys(const sarXattn& a, int b) { return a.k_lens ? min(max(a.k_lens[b], 0), a.Tk) : a.Tk; }
+__device__ __forceinline__ int live_rows(const sarXattn& a, int b) { return (a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq) * (a.Hq / a.Hkv); }
+
+struct Row { int t, h; };
+__device__ __forceinline__ Row row_of(const sarXattn& a, int hkv, int r) {
+    const int G = a.Hq / a.Hkv, t = r / G;
+    return {t, hkv * G + (r - t * G)};
+}
+// position of a row's statistics: lse is (B, Hq, Tq)
+__device__ __forceinline__ long stat_at(const sarXattn& a, int b, Row w) { return ((long)b * a.Hq + w.h) * a.Tq + w.t; }
+
+// the split form's partial results: O (splits, rows, D) fp32, then m and l (splits, rows); rows = B Hq Tq
+__device__ __host__ __forceinline__ long part_floats(long rows, int D, int splits) { return splits * rows * (D + 2); }
+
+// ---- host side: what a call may look like, and how far its key axis is cut
+static inline bool bad_shape(const sarXattn* a) {
+    if (!a || a->B < 1 || a->Tq < 1 || a->Tk < 0 || a->Hkv < 1 || a->Hq < 1 || a->Hq % a->Hkv || a->D < 8 || a->D > 128 || a->D % 8) return true;
+    const long R = (long)a->Tq * (a->Hq / a->Hkv);
+    return R > (1L << 30) || a->Tk > (1 << 30) || (R + 31) / 32 * a->B * a->Hkv > (1L << 24) || (a->Tk + 127L) / 128 * a->B * a->Hkv > (1L << 24);
+}
+static inline bool bad_strides(int elt_bytes, const long* s, int n) {
+    for (int i = 0; i < n; ++i)
+        if (s[i] < 0 || s[i] * elt_bytes % 16) return true;
+    return false;
+}
+static inline bool few_rows(const sarXattn* a) { return (long)a->Tq * (a->Hq / a->Hkv) <= 32; }
+// key slices: as many as bring the grid to `blocks`, of 256 keys at least, 64 at most (one lane each in the joining kernel)
+static inline int key_splits(const sarXattn* a, int rows_per_block, int blocks) {
+    const long R = (long)a->Tq * (a->Hq / a->Hkv), tiles = (R + rows_per_block - 1) / rows_per_block * a->B * a->Hkv, keys = (a->Tk + 255L) / 256;
+    long s = (blocks + tiles - 1) / tiles;
+    if (s > keys) s = keys;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+static inline int fwd_splits(const sarXattn* a) { return key_splits(a, 128, 512); }
+static inline int step_splits(const sarXattn* a) { return key_splits(a, 32, 1024); }
+static inline size_t part_bytes(const sarXattn* a, int splits) {
+    return splits > 1 ? 4 * (size_t)part_floats((long)a->B * a->Hq * a->Tq, a->D, splits) : 0;
+}
+static inline bool bad_workspace(const sarXattn* a, size_t need) { return need && (!a->ws || (uintptr_t)a->ws % 16 || a->ws_bytes < 0 || (size_t)a->ws_bytes < need); }
+
+// four consecutive values of a row
+template <typename T> __device__ __forceinline__ void store4(T* p, float x, float y, float z, float w) {
+    typename Num<T>::x4 v;
+    v[0] = (T)x; v[1] = (T)y; v[2] = (T)z; v[3] = (T)w;
+    *reinterpret_cast<typename Num<T>::x4*>(p) = v;
+}
+
+}  // namespace attn

@@ -1,0 +1,402 @@
+// Attention of a FEW rows (one token, a beam's tokens) to many keys: up to 32 folded rows (tokens x query heads of a key head) are the
+// columns n of one MFMA tile, every wave of a block walks its own 32-key tiles without a barrier, waves and key slices are joined at the end.
+// Reading the keys and values once is the whole cost, so what counts is bytes in flight: the next tile's K and V are loaded into registers
+// while the present one is computed.  K goes from memory straight into fragments; V passes through a wave's own piece of LDS, where
+// the transposing reads pick it up.
+//
+// The same kernel reads the 8-bit cache (include/sarnet.h: sarKv8): e4m3 values are converted exactly into the 16-bit operand type (bf16 for
+// bf16 and fp32 queries, fp16 for fp16 ones); the scale of a 64-key block multiplies the fp32 scores (K), and the fp32 sums as a ratio of
+// powers of two (V).  fp32 queries and probabilities enter as three bf16 planes (8 + 8 + 8 bits hold an fp32 mantissa): products are exact, sums fp32,
+// at a third of the bf16 rate instead of the fp32 MFMA's sixteenth.
+// Compiled once per element type: SAR_ELT 0 = fp32, 1 = bf16, 2 = fp16.
+#include "xattn.h"
+
+#if SAR_ELT == 0
+typedef float elt;
+typedef __bf16 wide8;
+#define SAR_FN(n) n##_f32
+#elif SAR_ELT == 1
+typedef __bf16 elt;
+typedef __bf16 wide8;
+#define SAR_FN(n) n##_bf16
+#else
+typedef _Float16 elt;
+typedef _Float16 wide8;
+#define SAR_FN(n) n##_f16
+#endif
+
+namespace attn {
+
+constexpr int KV_BLOCK = 64;            // frames that share a scale
+
+struct Kv8 { const unsigned char *k8, *v8; const float *ks, *vs; long frames; };   // (B, Hkv, frames, D), (B, Hkv, frames / 64)
+
+// eight e4m3 values -> eight 16-bit ones, exactly
+template <typename C> __device__ __forceinline__ u32x4 widen8(u32x2 w) {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int src = (int)w[i >> 1];
+        if constexpr (__is_same(C, __bf16)) {
+            const auto v = (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, 1.f, false);
+            o[i] = __builtin_bit_cast(unsigned, v);
+        } else {
+            const auto v = (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(src, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(src, 1.f, false);
+            o[i] = __builtin_bit_cast(unsigned, v);
+        }
+    }
+    return o;
+}
+// 16 bytes of a row of D bytes (D a multiple of 8) from dim d on, zero past D
+__device__ __forceinline__ u32x4 load8(const unsigned char* p, int d, int D, bool ok) {
+    u32x4 r = {0, 0, 0, 0};
+    if (ok && d + 16 <= D && (D & 15) == 0) r = *reinterpret_cast<const u32x4*>(p + d);
+    else {
+        if (ok && d < D) { const u32x2 w = *reinterpret_cast<const u32x2*>(p + d); r[0] = w[0]; r[1] = w[1]; }
+        if (ok && d + 8 < D) { const u32x2 w = *reinterpret_cast<const u32x2*>(p + d + 8); r[2] = w[0]; r[3] = w[1]; }
+    }
+    return r;
+}
+
+// a 32 x 32 fp32 result as operand planes of the 16-bit type: one (rounded), or three whose sum is the value
+template <typename C, int NPL> __device__ __forceinline__ void pack_planes(f32x16 s, u32x4 (*p)[4]) {
+#pragma unroll
+    for (int k = 0; k < NPL; ++k) {
+        pack<C>(s, p[k]);
+        if (k + 1 < NPL)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] -= (float)(C)s[i];
+    }
+}
+
+template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_bounds__(64 * NW) void xattn_step_kernel(sarXattn a, Kv8 kv, int row_tiles, int splits) {
+    constexpr int P = pitch<C, DP>(), ND = DP / 32, NPL = S8 && sizeof(T) == 4 ? 3 : 1;
+    constexpr int NC = DP * (int)sizeof(C) / 32;                  // operand chunks of a row
+    constexpr int CHV = DP * (S8 ? 1 : (int)sizeof(T)) / 16;      // stored 16-byte pieces of a row
+    constexpr int NKL = S8 ? DP / 32 : NC, NVL = 32 * CHV / 64;
+    extern __shared__ __attribute__((aligned(16))) char lds[];    // V tiles of the waves; afterwards their partial sums
+    __shared__ float lm[NW][32], ll[NW][32];
+    const long item = xcd_item((long)a.B * a.Hkv * row_tiles * splits);
+    if (item < 0) return;
+    const int sp = (int)(item % splits), rt = (int)((item / splits) % row_tiles), bh = (int)(item / splits / row_tiles);
+    const int b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
+    const int R = a.Tq * (a.Hq / a.Hkv), r = rt * 32 + n, rl = live_rows(a, b), len = live_keys(a, b);
+    const int tiles = (len + 31) / 32, per = (tiles + splits - 1) / splits;
+    const int t0 = min(sp * per, tiles), t1 = rt * 32 < rl ? min(t0 + per, tiles) : t0;
+    const Row me = row_of(a, hk, min(r, R - 1));
+    const float sl = a.scale * LOG2E;
+    char* tile = lds + w * 32 * P;
+
+    u32x4 qf[NPL][NC];
+    {
+        const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + me.t * a.q_st + me.h * a.q_sh;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            // the order of the dims among the contraction's slots follows the stored keys: 16 bytes a lane and half
+            const int d = S8 ? 32 * (c >> 1) + 16 * h + 8 * (c & 1) : (2 * c + h) * Num<T>::PER;
+            const bool ok = r < rl && d < a.D;
+            if constexpr (S8 && sizeof(T) == 4) {
+                f32x4 x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
+                if (ok) { x0 = *reinterpret_cast<const f32x4*>(qp + d); x1 = *reinterpret_cast<const f32x4*>(qp + d + 4); }
+#pragma unroll
+                for (int k = 0; k < NPL; ++k) {
+                    typename Num<C>::x16 v;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { v[j] = (C)x0[j]; v[4 + j] = (C)x1[j]; x0[j] -= (float)v[j]; x1[j] -= (float)v[4 + j]; }
+                    qf[k][c] = __builtin_bit_cast(u32x4, v);
+                }
+            } else {
+                qf[0][c] = u32x4{0, 0, 0, 0};
+                if (ok) qf[0][c] = *reinterpret_cast<const u32x4*>(qp + d);
+            }
+        }
+    }
+    const T* kb = S8 ? nullptr : reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
+    const T* vb = S8 ? nullptr : reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
+    const unsigned char* k8 = S8 ? kv.k8 + (long)bh * kv.frames * a.D : nullptr;
+    const unsigned char* v8 = S8 ? kv.v8 + (long)bh * kv.frames * a.D : nullptr;
+    const float* ks = S8 ? kv.ks + (long)bh * (kv.frames / KV_BLOCK) : nullptr;
+    const float* vs = S8 ? kv.vs + (long)bh * (kv.frames / KV_BLOCK) : nullptr;
+
+    u32x4 kr[NKL], vr[NVL];
+    float ksc = 1.f, vsc = 1.f;
+    const auto load = [&](int t) {
+        const int key = t * 32 + n;
+        if constexpr (S8) {
+#pragma unroll
+            for (int c = 0; c < NKL; ++c) kr[c] = load8(k8 + (long)key * a.D, 32 * c + 16 * h, a.D, key < len);
+#pragma unroll
+            for (int i = 0; i < NVL; ++i) {
+                const int idx = lane + 64 * i, row = t * 32 + idx / CHV;
+                vr[i] = load8(v8 + (long)row * a.D, 16 * (idx % CHV), a.D, row < len);
+            }
+            ksc = ks[t * 32 / KV_BLOCK]; vsc = vs[t * 32 / KV_BLOCK];
+        } else {
+            load_row<T, DP>(kb + (long)key * a.k_st, key < len, a.D, h, kr);
+#pragma unroll
+            for (int i = 0; i < NVL; ++i) {
+                const int idx = lane + 64 * i, row = t * 32 + idx / CHV, d = (idx % CHV) * Num<T>::PER;
+                vr[i] = u32x4{0, 0, 0, 0};
+                if (row < len && d < a.D) vr[i] = *reinterpret_cast<const u32x4*>(vb + (long)row * a.v_st + d);
+            }
+        }
+    };
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = NO_MAX, l = 0.f, unit = 1.f;                        // o holds sums in units of `unit` (a power of two; 1 without a cache)
+    if (t0 + w < t1) load(t0 + w);
+    if (S8 && t0 + w < t1) unit = vsc;
+    for (int t = t0 + w; t < t1; t += NW) {
+        f32x16 s;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+        if constexpr (S8) {
+#pragma unroll
+            for (int c = 0; c < NKL; ++c) {
+                const u32x4 lo = widen8<C>(u32x2{kr[c][0], kr[c][1]}), hi = widen8<C>(u32x2{kr[c][2], kr[c][3]});
+#pragma unroll
+                for (int k = NPL - 1; k >= 0; --k) { s = mma<C>(lo, qf[k][2 * c], s); s = mma<C>(hi, qf[k][2 * c + 1], s); }
+            }
+#pragma unroll
+            for (int i = 0; i < NVL; ++i) {
+                const int idx = lane + 64 * i, row = idx / CHV, ch = idx % CHV;
+                *reinterpret_cast<u32x4*>(tile + chunk_at<P>(row, 2 * ch)) = widen8<C>(u32x2{vr[i][0], vr[i][1]});
+                *reinterpret_cast<u32x4*>(tile + chunk_at<P>(row, 2 * ch + 1)) = widen8<C>(u32x2{vr[i][2], vr[i][3]});
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s = mma<T>(kr[c], qf[0][c], s);
+#pragma unroll
+            for (int i = 0; i < NVL; ++i) {
+                const int idx = lane + 64 * i;
+                *reinterpret_cast<u32x4*>(tile + chunk_at<P>(idx / CHV, idx % CHV)) = vr[i];
+            }
+        }
+        const float f = sl * ksc, nu = vsc;
+        if (t + NW < t1) load(t + NW);
+        float top = NO_MAX;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const bool in = t * 32 + 8 * (i >> 2) + 4 * h + (i & 3) < len;
+            s[i] = in ? s[i] * f : -INFINITY;
+            top = fmaxf(top, s[i]);
+        }
+        top = half_max(top);
+        if (__any(top > m + 8.f) || (S8 && nu != unit)) {
+            const float mn = fmaxf(m, top), e = __builtin_amdgcn_exp2f(m - mn), eo = S8 ? e * (unit / nu) : e;
+            m = mn; l *= e;
+            if (S8) unit = nu;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= eo;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(s[i] - m); l += s[i]; }
+        u32x4 p[NPL][4];
+        pack_planes<C, NPL>(s, p);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int k = NPL - 1; k >= 0; --k) o[d] = mma_down<C, P>(tile, 0, d, p[k], o[d], lane);
+        __builtin_amdgcn_wave_barrier();
+    }
+    l = half_sum(l);
+
+    // ---- join the waves: o, m, l of the live rows through LDS
+    const int nr = min(R - rt * 32, 32);
+    float* lo = reinterpret_cast<float*>(lds);
+    __syncthreads();                                              // every wave is done with its V tile
+    if (n < nr) {
+        float* op = lo + ((long)w * nr + n) * DP;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4*>(op + 32 * d + 8 * i + 4 * h) = f32x4{o[d][4 * i] * unit, o[d][4 * i + 1] * unit, o[d][4 * i + 2] * unit, o[d][4 * i + 3] * unit};
+        if (h == 0) { lm[w][n] = m; ll[w][n] = l; }
+    }
+    __syncthreads();
+    const int D4 = a.D / 4;
+    for (int e = threadIdx.x; e < nr * D4; e += 64 * NW) {
+        const int row = e / D4, d = (e - row * D4) * 4;
+        float M = lm[0][row];
+#pragma unroll
+        for (int x = 1; x < NW; ++x) M = fmaxf(M, lm[x][row]);
+        float L = 0.f;
+        f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+            const float g = __builtin_amdgcn_exp2f(lm[x][row] - M);
+            L = fmaf(ll[x][row], g, L);
+            v += *reinterpret_cast<const f32x4*>(lo + ((long)x * nr + row) * DP + d) * g;
+        }
+        const Row at = row_of(a, hk, rt * 32 + row);
+        if (splits == 1) {
+            const bool in = rt * 32 + row < rl && L != 0.f;
+            const float inv = 1.f / L;
+            store4<T>(reinterpret_cast<T*>(a.out) + b * a.o_sb + at.t * a.o_st + at.h * a.o_sh + d, in ? v[0] * inv : 0.f, in ? v[1] * inv : 0.f, in ? v[2] * inv : 0.f, in ? v[3] * inv : 0.f);
+            if (a.lse && d == 0) a.lse[stat_at(a, b, at)] = in ? M * LN2 + logf(L) : -INFINITY;
+        } else {
+            const long rows = (long)a.B * a.Hq * a.Tq, i = sp * rows + stat_at(a, b, at);
+            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.ws) + i * a.D + d) = v;
+            if (d == 0) {
+                float* ml = reinterpret_cast<float*>(a.ws) + splits * rows * a.D + i;
+                ml[0] = M; ml[splits * rows] = L;
+            }
+        }
+    }
+}
+
+// joins the key slices: one wave per row
+template <typename T> __global__ __launch_bounds__(256) void xattn_combine_kernel(sarXattn a, int splits) {
+    const long rows = (long)a.B * a.Hq * a.Tq, i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= rows) return;
+    const int t = (int)(i % a.Tq), hq = (int)(i / a.Tq % a.Hq), b = (int)(i / a.Tq / a.Hq), lane = threadIdx.x & 63;
+    const float* po = reinterpret_cast<const float*>(a.ws);
+    const float* pm = po + splits * rows * a.D;
+    const float m = lane < splits ? pm[lane * rows + i] : NO_MAX, l = lane < splits ? pm[(splits + lane) * rows + i] : 0.f;
+    const float M = wave_max(m), f = __builtin_amdgcn_exp2f(m - M), L = wave_sum(l * f);
+    const bool in = t < (a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq) && L != 0.f;
+    const int d = 2 * lane;
+    float x = 0.f, y = 0.f;
+    for (int s = 0; s < splits; ++s) {
+        const float g = __shfl(f, s, 64);
+        if (d < a.D) {
+            const float2 v = *reinterpret_cast<const float2*>(po + (s * rows + i) * a.D + d);
+            x = fmaf(v.x, g, x); y = fmaf(v.y, g, y);
+        }
+    }
+    const float inv = 1.f / L;
+    if (d < a.D) {
+        T* op = reinterpret_cast<T*>(a.out) + b * a.o_sb + t * a.o_st + hq * a.o_sh + d;
+        op[0] = (T)(in ? x * inv : 0.f); op[1] = (T)(in ? y * inv : 0.f);
+    }
+    if (a.lse && lane == 0) a.lse[i] = in ? M * LN2 + logf(L) : -INFINITY;
+}
+
+// ---- writing the cache: one block per (K or V, utterance, head, 64 frames): maximum, scale, conversion in one pass over its 64 D values
+struct Kv8Side { const void* x; long sb, st, sh; unsigned char* y; float* scale; };
+template <typename T> __global__ __launch_bounds__(256) void kv8_store_kernel(Kv8Side sk, Kv8Side sv, const int* __restrict__ lens, int* __restrict__ lens_out, int T_in, int H, int D,
+                                                                              long frames, int first, int blocks) {
+    __shared__ float red[4];
+    constexpr int V = 8;                                          // values a thread and step; D is a multiple of 8
+    const Kv8Side& sd = blockIdx.y ? sv : sk;
+    const T* x = reinterpret_cast<const T*>(sd.x);
+    const long sb = sd.sb, st = sd.st, sh = sd.sh;
+    const int j = blockIdx.x % blocks, bh = blockIdx.x / blocks, b = bh / H, hh = bh % H;
+    const int per = D / V, n = KV_BLOCK * per;                    // <= 1024: four steps
+    const int live = lens ? min(max(lens[b], 0), T_in) : T_in;
+    // the cache's length: an utterance without new frames keeps the one it has
+    if (j == 0 && hh == 0 && blockIdx.y == 0 && threadIdx.x == 0 && (live > 0 || first == 0)) lens_out[b] = first + live;
+    float v[4][V];
+    float top = 0.f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const int e = threadIdx.x + 256 * s, row = e / per, d = (e - row * per) * V, t = j * KV_BLOCK + row;
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[s][k] = 0.f;
+        if (e < n && t < live) {
+            const T* p = x + b * sb + (long)t * st + hh * sh + d;
+#pragma unroll
+            for (int q = 0; q < V; q += Num<T>::PER) {
+                const auto u = *reinterpret_cast<const typename Num<T>::x16*>(p + q);
+#pragma unroll
+                for (int k = 0; k < Num<T>::PER; ++k) v[s][q + k] = (float)u[k];
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) { const float m = fabsf(v[s][k]); if (m < INFINITY) top = fmaxf(top, m); }
+        }
+    }
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    // top = f 2^e, f in [1/2, 1): the smallest power of two with top / scale <= 448 = 7/8 2^9.  (Held at 2^-118 and above: its inverse stays finite.)
+    int e = 0;
+    const float f = frexpf(top, &e);
+    e = top == 0.f ? 0 : max(f <= 0.875f ? e - 9 : e - 8, -118);
+    const float inv = ldexpf(1.f, -e);
+    const long blk = (long)bh * (frames / KV_BLOCK) + first / KV_BLOCK + j;
+    if (threadIdx.x == 0) sd.scale[blk] = ldexpf(1.f, e);
+    unsigned char* o = sd.y + blk * KV_BLOCK * D;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const int q = threadIdx.x + 256 * s;
+        if (q >= n) continue;
+        u32x2 w;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            int p = 0;
+            p = __builtin_amdgcn_cvt_pk_fp8_f32(v[s][4 * k] * inv, v[s][4 * k + 1] * inv, p, false);
+            p = __builtin_amdgcn_cvt_pk_fp8_f32(v[s][4 * k + 2] * inv, v[s][4 * k + 3] * inv, p, true);
+            w[k] = (unsigned)p;
+        }
+        *reinterpret_cast<u32x2*>(o + (long)q * V) = w;
+    }
+}
+
+}  // namespace attn
+using namespace attn;
+
+template <typename C, bool S8, int DP> static int launch_step(const sarXattn& a, const Kv8& kv, int splits, hipStream_t st) {
+    constexpr int NW = 4;
+    const long R = (long)a.Tq * (a.Hq / a.Hkv);
+    const int rt = cdiv(R, 32);
+    const size_t tiles = (size_t)NW * 32 * pitch<C, DP>(), join = (size_t)NW * (R < 32 ? R : 32) * DP * 4, lds = tiles > join ? tiles : join;
+    auto* k = &xattn_step_kernel<elt, C, S8, DP, NW>;
+    static PerDeviceFlag raised;
+    if (lds > 64 * 1024 && !raised) {
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 2048) != hipSuccess) return SAR_ELAUNCH;
+        raised = true;
+    }
+    hipLaunchKernelGGL(k, dim3((unsigned)xcd_grid((long)rt * splits * a.B * a.Hkv)), dim3(64 * NW), lds, st, a, kv, rt, splits);
+    SAR_CHECK_LAUNCH();
+    return SAR_OK;
+}
+
+int SAR_FN(xattn_combine)(const sarXattn* a, int splits, hipStream_t stream) {
+    hipLaunchKernelGGL((xattn_combine_kernel<elt>), dim3((unsigned)cdiv((long)a->B * a->Hq * a->Tq, 4)), dim3(256), 0, stream, *a, splits);
+    SAR_CHECK_LAUNCH();
+    return SAR_OK;
+}
+
+template <typename C, bool S8> static int step(const sarXattn* a, const Kv8& kv, int splits, hipStream_t stream) {
+    const int rc = a->D <= 32 ? launch_step<C, S8, 32>(*a, kv, splits, stream) : a->D <= 64 ? launch_step<C, S8, 64>(*a, kv, splits, stream)
+                 : a->D <= 96 ? launch_step<C, S8, 96>(*a, kv, splits, stream) : launch_step<C, S8, 128>(*a, kv, splits, stream);
+    return rc == SAR_OK && splits > 1 ? SAR_FN(xattn_combine)(a, splits, stream) : rc;
+}
+int SAR_FN(xattn_step)(const sarXattn* a, int splits, hipStream_t stream) { return step<elt, false>(a, Kv8{}, splits, stream); }
+
+// ---- the 8-bit cache
+static bool bad8(const sarXattn* a, long frames) { return bad_shape(a) || frames < a->Tk || frames % KV_BLOCK || frames > (1L << 30); }
+#if SAR_ELT == 0      // the same for every type
+extern "C" size_t sar_kv8_attend_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, step_splits(a)); }
+#endif
+extern "C" int SAR_FN(sar_kv8_attend)(const sarXattn* a, const void* k8, const float* k_scale, const void* v8, const float* v_scale, long frames, hipStream_t stream) {
+    if (bad8(a, frames) || bad_strides(sizeof(elt), &a->q_sb, 3) || bad_strides(sizeof(elt), &a->o_sb, 3) || !a->q || !a->out || !k8 || !v8 || !k_scale || !v_scale) return SAR_EINVAL;
+    for (const void* p : {a->q, (const void*)a->out, k8, v8})
+        if ((uintptr_t)p % 16) return SAR_EINVAL;
+    if (bad_workspace(a, part_bytes(a, step_splits(a)))) return SAR_EINVAL;
+    return step<wide8, true>(a, Kv8{(const unsigned char*)k8, (const unsigned char*)v8, k_scale, v_scale, frames}, step_splits(a), stream);
+}
+extern "C" int SAR_FN(sar_kv8_store)(const void* k, long k_sb, long k_st, long k_sh, const void* v, long v_sb, long v_st, long v_sh, const int* lens, void* k8, float* k_scale,
+                                     void* v8, float* v_scale, int* lens_out, int B, int T, int H, int D, long frames, int first, hipStream_t stream) {
+    const long s[6] = {k_sb, k_st, k_sh, v_sb, v_st, v_sh};
+    if (bad_strides(sizeof(elt), s, 6) || !k_scale || !v_scale || !lens_out || B < 1 || T < 1 || H < 1 || D < 8 || D > 128 || D % 8 || frames % KV_BLOCK || frames > (1L << 30) ||
+        first < 0 || first % KV_BLOCK || first + (long)T > frames)
+        return SAR_EINVAL;
+    for (const void* p : {k, v, (const void*)k8, (const void*)v8})
+        if (!p || (uintptr_t)p % 16) return SAR_EINVAL;
+    const int blocks = cdiv(T, KV_BLOCK);
+    if ((long)B * H > (1L << 30) / blocks) return SAR_EINVAL;
+    hipLaunchKernelGGL((kv8_store_kernel<elt>), dim3((unsigned)(B * H * blocks), 2), dim3(256), 0, stream, Kv8Side{k, k_sb, k_st, k_sh, (unsigned char*)k8, k_scale},
+                       Kv8Side{v, v_sb, v_st, v_sh, (unsigned char*)v8, v_scale}, lens, lens_out, T, H, D, frames, first, blocks);
+    SAR_CHECK_LAUNCH();
+    return SAR_OK;
+}

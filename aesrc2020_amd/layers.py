@@ -8,6 +8,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .attention import cross_attention, cross_attention_grad
 from .engine import ACT, current_store, gemm, pick_splitk, he_normal, glorot_uniform, orthogonal
 
 _call = _lib.call
@@ -339,3 +340,30 @@ class L2Normalize(Layer):
         dx = dx_out if dx_out is not None else self.buf("dx", (self.B, self.dim))
         _call("sar_l2norm_rows_bwd_f32", dv, self.v, self.inv, dx, self.B, self.dim, 1 if accumulate_dx else 0)
         return dx
+
+
+class CrossAttention(Layer):
+    """Scaled dot-product attention of decoder rows to encoder rows (csrc/xattn.hip), no weights: the projections are Dense layers.
+    dim = heads * head width; kv_heads < heads: groups of query heads share a key head."""
+
+    def __init__(self, dim, heads, kv_heads=None, name=None):
+        super().__init__(name)
+        kv_heads = heads if kv_heads is None else kv_heads
+        if dim % heads or heads % kv_heads:
+            raise ValueError("%d wide over %d heads, %d key heads" % (dim, heads, kv_heads))
+        self.dim, self.heads, self.kv_heads, self.width = dim, heads, kv_heads, dim // heads
+        self.output_shape = (None, None, dim)
+
+    def forward(self, q, k, v, B, Lq, Lk, k_lens=None, q_lens=None):
+        """q (B * Lq, dim), k, v (B * Lk, kv_heads * width) rows -> (B * Lq, dim); k_lens, q_lens int32 (B,) or None."""
+        self.q, self.k, self.v = q.view(B, Lq, self.heads, self.width), k.view(B, Lk, self.kv_heads, self.width), v.view(B, Lk, self.kv_heads, self.width)
+        self.k_lens, self.q_lens = k_lens, q_lens
+        self.y, self.lse = self.buf("y", self.q.shape, q.dtype), self.buf("lse", (B, self.heads, Lq))
+        cross_attention(self.q, self.k, self.v, k_lens, q_lens, return_lse=True, out=self.y, lse=self.lse)
+        return self.y.view(B * Lq, self.dim)
+
+    def backward(self, dy):
+        """-> dq, dk, dv, as rows."""
+        dq, dk, dv = (self.buf(n, t.shape, t.dtype) for n, t in (("dq", self.q), ("dk", self.k), ("dv", self.v)))
+        cross_attention_grad(dy.view(self.q.shape), self.q, self.k, self.v, self.y, self.lse, self.k_lens, self.q_lens, dq=dq, dk=dk, dv=dv)
+        return dq.view(-1, self.dim), dk.view(-1, self.kv_heads * self.width), dv.view(-1, self.kv_heads * self.width)

@@ -583,6 +583,56 @@ int sar_adam_l2_step_f32(float* params, const float* grads, float* m, float* v, 
 int sar_grads_check_f32(const float* grads, void* ticket, long n, sarStream_t stream);
 int sar_adam_l2_update_f32(float* params, const float* grads, float* m, float* v, const float* chunk_l2, void* state, void* ticket,
                            float* l2_loss, long n, sarStream_t stream);
+/* ---- Cross attention to an encoder's states of another length (an attention decoder beside the CTC branch, model.py:117-119): forward,
+ * backward, single tokens.  Suffix = element type of q, k, v, out, dout, dq, dk, dv: f32 | bf16 | f16; statistics and sums are fp32.
+ *   s_ij = scale q_i . k_j for j < k_len;  p = softmax_j s;  o_i = sum_j p_ij v_j;  lse_i = log sum_j exp s_ij
+ * q, out, dout (B, Tq, Hq, D), k, v (B, Tk, Hkv, D): element strides of batch, time and head as given (non-negative, multiples of 16 bytes;
+ * the last axis is contiguous, pointers are 16-byte aligned); dq, dk, dv contiguous.  D: a multiple of 8 up to 128.  Hq a multiple of Hkv: query
+ * head h reads key head h / (Hq / Hkv), whose gradients sum over the group.  k_lens, q_lens (B) i32 or NULL (all); values outside
+ * [0, T] count as the nearer end.  Rows of K and V behind a length are not used, whatever they hold.  A row behind its q_len, and a
+ * row without keys, gets out = 0, lse = -inf and no gradient.  lse (B, Hq, Tq) fp32: optional in the forward, needed (with out) by the backward.
+ * ws: sar_xattn_fwd_workspace_bytes / _bwd_workspace_bytes of the same arguments, 16-byte aligned (0: none); nothing in it has to be initialised. */
+typedef struct {
+    const void *q, *k, *v, *dout;
+    void* out;
+    float* lse;
+    void *dq, *dk, *dv;
+    const int *k_lens, *q_lens;
+    void* ws;
+    long ws_bytes;
+    long q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, o_sb, o_st, o_sh, g_sb, g_st, g_sh;
+    int B, Tq, Tk, Hq, Hkv, D;
+    float scale;
+    int pad_;
+} sarXattn;
+size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a);
+size_t sar_xattn_bwd_workspace_bytes(const sarXattn* a);
+int sar_xattn_fwd_f32(const sarXattn* a, sarStream_t stream);
+int sar_xattn_fwd_bf16(const sarXattn* a, sarStream_t stream);
+int sar_xattn_fwd_f16(const sarXattn* a, sarStream_t stream);
+int sar_xattn_bwd_f32(const sarXattn* a, sarStream_t stream);
+int sar_xattn_bwd_bf16(const sarXattn* a, sarStream_t stream);
+int sar_xattn_bwd_f16(const sarXattn* a, sarStream_t stream);
+
+/* The encoder's keys and values held in 8 bits: written once per utterance, read by every token.  k8, v8 (B, H, frames, D) e4m3 (OCP), scales
+ * (B, H, frames / 64) fp32 powers of two, frames a multiple of 64: value = e4m3 * scale.  The scale of 64 frames of a head is the smallest power of
+ * two with max |x| / scale <= 448, so scaling is exact and the only rounding is e4m3's (to nearest even); 1 for a block of zeros, 2^-118 at least.
+ * A value that is not finite is held as NaN and left out of the maximum.
+ * sar_kv8_store: k, v (B, T, H, D) with element strides as above -> frames [first, first + T) (first a multiple of 64; the last block is
+ * filled with zeros); frames from lens[b] on are stored as zeros (lens NULL: all T are there).  lens_out[b] = first + lens[b]; with first > 0 an
+ * utterance without new frames keeps the length it has. */
+int sar_kv8_store_f32(const void* k, long k_sb, long k_st, long k_sh, const void* v, long v_sb, long v_st, long v_sh, const int* lens, void* k8, float* k_scale,
+                       void* v8, float* v_scale, int* lens_out, int B, int T, int H, int D, long frames, int first, sarStream_t stream);
+int sar_kv8_store_bf16(const void* k, long k_sb, long k_st, long k_sh, const void* v, long v_sb, long v_st, long v_sh, const int* lens, void* k8, float* k_scale,
+                       void* v8, float* v_scale, int* lens_out, int B, int T, int H, int D, long frames, int first, sarStream_t stream);
+int sar_kv8_store_f16(const void* k, long k_sb, long k_st, long k_sh, const void* v, long v_sb, long v_st, long v_sh, const int* lens, void* k8, float* k_scale,
+                       void* v8, float* v_scale, int* lens_out, int B, int T, int H, int D, long frames, int first, sarStream_t stream);
+/* sar_xattn_fwd over that cache (a->k, a->v and their strides are not read; a->Tk <= frames): any number of rows, made for a few. */
+size_t sar_kv8_attend_workspace_bytes(const sarXattn* a);
+int sar_kv8_attend_f32(const sarXattn* a, const void* k8, const float* k_scale, const void* v8, const float* v_scale, long frames, sarStream_t stream);
+int sar_kv8_attend_bf16(const sarXattn* a, const void* k8, const float* k_scale, const void* v8, const float* v_scale, long frames, sarStream_t stream);
+int sar_kv8_attend_f16(const sarXattn* a, const void* k8, const float* k_scale, const void* v8, const float* v_scale, long frames, sarStream_t stream);
+
 /* ---- data feeder: utils.py:35-36 feat_norm (sklearn MinMaxScaler.fit_transform per utterance: every
  * feature column scaled to [0,1] over ALL frames of the utterance; constant column -> 0) + utils.py:39-46 feat_reshape
  * (truncate / zero-pad to T frames).  frames = the batch's utterances back to back (sum_n, D) f32; offsets (B+1) i32 frame
