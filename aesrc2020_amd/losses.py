@@ -4,9 +4,12 @@ SphereFace / CosFace / ArcFace keep the reference constructor (n_classes, s, m, 
 `layer([x, y_onehot]) -> softmax probabilities` (losses.py:28-47, 74-91, 121-144); weight `W (D, n_classes)`,
 glorot_uniform (losses.py:22-26).  circle_loss(y_true, y_pred, gamma, margin) -> per-sample loss (losses.py:157-172).
 """
-import numpy as np
+import ctypes
+
+import torch
 
 from . import _lib
+from .attention import _SFX, _launch, _result
 from .engine import glorot_uniform
 from .layers import Layer
 
@@ -140,3 +143,107 @@ class CategoricalCrossentropy:
         dp = self.bufs.get(self.key + "/dp", (B, A))
         _call("sar_cce_bwd_f32", self.y, self.p, dloss, dp, B, A)
         return dp
+
+
+# ---- softmax cross entropy over a vocabulary, from the hidden rows and the output layer's kernel (csrc/vocab_ce.hip)
+class _VocabCe(ctypes.Structure):
+    """include/sarnet.h: sarVocabCe."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "kernel", "bias", "labels", "dloss", "loss", "lse", "dx", "dkernel", "dbias", "ws")] + \
+               [(n, ctypes.c_long) for n in ("ws_bytes", "ldx", "ldk")] + [(n, ctypes.c_int) for n in ("R", "D", "V", "label_bytes", "accumulate", "pad_")]
+
+
+def _vocab_args(x, kernel, labels, bias):
+    """-> x, kernel (rows contiguous), bias, labels as the kernels take them."""
+    if x.dim() != 2 or kernel.dim() != 2 or x.shape[1] != kernel.shape[0] or kernel.shape[1] < 1 or kernel.shape[0] < 1:
+        raise ValueError("x %r and kernel %r have to be (rows, D) and (D, vocabulary)" % (tuple(x.shape), tuple(kernel.shape)))
+    if x.dtype not in _SFX or not x.is_cuda:
+        raise ValueError("x has to be a float32, bfloat16 or float16 tensor on a HIP device, got %s on %s" % (x.dtype, x.device))
+    if kernel.dtype != x.dtype or kernel.device != x.device:
+        raise ValueError("kernel is %s on %s, x is %s on %s" % (kernel.dtype, kernel.device, x.dtype, x.device))
+    R, (D, V) = x.shape[0], kernel.shape
+    if bias is not None and (tuple(bias.shape) != (V,) or bias.dtype != x.dtype or bias.device != x.device or not bias.is_contiguous()):
+        raise ValueError("bias has to be a contiguous %s tensor of %d values on %s" % (x.dtype, V, x.device))
+    if tuple(labels.shape) != (R,) or labels.dtype not in (torch.int32, torch.int64) or labels.device != x.device or not labels.is_contiguous():
+        raise ValueError("labels have to be a contiguous int32 or int64 tensor of %d values on %s" % (R, x.device))
+    if R > 1 << 24 or V > 1 << 24 or D > 1 << 16:
+        raise ValueError("%d rows, %d wide, over %d classes: at most 2^24, 2^16 and 2^24 are taken" % (R, D, V))
+    x = x if x.stride(1) == 1 and x.stride(0) >= D or R == 0 else x.clone(memory_format=torch.contiguous_format)
+    kernel = kernel if kernel.stride(1) == 1 and kernel.stride(0) >= V else kernel.clone(memory_format=torch.contiguous_format)
+    return x, kernel, bias
+
+
+def _vocab_launch(direction, a, x):
+    name = "sar_vocab_ce_%s_%s" % (direction, _SFX[x.dtype])
+    n = _lib.lib().fn[name + "_workspace_bytes"](ctypes.byref(a))
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)                  # (torch's blocks are 512-byte aligned)
+    a.ws, a.ws_bytes = ws.data_ptr(), n
+    _launch(name, x.device, ctypes.byref(a))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rowstride(t, width):
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+
+
+def vocab_crossentropy(x, kernel, labels, bias=None, return_lse=False, loss=None, lse=None):
+    """-log softmax(x @ kernel + bias)[label] of every row, without keeping the logits.
+
+    x (R, D) hidden rows, kernel (D, V) in the Dense layout, bias (V) or None: all fp32, bf16 or fp16; labels (R) int32 or int64, a label outside
+    [0, V) leaves its row out (loss 0).  -> loss (R) fp32, and with return_lse the rows' log-sum-exp (R) fp32 that vocab_crossentropy_grad needs."""
+    x, kernel, bias = _vocab_args(x, kernel, labels, bias)
+    R, (D, V) = x.shape[0], kernel.shape
+    loss = _result("loss", loss, (R,), torch.float32, x.device)
+    if return_lse or lse is not None:
+        lse = _result("lse", lse, (R,), torch.float32, x.device)
+    if R:
+        _vocab_launch("fwd", _VocabCe(x.data_ptr(), kernel.data_ptr(), _ptr(bias), labels.data_ptr(), None, loss.data_ptr(), _ptr(lse), None, None, None, None, 0,
+                                      _rowstride(x, D), _rowstride(kernel, V), R, D, V, labels.element_size(), 0, 0), x)
+    return (loss, lse) if return_lse else loss
+
+
+def vocab_crossentropy_grad(dloss, x, kernel, labels, lse, bias=None, dx=None, dkernel=None, dbias=None, accumulate=False, need_dx=True):
+    """Gradients of vocab_crossentropy: dloss (R) fp32 -> (dx, dkernel, dbias | None) of the inputs' type, each element rounded once from an fp32
+    sum.  accumulate (fp32 only): add to the `dkernel`, `dbias` given, as parameter gradients of this package are.  need_dx=False: dx is None.
+    No atomics: the same inputs give the same bits."""
+    x, kernel, bias = _vocab_args(x, kernel, labels, bias)
+    R, (D, V) = x.shape[0], kernel.shape
+    if accumulate and (x.dtype != torch.float32 or dkernel is None or (bias is not None and dbias is None)):
+        raise ValueError("accumulate needs fp32 and the buffers to add to")
+    dloss, lse = _result("dloss", dloss, (R,), torch.float32, x.device), _result("lse", lse, (R,), torch.float32, x.device)
+    dx = _result("dx", dx, (R, D), x.dtype, x.device) if need_dx else None
+    dkernel = _result("dkernel", dkernel, (D, V), x.dtype, x.device)
+    dbias = None if bias is None else _result("dbias", dbias, (V,), x.dtype, x.device)
+    if R:
+        _vocab_launch("bwd", _VocabCe(x.data_ptr(), kernel.data_ptr(), _ptr(bias), labels.data_ptr(), dloss.data_ptr(), None, lse.data_ptr(), _ptr(dx), dkernel.data_ptr(), _ptr(dbias), None, 0,
+                                      _rowstride(x, D), _rowstride(kernel, V), R, D, V, labels.element_size(), 1 if accumulate else 0, 0), x)
+    elif not accumulate:
+        dkernel.zero_()
+        if dbias is not None:
+            dbias.zero_()
+    return dx, dkernel, dbias
+
+
+class VocabCrossentropy:
+    """Softmax layer + cross entropy of a label-synchronous branch as one object with explicit backward: what Dense(..., "softmax") followed by
+    CategoricalCrossentropy computes, for the weights of a Dense layer (bias or none) and integer labels."""
+
+    def __init__(self, bufs, key, dense):
+        self.bufs, self.key, self.dense = bufs, key, dense
+
+    def forward(self, x, labels):
+        R = x.numel() // self.dense.in_dim
+        self.x, self.labels = x.view(R, self.dense.in_dim), labels
+        self.bias = None if self.dense.bias is None else self.dense.bias.w
+        self.loss, self.lse = self.bufs.get(self.key + "/loss", (R,)), self.bufs.get(self.key + "/lse", (R,))
+        vocab_crossentropy(self.x, self.dense.kernel.w, labels, self.bias, True, self.loss, self.lse)
+        return self.loss
+
+    def backward(self, dloss, need_dx=True):
+        """-> dx; the layer's kernel and bias gradients are accumulated."""
+        dx = self.bufs.get(self.key + "/dx", tuple(self.x.shape)) if need_dx else None
+        vocab_crossentropy_grad(dloss, self.x, self.dense.kernel.w, self.labels, self.lse, self.bias, dx, self.dense.kernel.g,
+                                None if self.bias is None else self.dense.bias.g, accumulate=True, need_dx=need_dx)
+        return dx

@@ -633,6 +633,37 @@ int sar_kv8_attend_f32(const sarXattn* a, const void* k8, const float* k_scale, 
 int sar_kv8_attend_bf16(const sarXattn* a, const void* k8, const float* k_scale, const void* v8, const float* v_scale, long frames, sarStream_t stream);
 int sar_kv8_attend_f16(const sarXattn* a, const void* k8, const float* k_scale, const void* v8, const float* v_scale, long frames, sarStream_t stream);
 
+/* ---- Softmax cross entropy over a vocabulary, straight from the hidden rows and the output Dense kernel (the form of model.py:119's softmax
+ * layer followed by a cross entropy, for label-synchronous branches), in pieces of the vocabulary and without an (R, V) array of logits.
+ * Suffix = type of x, kernel, bias and their gradients: f32 | bf16 | f16.
+ *   z = x W + b;  lse_r = log sum_v exp z_rv;  loss_r = lse_r - z_{r, label_r};  dz = dloss_r (softmax(z) - onehot);  dx = dz W^T, dkernel = x^T dz, dbias = sum_r dz
+ * x (R, D) with row stride ldx, kernel (D, V) with row stride ldk (elements; the Keras Dense layout), bias (V) or NULL, labels (R) of
+ * label_bytes 4 or 8; a label outside [0, V) leaves its row out: loss 0, no gradient.  loss, lse, dloss (R) fp32 (forward: either may be NULL; backward:
+ * lse of the forward).  dx (R, D), dkernel (D, V), dbias (V) contiguous, each may be NULL; accumulate (f32 only): dkernel and dbias are added to.
+ * ws: the matching _workspace_bytes of the same struct, 256-byte aligned; nothing in it has to be initialised, nothing is kept there. */
+typedef struct {
+    const void *x, *kernel, *bias, *labels;
+    const float* dloss;
+    float *loss, *lse;
+    void *dx, *dkernel, *dbias;
+    void* ws;
+    long ws_bytes;
+    long ldx, ldk;
+    int R, D, V, label_bytes, accumulate, pad_;
+} sarVocabCe;
+size_t sar_vocab_ce_fwd_f32_workspace_bytes(const sarVocabCe* a);
+int sar_vocab_ce_fwd_f32(const sarVocabCe* a, sarStream_t stream);
+size_t sar_vocab_ce_fwd_bf16_workspace_bytes(const sarVocabCe* a);
+int sar_vocab_ce_fwd_bf16(const sarVocabCe* a, sarStream_t stream);
+size_t sar_vocab_ce_fwd_f16_workspace_bytes(const sarVocabCe* a);
+int sar_vocab_ce_fwd_f16(const sarVocabCe* a, sarStream_t stream);
+size_t sar_vocab_ce_bwd_f32_workspace_bytes(const sarVocabCe* a);
+int sar_vocab_ce_bwd_f32(const sarVocabCe* a, sarStream_t stream);
+size_t sar_vocab_ce_bwd_bf16_workspace_bytes(const sarVocabCe* a);
+int sar_vocab_ce_bwd_bf16(const sarVocabCe* a, sarStream_t stream);
+size_t sar_vocab_ce_bwd_f16_workspace_bytes(const sarVocabCe* a);
+int sar_vocab_ce_bwd_f16(const sarVocabCe* a, sarStream_t stream);
+
 /* ---- data feeder: utils.py:35-36 feat_norm (sklearn MinMaxScaler.fit_transform per utterance: every
  * feature column scaled to [0,1] over ALL frames of the utterance; constant column -> 0) + utils.py:39-46 feat_reshape
  * (truncate / zero-pad to T frames).  frames = the batch's utterances back to back (sum_n, D) f32; offsets (B+1) i32 frame
