@@ -130,11 +130,49 @@ __device__ __forceinline__ void halves(float v, float& lo, float& hi) {
 __device__ __forceinline__ float half_max(float v) { float a, b; halves(v, a, b); return fmaxf(a, b); }
 __device__ __forceinline__ float half_sum(float v) { float a, b; halves(v, a, b); return a + b; }
 
+// ---- tiles straight from memory into LDS.  A buffer descriptor over the rows that exist makes the hardware deliver zeros for all others (no
+// branches, no clamps, and a row behind a length can hold anything); the lanes' 16-byte pieces land in LDS in lane order, so the swizzle is
+// applied to WHICH piece a lane fetches.
+__device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
+__device__ __forceinline__ u32x4 descriptor(const void* base, unsigned bytes) {
+    const uintptr_t b = (uintptr_t)base;
+    return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)b), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(b >> 32)) & 0xffffu,
+                 (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00027000u};
+}
+// (m0 is put back: the compiler does not know that the statement uses it.  The loads are waited for with tile_barrier().)
+__device__ __forceinline__ void dma16(u32x4 rsrc, unsigned offset, unsigned lds) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(lds), "v"(offset), "s"(rsrc) : "memory");
+}
+// this wave's tile loads have arrived, its LDS reads are done, and so are every other wave's of the block
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// ROWS rows of `bytes` useful bytes each, `stride` bytes apart, by the block's four waves
+template <int PITCH, int ROWS> struct TileLoader {
+    static constexpr int CPR = PITCH / 16, ALL = ROWS * PITCH / 1024, N = (ALL + 3) / 4;
+    unsigned first, step;
+    __device__ __forceinline__ TileLoader(unsigned stride, unsigned bytes) {
+        const int slot = threadIdx.x, row = slot / CPR, pos = slot % CPR;
+        const unsigned ch = (unsigned)((chunk_at<PITCH>(row, pos) - row * PITCH) >> 4);      // (an involution: the piece that belongs at `pos`)
+        first = ch * 16 < bytes ? row * stride + ch * 16 : 0x80000000u;                        // behind the row: out of any range
+        step = 256 / CPR * stride;
+    }
+    // `rows` (>= 1) of the tile's rows exist
+    __device__ __forceinline__ void load(const void* base, int rows, unsigned stride, unsigned bytes, char* tile, int wave) const {
+        const u32x4 rsrc = descriptor(base, (unsigned)(min(rows, ROWS) - 1) * stride + bytes);
+        const unsigned dst = lds_addr(tile);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (ALL % 4 == 0 || 4 * i + wave < ALL) dma16(rsrc, first + i * step, dst + (4 * i + wave) * 1024);
+    }
+};
+
 // blockIdx -> work item such that consecutive items (which share keys and values) land on ONE of the eight XCDs, whose L2 then holds them;
 // the grid is rounded up to a multiple of 8, surplus blocks get -1
-__device__ __forceinline__ long xcd_item(long n) {
-    const long per = (n + 7) >> 3, i = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    return (long)(blockIdx.x >> 3) < per && i < n ? i : -1;
+__device__ __forceinline__ int xcd_item(int n) {
+    const int per = (n + 7) >> 3, at = blockIdx.x >> 3, i = (int)(blockIdx.x & 7) * per + at;
+    return at < per && i < n ? i : -1;
 }
 static inline long xcd_grid(long n) { return ((n + 7) >> 3) << 3; }
 

@@ -4,7 +4,7 @@
 //   z = x W + b    lse_r = log sum_v exp z_rv    loss_r = lse_r - z_{r, label}    (0 for a label outside [0, V))
 //   dz_rv = g_r (exp(z_rv - lse_r) - [v = label_r])    dx = dz W^T    dW = x^T dz    db = sum_r dz
 //
-// Forward: one product whose epilogue keeps the maximum and the sum of every 256 (128) vocabulary entries of a row; a small kernel joins them.
+// Forward: one product whose epilogue keeps the maximum and the sum of every 64 vocabulary entries of a row; a small kernel joins them.
 // Backward, in pieces of the vocabulary: the piece's logits are computed again, turned into dz in the epilogue and written once in the
 // operand type; two more products read that piece (it stays in the last-level cache) for dx and dW.
 //
@@ -171,9 +171,9 @@ __device__ __forceinline__ long label_of(const Epi& e, int r) {
 template <int MT, int NT, bool ADOWN, bool BDOWN, int EPI> __global__ __launch_bounds__(256) void product_kernel(Side A, Side B, Epi e, int mtiles, int ntiles, int ksteps, int slices) {
     constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * 2, SB = BN * BK * 2;
     __shared__ __attribute__((aligned(16))) char lds[2][SA + SB];
-    const long item = attn::xcd_item((long)mtiles * ntiles * slices);
+    const int item = attn::xcd_item(mtiles * ntiles * slices);
     if (item < 0) return;
-    const int nt = (int)(item % ntiles), mt = (int)(item / ntiles % mtiles), sl = (int)(item / ntiles / mtiles);
+    const int nt = item % ntiles, mt = item / ntiles % mtiles, sl = item / ntiles / mtiles;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w >> 1, wn = w & 1, h = lane >> 5;
     const int m0 = mt * BM, n0 = nt * BN;
     const int per = (ksteps + slices - 1) / slices, k_lo = min(sl * per, ksteps), k_hi = min(k_lo + per, ksteps), steps = (k_hi - k_lo) * PAIRS;
@@ -382,7 +382,8 @@ static int cut(long tiles, int ksteps) {                          // slices of a
 }
 
 static bool bad(const sarVocabCe* a) {
-    return !a || a->R < 1 || a->D < 1 || a->V < 1 || a->R > (1 << 24) || a->D > (1 << 16) || a->V > (1 << 24) || (a->label_bytes != 4 && a->label_bytes != 8) || a->ldx < a->D || a->ldk < a->V;
+    return !a || a->R < 1 || a->D < 1 || a->V < 1 || a->R > (1 << 24) || a->D > (1 << 16) || a->V > (1 << 24) || (a->label_bytes != 4 && a->label_bytes != 8) || a->ldx < a->D || a->ldk < a->V ||
+           (a->R + 127L) / 128 * ((a->V + 127L) / 128) > (1L << 28);
 }
 static Plan plan(const sarVocabCe* a, bool grad) {
     Plan p = {};
@@ -395,7 +396,7 @@ static Plan plan(const sarVocabCe* a, bool grad) {
     p.parts = take(3 * PARTS * 4);
     if (p.pack_x) p.xo = take((size_t)a->R * p.Dp * 2 * NPL);
     if (p.pack_w) p.wo = take((size_t)a->D * p.Vp * 2 * NPL);
-    p.lse_slices = 2 * cdiv(a->V, 256);
+    p.lse_slices = 2 * cdiv(a->V, 128);
     if (!grad) {
         p.a = take((size_t)p.lse_slices * p.Rp * 4); p.b = take((size_t)p.lse_slices * p.Rp * 4);
         p.zl = take((size_t)p.Rp * 4);
@@ -468,7 +469,7 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = a->labels; e.label_bytes = a->label_bytes;
     e.pm = reinterpret_cast<float*>(ws + p.a); e.pl = reinterpret_cast<float*>(ws + p.b); e.zl = reinterpret_cast<float*>(ws + p.zl);
     e.R = a->R; e.V = a->V; e.Rp = p.Rp;
-    product<4, 2, true, false, E_LSE>(w, x, e, a->V, a->R, p.Dp / BK, 1, st);
+    product<2, 2, true, false, E_LSE>(w, x, e, a->V, a->R, p.Dp / BK, 1, st);
     hipLaunchKernelGGL(finish_kernel, dim3((unsigned)cdiv(a->R, 32)), dim3(256), 0, st, e.pm, e.pl, e.zl, a->labels, a->label_bytes, a->loss, a->lse, a->R, p.Rp, a->V, p.lse_slices);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
@@ -495,7 +496,7 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         Side ws_ = w, xs = x;
         ws_.p += v0; ws_.len = (p.pack_w ? p.Vp : a->V) - v0; ws_.k = a->D;
         xs.len = a->R; xs.k = p.Dp;
-        product<4, 2, true, false, E_DZ>(ws_, xs, e, ld, p.Rp, p.Dp / BK, 1, st);
+        product<2, 2, true, false, E_DZ>(ws_, xs, e, ld, p.Rp, p.Dp / BK, 1, st);
         if (a->dx) {
             Epi o = e;
             o.R = a->R; o.V = a->D; o.operands = 1; o.ldo = a->D;

@@ -1,6 +1,7 @@
 // Arguments and row folding shared by the cross-attention kernels (xattn.hip, xattn_step.hip).
 #pragma once
 #include "attn_tiles.h"
+#include <initializer_list>
 
 // include/sarnet.h: sarXattn (kept field for field)
 struct sarXattn {
@@ -46,7 +47,13 @@ static inline bool bad_shape(const sarXattn* a) {
 }
 static inline bool bad_strides(int elt_bytes, const long* s, int n) {
     for (int i = 0; i < n; ++i)
-        if (s[i] < 0 || s[i] * elt_bytes % 16) return true;
+        if (s[i] < 0 || s[i] > (1L << 40) || s[i] * elt_bytes % 16) return true;
+    return false;
+}
+// a tile's rows are addressed with 32-bit offsets from its first: rows at most 16 MB apart
+static inline bool wide_rows(int elt_bytes, std::initializer_list<long> strides) {
+    for (long s : strides)
+        if (s * elt_bytes > (1L << 24)) return true;
     return false;
 }
 static inline bool few_rows(const sarXattn* a) { return (long)a->Tq * (a->Hq / a->Hkv) <= 32; }
@@ -57,7 +64,14 @@ static inline int key_splits(const sarXattn* a, int rows_per_block, int blocks) 
     if (s > keys) s = keys;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
-static inline int fwd_splits(const sarXattn* a) { return key_splits(a, 128, 512); }
+// the forward for many rows: four waves on 128 rows where those blocks fill the chip's 256 CUs twice; else two pairs of waves on 64; the key axis
+// is cut only where even those are fewer than the CUs (partial results cost their writing and reading)
+struct FwdPlan { int waves, splits; };
+static inline FwdPlan fwd_plan(const sarXattn* a) {
+    const long R = (long)a->Tq * (a->Hq / a->Hkv), bh = (long)a->B * a->Hkv;
+    if ((R + 127) / 128 * bh >= 512) return {4, 1};
+    return {2, (R + 63) / 64 * bh >= 192 ? 1 : key_splits(a, 64, 384)};
+}
 static inline int step_splits(const sarXattn* a) { return key_splits(a, 32, 1024); }
 static inline size_t part_bytes(const sarXattn* a, int splits) {
     return splits > 1 ? 4 * (size_t)part_floats((long)a->B * a->Hq * a->Tq, a->D, splits) : 0;

@@ -24,93 +24,107 @@ int SAR_FN(xattn_combine)(const sarXattn* a, int splits, hipStream_t stream);
 
 namespace attn {
 
-template <typename T> constexpr int key_tile() { return sizeof(T) == 4 ? 32 : 64; }
+// Streamed tiles: rows of the streamed side per step, two buffers.  WN waves of a block hold different columns n (32 each), WM = 4 / WN waves share
+// columns and take different 32-row parts of every step; their sums are added through LDS at the end.
+template <typename T, int WN> constexpr int step_rows() { return sizeof(T) == 4 && WN == 4 ? 32 : 64; }
+// two waves per SIMD where the accumulators and fragments leave room for it: the compiler then keeps everything in one register file
+template <typename T, int DP> constexpr int min_waves() { return sizeof(T) == 4 && DP > 64 ? 1 : 2; }
 
-// rows [first, first + ROWS) of a (T, D) operand, zero from `live` on and past D, through registers into a swizzled LDS tile
-template <typename T, int DP, int ROWS> struct Stage {
-    static constexpr int CH = DP * (int)sizeof(T) / 16, ALL = ROWS * CH, N = (ALL + 255) / 256, P = pitch<T, DP>();
-    u32x4 r[N];
-    // element offset of row `row`: a plain stride, or the folded rows of the queries
-    template <typename F> __device__ __forceinline__ void load(const T* base, F offset, int first, int live, int D) {
+template <int N> __device__ __forceinline__ void clear(f32x16 (&o)[N]) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int idx = threadIdx.x + 256 * i, row = first + idx / CH, ch = idx % CH;
-            r[i] = u32x4{0, 0, 0, 0};
-            if (row < live && ch * Num<T>::PER < D && (ALL % 256 == 0 || idx < ALL)) r[i] = *reinterpret_cast<const u32x4*>(base + offset(row) + ch * Num<T>::PER);
-        }
-    }
-    __device__ __forceinline__ void store(char* tile) const {
+    for (int d = 0; d < N; ++d)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int idx = threadIdx.x + 256 * i;
-            if (ALL % 256 == 0 || idx < ALL) *reinterpret_cast<u32x4*>(tile + chunk_at<P>(idx / CH, idx % CH)) = r[i];
-        }
-    }
-};
-
-// ---- forward: a block of four waves takes 128 rows (32 a wave, as columns n) against one slice of the keys
-template <typename T, int DP> __global__ __launch_bounds__(256) void xattn_fwd_kernel(sarXattn a, int row_tiles, int splits) {
-    constexpr int KT = key_tile<T>(), P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, NS = KT / 32;
-    __shared__ __attribute__((aligned(16))) char lk[KT * P];
-    __shared__ __attribute__((aligned(16))) char lv[KT * P];
-    const long item = xcd_item((long)a.B * a.Hkv * splits * row_tiles);
-    if (item < 0) return;
-    const int rt = (int)(item % row_tiles), sp = (int)((item / row_tiles) % splits), bh = (int)(item / row_tiles / splits);
-    const int b = bh / a.Hkv, hk = bh % a.Hkv;
-    const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
-    const int R = a.Tq * (a.Hq / a.Hkv), row0 = rt * 128 + (threadIdx.x >> 6) * 32, r = row0 + n;
-    const int rl = live_rows(a, b), len = live_keys(a, b);
-    const int per = ((len + KT - 1) / KT + splits - 1) / splits * KT;
-    const int k0 = min(sp * per, len), k1 = rt * 128 < rl ? min(k0 + per, len) : k0;
-    const Row me = row_of(a, hk, min(r, R - 1));
-    const float sl = a.scale * LOG2E;
-
-    u32x4 qf[NC];
-    load_row<T, DP>(reinterpret_cast<const T*>(a.q) + b * a.q_sb + me.t * a.q_st + me.h * a.q_sh, r < rl, a.D, h, qf);
-    const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
-    const T* vb = reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
-    const auto krow = [&](int j) { return j * a.k_st; };
-    const auto vrow = [&](int j) { return j * a.v_st; };
-
-    f32x16 o[ND];
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+}
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+// accumulators to and from LDS, one float per lane and place
+template <int N> __device__ __forceinline__ void put(float* p, const f32x16 (&o)[N], int lane) {
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[(d * 16 + i) * 64 + lane] = o[d][i];
+}
+template <int N> __device__ __forceinline__ void add(const float* p, f32x16 (&o)[N], int lane) {
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] += p[(d * 16 + i) * 64 + lane];
+}
+// a wave's column of D values: lane holds column n, values 32 d + 8 i + 4 h + (0..3)
+template <typename T, int ND> __device__ __forceinline__ void store_column(T* p, const f32x16 (&o)[ND], float f, bool in, int D, int h) {
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-    float m = NO_MAX, l = 0.f;
+        for (int i = 0; i < 4; ++i) {
+            const int dd = 32 * d + 8 * i + 4 * h;
+            if (dd < D) store4<T>(p + dd, in ? o[d][4 * i] * f : 0.f, in ? o[d][4 * i + 1] * f : 0.f, in ? o[d][4 * i + 2] * f : 0.f, in ? o[d][4 * i + 3] * f : 0.f);
+        }
+}
 
-    Stage<T, DP, KT> sk, sv;
-    sk.load(kb, krow, k0, k1, a.D); sv.load(vb, vrow, k0, k1, a.D);
-    for (int j = k0; j < k1; j += KT) {
-        __syncthreads();
-        sk.store(lk); sv.store(lv);
-        __syncthreads();
-        if (j + KT < k1) { sk.load(kb, krow, j + KT, k1, a.D); sv.load(vb, vrow, j + KT, k1, a.D); }
-        if (row0 >= rl) continue;
+// ---- forward: a block takes 32 WN rows (as columns n) against one slice of the keys
+template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_fwd_kernel(sarXattn a, int row_tiles, int splits) {
+    constexpr int KT = step_rows<T, WN>(), P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, WM = 4 / WN, NS = KT / 32 / WM, TILE = KT * P;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];                // K, V; two of each
+    const int item = xcd_item(a.B * a.Hkv * splits * row_tiles);
+    if (item < 0) return;
+    const int rt = item % row_tiles, sp = item / row_tiles % splits, bh = item / row_tiles / splits;
+    const int b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31, wn = w % WN, wm = w / WN;
+    const int R = a.Tq * (a.Hq / a.Hkv), row0 = (rt * WN + wn) * 32, r = row0 + n;
+    const int rl = live_rows(a, b), len = live_keys(a, b);
+    const int per = ((len + KT - 1) / KT + splits - 1) / splits * KT;
+    const int k0 = min(sp * per, len), k1 = rt * 32 * WN < rl ? min(k0 + per, len) : k0;
+    const Row me = row_of(a, hk, min(r, R - 1));
+    const float sl = a.scale * LOG2E;
+
+    const unsigned ks = (unsigned)(a.k_st * sizeof(T)), vs = (unsigned)(a.v_st * sizeof(T)), db = (unsigned)(a.D * sizeof(T));
+    const TileLoader<P, KT> tk(ks, db), tv(vs, db);
+    const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
+    const T* vb = reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
+    const auto load = [&](int j, char* to) {
+        tk.load(kb + j * a.k_st, k1 - j, ks, db, to, w);
+        tv.load(vb + j * a.v_st, k1 - j, vs, db, to + TILE, w);
+    };
+    if (k0 < k1) load(k0, lds);
+    u32x4 qf[NC];
+    load_row<T, DP>(reinterpret_cast<const T*>(a.q) + b * a.q_sb + me.t * a.q_st + me.h * a.q_sh, r < rl, a.D, h, qf);
+    f32x16 o[ND];
+    clear(o);
+    float m = NO_MAX, l = 0.f;
+    int cur = 0;
+    for (int j = k0; j < k1; j += KT, cur ^= 2 * TILE) {
+        tile_barrier();
+        if (j + KT < k1) load(j + KT, lds + (cur ^ (2 * TILE)));
+        if (row0 >= rl || (WM > 1 && j + 32 * wm >= k1)) continue;
+        const char *lk = lds + cur, *lv = lds + cur + TILE;
         f32x16 s[NS];
         float top = NO_MAX;
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
+            s[u] = zero16();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) s[u] = mma<T>(frag<P>(lk, 32 * u + n, c, h), qf[c], s[u]);
+            for (int c = 0; c < NC; ++c) s[u] = mma<T>(frag<P>(lk, 32 * (u * WM + wm) + n, c, h), qf[c], s[u]);
         }
         if (j + KT > k1) {
 #pragma unroll
             for (int u = 0; u < NS; ++u)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const bool in = j + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3) < k1;
-                    s[u][i] = in ? s[u][i] * sl : -INFINITY;
-                    top = fmaxf(top, s[u][i]);
-                }
+                for (int i = 0; i < 16; ++i) s[u][i] = j + 32 * (u * WM + wm) + 8 * (i >> 2) + 4 * h + (i & 3) < k1 ? s[u][i] * sl : -INFINITY;
         } else {
 #pragma unroll
             for (int u = 0; u < NS; ++u)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) { s[u][i] *= sl; top = fmaxf(top, s[u][i]); }
+                for (int i = 0; i < 16; ++i) s[u][i] *= sl;
         }
+#pragma unroll
+        for (int u = 0; u < NS; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
         top = half_max(top);
         // the maximum follows only where it grew by more than 2^8: below that p <= 2^8 loses nothing in any of the types, and most
         // tiles skip the rescaling
@@ -129,242 +143,269 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void xattn_fwd_k
             u32x4 p[4];
             pack<T>(s[u], p);
 #pragma unroll
-            for (int d = 0; d < ND; ++d) o[d] = mma_down<T, P>(lv, 32 * u, d, p, o[d], lane);
+            for (int d = 0; d < ND; ++d) o[d] = mma_down<T, P>(lv, 32 * (u * WM + wm), d, p, o[d], lane);
         }
+    }
+    if constexpr (WM > 1) {                                       // two waves per column: bring both to one maximum, add
+        static_assert(WM == 2, "");
+        float* join = reinterpret_cast<float*>(lds) + wn * (ND * 16 + 2) * 64;
+        static_assert(WN * (ND * 16 + 2) * 64 * 4 <= 4 * TILE, "");
+        __syncthreads();
+        if (wm) {
+            put(join, o, lane);
+            join[ND * 1024 + lane] = m; join[ND * 1024 + 64 + lane] = l;
+        }
+        __syncthreads();
+        if (wm) return;
+        const float m2 = join[ND * 1024 + lane], mn = fmaxf(m, m2), f = __builtin_amdgcn_exp2f(m - mn), g = __builtin_amdgcn_exp2f(m2 - mn);
+        l = l * f + join[ND * 1024 + 64 + lane] * g;
+        m = mn;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * f + join[(d * 16 + i) * 64 + lane] * g;
     }
     l = half_sum(l);
     if (r >= R) return;
     if (splits == 1) {
         const bool in = r < rl && l != 0.f;                       // rows behind the length, and rows without keys: zeros
-        const float inv = 1.f / l;
-        T* op = reinterpret_cast<T*>(a.out) + b * a.o_sb + me.t * a.o_st + me.h * a.o_sh;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int dd = 32 * d + 8 * i + 4 * h;
-                if (dd < a.D)
-                    store4<T>(op + dd, in ? o[d][4 * i] * inv : 0.f, in ? o[d][4 * i + 1] * inv : 0.f, in ? o[d][4 * i + 2] * inv : 0.f, in ? o[d][4 * i + 3] * inv : 0.f);
-            }
+        store_column<T, ND>(reinterpret_cast<T*>(a.out) + b * a.o_sb + me.t * a.o_st + me.h * a.o_sh, o, 1.f / l, in, a.D, h);
         if (a.lse && h == 0) a.lse[stat_at(a, b, me)] = in ? m * LN2 + logf(l) : -INFINITY;
     } else {
         const long rows = (long)a.B * a.Hq * a.Tq, at = sp * rows + stat_at(a, b, me);
-        float* op = reinterpret_cast<float*>(a.ws) + at * a.D;
+        store_column<float, ND>(reinterpret_cast<float*>(a.ws) + at * a.D, o, 1.f, true, a.D, h);
         float* ml = reinterpret_cast<float*>(a.ws) + splits * rows * a.D + at;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int dd = 32 * d + 8 * i + 4 * h;
-                if (dd < a.D) *reinterpret_cast<f32x4*>(op + dd) = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-            }
         if (h == 0) { ml[0] = m; ml[splits * rows] = l; }
     }
 }
 
-// delta_i = do_i . o_i, one wave per row
-template <typename T> __global__ __launch_bounds__(256) void xattn_delta_kernel(sarXattn a, float* delta) {
-    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= (long)a.B * a.Hq * a.Tq) return;
-    const int t = (int)(i % a.Tq), hq = (int)(i / a.Tq % a.Hq), b = (int)(i / a.Tq / a.Hq);
-    const T* o = reinterpret_cast<const T*>(a.out) + b * a.o_sb + t * a.o_st + hq * a.o_sh;
-    const T* g = reinterpret_cast<const T*>(a.dout) + b * a.g_sb + t * a.g_st + hq * a.g_sh;
-    float s = 0.f;
-    for (int d = threadIdx.x & 63; d < a.D; d += 64) s = fmaf((float)o[d], (float)g[d], s);
-    s = wave_sum(s);
-    if ((threadIdx.x & 63) == 0) delta[i] = s;
-}
-
-// ---- dK, dV: a wave holds 32 keys as columns n (their K and V fragments in registers), the rows stream through LDS
-template <typename T, int DP> __global__ __launch_bounds__(256) void xattn_dkv_kernel(sarXattn a, const float* __restrict__ delta, int key_tiles) {
-    constexpr int RT = 32, P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32;
-    __shared__ __attribute__((aligned(16))) char lq[RT * P];
-    __shared__ __attribute__((aligned(16))) char lg[RT * P];
-    __shared__ __attribute__((aligned(16))) float ls[2][RT];      // lse (in powers of two) and delta of the tile's rows
-    const long item = xcd_item((long)a.B * a.Hkv * key_tiles);
+// ---- dQ (and delta): as the forward, a wave holds 32 rows as columns n, the keys and values stream through LDS.  It also leaves {lse log2 e,
+// delta} of every row in `stats` (B, Hq, Tq, 2) for the dK, dV kernel.
+template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dq_kernel(sarXattn a, float2* __restrict__ stats, int row_tiles) {
+    constexpr int KT = step_rows<T, WN>(), P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, WM = 4 / WN, NS = KT / 32 / WM, TILE = KT * P;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
+    const int item = xcd_item(a.B * a.Hkv * row_tiles);
     if (item < 0) return;
-    const int kt = (int)(item % key_tiles), bh = (int)(item / key_tiles), b = bh / a.Hkv, hk = bh % a.Hkv;
-    const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
-    const int len = live_keys(a, b), key0 = kt * 128 + (threadIdx.x >> 6) * 32, key = key0 + n;
-    const int rl = kt * 128 < len ? live_rows(a, b) : 0;
-    const float sl = a.scale * LOG2E;
-    u32x4 kf[NC], vf[NC];
-    load_row<T, DP>(reinterpret_cast<const T*>(a.k) + b * a.k_sb + min(key, a.Tk - 1) * a.k_st + hk * a.k_sh, key < len, a.D, h, kf);
-    load_row<T, DP>(reinterpret_cast<const T*>(a.v) + b * a.v_sb + min(key, a.Tk - 1) * a.v_st + hk * a.v_sh, key < len, a.D, h, vf);
-    const T* qb = reinterpret_cast<const T*>(a.q) + b * a.q_sb;
-    const T* gb = reinterpret_cast<const T*>(a.dout) + b * a.g_sb;
-    const auto qrow = [&](int r) { const Row w = row_of(a, hk, r); return w.t * a.q_st + w.h * a.q_sh; };
-    const auto grow = [&](int r) { const Row w = row_of(a, hk, r); return w.t * a.g_st + w.h * a.g_sh; };
-    f32x16 dk[ND], dv[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) { dk[d][i] = 0.f; dv[d][i] = 0.f; }
-    Stage<T, DP, RT> sq, sg;
-    float st = 0.f;
-    const auto load_stats = [&](int r0) {
-        if (threadIdx.x < 2 * RT) {
-            const int r = r0 + (threadIdx.x & (RT - 1));
-            st = threadIdx.x < RT ? INFINITY : 0.f;               // a row that does not exist: p = exp2(s - inf) = 0
-            if (r < rl) {
-                const long at = stat_at(a, b, row_of(a, hk, r));
-                const float v = threadIdx.x < RT ? a.lse[at] * LOG2E : delta[at];
-                st = threadIdx.x < RT && v == -INFINITY ? INFINITY : v;
-            }
-        }
-    };
-    sq.load(qb, qrow, 0, rl, a.D); sg.load(gb, grow, 0, rl, a.D); load_stats(0);
-    for (int r0 = 0; r0 < rl; r0 += RT) {
-        __syncthreads();
-        sq.store(lq); sg.store(lg);
-        if (threadIdx.x < 2 * RT) ls[threadIdx.x / RT][threadIdx.x & (RT - 1)] = st;
-        __syncthreads();
-        if (r0 + RT < rl) { sq.load(qb, qrow, r0 + RT, rl, a.D); sg.load(gb, grow, r0 + RT, rl, a.D); load_stats(r0 + RT); }
-        if (key0 >= len) continue;
-        f32x16 s, dp;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) s = mma<T>(frag<P>(lq, n, c, h), kf[c], s);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) dp = mma<T>(frag<P>(lg, n, c, h), vf[c], dp);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const f32x4 e = *reinterpret_cast<const f32x4*>(&ls[0][8 * x + 4 * h]), dl = *reinterpret_cast<const f32x4*>(&ls[1][8 * x + 4 * h]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * x + c], sl, -e[c]));
-                s[4 * x + c] = p;
-                dp[4 * x + c] = p * (dp[4 * x + c] - dl[c]);
-            }
-        }
-        u32x4 pf[4], df[4];
-        pack<T>(s, pf); pack<T>(dp, df);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            dv[d] = mma_down<T, P>(lg, 0, d, pf, dv[d], lane);
-            dk[d] = mma_down<T, P>(lq, 0, d, df, dk[d], lane);
-        }
-    }
-    if (key >= a.Tk) return;
-    const bool in = key < len;                                    // frames behind the length: their gradient is zero
-    T* kp = reinterpret_cast<T*>(a.dk) + (((long)b * a.Tk + key) * a.Hkv + hk) * a.D;
-    T* vp = reinterpret_cast<T*>(a.dv) + (((long)b * a.Tk + key) * a.Hkv + hk) * a.D;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int dd = 32 * d + 8 * i + 4 * h;
-            if (dd >= a.D) continue;
-            const float f = a.scale;
-            store4<T>(kp + dd, in ? dk[d][4 * i] * f : 0.f, in ? dk[d][4 * i + 1] * f : 0.f, in ? dk[d][4 * i + 2] * f : 0.f, in ? dk[d][4 * i + 3] * f : 0.f);
-            store4<T>(vp + dd, in ? dv[d][4 * i] : 0.f, in ? dv[d][4 * i + 1] : 0.f, in ? dv[d][4 * i + 2] : 0.f, in ? dv[d][4 * i + 3] : 0.f);
-        }
-}
-
-// ---- dQ: as the forward, a wave holds 32 rows as columns n, the keys and values stream through LDS
-template <typename T, int DP> __global__ __launch_bounds__(256) void xattn_dq_kernel(sarXattn a, const float* __restrict__ delta, int row_tiles) {
-    constexpr int KT = 32, P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32;
-    __shared__ __attribute__((aligned(16))) char lk[KT * P];
-    __shared__ __attribute__((aligned(16))) char lv[KT * P];
-    const long item = xcd_item((long)a.B * a.Hkv * row_tiles);
-    if (item < 0) return;
-    const int rt = (int)(item % row_tiles), bh = (int)(item / row_tiles), b = bh / a.Hkv, hk = bh % a.Hkv;
-    const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
-    const int R = a.Tq * (a.Hq / a.Hkv), row0 = rt * 128 + (threadIdx.x >> 6) * 32, r = row0 + n;
-    const int rl = live_rows(a, b), len = rt * 128 < rl ? live_keys(a, b) : 0;
+    const int rt = item % row_tiles, bh = item / row_tiles, b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31, wn = w % WN, wm = w / WN;
+    const int R = a.Tq * (a.Hq / a.Hkv), row0 = (rt * WN + wn) * 32, r = row0 + n;
+    const int rl = live_rows(a, b), len = rt * 32 * WN < rl ? live_keys(a, b) : 0;
     const Row me = row_of(a, hk, min(r, R - 1));
     const float sl = a.scale * LOG2E;
-    u32x4 qf[NC], gf[NC];
-    load_row<T, DP>(reinterpret_cast<const T*>(a.q) + b * a.q_sb + me.t * a.q_st + me.h * a.q_sh, r < rl, a.D, h, qf);
-    load_row<T, DP>(reinterpret_cast<const T*>(a.dout) + b * a.g_sb + me.t * a.g_st + me.h * a.g_sh, r < rl, a.D, h, gf);
-    float e = r < rl ? a.lse[stat_at(a, b, me)] * LOG2E : INFINITY;
-    if (e == -INFINITY) e = INFINITY;
-    const float dl = r < rl ? delta[stat_at(a, b, me)] : 0.f;
+    const unsigned ks = (unsigned)(a.k_st * sizeof(T)), vs = (unsigned)(a.v_st * sizeof(T)), db = (unsigned)(a.D * sizeof(T));
+    const TileLoader<P, KT> tk(ks, db), tv(vs, db);
     const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
     const T* vb = reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
-    const auto krow = [&](int j) { return j * a.k_st; };
-    const auto vrow = [&](int j) { return j * a.v_st; };
-    f32x16 dq[ND];
+    const auto load = [&](int j, char* to) {
+        tk.load(kb + j * a.k_st, len - j, ks, db, to, w);
+        tv.load(vb + j * a.v_st, len - j, vs, db, to + TILE, w);
+    };
+    if (0 < len) load(0, lds);
+    u32x4 qf[NC], gf[NC];
+    float e = 0.f, dl = 0.f;
+    {
+        u32x4 of[NC];
+        load_row<T, DP>(reinterpret_cast<const T*>(a.q) + b * a.q_sb + me.t * a.q_st + me.h * a.q_sh, r < rl, a.D, h, qf);
+        load_row<T, DP>(reinterpret_cast<const T*>(a.dout) + b * a.g_sb + me.t * a.g_st + me.h * a.g_sh, r < rl, a.D, h, gf);
+        load_row<T, DP>(reinterpret_cast<const T*>(a.out) + b * a.o_sb + me.t * a.o_st + me.h * a.o_sh, r < rl, a.D, h, of);
+        if (r < rl) e = a.lse[stat_at(a, b, me)] * LOG2E;
+        if (e == -INFINITY) e = 0.f;                              // a row without keys meets no key
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
-    Stage<T, DP, KT> sk, sv;
-    sk.load(kb, krow, 0, len, a.D); sv.load(vb, vrow, 0, len, a.D);
-    for (int j = 0; j < len; j += KT) {
-        __syncthreads();
-        sk.store(lk); sv.store(lv);
-        __syncthreads();
-        if (j + KT < len) { sk.load(kb, krow, j + KT, len, a.D); sv.load(vb, vrow, j + KT, len, a.D); }
-        if (row0 >= rl) continue;
-        f32x16 s, dp;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) s = mma<T>(frag<P>(lk, n, c, h), qf[c], s);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) dp = mma<T>(frag<P>(lv, n, c, h), gf[c], dp);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const bool in = j + 8 * (i >> 2) + 4 * h + (i & 3) < len;
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], sl, -e));
-            dp[i] = in ? p * (dp[i] - dl) : 0.f;
-        }
-        u32x4 df[4];
-        pack<T>(dp, df);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) dq[d] = mma_down<T, P>(lk, 0, d, df, dq[d], lane);
+            for (int i = 0; i < Num<T>::PER; ++i) dl = fmaf((float)as16<T>(gf[c])[i], (float)as16<T>(of[c])[i], dl);
+        dl = half_sum(dl);
+        if (wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
     }
-    if (r >= R) return;
-    T* op = reinterpret_cast<T*>(a.dq) + (((long)b * a.Tq + me.t) * a.Hq + me.h) * a.D;
-    const bool in = r < rl;
-    const float f = a.scale;
+    f32x16 dq[ND];
+    clear(dq);
+    int cur = 0;
+    for (int j = 0; j < len; j += KT, cur ^= 2 * TILE) {
+        tile_barrier();
+        if (j + KT < len) load(j + KT, lds + (cur ^ (2 * TILE)));
+        if (row0 >= rl || (WM > 1 && j + 32 * wm >= len)) continue;
+        const char *lk = lds + cur, *lv = lds + cur + TILE;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+        for (int u = 0; u < NS; ++u) {
+            const int at = 32 * (u * WM + wm);
+            f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int dd = 32 * d + 8 * i + 4 * h;
-            if (dd < a.D)
-                store4<T>(op + dd, in ? dq[d][4 * i] * f : 0.f, in ? dq[d][4 * i + 1] * f : 0.f, in ? dq[d][4 * i + 2] * f : 0.f, in ? dq[d][4 * i + 3] * f : 0.f);
+            for (int c = 0; c < NC; ++c) s = mma<T>(frag<P>(lk, at + n, c, h), qf[c], s);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) dp = mma<T>(frag<P>(lv, at + n, c, h), gf[c], dp);
+            if (j + KT > len) {                                   // (a key behind the length is a zero row: its p is no number to be trusted)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = j + at + 8 * (i >> 2) + 4 * h + (i & 3) < len ? fmaf(s[i], sl, -e) : -INFINITY;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], sl, -e);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] = __builtin_amdgcn_exp2f(s[i]) * (dp[i] - dl);
+            u32x4 df[4];
+            pack<T>(dp, df);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) dq[d] = mma_down<T, P>(lk, at, d, df, dq[d], lane);
         }
+    }
+    if constexpr (WM > 1) {
+        static_assert(WM == 2, "");
+        float* join = reinterpret_cast<float*>(lds) + wn * ND * 1024;
+        static_assert(WN * ND * 1024 * 4 <= 4 * TILE, "");
+        __syncthreads();
+        if (wm) put(join, dq, lane);
+        __syncthreads();
+        if (wm) return;
+        add(join, dq, lane);
+    }
+    if (r < R) store_column<T, ND>(reinterpret_cast<T*>(a.dq) + (((long)b * a.Tq + me.t) * a.Hq + me.h) * a.D, dq, a.scale, r < rl, a.D, h);
+}
+
+// ---- dK, dV: a wave holds 32 keys as columns n; the rows of one query head after the other stream through LDS
+template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dkv_kernel(sarXattn a, const float2* __restrict__ stats, int key_tiles) {
+    constexpr int WM = 4 / WN, RT = 32 * WM, P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, TILE = RT * P, BUF = 2 * TILE;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * BUF];                 // Q, dO; two of each
+    __shared__ __attribute__((aligned(16))) float2 row_stats[2][RT];
+    // 128 wide, both fragments and both sums do not fit 256 registers: the K fragments stay in the wave's own piece of LDS, in lane order
+    constexpr bool KL = sizeof(T) == 2 && DP == 128;
+    __shared__ __attribute__((aligned(16))) u32x4 k_frags[KL ? 4 : 1][KL ? NC : 1][KL ? 64 : 1];
+    const int item = xcd_item(a.B * a.Hkv * key_tiles);
+    if (item < 0) return;
+    const int kt = item % key_tiles, bh = item / key_tiles, b = bh / a.Hkv, hk = bh % a.Hkv, G = a.Hq / a.Hkv;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31, wn = w % WN, wm = w / WN;
+    const int len = live_keys(a, b), key0 = (kt * WN + wn) * 32, key = key0 + n;
+    const int tl = kt * 32 * WN < len ? live_rows(a, b) / G : 0;                 // tokens
+    const float sl = a.scale * LOG2E;
+    const unsigned qs = (unsigned)(a.q_st * sizeof(T)), gs = (unsigned)(a.g_st * sizeof(T)), db = (unsigned)(a.D * sizeof(T));
+    const TileLoader<P, RT> tq(qs, db), tg(gs, db);
+    const T* qb = reinterpret_cast<const T*>(a.q) + b * a.q_sb + (long)hk * G * a.q_sh;
+    const T* gb = reinterpret_cast<const T*>(a.dout) + b * a.g_sb + (long)hk * G * a.g_sh;
+    const float2* sb = stats + ((long)b * a.Hq + hk * G) * a.Tq;
+    const auto load = [&](int g, int t, char* to) {
+        tq.load(qb + g * a.q_sh + t * a.q_st, tl - t, qs, db, to, w);
+        tg.load(gb + g * a.g_sh + t * a.g_st, tl - t, gs, db, to + TILE, w);
+    };
+    // {lse log2 e, delta} of the tile's rows.  Rows behind the last one get zeros as their Q and dO do: p = exp2(0), which meets zero rows.
+    const auto load_stats = [&](int g, int t) {
+        const int i = t + (int)threadIdx.x;
+        return threadIdx.x < RT && i < tl ? sb[(long)g * a.Tq + i] : make_float2(0.f, 0.f);
+    };
+    if (tl > 0) {
+        load(0, 0, lds);
+        if (threadIdx.x < RT) row_stats[0][threadIdx.x] = load_stats(0, 0);
+    }
+    u32x4 kf[NC], vf[NC];
+    load_row<T, DP>(reinterpret_cast<const T*>(a.k) + b * a.k_sb + min(key, a.Tk - 1) * a.k_st + hk * a.k_sh, key < len, a.D, h, kf);
+    if constexpr (KL) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) k_frags[w][c][lane] = kf[c];
+    }
+    load_row<T, DP>(reinterpret_cast<const T*>(a.v) + b * a.v_sb + min(key, a.Tk - 1) * a.v_st + hk * a.v_sh, key < len, a.D, h, vf);
+    f32x16 dk[ND], dv[ND];
+    clear(dk); clear(dv);
+    int g = 0, t = 0, cur = 0, par = 0;
+    while (g < G && tl > 0) {
+        tile_barrier();
+        int gn = g, tn = t + RT;
+        if (tn >= tl) { ++gn; tn = 0; }
+        float2 next = make_float2(0.f, 0.f);
+        if (gn < G) { next = load_stats(gn, tn); load(gn, tn, lds + (cur ^ BUF)); }
+        if (key0 < len && (WM == 1 || t + 32 * wm < tl)) {
+            const char *lq = lds + cur, *lg = lds + cur + TILE;
+            const float* st = reinterpret_cast<const float*>(row_stats[par]) + wm * 64;
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s = mma<T>(frag<P>(lq, 32 * wm + n, c, h), KL ? k_frags[w][KL ? c : 0][KL ? lane : 0] : kf[c], s);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[4 * x + c] = __builtin_amdgcn_exp2f(fmaf(s[4 * x + c], sl, -st[2 * (8 * x + 4 * h + c)]));
+            u32x4 pf[4];
+            pack<T>(s, pf);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) dv[d] = mma_down<T, P>(lg, 32 * wm, d, pf, dv[d], lane);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) dp = mma<T>(frag<P>(lg, 32 * wm + n, c, h), vf[c], dp);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) dp[4 * x + c] = s[4 * x + c] * (dp[4 * x + c] - st[2 * (8 * x + 4 * h + c) + 1]);
+            pack<T>(dp, pf);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) dk[d] = mma_down<T, P>(lq, 32 * wm, d, pf, dk[d], lane);
+        }
+        g = gn; t = tn; cur ^= BUF; par ^= 1;
+        if (threadIdx.x < RT) row_stats[par][threadIdx.x] = next;
+    }
+    if constexpr (WM > 1) {
+        static_assert(WM == 2, "");
+        float* join = reinterpret_cast<float*>(lds) + wn * 2 * ND * 1024;
+        static_assert(WN * 2 * ND * 1024 * 4 <= 2 * BUF, "");
+        __syncthreads();
+        if (wm) { put(join, dk, lane); put(join + ND * 1024, dv, lane); }
+        __syncthreads();
+        if (wm) return;
+        add(join, dk, lane); add(join + ND * 1024, dv, lane);
+    }
+    if (key >= a.Tk) return;
+    const long at = (((long)b * a.Tk + key) * a.Hkv + hk) * a.D;  // frames behind the length: their gradient is zero
+    store_column<T, ND>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, key < len, a.D, h);
+    store_column<T, ND>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, key < len, a.D, h);
 }
 
 }  // namespace attn
 using namespace attn;
 
 static bool bad(const sarXattn* a) {
-    if (bad_shape(a) || bad_strides(sizeof(elt), &a->q_sb, 12)) return true;
+    if (bad_shape(a) || bad_strides(sizeof(elt), &a->q_sb, 12) || wide_rows(sizeof(elt), {a->q_st, a->k_st, a->v_st})) return true;
     for (const void* p : {a->q, a->k, a->v, (const void*)a->out})
         if (!p || (uintptr_t)p % 16) return true;
     return false;
 }
 
-template <int DP> static void launch_fwd(const sarXattn& a, int splits, hipStream_t st) {
-    const int rt = cdiv((long)a.Tq * (a.Hq / a.Hkv), 128);
-    hipLaunchKernelGGL((xattn_fwd_kernel<elt, DP>), dim3((unsigned)xcd_grid((long)rt * splits * a.B * a.Hkv)), dim3(256), 0, st, a, rt, splits);
+// fp32 heads wider than 64 have no two-waves-per-column form: its tiles would pass 64 KB of LDS
+template <int DP> constexpr bool paired() { return sizeof(elt) == 2 || DP <= 64; }
+template <int DP> static void launch_fwd(const sarXattn& a, hipStream_t st) {
+    const FwdPlan p = fwd_plan(&a);
+    const bool two = paired<DP>() && p.waves == 2;
+    const int rt = cdiv((long)a.Tq * (a.Hq / a.Hkv), two ? 64 : 128);
+    const dim3 grid((unsigned)xcd_grid((long)rt * p.splits * a.B * a.Hkv));
+    if constexpr (paired<DP>()) {
+        if (two) hipLaunchKernelGGL((xattn_fwd_kernel<elt, DP, 2>), grid, dim3(256), 0, st, a, rt, p.splits);
+    }
+    if (!two) hipLaunchKernelGGL((xattn_fwd_kernel<elt, DP, 4>), grid, dim3(256), 0, st, a, rt, p.splits);
 }
-template <int DP> static void launch_bwd(const sarXattn& a, float* delta, hipStream_t st) {
-    const int kt = cdiv(a.Tk, 128), rt = cdiv((long)a.Tq * (a.Hq / a.Hkv), 128);
-    hipLaunchKernelGGL((xattn_delta_kernel<elt>), dim3((unsigned)cdiv((long)a.B * a.Hq * a.Tq, 4)), dim3(256), 0, st, a, delta);
-    if (kt) hipLaunchKernelGGL((xattn_dkv_kernel<elt, DP>), dim3((unsigned)xcd_grid((long)kt * a.B * a.Hkv)), dim3(256), 0, st, a, delta, kt);
-    hipLaunchKernelGGL((xattn_dq_kernel<elt, DP>), dim3((unsigned)xcd_grid((long)rt * a.B * a.Hkv)), dim3(256), 0, st, a, delta, rt);
+template <int DP> static void launch_bwd(const sarXattn& a, float2* stats, hipStream_t st) {
+    const long R = (long)a.Tq * (a.Hq / a.Hkv), bh = (long)a.B * a.Hkv;
+    // four waves on 128 columns where those blocks fill the chip twice, else two pairs on 64
+    const bool few_q = paired<DP>() && cdiv(R, 128) * bh < 512, few_k = paired<DP>() && cdiv(a.Tk, 128) * bh < 512;
+    const int rt = cdiv(R, few_q ? 64 : 128), kt = cdiv(a.Tk, few_k ? 64 : 128);
+    const dim3 gq((unsigned)xcd_grid(rt * bh)), gk((unsigned)xcd_grid(kt * bh));
+    if constexpr (paired<DP>()) {
+        if (few_q) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2>), gq, dim3(256), 0, st, a, stats, rt);
+    }
+    if (!few_q) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4>), gq, dim3(256), 0, st, a, stats, rt);
+    if (!kt) return;
+    if constexpr (paired<DP>()) {
+        if (few_k) hipLaunchKernelGGL((xattn_dkv_kernel<elt, DP, 2>), gk, dim3(256), 0, st, a, stats, kt);
+    }
+    if (!few_k) hipLaunchKernelGGL((xattn_dkv_kernel<elt, DP, 4>), gk, dim3(256), 0, st, a, stats, kt);
 }
 
 #if SAR_ELT == 0      // the same for every type
-extern "C" size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, few_rows(a) ? step_splits(a) : fwd_splits(a)); }
-extern "C" size_t sar_xattn_bwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : 4 * (size_t)a->B * a->Hq * a->Tq; }
+extern "C" size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, few_rows(a) ? step_splits(a) : fwd_plan(a).splits); }
+extern "C" size_t sar_xattn_bwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : 8 * (size_t)a->B * a->Hq * a->Tq; }
 #endif
 
 extern "C" int SAR_FN(sar_xattn_fwd)(const sarXattn* a, hipStream_t stream) {
     if (bad(a)) return SAR_EINVAL;
-    if (bad_workspace(a, part_bytes(a, few_rows(a) ? step_splits(a) : fwd_splits(a)))) return SAR_EINVAL;
+    if (bad_workspace(a, part_bytes(a, few_rows(a) ? step_splits(a) : fwd_plan(a).splits))) return SAR_EINVAL;
     if (few_rows(a)) return SAR_FN(xattn_step)(a, step_splits(a), stream);
-    const int splits = fwd_splits(a);
-    if (a->D <= 32) launch_fwd<32>(*a, splits, stream);
-    else if (a->D <= 64) launch_fwd<64>(*a, splits, stream);
-    else if (a->D <= 96) launch_fwd<96>(*a, splits, stream);
-    else launch_fwd<128>(*a, splits, stream);
+    const int splits = fwd_plan(a).splits;
+    if (a->D <= 32) launch_fwd<32>(*a, stream);
+    else if (a->D <= 64) launch_fwd<64>(*a, stream);
+    else if (a->D <= 96) launch_fwd<96>(*a, stream);
+    else launch_fwd<128>(*a, stream);
     SAR_CHECK_LAUNCH();
     return splits > 1 ? SAR_FN(xattn_combine)(a, splits, stream) : SAR_OK;
 }
@@ -373,12 +414,12 @@ extern "C" int SAR_FN(sar_xattn_bwd)(const sarXattn* a, hipStream_t stream) {
     if (bad(a) || !a->lse || !a->dout || !a->dq || !a->dk || !a->dv || !a->ws) return SAR_EINVAL;
     for (const void* p : {a->dout, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
         if ((uintptr_t)p % 16) return SAR_EINVAL;
-    if (bad_strides(sizeof(elt), &a->g_sb, 3) || bad_workspace(a, 4 * (size_t)a->B * a->Hq * a->Tq)) return SAR_EINVAL;
-    float* delta = reinterpret_cast<float*>(a->ws);
-    if (a->D <= 32) launch_bwd<32>(*a, delta, stream);
-    else if (a->D <= 64) launch_bwd<64>(*a, delta, stream);
-    else if (a->D <= 96) launch_bwd<96>(*a, delta, stream);
-    else launch_bwd<128>(*a, delta, stream);
+    if (bad_strides(sizeof(elt), &a->g_sb, 3) || wide_rows(sizeof(elt), {a->g_st}) || bad_workspace(a, 8 * (size_t)a->B * a->Hq * a->Tq)) return SAR_EINVAL;
+    float2* stats = reinterpret_cast<float2*>(a->ws);
+    if (a->D <= 32) launch_bwd<32>(*a, stats, stream);
+    else if (a->D <= 64) launch_bwd<64>(*a, stats, stream);
+    else if (a->D <= 96) launch_bwd<96>(*a, stats, stream);
+    else launch_bwd<128>(*a, stats, stream);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
 }

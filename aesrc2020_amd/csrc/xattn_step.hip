@@ -76,9 +76,9 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
     constexpr int NKL = S8 ? DP / 32 : NC, NVL = 32 * CHV / 64;
     extern __shared__ __attribute__((aligned(16))) char lds[];    // V tiles of the waves; afterwards their partial sums
     __shared__ float lm[NW][32], ll[NW][32];
-    const long item = xcd_item((long)a.B * a.Hkv * row_tiles * splits);
+    const int item = xcd_item(a.B * a.Hkv * row_tiles * splits);
     if (item < 0) return;
-    const int sp = (int)(item % splits), rt = (int)((item / splits) % row_tiles), bh = (int)(item / splits / row_tiles);
+    const int sp = item % splits, rt = item / splits % row_tiles, bh = item / splits / row_tiles;
     const int b = bh / a.Hkv, hk = bh % a.Hkv;
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
     const int R = a.Tq * (a.Hq / a.Hkv), r = rt * 32 + n, rl = live_rows(a, b), len = live_keys(a, b);
