@@ -165,10 +165,10 @@ def _vocab_args(x, kernel, labels, bias):
         raise ValueError("bias has to be a contiguous %s tensor of %d values on %s" % (x.dtype, V, x.device))
     if tuple(labels.shape) != (R,) or labels.dtype not in (torch.int32, torch.int64) or labels.device != x.device or not labels.is_contiguous():
         raise ValueError("labels have to be a contiguous int32 or int64 tensor of %d values on %s" % (R, x.device))
-    if R > 1 << 24 or V > 1 << 24 or D > 1 << 16:
-        raise ValueError("%d rows, %d wide, over %d classes: at most 2^24, 2^16 and 2^24 are taken" % (R, D, V))
-    x = x if x.stride(1) == 1 and x.stride(0) >= D or R == 0 else x.clone(memory_format=torch.contiguous_format)
-    kernel = kernel if kernel.stride(1) == 1 and kernel.stride(0) >= V else kernel.clone(memory_format=torch.contiguous_format)
+    if R > 1 << 22 or V > 1 << 22 or D > 1 << 16 or (R // 64 + 1) * (V // 64 + 1) > 1 << 28:
+        raise ValueError("%d rows, %d wide, over %d classes: at most 2^22, 2^16 and 2^22 are taken, and 2^40 logits" % (R, D, V))
+    x = x if x.stride(1) == 1 and D <= x.stride(0) <= 1 << 22 or R == 0 else x.clone(memory_format=torch.contiguous_format)
+    kernel = kernel if kernel.stride(1) == 1 and V <= kernel.stride(0) <= 1 << 22 else kernel.clone(memory_format=torch.contiguous_format)
     return x, kernel, bias
 
 

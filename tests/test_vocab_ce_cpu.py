@@ -16,7 +16,7 @@ def _args(**kw):
 
 @pytest.mark.parametrize("sfx", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("kw", [dict(x=None), dict(kernel=None), dict(labels=None), dict(R=0), dict(D=0), dict(V=0), dict(ldx=63), dict(ldk=999), dict(label_bytes=2), dict(ws=None),
-                                dict(ws=4100), dict(ws_bytes=100), dict(R=1 << 25), dict(V=1 << 25, ldk=1 << 25)], ids=lambda k: "-".join("%s=%s" % i for i in k.items()))
+                                dict(ws=4100), dict(ws_bytes=100), dict(R=1 << 25), dict(V=1 << 25, ldk=1 << 25), dict(ldx=1 << 23), dict(R=1 << 22, V=1 << 22, ldk=1 << 22)], ids=lambda k: "-".join("%s=%s" % i for i in k.items()))
 def test_c_refuses(sfx, kw):
     from aesrc2020_amd import _lib
     L = _lib.lib().fn
