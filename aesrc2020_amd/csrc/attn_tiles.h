@@ -52,10 +52,9 @@ template <typename T, int DP> constexpr int pitch() {
 }
 // 16-byte chunk `ch` of row `row`: eight consecutive rows put one chunk into eight different bank groups of 16 bytes (row-wise 16-byte
 // reads), four consecutive rows put a PAIR of chunks into four different ones (the transposing reads)
-template <int PITCH> __device__ __forceinline__ int chunk_at(int row, int ch) {
-    const int f = PITCH == 64 ? (row & 2) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1);
-    return row * PITCH + ((ch ^ f) << 4);
-}
+// (every bit of the swizzle is one bit of the row: the swizzle of a sum of rows without common bits is the two swizzles' xor)
+template <int PITCH> __device__ __forceinline__ constexpr int swizzle(int row) { return PITCH == 64 ? (row & 2) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1); }
+template <int PITCH> __device__ __forceinline__ int chunk_at(int row, int ch) { return row * PITCH + ((ch ^ swizzle<PITCH>(row)) << 4); }
 // fragment of chunk c: row `row`
 template <int PITCH> __device__ __forceinline__ u32x4 frag(const char* tile, int row, int c, int h) {
     return *reinterpret_cast<const u32x4*>(tile + chunk_at<PITCH>(row, 2 * c + h));
@@ -154,7 +153,7 @@ template <int PITCH, int ROWS> struct TileLoader {
     unsigned first, step;
     __device__ __forceinline__ TileLoader(unsigned stride, unsigned bytes) {
         const int slot = threadIdx.x, row = slot / CPR, pos = slot % CPR;
-        const unsigned ch = (unsigned)((chunk_at<PITCH>(row, pos) - row * PITCH) >> 4);      // (an involution: the piece that belongs at `pos`)
+        const unsigned ch = pos ^ swizzle<PITCH>(row);            // the piece that belongs at `pos`
         first = ch * 16 < bytes ? row * stride + ch * 16 : 0x80000000u;                        // behind the row: out of any range
         step = 256 / CPR * stride;
     }
@@ -165,6 +164,25 @@ template <int PITCH, int ROWS> struct TileLoader {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (ALL % 4 == 0 || 4 * i + wave < ALL) dma16(rsrc, first + i * step, dst + (4 * i + wave) * 1024);
+    }
+};
+
+// the same for one wave alone: 32 rows, waited for with the wave's own count of loads
+template <int PITCH> struct WaveLoader {
+    static constexpr int CPR = PITCH / 16, RPI = 64 / CPR, N = 32 / RPI;
+    unsigned row, piece;
+    __device__ __forceinline__ WaveLoader(unsigned stride) {
+        const int lane = threadIdx.x & 63, r = lane / CPR;
+        row = r * stride;
+        piece = lane % CPR ^ swizzle<PITCH>(r);
+    }
+    __device__ __forceinline__ void load(const void* base, int rows, unsigned stride, unsigned bytes, unsigned dst) const {
+        const u32x4 rsrc = descriptor(base, (unsigned)(min(rows, 32) - 1) * stride + bytes);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const unsigned at = (piece ^ swizzle<PITCH>(i * RPI)) * 16;
+            dma16(rsrc, at < bytes ? row + i * RPI * stride + at : 0x80000000u, dst + i * 1024);
+        }
     }
 };
 

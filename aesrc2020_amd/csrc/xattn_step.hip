@@ -1,8 +1,7 @@
 // Attention of a FEW rows (one token, a beam's tokens) to many keys: up to 32 folded rows (tokens x query heads of a key head) are the
 // columns n of one MFMA tile, every wave of a block walks its own 32-key tiles without a barrier, waves and key slices are joined at the end.
-// Reading the keys and values once is the whole cost, so what counts is bytes in flight: the next tile's K and V are loaded into registers
-// while the present one is computed.  K goes from memory straight into fragments; V passes through a wave's own piece of LDS, where
-// the transposing reads pick it up.
+// Reading the keys and values once is the whole cost, so what counts is bytes in flight: a wave has two buffers for a K and a V tile in LDS and
+// loads the next tile straight into one (whole rows, coalesced) while it computes from the other.
 //
 // The same kernel reads the 8-bit cache (include/sarnet.h: sarKv8): e4m3 values are converted exactly into the 16-bit operand type (bf16 for
 // bf16 and fp32 queries, fp16 for fp16 ones); the scale of a 64-key block multiplies the fp32 scores (K), and the fp32 sums as a ratio of
@@ -47,15 +46,12 @@ template <typename C> __device__ __forceinline__ u32x4 widen8(u32x2 w) {
     }
     return o;
 }
-// 16 bytes of a row of D bytes (D a multiple of 8) from dim d on, zero past D
-__device__ __forceinline__ u32x4 load8(const unsigned char* p, int d, int D, bool ok) {
-    u32x4 r = {0, 0, 0, 0};
-    if (ok && d + 16 <= D && (D & 15) == 0) r = *reinterpret_cast<const u32x4*>(p + d);
-    else {
-        if (ok && d < D) { const u32x2 w = *reinterpret_cast<const u32x2*>(p + d); r[0] = w[0]; r[1] = w[1]; }
-        if (ok && d + 8 < D) { const u32x2 w = *reinterpret_cast<const u32x2*>(p + d + 8); r[2] = w[0]; r[3] = w[1]; }
-    }
-    return r;
+// mma_down (attn_tiles.h) over a tile of e4m3 rows: the transposing read hands a lane eight rows of one column as bytes
+template <typename C, int PITCH> __device__ __forceinline__ u32x4 down8(const char* tile, int dt, int s, int lane) {
+    const int i = lane & 15, slot = i >> 1, r = 16 * s + 4 * (lane >> 5) + (slot & 3) + 8 * (slot >> 2);
+    typedef __attribute__((ext_vector_type(2))) int i32x2;
+    const i32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(tile + chunk_at<PITCH>(r, 2 * dt + ((lane >> 4) & 1)) + (i & 1) * 8));
+    return widen8<C>(__builtin_bit_cast(u32x2, v));
 }
 
 // a 32 x 32 fp32 result as operand planes of the 16-bit type: one (rounded), or three whose sum is the value
@@ -69,24 +65,42 @@ template <typename C, int NPL> __device__ __forceinline__ void pack_planes(f32x1
     }
 }
 
-template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_bounds__(64 * NW) void xattn_step_kernel(sarXattn a, Kv8 kv, int row_tiles, int splits) {
-    constexpr int P = pitch<C, DP>(), ND = DP / 32, NPL = S8 && sizeof(T) == 4 ? 3 : 1;
+template <typename T, bool S8, int DP> constexpr int step_pitch() { return S8 ? (DP <= 64 ? 64 : 128) : pitch<T, DP>(); }
+// waves of a block: each has two buffers of a K and a V tile
+template <typename T, bool S8, int DP> constexpr int step_waves() { return step_pitch<T, S8, DP>() <= 256 ? 4 : 2; }
+
+template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_bounds__(64 * NW, 2) void xattn_step_kernel(sarXattn a, Kv8 kv, int row_tiles, int splits) {
+    constexpr int P = step_pitch<T, S8, DP>(), ND = DP / 32, NPL = S8 && sizeof(T) == 4 ? 3 : 1, TILE = 32 * P;
     constexpr int NC = DP * (int)sizeof(C) / 32;                  // operand chunks of a row
-    constexpr int CHV = DP * (S8 ? 1 : (int)sizeof(T)) / 16;      // stored 16-byte pieces of a row
-    constexpr int NKL = S8 ? DP / 32 : NC, NVL = 32 * CHV / 64;
-    extern __shared__ __attribute__((aligned(16))) char lds[];    // V tiles of the waves; afterwards their partial sums
+    typedef WaveLoader<P> Loader;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];  // K and V tiles of the waves; afterwards their partial sums
     __shared__ float lm[NW][32], ll[NW][32];
     const int item = xcd_item(a.B * a.Hkv * row_tiles * splits);
     if (item < 0) return;
     const int sp = item % splits, rt = item / splits % row_tiles, bh = item / splits / row_tiles;
     const int b = bh / a.Hkv, hk = bh % a.Hkv;
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
     const int R = a.Tq * (a.Hq / a.Hkv), r = rt * 32 + n, rl = live_rows(a, b), len = live_keys(a, b);
     const int tiles = (len + 31) / 32, per = (tiles + splits - 1) / splits;
     const int t0 = min(sp * per, tiles), t1 = rt * 32 < rl ? min(t0 + per, tiles) : t0;
     const Row me = row_of(a, hk, min(r, R - 1));
     const float sl = a.scale * LOG2E;
-    char* tile = lds + w * 32 * P;
+
+    const unsigned bytes = (unsigned)(a.D * (S8 ? 1 : (int)sizeof(T)));
+    const long k_st = S8 ? a.D : a.k_st * (long)sizeof(T), v_st = S8 ? a.D : a.v_st * (long)sizeof(T);
+    const char* kb = S8 ? reinterpret_cast<const char*>(kv.k8) + (long)bh * kv.frames * a.D : reinterpret_cast<const char*>(a.k) + (b * a.k_sb + hk * a.k_sh) * (long)sizeof(T);
+    const char* vb = S8 ? reinterpret_cast<const char*>(kv.v8) + (long)bh * kv.frames * a.D : reinterpret_cast<const char*>(a.v) + (b * a.v_sb + hk * a.v_sh) * (long)sizeof(T);
+    // (scalar loads: a vector load among the tile loads would be waited for with them)
+    typedef const __attribute__((address_space(4))) float* scales;
+    const scales ks = S8 ? (scales)(uintptr_t)(kv.ks + (long)bh * (kv.frames / KV_BLOCK)) : nullptr, vs = S8 ? (scales)(uintptr_t)(kv.vs + (long)bh * (kv.frames / KV_BLOCK)) : nullptr;
+    const Loader lk((unsigned)k_st), lv((unsigned)v_st);
+    char* mine = lds + w * 4 * TILE;
+    const unsigned to = lds_addr(mine);
+    const auto load = [&](int t, int buf) {
+        lk.load(kb + t * 32 * k_st, len - t * 32, (unsigned)k_st, bytes, to + buf);
+        lv.load(vb + t * 32 * v_st, len - t * 32, (unsigned)v_st, bytes, to + buf + TILE);
+    };
+    if (t0 + w < t1) load(t0 + w, 0);
 
     u32x4 qf[NPL][NC];
     {
@@ -112,79 +126,51 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
             }
         }
     }
-    const T* kb = S8 ? nullptr : reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
-    const T* vb = S8 ? nullptr : reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
-    const unsigned char* k8 = S8 ? kv.k8 + (long)bh * kv.frames * a.D : nullptr;
-    const unsigned char* v8 = S8 ? kv.v8 + (long)bh * kv.frames * a.D : nullptr;
-    const float* ks = S8 ? kv.ks + (long)bh * (kv.frames / KV_BLOCK) : nullptr;
-    const float* vs = S8 ? kv.vs + (long)bh * (kv.frames / KV_BLOCK) : nullptr;
-
-    u32x4 kr[NKL], vr[NVL];
-    float ksc = 1.f, vsc = 1.f;
-    const auto load = [&](int t) {
-        const int key = t * 32 + n;
-        if constexpr (S8) {
-#pragma unroll
-            for (int c = 0; c < NKL; ++c) kr[c] = load8(k8 + (long)key * a.D, 32 * c + 16 * h, a.D, key < len);
-#pragma unroll
-            for (int i = 0; i < NVL; ++i) {
-                const int idx = lane + 64 * i, row = t * 32 + idx / CHV;
-                vr[i] = load8(v8 + (long)row * a.D, 16 * (idx % CHV), a.D, row < len);
-            }
-            ksc = ks[t * 32 / KV_BLOCK]; vsc = vs[t * 32 / KV_BLOCK];
-        } else {
-            load_row<T, DP>(kb + (long)key * a.k_st, key < len, a.D, h, kr);
-#pragma unroll
-            for (int i = 0; i < NVL; ++i) {
-                const int idx = lane + 64 * i, row = t * 32 + idx / CHV, d = (idx % CHV) * Num<T>::PER;
-                vr[i] = u32x4{0, 0, 0, 0};
-                if (row < len && d < a.D) vr[i] = *reinterpret_cast<const u32x4*>(vb + (long)row * a.v_st + d);
-            }
-        }
-    };
     f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = NO_MAX, l = 0.f, unit = 1.f;                        // o holds sums in units of `unit` (a power of two; 1 without a cache)
-    if (t0 + w < t1) load(t0 + w);
-    if (S8 && t0 + w < t1) unit = vsc;
-    for (int t = t0 + w; t < t1; t += NW) {
+    if (S8 && t0 + w < t1) unit = vs[(t0 + w) * 32 / KV_BLOCK];
+    int cur = 0;
+    for (int t = t0 + w; t < t1; t += NW, cur ^= 2 * TILE) {
+        if (t + NW < t1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // the reads of the buffer that is loaded next are done
+            load(t + NW, cur ^ (2 * TILE));
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Loader::N) : "memory");
+        } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const char *tk = mine + cur, *tv = tk + TILE;
         f32x16 s;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = 0.f;
         if constexpr (S8) {
 #pragma unroll
-            for (int c = 0; c < NKL; ++c) {
-                const u32x4 lo = widen8<C>(u32x2{kr[c][0], kr[c][1]}), hi = widen8<C>(u32x2{kr[c][2], kr[c][3]});
+            for (int c = 0; c < DP / 32; ++c) {
+                u32x4 x = frag<P>(tk, n, c, h);
+                if (a.D & 8) {                                    // a row ends inside a piece: what follows is the next row
+                    const bool half = 32 * c + 16 * h + 8 >= a.D;
+                    x[2] = half ? 0 : x[2]; x[3] = half ? 0 : x[3];
+                }
+                const u32x4 lo = widen8<C>(u32x2{x[0], x[1]}), hi = widen8<C>(u32x2{x[2], x[3]});
 #pragma unroll
                 for (int k = NPL - 1; k >= 0; --k) { s = mma<C>(lo, qf[k][2 * c], s); s = mma<C>(hi, qf[k][2 * c + 1], s); }
             }
-#pragma unroll
-            for (int i = 0; i < NVL; ++i) {
-                const int idx = lane + 64 * i, row = idx / CHV, ch = idx % CHV;
-                *reinterpret_cast<u32x4*>(tile + chunk_at<P>(row, 2 * ch)) = widen8<C>(u32x2{vr[i][0], vr[i][1]});
-                *reinterpret_cast<u32x4*>(tile + chunk_at<P>(row, 2 * ch + 1)) = widen8<C>(u32x2{vr[i][2], vr[i][3]});
-            }
         } else {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) s = mma<T>(kr[c], qf[0][c], s);
-#pragma unroll
-            for (int i = 0; i < NVL; ++i) {
-                const int idx = lane + 64 * i;
-                *reinterpret_cast<u32x4*>(tile + chunk_at<P>(idx / CHV, idx % CHV)) = vr[i];
-            }
+            for (int c = 0; c < NC; ++c) s = mma<T>(frag<P>(tk, n, c, h), qf[0][c], s);
         }
-        const float f = sl * ksc, nu = vsc;
-        if (t + NW < t1) load(t + NW);
+        const float f = S8 ? sl * ks[t * 32 / KV_BLOCK] : sl, nu = S8 ? vs[t * 32 / KV_BLOCK] : 1.f;
         float top = NO_MAX;
+        if (t * 32 + 32 > len) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const bool in = t * 32 + 8 * (i >> 2) + 4 * h + (i & 3) < len;
-            s[i] = in ? s[i] * f : -INFINITY;
-            top = fmaxf(top, s[i]);
+            for (int i = 0; i < 16; ++i) s[i] = t * 32 + 8 * (i >> 2) + 4 * h + (i & 3) < len ? s[i] * f : -INFINITY;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] *= f;
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
         top = half_max(top);
         if (__any(top > m + 8.f) || (S8 && nu != unit)) {
             const float mn = fmaxf(m, top), e = __builtin_amdgcn_exp2f(m - mn), eo = S8 ? e * (unit / nu) : e;
@@ -199,12 +185,17 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
         for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(s[i] - m); l += s[i]; }
         u32x4 p[NPL][4];
         pack_planes<C, NPL>(s, p);
-        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d) {
+            if constexpr (S8) {
 #pragma unroll
-            for (int k = NPL - 1; k >= 0; --k) o[d] = mma_down<C, P>(tile, 0, d, p[k], o[d], lane);
-        __builtin_amdgcn_wave_barrier();
+                for (int x = 0; x < 2; ++x) {
+                    const u32x4 v = down8<C, P>(tv, d, x, lane);
+#pragma unroll
+                    for (int k = NPL - 1; k >= 0; --k) o[d] = mma<C>(v, p[k][x], o[d]);
+                }
+            } else o[d] = mma_down<C, P>(tv, 0, d, p[0], o[d], lane);
+        }
     }
     l = half_sum(l);
 
@@ -345,10 +336,10 @@ template <typename T> __global__ __launch_bounds__(256) void kv8_store_kernel(Kv
 using namespace attn;
 
 template <typename C, bool S8, int DP> static int launch_step(const sarXattn& a, const Kv8& kv, int splits, hipStream_t st) {
-    constexpr int NW = 4;
+    constexpr int NW = step_waves<elt, S8, DP>();
     const long R = (long)a.Tq * (a.Hq / a.Hkv);
     const int rt = cdiv(R, 32);
-    const size_t tiles = (size_t)NW * 32 * pitch<C, DP>(), join = (size_t)NW * (R < 32 ? R : 32) * DP * 4, lds = tiles > join ? tiles : join;
+    const size_t tiles = (size_t)NW * 4 * 32 * step_pitch<elt, S8, DP>(), join = (size_t)NW * (R < 32 ? R : 32) * DP * 4, lds = tiles > join ? tiles : join;
     auto* k = &xattn_step_kernel<elt, C, S8, DP, NW>;
     static PerDeviceFlag raised;
     if (lds > 64 * 1024 && !raised) {
