@@ -110,13 +110,14 @@ template <typename T> __device__ __forceinline__ void pack(const f32x16& s, u32x
 }
 
 // the fragments of one row (a wave's column n), zero past D and for rows that do not exist
-template <typename T, int DP> __device__ __forceinline__ void load_row(const T* p, bool ok, int D, int h, u32x4* f) {
+template <typename T, int DP> __device__ __forceinline__ void load_row(const T* p, bool ok, int D, int h, u32x4* f, bool negate = false) {
     constexpr int NC = DP * (int)sizeof(T) / 32;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int d = (2 * c + h) * Num<T>::PER;
         f[c] = u32x4{0, 0, 0, 0};
         if (ok && d < D) f[c] = *reinterpret_cast<const u32x4*>(p + d);
+        if (negate) f[c] = f[c] ^ (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
     }
 }
 
@@ -157,9 +158,9 @@ template <int PITCH, int ROWS> struct TileLoader {
         first = ch * 16 < bytes ? row * stride + ch * 16 : 0x80000000u;                        // behind the row: out of any range
         step = 256 / CPR * stride;
     }
-    // `rows` (>= 1) of the tile's rows exist
+    // `rows` of the tile's rows exist (none: zeros)
     __device__ __forceinline__ void load(const void* base, int rows, unsigned stride, unsigned bytes, char* tile, int wave) const {
-        const u32x4 rsrc = descriptor(base, (unsigned)(min(rows, ROWS) - 1) * stride + bytes);
+        const u32x4 rsrc = descriptor(base, rows > 0 ? (unsigned)(min(rows, ROWS) - 1) * stride + bytes : 0);
         const unsigned dst = lds_addr(tile);
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -177,7 +178,7 @@ template <int PITCH> struct WaveLoader {
         piece = lane % CPR ^ swizzle<PITCH>(r);
     }
     __device__ __forceinline__ void load(const void* base, int rows, unsigned stride, unsigned bytes, unsigned dst) const {
-        const u32x4 rsrc = descriptor(base, (unsigned)(min(rows, 32) - 1) * stride + bytes);
+        const u32x4 rsrc = descriptor(base, rows > 0 ? (unsigned)(min(rows, 32) - 1) * stride + bytes : 0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const unsigned at = (piece ^ swizzle<PITCH>(i * RPI)) * 16;

@@ -55,7 +55,6 @@ using attn::chunk_at;
 using attn::as16;
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int BK = 32;                  // contraction elements per LDS stage
 constexpr int NPL = SAR_ELT == 0 ? 2 : 1;
 constexpr bool FWD_SCALED = SAR_ELT == 0, BWD_SCALED = SAR_ELT != 2;           // operands packed under a power of two per tensor
 constexpr int DZ_BITS = 14;
@@ -81,28 +80,37 @@ __device__ __forceinline__ int g_exp(float v) {                   // v 2^-e in [
 struct MaxJob { const void* x; long rows, ld; int cols, f32; };
 struct MaxJobs { MaxJob j[3]; };
 // partial maxima of the finite |values| of up to three tensors (blockIdx.y): PARTS places each
-__global__ __launch_bounds__(256) void absmax_kernel(MaxJobs jobs, float* __restrict__ part) {
+__global__ __launch_bounds__(1024) void absmax_kernel(MaxJobs jobs, float* __restrict__ part) {
     __shared__ float red[16];
     const MaxJob j = jobs.j[blockIdx.y];
     float m = 0.f;
     const auto see = [&](float v) { v = fabsf(v); if (v < INFINITY) m = fmaxf(m, v); };
-    if (j.rows == 1) {
-        for (long c = blockIdx.x * 256 + threadIdx.x; c < j.cols; c += PARTS * 256)
-            see(j.f32 ? reinterpret_cast<const float*>(j.x)[c] : (float)reinterpret_cast<const elt*>(j.x)[c]);
+    if (j.f32) {
+        for (long c = blockIdx.x * 1024 + threadIdx.x; c < j.cols; c += PARTS * 1024) see(reinterpret_cast<const float*>(j.x)[c]);
     } else {
-        // a block walks rows; eight elements a thread where rows are aligned for it
+        // sixteen bytes a thread where rows are aligned for it; whole tensors without gaps as one row
         constexpr int V = Num<elt>::PER;
-        const bool wide = j.cols % V == 0 && j.ld % V == 0 && (uintptr_t)j.x % 16 == 0;
-        for (long r = blockIdx.x; r < j.rows; r += PARTS) {
-            const elt* p = reinterpret_cast<const elt*>(j.x) + r * j.ld;
-            if (wide)
-                for (int c = threadIdx.x; c < j.cols / V; c += 256) {
-                    const auto v = reinterpret_cast<const typename Num<elt>::x16*>(p)[c];
+        const bool flat = j.ld == j.cols, wide = (flat ? j.rows * j.cols : j.cols) % V == 0 && (flat || j.ld % V == 0) && (uintptr_t)j.x % 16 == 0;
+        const elt* x = reinterpret_cast<const elt*>(j.x);
+        const long rows = flat ? 1 : j.rows, cols = flat ? j.rows * j.cols : j.cols, n = wide ? cols / V : cols;
+        const long first = flat ? (long)blockIdx.x * 1024 + threadIdx.x : threadIdx.x, step = flat ? PARTS * 1024 : 1024;
+        for (long r = flat ? 0 : blockIdx.x; r < rows; r += PARTS) {
+            const elt* p = x + r * j.ld;
+            if (wide) {
+                const auto* q = reinterpret_cast<const typename Num<elt>::x16*>(p);
+                long c = first;
+                for (; c + 3 * step < n; c += 4 * step) {         // four loads in flight
+                    const auto a = q[c], b = q[c + step], d = q[c + 2 * step], e = q[c + 3 * step];
 #pragma unroll
-                    for (int k = 0; k < V; ++k) see((float)v[k]);
+                    for (int k = 0; k < V; ++k) { see((float)a[k]); see((float)b[k]); see((float)d[k]); see((float)e[k]); }
                 }
-            else
-                for (int c = threadIdx.x; c < j.cols; c += 256) see((float)p[c]);
+                for (; c < n; c += step) {
+                    const auto a = q[c];
+#pragma unroll
+                    for (int k = 0; k < V; ++k) see((float)a[k]);
+                }
+            } else
+                for (long c = first; c < n; c += step) see((float)p[c]);
         }
     }
     m = block_max(m, red);
@@ -149,7 +157,7 @@ template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_
 struct Side { const void* p; long plane, ld; int len, k; };
 
 // an operand's LDS tile of one stage: ROWS of the output's side, BK of the contraction; everything outside the tensor arrives as zeros
-template <typename OP, int ROWS, bool DOWN> struct Operand {
+template <typename OP, int BK, int ROWS, bool DOWN> struct Operand {
     static constexpr int P = DOWN ? ROWS * 2 : BK * 2, LINES = DOWN ? BK : ROWS, BYTES = ROWS * BK * 2, N = attn::TileLoader<P, LINES>::N;
     attn::TileLoader<P, LINES> loader;
     const OP* base;
@@ -194,10 +202,10 @@ __device__ __forceinline__ long label_of(const Epi& e, int r) {
 // C = A B^T over k, four waves as 2 x 2, each MT x NT tiles of 32 x 32.  ST stages of LDS, loads ST - 1 steps ahead.
 // What bounds it: the LDS reads of 64 x 64 per wave (four 16-byte fragments for four matrix instructions) plus the stages' writes come to 1.5 times the
 // matrix instructions' cycles at the peak rate; several blocks per CU keep both busy.
-template <typename OP, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> __global__ __launch_bounds__(256, 2) void product_kernel(Side A, Side B, Epi e, int mtiles, int ntiles, int ksteps, int slices) {
+template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> __global__ __launch_bounds__(256, 2) void product_kernel(Side A, Side B, Epi e, int mtiles, int ntiles, int ksteps, int slices) {
     constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * 2, SB = BN * BK * 2, STAGE = NPL * (SA + SB), ST = 49152 / STAGE < 4 ? (49152 / STAGE > 2 ? 49152 / STAGE : 2) : 4;
-    typedef Operand<OP, BM, AD> OA;
-    typedef Operand<OP, BN, BD> OB;
+    typedef Operand<OP, BK, BM, AD> OA;
+    typedef Operand<OP, BK, BN, BD> OB;
     constexpr int LOADS = NPL * (OA::N + OB::N);
     __shared__ __attribute__((aligned(1024))) char lds[ST * STAGE];
     const int item = attn::xcd_item(mtiles * ntiles * slices);
@@ -435,7 +443,16 @@ __global__ __launch_bounds__(256) void sum_slices_kernel(SumJobs jobs) {
         const int c = (int)(i - r * across) * 256 + threadIdx.x;
         if (c >= j.cols) continue;
         float v = 0.f;
-        for (int s = 0; s < j.slices; ++s) v += j.part[s * j.slice + r * j.ldp + c];
+        const float* p = j.part + r * j.ldp + c;
+        int s = 0;
+        for (; s + 8 <= j.slices; s += 8) {                       // eight loads in flight
+            float t[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = p[(s + k) * j.slice];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += t[k];
+        }
+        for (; s < j.slices; ++s) v += p[s * j.slice];
         elt* o = j.out + r * j.ldo + c;
         *o = (elt)(j.accumulate ? (float)*o + v : v);
     }
@@ -443,7 +460,7 @@ __global__ __launch_bounds__(256) void sum_slices_kernel(SumJobs jobs) {
 
 // ---- plan of a call: what is packed, the pieces, the tiles, the workspace
 struct Plan {
-    int Rp, Dp, Vp;                     // rows, hidden width and vocabulary rounded up to the contraction step
+    int Rp, Dp, Vp;                     // rows, hidden width and vocabulary rounded up to the contraction steps
     bool pack_x, pack_w;
     int piece, pieces;
     bool small_z, small_dx, small_dw;   // 64 x 64 tiles instead of 128 x 128
@@ -452,7 +469,7 @@ struct Plan {
     size_t parts, xo, wo, a, b, zl, dz, dxp, dwp, dbp, bytes;      // offsets
 };
 static size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
-static int up32(int n) { return (n + 31) & ~31; }
+static int up64(int n) { return (n + 63) & ~63; }
 static long tiles(int m, int n, int t) { return (long)cdiv(m, t) * cdiv(n, t); }
 // 64 x 64 tiles where 128 x 128 ones leave CUs without work
 static bool small(int m, int n) { return tiles(m, n, 128) < 256; }
@@ -469,11 +486,11 @@ static bool bad(const sarVocabCe* a) {
 }
 static Plan plan(const sarVocabCe* a, bool grad) {
     Plan p = {};
-    p.Rp = up32(a->R); p.Dp = up32(a->D); p.Vp = up32(a->V);
+    p.Rp = up64(a->R); p.Dp = up64(a->D); p.Vp = up64(a->V);
     // operands are read where they lie when they have the products' type, their rows are 16-byte aligned and no row ends inside a contraction step
     const bool scaled = grad ? BWD_SCALED : FWD_SCALED;
-    p.pack_x = scaled || a->D % 32 || a->ldx % 8 || (uintptr_t)a->x % 16;
-    p.pack_w = scaled || a->V % 32 || a->ldk % 8 || (uintptr_t)a->kernel % 16;
+    p.pack_x = scaled || a->D % 64 || a->ldx % 8 || (uintptr_t)a->x % 16;
+    p.pack_w = scaled || a->V % 64 || a->ldk % 8 || (uintptr_t)a->kernel % 16;
     size_t at = 0;
     const auto take = [&](size_t n) { const size_t o = at; at += up(n); return o; };
     p.parts = take(3 * PARTS * 4);
@@ -506,14 +523,18 @@ static Plan plan(const sarVocabCe* a, bool grad) {
     return p;
 }
 
+// contraction elements per LDS stage.  64 (two stages) where an operand is read along the contraction on both sides -- whole 128-byte lines -- or on
+// neither: dx 189 -> 159 us, dW 158 -> 141 us for an 8192 x 8192 piece against 1024; 32 (three stages, three blocks per CU) for the logits:
+// 595 against 614 us for 8192 x 32000 x 1024.  fp32 (two planes): 32.
+constexpr int step_of(bool ad, bool bd) { return NPL == 2 || ad != bd ? 32 : 64; }
 static unsigned some_blocks(long n) { return (unsigned)(n < 1 ? 1 : n < 4096 ? n : 4096); }
 // the operands as the products read them
 template <typename OP, bool SCALED> static void operands(const sarVocabCe* a, const Plan& p, bool grad, Side& x, Side& w, hipStream_t st) {
     char* ws = reinterpret_cast<char*>(a->ws);
     float* parts = reinterpret_cast<float*>(ws + p.parts);
     const MaxJobs all = {{{a->x, a->R, a->ldx, a->D, 0}, {a->kernel, a->D, a->ldk, a->V, 0}, {a->dloss, 1, a->R, a->R, 1}}}, gradient = {{all.j[2]}};
-    if (SCALED) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, grad ? 3 : 2), dim3(256), 0, st, all, parts);
-    else if (grad) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, 1), dim3(256), 0, st, gradient, parts + 2 * PARTS);
+    if (SCALED) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, grad ? 3 : 2), dim3(1024), 0, st, all, parts);
+    else if (grad) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, 1), dim3(1024), 0, st, gradient, parts + 2 * PARTS);
     x = {a->x, 0, a->ldx, 0, 0};
     w = {a->kernel, 0, a->ldk, 0, 0};
     PackJobs jobs = {};
@@ -529,11 +550,13 @@ template <typename OP, bool SCALED> static void operands(const sarVocabCe* a, co
     if (p.pack_w) pack(w, p.wo, a->D, a->V, p.Vp, parts + PARTS);
     if (n) hipLaunchKernelGGL((pack_kernel<OP, SCALED>), dim3(some_blocks(blocks), n), dim3(256), 0, st, jobs);
 }
-template <typename OP, bool AD, bool BD, int EPI, bool SCALED> static void product(Side A, Side B, const Epi& e, int m, int n, int ksteps, int slices, bool small_tiles, hipStream_t st) {
+template <typename OP, bool AD, bool BD, int EPI, bool SCALED> static void product(Side A, Side B, const Epi& e, int m, int n, int k, int slices, bool small_tiles, hipStream_t st) {
+    constexpr int BK = step_of(AD, BD);
+    const int ksteps = k / BK;
     const int t = small_tiles ? 64 : 128, mt = cdiv(m, t), nt = cdiv(n, t);
     const dim3 grid((unsigned)attn::xcd_grid((long)mt * nt * slices));
-    if (small_tiles) hipLaunchKernelGGL((product_kernel<OP, 1, 1, AD, BD, EPI, SCALED>), grid, dim3(256), 0, st, A, B, e, mt, nt, ksteps, slices);
-    else hipLaunchKernelGGL((product_kernel<OP, 2, 2, AD, BD, EPI, SCALED>), grid, dim3(256), 0, st, A, B, e, mt, nt, ksteps, slices);
+    if (small_tiles) hipLaunchKernelGGL((product_kernel<OP, BK, 1, 1, AD, BD, EPI, SCALED>), grid, dim3(256), 0, st, A, B, e, mt, nt, ksteps, slices);
+    else hipLaunchKernelGGL((product_kernel<OP, BK, 2, 2, AD, BD, EPI, SCALED>), grid, dim3(256), 0, st, A, B, e, mt, nt, ksteps, slices);
 }
 
 }
@@ -556,7 +579,7 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = a->labels; e.label_bytes = a->label_bytes;
     e.pm = reinterpret_cast<float*>(ws + p.a); e.pl = reinterpret_cast<float*>(ws + p.b); e.zl = reinterpret_cast<float*>(ws + p.zl);
     e.R = a->R; e.V = a->V; e.Rp = p.Rp;
-    product<fwd16, true, false, E_LSE, FWD_SCALED>(w, x, e, a->V, a->R, p.Dp / BK, 1, p.small_z, st);
+    product<fwd16, true, false, E_LSE, FWD_SCALED>(w, x, e, a->V, a->R, p.Dp, 1, p.small_z, st);
     hipLaunchKernelGGL(finish_kernel, dim3((unsigned)cdiv(a->R, 16)), dim3(256), 0, st, e.pm, e.pl, e.zl, a->labels, a->label_bytes, a->loss, a->lse, a->R, p.Rp, a->V, p.lse_slices);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
@@ -572,7 +595,7 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
     operands<bwd16, BWD_SCALED>(a, p, true, x, w, st);
     const auto from = [](const Side& s, int v) { Side t = s; t.p = reinterpret_cast<const bwd16*>(s.p) + v; return t; };
     for (int i = 0; i < p.pieces; ++i) {
-        const int v0 = i * p.piece, cols = a->V - v0 < p.piece ? a->V - v0 : p.piece, ld = up32(cols);
+        const int v0 = i * p.piece, cols = a->V - v0 < p.piece ? a->V - v0 : p.piece, ld = up64(cols);
         const long plane = (long)p.Rp * ld;
         Epi e = {};
         e.parts = reinterpret_cast<float*>(ws + p.parts);
@@ -583,7 +606,7 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         Side wz = from(w, v0), xz = x;
         wz.len = (p.pack_w ? p.Vp : a->V) - v0; wz.k = a->D;
         xz.len = a->R; xz.k = p.Dp;
-        product<bwd16, true, false, E_DZ, BWD_SCALED>(wz, xz, e, ld, p.Rp, p.Dp / BK, 1, p.small_z, st);
+        product<bwd16, true, false, E_DZ, BWD_SCALED>(wz, xz, e, ld, p.Rp, p.Dp, 1, p.small_z, st);
         SumJobs sums = {};
         int ns = 0;
         long blocks = 0;
@@ -599,11 +622,11 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
             elt* out = reinterpret_cast<elt*>(a->dkernel) + v0;
             if (p.dw_slices > 1) {
                 o.out = ws + p.dwp; o.slice = (long)a->D * ld; o.ldo = ld;
-                product<bwd16, true, true, E_PART, BWD_SCALED>(A, B, o, a->D, cols, p.Rp / BK, p.dw_slices, p.small_dw, st);
+                product<bwd16, true, true, E_PART, BWD_SCALED>(A, B, o, a->D, cols, p.Rp, p.dw_slices, p.small_dw, st);
                 sum(p.dwp, p.dw_slices, o.slice, a->D, cols, ld, out, a->V, a->accumulate);
             } else {
                 o.out = out; o.ldo = a->V; o.accumulate = a->accumulate;
-                product<bwd16, true, true, E_OUT, BWD_SCALED>(A, B, o, a->D, cols, p.Rp / BK, 1, p.small_dw, st);
+                product<bwd16, true, true, E_OUT, BWD_SCALED>(A, B, o, a->D, cols, p.Rp, 1, p.small_dw, st);
             }
         }
         if (a->dbias) sum(p.dbp, p.db_slices, ld, 1, cols, ld, reinterpret_cast<elt*>(a->dbias) + v0, cols, a->accumulate);
@@ -613,11 +636,11 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
             const Side A = {dz, plane, ld, p.Rp, ld}, B0 = from(w, v0), B = {B0.p, w.plane, w.ld, a->D, ld};
             if (p.dx_parts) {
                 o.out = ws + p.dxp; o.slice = (long)a->R * a->D; o.accumulate = i > 0;
-                product<bwd16, false, false, E_PART, BWD_SCALED>(A, B, o, a->R, a->D, ld / BK, p.dx_slices, p.small_dx, st);
+                product<bwd16, false, false, E_PART, BWD_SCALED>(A, B, o, a->R, a->D, ld, p.dx_slices, p.small_dx, st);
                 if (i == p.pieces - 1) sum(p.dxp, p.dx_slices, o.slice, a->R, a->D, a->D, reinterpret_cast<elt*>(a->dx), a->D, 0);
             } else {
                 o.out = a->dx;
-                product<bwd16, false, false, E_OUT, BWD_SCALED>(A, B, o, a->R, a->D, ld / BK, 1, p.small_dx, st);
+                product<bwd16, false, false, E_OUT, BWD_SCALED>(A, B, o, a->R, a->D, ld, 1, p.small_dx, st);
             }
         }
         if (ns) hipLaunchKernelGGL(sum_slices_kernel, dim3(some_blocks(blocks), ns), dim3(256), 0, st, sums);

@@ -28,6 +28,9 @@ constexpr float NO_MAX = -1e30f;        // the running maximum before any key: f
 __device__ __forceinline__ int live_keys(const sarXattn& a, int b) { return a.k_lens ? min(max(a.k_lens[b], 0), a.Tk) : a.Tk; }
 __device__ __forceinline__ int live_rows(const sarXattn& a, int b) { return (a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq) * (a.Hq / a.Hkv); }
 
+// |scale| log2 e; for a scale of 0 a number that makes any finite product 0 and leaves -inf what it is
+__device__ __forceinline__ float score_factor(const sarXattn& a) { return fmaxf(fabsf(a.scale) * LOG2E, 1e-37f); }
+
 struct Row { int t, h; };
 __device__ __forceinline__ Row row_of(const sarXattn& a, int hkv, int r) {
     const int G = a.Hq / a.Hkv, t = r / G;

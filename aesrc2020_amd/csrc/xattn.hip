@@ -80,7 +80,8 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     const int per = ((len + KT - 1) / KT + splits - 1) / splits * KT;
     const int k0 = min(sp * per, len), k1 = rt * 32 * WN < rl ? min(k0 + per, len) : k0;
     const Row me = row_of(a, hk, min(r, R - 1));
-    const float sl = a.scale * LOG2E;
+    // scores by |scale|, the sign in the queries: the maximum of the products is then the maximum of the scores
+    const float sl = score_factor(a);
 
     const unsigned ks = (unsigned)(a.k_st * sizeof(T)), vs = (unsigned)(a.v_st * sizeof(T)), db = (unsigned)(a.D * sizeof(T));
     const TileLoader<P, KT> tk(ks, db), tv(vs, db);
@@ -92,7 +93,7 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     };
     if (k0 < k1) load(k0, lds);
     u32x4 qf[NC];
-    load_row<T, DP>(reinterpret_cast<const T*>(a.q) + b * a.q_sb + me.t * a.q_st + me.h * a.q_sh, r < rl, a.D, h, qf);
+    load_row<T, DP>(reinterpret_cast<const T*>(a.q) + b * a.q_sb + me.t * a.q_st + me.h * a.q_sh, r < rl, a.D, h, qf, a.scale < 0.f);
     f32x16 o[ND];
     clear(o);
     float m = NO_MAX, l = 0.f;
@@ -114,18 +115,13 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
 #pragma unroll
             for (int u = 0; u < NS; ++u)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[u][i] = j + 32 * (u * WM + wm) + 8 * (i >> 2) + 4 * h + (i & 3) < k1 ? s[u][i] * sl : -INFINITY;
-        } else {
-#pragma unroll
-            for (int u = 0; u < NS; ++u)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[u][i] *= sl;
+                for (int i = 0; i < 16; ++i) s[u][i] = j + 32 * (u * WM + wm) + 8 * (i >> 2) + 4 * h + (i & 3) < k1 ? s[u][i] : -INFINITY;
         }
 #pragma unroll
         for (int u = 0; u < NS; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
-        top = half_max(top);
+        top = half_max(top) * sl;
         // the maximum follows only where it grew by more than 2^8: below that p <= 2^8 loses nothing in any of the types, and most
         // tiles skip the rescaling
         if (__any(top > m + 8.f)) {
@@ -139,7 +135,7 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) { s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - m); l += s[u][i]; }
+            for (int i = 0; i < 16; ++i) { s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], sl, -m)); l += s[u][i]; }
             u32x4 p[4];
             pack<T>(s[u], p);
 #pragma unroll

@@ -84,7 +84,8 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
     const int tiles = (len + 31) / 32, per = (tiles + splits - 1) / splits;
     const int t0 = min(sp * per, tiles), t1 = rt * 32 < rl ? min(t0 + per, tiles) : t0;
     const Row me = row_of(a, hk, min(r, R - 1));
-    const float sl = a.scale * LOG2E;
+    const float sl = score_factor(a);                             // (the scale's sign is in the queries: xattn.hip)
+    const bool negate = a.scale < 0.f;
 
     const unsigned bytes = (unsigned)(a.D * (S8 ? 1 : (int)sizeof(T)));
     const long k_st = S8 ? a.D : a.k_st * (long)sizeof(T), v_st = S8 ? a.D : a.v_st * (long)sizeof(T);
@@ -113,6 +114,7 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
             if constexpr (S8 && sizeof(T) == 4) {
                 f32x4 x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
                 if (ok) { x0 = *reinterpret_cast<const f32x4*>(qp + d); x1 = *reinterpret_cast<const f32x4*>(qp + d + 4); }
+                if (negate) { x0 = -x0; x1 = -x1; }
 #pragma unroll
                 for (int k = 0; k < NPL; ++k) {
                     typename Num<C>::x16 v;
@@ -123,6 +125,7 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
             } else {
                 qf[0][c] = u32x4{0, 0, 0, 0};
                 if (ok) qf[0][c] = *reinterpret_cast<const u32x4*>(qp + d);
+                if (negate) qf[0][c] = qf[0][c] ^ (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
             }
         }
     }
@@ -164,14 +167,11 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
         float top = NO_MAX;
         if (t * 32 + 32 > len) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = t * 32 + 8 * (i >> 2) + 4 * h + (i & 3) < len ? s[i] * f : -INFINITY;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] *= f;
+            for (int i = 0; i < 16; ++i) s[i] = t * 32 + 8 * (i >> 2) + 4 * h + (i & 3) < len ? s[i] : -INFINITY;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
-        top = half_max(top);
+        top = half_max(top) * f;
         if (__any(top > m + 8.f) || (S8 && nu != unit)) {
             const float mn = fmaxf(m, top), e = __builtin_amdgcn_exp2f(m - mn), eo = S8 ? e * (unit / nu) : e;
             m = mn; l *= e;
@@ -182,7 +182,7 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
                 for (int i = 0; i < 16; ++i) o[d][i] *= eo;
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(s[i] - m); l += s[i]; }
+        for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], f, -m)); l += s[i]; }
         u32x4 p[NPL][4];
         pack_planes<C, NPL>(s, p);
 #pragma unroll

@@ -178,7 +178,7 @@ def test_large_scores_given_scale_and_out_buffers(dt):
     A = _att()
     q, k, v, g = make(1, 64, 200, 2, 2, 64, DT[dt], seed=2)
     q = (q.float() * 12).to(DT[dt])
-    for scale in (1.0, -0.3):
+    for scale in (1.0, -0.3, 0.0):
         o = torch.full_like(q, 7.0); l = torch.empty(1, 2, 64, device="cuda")
         out, lse = A.cross_attention(q, k, v, scale=scale, return_lse=True, out=o, lse=l)
         assert out is o and lse is l
