@@ -23,17 +23,18 @@ class Xattn(ctypes.Structure):
 
 
 def _rows(name, x, like=None):
-    """x as the kernels take it: 4-D, last axis contiguous, rows on 16-byte boundaries -- a view that is not is copied."""
+    """x as the kernels take it: 4-D, last axis contiguous, rows on 16-byte boundaries and at most 16 MB apart -- a view that is not is copied."""
     if x.dim() != 4:
         raise ValueError("%s has to be (batch, time, heads, dim), got shape %r" % (name, tuple(x.shape)))
-    if x.dtype not in _SFX:
-        raise ValueError("%s has to be float32, bfloat16 or float16, got %s" % (name, x.dtype))
-    if like is not None and (x.dtype != like.dtype or x.device != like.device):
+    if like is None:
+        if x.dtype not in _SFX:
+            raise ValueError("%s has to be float32, bfloat16 or float16, got %s" % (name, x.dtype))
+        if not x.is_cuda:
+            raise ValueError("%s is on %s: the kernels need a HIP device, there is no CPU fallback" % (name, x.device))
+    elif x.dtype != like.dtype or x.device != like.device:
         raise ValueError("%s is %s on %s, the queries are %s on %s" % (name, x.dtype, x.device, like.dtype, like.device))
-    if like is None and not x.is_cuda:
-        raise ValueError("%s is on %s: the kernels need a HIP device, there is no CPU fallback" % (name, x.device))
     sb, st, sh, sd = x.stride()
-    if sd != 1 and x.shape[3] != 1 or (sb | st | sh) * x.element_size() % 16 or x.data_ptr() % 16:
+    if sd != 1 and x.shape[3] != 1 or (sb | st | sh) * x.element_size() & 15 or x.data_ptr() & 15 or st > 1 << 22:
         return x.clone(memory_format=torch.contiguous_format)          # (a fresh allocation is aligned; contiguous() may hand x back)
     return x
 
@@ -41,7 +42,7 @@ def _rows(name, x, like=None):
 def _lens(name, lens, B, device):
     if lens is None:
         return None
-    if lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != B or lens.device != device or not lens.is_contiguous():
+    if lens.dtype != torch.int32 or lens.shape != (B,) or lens.device != device or not lens.is_contiguous():
         raise ValueError("%s has to be a contiguous int32 tensor of %d lengths on %s" % (name, B, device))
     return lens.data_ptr()
 
@@ -54,13 +55,14 @@ def _heads(Hq, Hkv, D):
 
 
 def _launch(name, device, *args):
-    L = _lib.lib()
+    """Call an entry point on the current stream of the tensors' device."""
+    fn = _lib.lib().fn[name]
     index = device.index
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
-            rc = L.fn[name](*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
     else:
-        rc = L.fn[name](*args, torch.cuda.current_stream().cuda_stream)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))      # (torch.cuda.current_stream().cuda_stream without the Stream object: 2 us less)
     if rc != 0:
         raise RuntimeError("%s failed with status %d" % (name, rc))
 
@@ -83,9 +85,10 @@ def _result(name, t, shape, dtype, device):
 
 def _check_kv(q, k, v):
     k, v = _rows("k", k, q), _rows("v", v, q)
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise ValueError("q %r, k %r and v %r do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    _heads(q.shape[2], k.shape[2], q.shape[3])
+    ks, qs = k.shape, q.shape
+    if ks != v.shape or ks[0] != qs[0] or ks[3] != qs[3]:
+        raise ValueError("q %r, k %r and v %r do not fit" % (tuple(qs), tuple(ks), tuple(v.shape)))
+    _heads(qs[2], ks[2], qs[3])
     return k, v
 
 
@@ -109,7 +112,7 @@ def cross_attention(q, k, v, k_lens=None, q_lens=None, scale=None, return_lse=Fa
         a = Xattn(q.data_ptr(), kv[0], kv[1], None, out.data_ptr(), None if lse is None else lse.data_ptr(), None, None, None, kl, ql, None, 0,
                   *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], 0, 0, 0, B, Tq, Tk, Hq, Hkv, D,
                   1.0 / math.sqrt(D) if scale is None else float(scale), 0)
-        ws = _workspace("sar_xattn_fwd_workspace_bytes", a, q.device)                            # noqa: F841  (alive until launched)
+        ws = _workspace("sar_xattn_fwd_workspace_bytes", a, q.device) if Tk > 256 else None      # noqa: F841  (alive until launched; sarnet.h: 256 keys never need one)
         _launch("sar_xattn_fwd_" + _SFX[q.dtype], q.device, ctypes.byref(a))
     return (out, lse) if return_lse else out
 
@@ -157,9 +160,9 @@ class EncoderCache8:
             raise ValueError("a cache needs at least one utterance and one frame, got %d and %d" % (batch, frames))
         self.batch, self.frames, self.heads, self.dim = batch, frames, heads, dim
         n = -(-frames // self.BLOCK)
-        self.k8, self.v8 = (torch.zeros(batch, heads, n * self.BLOCK, dim, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
-        self.k_scale, self.v_scale = (torch.ones(batch, heads, n, dtype=torch.float32, device=device) for _ in range(2))
-        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.k8, self.v8 = (torch.empty(batch, heads, n * self.BLOCK, dim, dtype=torch.float8_e4m3fn, device=device) for _ in range(2))
+        self.k_scale, self.v_scale = (torch.empty(batch, heads, n, dtype=torch.float32, device=device) for _ in range(2))
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)                         # (nothing behind a length is ever read)
         self.device = self.k8.device
 
     def store(self, k, v, k_lens=None, first=0):
@@ -191,7 +194,7 @@ class EncoderCache8:
             a = Xattn(q.data_ptr(), None, None, None, out.data_ptr(), None, None, None, None, self.lens.data_ptr(), _lens("q_lens", q_lens, B, q.device), None, 0,
                       *q.stride()[:3], 0, 0, 0, 0, 0, 0, *out.stride()[:3], 0, 0, 0, B, Tq, self.frames, Hq, self.heads, D,
                       1.0 / math.sqrt(D) if scale is None else float(scale), 0)
-            ws = _workspace("sar_kv8_attend_workspace_bytes", a, q.device)                       # noqa: F841
+            ws = _workspace("sar_kv8_attend_workspace_bytes", a, q.device) if self.frames > 256 else None       # noqa: F841
             _launch("sar_kv8_attend_" + _SFX[q.dtype], q.device, ctypes.byref(a), self.k8.data_ptr(), self.k_scale.data_ptr(), self.v8.data_ptr(),
                     self.v_scale.data_ptr(), self.k8.shape[2])
         return out

@@ -54,7 +54,7 @@ using attn::Num;
 using attn::chunk_at;
 using attn::as16;
 
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int NPL = SAR_ELT == 0 ? 2 : 1;
 constexpr bool FWD_SCALED = SAR_ELT == 0, BWD_SCALED = SAR_ELT != 2;           // operands packed under a power of two per tensor
 constexpr int DZ_BITS = 14;
@@ -202,7 +202,7 @@ __device__ __forceinline__ long label_of(const Epi& e, int r) {
 // C = A B^T over k, four waves as 2 x 2, each MT x NT tiles of 32 x 32.  ST stages of LDS, loads ST - 1 steps ahead.
 // What bounds it: the LDS reads of 64 x 64 per wave (four 16-byte fragments for four matrix instructions) plus the stages' writes come to 1.5 times the
 // matrix instructions' cycles at the peak rate; several blocks per CU keep both busy.
-template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> __global__ __launch_bounds__(256, 2) void product_kernel(Side A, Side B, Epi e, int mtiles, int ntiles, int ksteps, int slices) {
+template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> __global__ __launch_bounds__(256, (NPL == 1 && BK == 32 ? 3 : 2)) void product_kernel(Side A, Side B, Epi e, int mtiles, int ntiles, int ksteps, int slices) {
     constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * 2, SB = BN * BK * 2, STAGE = NPL * (SA + SB), ST = 49152 / STAGE < 4 ? (49152 / STAGE > 2 ? 49152 / STAGE : 2) : 4;
     typedef Operand<OP, BK, BM, AD> OA;
     typedef Operand<OP, BK, BN, BD> OB;
@@ -263,34 +263,65 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
         cur = cur == ST - 1 ? 0 : cur + 1;
     }
     const int mw = wm * MT * 32, nw = wn * NT * 32;               // the wave's corner of the tile
-    if constexpr (EPI == E_LSE) {                                 // m: vocabulary entries, n: rows of x
-        const float f = SCALED ? ldexpf(1.f, -up_exp(max_of(e.parts)) - up_exp(max_of(e.parts + PARTS))) : 1.f;
-        float* join = reinterpret_cast<float*>(lds);              // (2, BN) maxima and sums of the lower waves
-        float top[NT], l[NT];
+    // logits in powers of two: y = (acc f + b) log2 e, entries behind the vocabulary -inf
+    const auto logits = [&](int v0) {
+        const float f = LOG2E * (SCALED ? ldexpf(1.f, -up_exp(max_of(e.parts)) - up_exp(max_of(e.parts + PARTS))) : 1.f);
+        const int first = v0 + m0 + mw + 4 * h;
+        if (v0 + m0 + BM <= e.V) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int r = n0 + nw + 32 * j + (lane & 31);
-            const long lab = r < e.R ? label_of(e, r) : -1;
-            top[j] = -INFINITY;
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    float b[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (e.bias)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) b[x] = (float)e.bias[first + 32 * i + 8 * a + x] * LOG2E;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) acc[i][j][4 * a + x] = fmaf(acc[i][j][4 * a + x], f, b[x]);
+                }
+        } else {
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const int v = m0 + mw + 32 * i + 8 * (x >> 2) + 4 * h + (x & 3);
-                    float z = acc[i][j][x] * f;
-                    if (e.bias) z += v < e.V ? (float)e.bias[v] : 0.f;
-                    if (v == lab && v < e.V) e.zl[r] = z;
-                    z = v < e.V ? z : -INFINITY;
-                    acc[i][j][x] = z;
-                    top[j] = fmaxf(top[j], z);
+                    const int v = first + 32 * i + 8 * (x >> 2) + (x & 3);
+                    const float b = e.bias && v < e.V ? (float)e.bias[v] * LOG2E : 0.f;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j][x] = v < e.V ? fmaf(acc[i][j][x], f, b) : -INFINITY;
                 }
+        }
+    };
+    // f(i, x) for the place of entry `at` (of the wave's corner), if the lane holds it
+    const auto place = [&](long at, auto&& f) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+                if (at == 32 * i + 8 * (x >> 2) + 4 * h + (x & 3)) f(i, x);
+    };
+    if constexpr (EPI == E_LSE) {                                 // m: vocabulary entries, n: rows of x
+        float* join = reinterpret_cast<float*>(lds);              // (2, BN) maxima and sums of the lower waves
+        float top[NT], l[NT];
+        logits(0);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int r = n0 + nw + 32 * j + (lane & 31);
+            const long lab = r < e.R ? label_of(e, r) : -1, at = lab - m0 - mw;
+            if (__any(at >= 0 && at < 32 * MT && lab < e.V)) place(lab < e.V ? at : -1, [&](int i, int x) { e.zl[r] = acc[i][j][x]; });
+            top[j] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) top[j] = fmaxf(top[j], acc[i][j][x]);
             top[j] = attn::half_max(top[j]);
             const float base = top[j] == -INFINITY ? 0.f : top[j];
             l[j] = 0.f;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) l[j] += __builtin_amdgcn_exp2f((acc[i][j][x] - base) * LOG2E);
+                for (int x = 0; x < 16; ++x) l[j] += __builtin_amdgcn_exp2f(acc[i][j][x] - base);
             l[j] = attn::half_sum(l[j]);
         }
         __syncthreads();
@@ -304,26 +335,24 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
             if (wm || h || r >= e.Rp) continue;
             const float t2 = join[nw + 32 * j + lane], l2 = join[BN + nw + 32 * j + lane], M = fmaxf(top[j], t2), base = M == -INFINITY ? 0.f : M;
             e.pm[(long)mt * e.Rp + r] = M;
-            e.pl[(long)mt * e.Rp + r] = l[j] * __builtin_amdgcn_exp2f((top[j] - base) * LOG2E) + l2 * __builtin_amdgcn_exp2f((t2 - base) * LOG2E);
+            e.pl[(long)mt * e.Rp + r] = l[j] * __builtin_amdgcn_exp2f(top[j] - base) + l2 * __builtin_amdgcn_exp2f(t2 - base);
         }
     } else if constexpr (EPI == E_DZ) {                           // m: vocabulary entries from v0 on, n: rows of x
-        const float f = SCALED ? ldexpf(1.f, -up_exp(max_of(e.parts)) - up_exp(max_of(e.parts + PARTS))) : 1.f;
         const float gs = ldexpf(1.f, DZ_BITS - g_exp(max_of(e.parts + 2 * PARTS)));
+        logits(e.v0);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int r = n0 + nw + 32 * j + (lane & 31);
             const long lab = r < e.R ? label_of(e, r) : -1;
             const bool has = lab >= 0 && lab < e.V;
-            const float g = has ? e.dloss[r] * gs : 0.f, lse = has ? e.lse[r] : INFINITY;
+            // a row that is left out: p = exp2(-inf) = 0 and g = 0
+            const float g = has ? e.dloss[r] * gs : 0.f, lse = has ? e.lse[r] * LOG2E : INFINITY;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const int v = e.v0 + m0 + mw + 32 * i + 8 * (x >> 2) + 4 * h + (x & 3);
-                    float z = acc[i][j][x] * f;
-                    if (e.bias) z += v < e.V ? (float)e.bias[v] : 0.f;
-                    acc[i][j][x] = has && v < e.V ? g * (__builtin_amdgcn_exp2f((z - lse) * LOG2E) - (v == lab ? 1.f : 0.f)) : 0.f;
-                }
+                for (int x = 0; x < 16; ++x) acc[i][j][x] = has ? g * __builtin_amdgcn_exp2f(acc[i][j][x] - lse) : 0.f;
+            const long at = lab - e.v0 - m0 - mw;
+            if (__any(has && at >= 0 && at < 32 * MT)) place(has ? at : -1, [&](int i, int x) { acc[i][j][x] -= g; });
         }
         // through LDS into whole row pieces of the (rows, piece) array; the column sums (db) on the way
         constexpr int CH = BM / 8, REP = BN * CH / 256;
@@ -406,7 +435,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ p
     const int c = threadIdx.x & 15, g = threadIdx.x >> 4, r = blockIdx.x * 16 + c;
     const auto join = [](float& m, float& l, float m2, float l2) {
         const float M = fmaxf(m, m2), base = M == -INFINITY ? 0.f : M;
-        l = l * __builtin_amdgcn_exp2f((m - base) * LOG2E) + l2 * __builtin_amdgcn_exp2f((m2 - base) * LOG2E);
+        l = l * __builtin_amdgcn_exp2f(m - base) + l2 * __builtin_amdgcn_exp2f(m2 - base);
         m = M;
     };
     float m = -INFINITY, l = 0.f;
@@ -426,10 +455,10 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ p
     if (g || r >= R) return;
 #pragma unroll
     for (int x = 1; x < 16; ++x) join(m, l, sm[x][c], ss[x][c]);
-    const float s = m + logf(l);
+    const float s = (m + __builtin_amdgcn_logf(l)) * LN2;         // (maxima, sums and label logits are in powers of two)
     const long lab = label_bytes == 8 ? (long)reinterpret_cast<const long long*>(labels)[r] : (long)reinterpret_cast<const int*>(labels)[r];
     if (lse) lse[r] = s;
-    if (loss) loss[r] = lab >= 0 && lab < V ? s - zl[r] : 0.f;
+    if (loss) loss[r] = lab >= 0 && lab < V ? (m - zl[r] + __builtin_amdgcn_logf(l)) * LN2 : 0.f;
 }
 
 // out (rows, cols) (+)= sum of the slices, for up to three results (blockIdx.y)

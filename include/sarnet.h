@@ -591,7 +591,8 @@ int sar_adam_l2_update_f32(float* params, const float* grads, float* m, float* v
  * head h reads key head h / (Hq / Hkv), whose gradients sum over the group.  k_lens, q_lens (B) i32 or NULL (all); values outside
  * [0, T] count as the nearer end.  Rows of K and V behind a length are not used, whatever they hold.  A row behind its q_len, and a
  * row without keys, gets out = 0, lse = -inf and no gradient.  lse (B, Hq, Tq) fp32: optional in the forward, needed (with out) by the backward.
- * ws: sar_xattn_fwd_workspace_bytes / _bwd_workspace_bytes of the same arguments, 16-byte aligned (0: none); nothing in it has to be initialised. */
+ * ws: sar_xattn_fwd_workspace_bytes / _bwd_workspace_bytes of the same arguments, 16-byte aligned (0: none; a forward over at most 256 keys never
+ * needs one); nothing in it has to be initialised.  Time strides: at most 16 MB. */
 typedef struct {
     const void *q, *k, *v, *dout;
     void* out;
