@@ -72,7 +72,7 @@ static inline int key_splits(const sarXattn* a, int rows_per_block, int blocks) 
 struct FwdPlan { int waves, splits; };
 static inline FwdPlan fwd_plan(const sarXattn* a) {
     const long R = (long)a->Tq * (a->Hq / a->Hkv), bh = (long)a->B * a->Hkv;
-    if ((R + 127) / 128 * bh >= 512) return {4, 1};
+    if (R > 64 && (R + 127) / 128 * bh >= 512) return {4, 1};
     return {2, (R + 63) / 64 * bh >= 192 ? 1 : key_splits(a, 64, 384)};
 }
 static inline int step_splits(const sarXattn* a) { return key_splits(a, 32, 1024); }

@@ -373,8 +373,8 @@ template <int DP> static void launch_fwd(const sarXattn& a, hipStream_t st) {
 }
 template <int DP> static void launch_bwd(const sarXattn& a, float2* stats, hipStream_t st) {
     const long R = (long)a.Tq * (a.Hq / a.Hkv), bh = (long)a.B * a.Hkv;
-    // four waves on 128 columns where those blocks fill the chip twice, else two pairs on 64
-    const bool few_q = paired<DP>() && cdiv(R, 128) * bh < 512, few_k = paired<DP>() && cdiv(a.Tk, 128) * bh < 512;
+    // four waves on 128 columns where those blocks fill the chip twice, else two pairs on 64 -- and where 64 are all there are
+    const bool few_q = paired<DP>() && (R <= 64 || cdiv(R, 128) * bh < 512), few_k = paired<DP>() && (a.Tk <= 64 || cdiv(a.Tk, 128) * bh < 512);
     const int rt = cdiv(R, few_q ? 64 : 128), kt = cdiv(a.Tk, few_k ? 64 : 128);
     const dim3 gq((unsigned)xcd_grid(rt * bh)), gk((unsigned)xcd_grid(kt * bh));
     if constexpr (paired<DP>()) {
