@@ -6,6 +6,7 @@ Everything runs on the current HIP stream of the tensors' device, allocates thro
 raises ValueError for arguments it does not take.  layers.CrossAttention is the Layer over the same calls."""
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -20,6 +21,9 @@ class Xattn(ctypes.Structure):
     _fields_ = [(n, _P) for n in ("q", "k", "v", "dout", "out", "lse", "dq", "dk", "dv", "k_lens", "q_lens", "ws")] + [("ws_bytes", _L)] + \
                [(n, _L) for n in ("q_sb", "q_st", "q_sh", "k_sb", "k_st", "k_sh", "v_sb", "v_st", "v_sh", "o_sb", "o_st", "o_sh", "g_sb", "g_st", "g_sh")] + \
                [(n, _I) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "D")] + [("scale", ctypes.c_float), ("pad_", _I)]
+
+
+_XATTN = struct.Struct("12Ql15l6ifi")                                  # the same fields: packing bytes costs a fifth of filling the Structure
 
 
 def _rows(name, x, like=None):
@@ -41,7 +45,7 @@ def _rows(name, x, like=None):
 
 def _lens(name, lens, B, device):
     if lens is None:
-        return None
+        return 0
     if lens.dtype != torch.int32 or lens.shape != (B,) or lens.device != device or not lens.is_contiguous():
         raise ValueError("%s has to be a contiguous int32 tensor of %d lengths on %s" % (name, B, device))
     return lens.data_ptr()
@@ -67,12 +71,15 @@ def _launch(name, device, *args):
         raise RuntimeError("%s failed with status %d" % (name, rc))
 
 
-def _workspace(query, a, device):
-    n = _lib.lib().fn[query](ctypes.byref(a))
-    if n:
-        ws = torch.empty(n, dtype=torch.uint8, device=device)
-        a.ws, a.ws_bytes = ws.data_ptr(), n
-        return ws
+def _xattn(query, device, ptrs, strides, sizes, scale, may_need):
+    """sarXattn as bytes, with a workspace where the call needs one -> (bytes, workspace to keep until the launch)."""
+    scale = 1.0 / math.sqrt(sizes[5]) if scale is None else float(scale)
+    a = _XATTN.pack(*ptrs, 0, 0, *strides, *sizes, scale, 0)
+    n = _lib.lib().fn[query](a) if may_need else 0
+    if not n:
+        return a, None
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    return _XATTN.pack(*ptrs, ws.data_ptr(), n, *strides, *sizes, scale, 0), ws
 
 
 def _result(name, t, shape, dtype, device):
@@ -108,12 +115,11 @@ def cross_attention(q, k, v, k_lens=None, q_lens=None, scale=None, return_lse=Fa
         lse = _result("lse", lse, (B, Hq, Tq), torch.float32, q.device)
     kl, ql = _lens("k_lens", k_lens, B, q.device), _lens("q_lens", q_lens, B, q.device)
     if out.numel():
-        kv = (k.data_ptr(), v.data_ptr()) if Tk else (q.data_ptr(), q.data_ptr())                # (no frames: never read)
-        a = Xattn(q.data_ptr(), kv[0], kv[1], None, out.data_ptr(), None if lse is None else lse.data_ptr(), None, None, None, kl, ql, None, 0,
-                  *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], 0, 0, 0, B, Tq, Tk, Hq, Hkv, D,
-                  1.0 / math.sqrt(D) if scale is None else float(scale), 0)
-        ws = _workspace("sar_xattn_fwd_workspace_bytes", a, q.device) if Tk > 256 else None      # noqa: F841  (alive until launched; sarnet.h: 256 keys never need one)
-        _launch("sar_xattn_fwd_" + _SFX[q.dtype], q.device, ctypes.byref(a))
+        qp = q.data_ptr()
+        ptrs = (qp, k.data_ptr() if Tk else qp, v.data_ptr() if Tk else qp, 0, out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, kl, ql)      # (no frames: never read)
+        a, ws = _xattn("sar_xattn_fwd_workspace_bytes", q.device, ptrs, q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + out.stride()[:3] + (0, 0, 0),
+                       (B, Tq, Tk, Hq, Hkv, D), scale, Tk > 256)       # (sarnet.h: 256 keys never need one)
+        _launch("sar_xattn_fwd_" + _SFX[q.dtype], q.device, a)
     return (out, lse) if return_lse else out
 
 
@@ -135,12 +141,12 @@ def cross_attention_grad(dout, q, k, v, out, lse, k_lens=None, q_lens=None, scal
     if Tq == 0:
         dk.zero_(); dv.zero_()
     elif q.numel():
-        kv = (k.data_ptr(), v.data_ptr(), dk.data_ptr(), dv.data_ptr()) if Tk else (q.data_ptr(),) * 4                # (no frames: never read or written)
-        a = Xattn(q.data_ptr(), kv[0], kv[1], dout.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), kv[2], kv[3], kl, ql, None, 0,
-                  *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *dout.stride()[:3], B, Tq, Tk, Hq, Hkv, D,
-                  1.0 / math.sqrt(D) if scale is None else float(scale), 0)
-        ws = _workspace("sar_xattn_bwd_workspace_bytes", a, q.device)                            # noqa: F841
-        _launch("sar_xattn_bwd_" + _SFX[q.dtype], q.device, ctypes.byref(a))
+        qp = q.data_ptr()
+        ptrs = (qp, k.data_ptr() if Tk else qp, v.data_ptr() if Tk else qp, dout.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(),
+                dk.data_ptr() if Tk else qp, dv.data_ptr() if Tk else qp, kl, ql)                # (no frames: never read or written)
+        a, ws = _xattn("sar_xattn_bwd_workspace_bytes", q.device, ptrs, q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + out.stride()[:3] + dout.stride()[:3],
+                       (B, Tq, Tk, Hq, Hkv, D), scale, True)
+        _launch("sar_xattn_bwd_" + _SFX[q.dtype], q.device, a)
     return dq, dk, dv
 
 
@@ -191,10 +197,8 @@ class EncoderCache8:
         _heads(Hq, self.heads, D)
         out = _result("out", out, q.shape, q.dtype, q.device)
         if out.numel():
-            a = Xattn(q.data_ptr(), None, None, None, out.data_ptr(), None, None, None, None, self.lens.data_ptr(), _lens("q_lens", q_lens, B, q.device), None, 0,
-                      *q.stride()[:3], 0, 0, 0, 0, 0, 0, *out.stride()[:3], 0, 0, 0, B, Tq, self.frames, Hq, self.heads, D,
-                      1.0 / math.sqrt(D) if scale is None else float(scale), 0)
-            ws = _workspace("sar_kv8_attend_workspace_bytes", a, q.device) if self.frames > 256 else None       # noqa: F841
-            _launch("sar_kv8_attend_" + _SFX[q.dtype], q.device, ctypes.byref(a), self.k8.data_ptr(), self.k_scale.data_ptr(), self.v8.data_ptr(),
-                    self.v_scale.data_ptr(), self.k8.shape[2])
+            ptrs = (q.data_ptr(), 0, 0, 0, out.data_ptr(), 0, 0, 0, 0, self.lens.data_ptr(), _lens("q_lens", q_lens, B, q.device))
+            a, ws = _xattn("sar_kv8_attend_workspace_bytes", q.device, ptrs, q.stride()[:3] + (0,) * 6 + out.stride()[:3] + (0, 0, 0),
+                           (B, Tq, self.frames, Hq, self.heads, D), scale, self.frames > 256)
+            _launch("sar_kv8_attend_" + _SFX[q.dtype], q.device, a, self.k8.data_ptr(), self.k_scale.data_ptr(), self.v8.data_ptr(), self.v_scale.data_ptr(), self.k8.shape[2])
         return out

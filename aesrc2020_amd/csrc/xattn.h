@@ -67,6 +67,8 @@ static inline int key_splits(const sarXattn* a, int rows_per_block, int blocks) 
     if (s > keys) s = keys;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
+// a few rows: `waves` waves of a block can take eight 32-key tiles each before a second launch (joining slices: 5 us) costs less than going on
+static inline int step_splits(const sarXattn* a, int waves) { return a->Tk <= waves * 256 ? 1 : key_splits(a, 32, 1024); }
 // the forward for many rows: four waves on 128 rows where those blocks fill the chip's 256 CUs twice; else two pairs of waves on 64; the key axis
 // is cut only where even those are fewer than the CUs (partial results cost their writing and reading)
 struct FwdPlan { int waves, splits; };
@@ -75,7 +77,6 @@ static inline FwdPlan fwd_plan(const sarXattn* a) {
     if (R > 64 && (R + 127) / 128 * bh >= 512) return {4, 1};
     return {2, (R + 63) / 64 * bh >= 192 ? 1 : key_splits(a, 64, 384)};
 }
-static inline int step_splits(const sarXattn* a) { return key_splits(a, 32, 1024); }
 static inline size_t part_bytes(const sarXattn* a, int splits) {
     return splits > 1 ? 4 * (size_t)part_floats((long)a->B * a->Hq * a->Tq, a->D, splits) : 0;
 }

@@ -19,7 +19,7 @@ typedef _Float16 elt;
 #define SAR_FN(n) n##_f16
 #endif
 
-int SAR_FN(xattn_step)(const sarXattn* a, int splits, hipStream_t stream);       // xattn_step.hip
+int SAR_FN(xattn_step)(const sarXattn* a, hipStream_t stream);       // xattn_step.hip
 int SAR_FN(xattn_combine)(const sarXattn* a, int splits, hipStream_t stream);
 
 namespace attn {
@@ -389,15 +389,15 @@ template <int DP> static void launch_bwd(const sarXattn& a, float2* stats, hipSt
 }
 
 #if SAR_ELT == 0      // the same for every type
-extern "C" size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, few_rows(a) ? step_splits(a) : fwd_plan(a).splits); }
+extern "C" size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, few_rows(a) ? step_splits(a, a->D <= 32 ? 8 : a->D <= 64 ? 4 : 2) : fwd_plan(a).splits); }   // (the widest type's waves)
 extern "C" size_t sar_xattn_bwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : 8 * (size_t)a->B * a->Hq * a->Tq; }
 #endif
 
 extern "C" int SAR_FN(sar_xattn_fwd)(const sarXattn* a, hipStream_t stream) {
     if (bad(a)) return SAR_EINVAL;
-    if (bad_workspace(a, part_bytes(a, few_rows(a) ? step_splits(a) : fwd_plan(a).splits))) return SAR_EINVAL;
-    if (few_rows(a)) return SAR_FN(xattn_step)(a, step_splits(a), stream);
+    if (few_rows(a)) return SAR_FN(xattn_step)(a, stream);
     const int splits = fwd_plan(a).splits;
+    if (bad_workspace(a, part_bytes(a, splits))) return SAR_EINVAL;
     if (a->D <= 32) launch_fwd<32>(*a, stream);
     else if (a->D <= 64) launch_fwd<64>(*a, stream);
     else if (a->D <= 96) launch_fwd<96>(*a, stream);

@@ -66,8 +66,9 @@ template <typename C, int NPL> __device__ __forceinline__ void pack_planes(f32x1
 }
 
 template <typename T, bool S8, int DP> constexpr int step_pitch() { return S8 ? (DP <= 64 ? 64 : 128) : pitch<T, DP>(); }
-// waves of a block: each has two buffers of a K and a V tile
+// waves of a block: each has two buffers of a K and a V tile (128 KB of LDS at most); narrow rows leave room for eight
 template <typename T, bool S8, int DP> constexpr int step_waves() { return step_pitch<T, S8, DP>() <= 256 ? 4 : 2; }
+template <typename T, bool S8, int DP> constexpr int most_waves() { return step_pitch<T, S8, DP>() <= 128 ? 8 : step_waves<T, S8, DP>(); }
 
 template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_bounds__(64 * NW, 2) void xattn_step_kernel(sarXattn a, Kv8 kv, int row_tiles, int splits) {
     constexpr int P = step_pitch<T, S8, DP>(), ND = DP / 32, NPL = S8 && sizeof(T) == 4 ? 3 : 1, TILE = 32 * P;
@@ -335,20 +336,32 @@ template <typename T> __global__ __launch_bounds__(256) void kv8_store_kernel(Kv
 }  // namespace attn
 using namespace attn;
 
-template <typename C, bool S8, int DP> static int launch_step(const sarXattn& a, const Kv8& kv, int splits, hipStream_t st) {
-    constexpr int NW = step_waves<elt, S8, DP>();
+int SAR_FN(xattn_combine)(const sarXattn* a, int splits, hipStream_t stream);
+
+template <typename C, bool S8, int DP, int NW> static int launch_waves(const sarXattn& a, const Kv8& kv, int splits, hipStream_t st) {
     const long R = (long)a.Tq * (a.Hq / a.Hkv);
     const int rt = cdiv(R, 32);
     const size_t tiles = (size_t)NW * 4 * 32 * step_pitch<elt, S8, DP>(), join = (size_t)NW * (R < 32 ? R : 32) * DP * 4, lds = tiles > join ? tiles : join;
     auto* k = &xattn_step_kernel<elt, C, S8, DP, NW>;
     static PerDeviceFlag raised;
     if (lds > 64 * 1024 && !raised) {
-        if (hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 2048) != hipSuccess) return SAR_ELAUNCH;
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 4096) != hipSuccess) return SAR_ELAUNCH;
         raised = true;
     }
     hipLaunchKernelGGL(k, dim3((unsigned)xcd_grid((long)rt * splits * a.B * a.Hkv)), dim3(64 * NW), lds, st, a, kv, rt, splits);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
+}
+// without key slices, the wider block where the keys are many for four waves
+template <typename C, bool S8, int DP> static int launch_step(const sarXattn& a, const Kv8& kv, hipStream_t st) {
+    constexpr int NW = step_waves<elt, S8, DP>(), MW = most_waves<elt, S8, DP>();
+    const int splits = step_splits(&a, MW);
+    if (bad_workspace(&a, part_bytes(&a, splits))) return SAR_EINVAL;
+    if constexpr (MW > NW) {
+        if (splits == 1 && a.Tk > 256) return launch_waves<C, S8, DP, MW>(a, kv, 1, st);
+    }
+    const int rc = launch_waves<C, S8, DP, NW>(a, kv, splits, st);
+    return rc == SAR_OK && splits > 1 ? SAR_FN(xattn_combine)(&a, splits, st) : rc;
 }
 
 int SAR_FN(xattn_combine)(const sarXattn* a, int splits, hipStream_t stream) {
@@ -357,24 +370,22 @@ int SAR_FN(xattn_combine)(const sarXattn* a, int splits, hipStream_t stream) {
     return SAR_OK;
 }
 
-template <typename C, bool S8> static int step(const sarXattn* a, const Kv8& kv, int splits, hipStream_t stream) {
-    const int rc = a->D <= 32 ? launch_step<C, S8, 32>(*a, kv, splits, stream) : a->D <= 64 ? launch_step<C, S8, 64>(*a, kv, splits, stream)
-                 : a->D <= 96 ? launch_step<C, S8, 96>(*a, kv, splits, stream) : launch_step<C, S8, 128>(*a, kv, splits, stream);
-    return rc == SAR_OK && splits > 1 ? SAR_FN(xattn_combine)(a, splits, stream) : rc;
+template <typename C, bool S8> static int step(const sarXattn* a, const Kv8& kv, hipStream_t stream) {
+    return a->D <= 32 ? launch_step<C, S8, 32>(*a, kv, stream) : a->D <= 64 ? launch_step<C, S8, 64>(*a, kv, stream)
+         : a->D <= 96 ? launch_step<C, S8, 96>(*a, kv, stream) : launch_step<C, S8, 128>(*a, kv, stream);
 }
-int SAR_FN(xattn_step)(const sarXattn* a, int splits, hipStream_t stream) { return step<elt, false>(a, Kv8{}, splits, stream); }
+int SAR_FN(xattn_step)(const sarXattn* a, hipStream_t stream) { return step<elt, false>(a, Kv8{}, stream); }
 
 // ---- the 8-bit cache
 static bool bad8(const sarXattn* a, long frames) { return bad_shape(a) || frames < a->Tk || frames % KV_BLOCK || frames > (1L << 30); }
 #if SAR_ELT == 0      // the same for every type
-extern "C" size_t sar_kv8_attend_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, step_splits(a)); }
+extern "C" size_t sar_kv8_attend_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, step_splits(a, 8)); }   // (its rows are at most 128 bytes: eight waves)
 #endif
 extern "C" int SAR_FN(sar_kv8_attend)(const sarXattn* a, const void* k8, const float* k_scale, const void* v8, const float* v_scale, long frames, hipStream_t stream) {
     if (bad8(a, frames) || bad_strides(sizeof(elt), &a->q_sb, 3) || bad_strides(sizeof(elt), &a->o_sb, 3) || !a->q || !a->out || !k8 || !v8 || !k_scale || !v_scale) return SAR_EINVAL;
     for (const void* p : {a->q, (const void*)a->out, k8, v8})
         if ((uintptr_t)p % 16) return SAR_EINVAL;
-    if (bad_workspace(a, part_bytes(a, step_splits(a)))) return SAR_EINVAL;
-    return step<wide8, true>(a, Kv8{(const unsigned char*)k8, (const unsigned char*)v8, k_scale, v_scale, frames}, step_splits(a), stream);
+    return step<wide8, true>(a, Kv8{(const unsigned char*)k8, (const unsigned char*)v8, k_scale, v_scale, frames}, stream);
 }
 extern "C" int SAR_FN(sar_kv8_store)(const void* k, long k_sb, long k_st, long k_sh, const void* v, long v_sb, long v_st, long v_sh, const int* lens, void* k8, float* k_scale,
                                      void* v8, float* v_scale, int* lens_out, int B, int T, int H, int D, long frames, int first, hipStream_t stream) {
