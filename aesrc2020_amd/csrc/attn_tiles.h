@@ -189,10 +189,11 @@ template <int PITCH> struct WaveLoader {
 
 // blockIdx -> work item such that consecutive items (which share keys and values) land on ONE of the eight XCDs, whose L2 then holds them;
 // the grid is rounded up to a multiple of 8, surplus blocks get -1
-__device__ __forceinline__ int xcd_item(int n) {
-    const int per = (n + 7) >> 3, at = blockIdx.x >> 3, i = (int)(blockIdx.x & 7) * per + at;
+__device__ __forceinline__ int xcd_item(int n, int block) {
+    const int per = (n + 7) >> 3, at = block >> 3, i = (block & 7) * per + at;
     return at < per && i < n ? i : -1;
 }
+__device__ __forceinline__ int xcd_item(int n) { return xcd_item(n, blockIdx.x); }
 static inline long xcd_grid(long n) { return ((n + 7) >> 3) << 3; }
 
 }  // namespace attn

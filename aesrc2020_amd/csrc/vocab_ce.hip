@@ -157,19 +157,25 @@ template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_
 struct Side { const void* p; long plane, ld; int len, k; };
 
 // an operand's LDS tile of one stage: ROWS of the output's side, BK of the contraction; everything outside the tensor arrives as zeros
-template <typename OP, int BK, int ROWS, bool DOWN> struct Operand {
+// TAIL: the contraction may end inside a step (64 x 64 tiles; the larger ones' loads are 3 % slower with it and take packed operands instead)
+template <typename OP, int BK, int ROWS, bool DOWN, bool TAIL> struct Operand {
     static constexpr int P = DOWN ? ROWS * 2 : BK * 2, LINES = DOWN ? BK : ROWS, BYTES = ROWS * BK * 2, N = attn::TileLoader<P, LINES>::N;
     attn::TileLoader<P, LINES> loader;
+    unsigned tail;                               // the loader's offsets for the last, shorter step along the contraction
     const OP* base;
     long ld;
-    int lines;
+    int lines, last;
     unsigned useful;
     __device__ __forceinline__ Operand(const Side& s, int i0)
-        : loader((unsigned)(s.ld * 2), DOWN ? (unsigned)min(ROWS, s.len - i0) * 2 : BK * 2), base(reinterpret_cast<const OP*>(s.p) + (DOWN ? i0 : i0 * s.ld)), ld(s.ld),
-          lines(DOWN ? s.k : s.len - i0), useful(DOWN ? (unsigned)min(ROWS, s.len - i0) * 2 : BK * 2) {}
-    __device__ __forceinline__ void load(int k, long plane, char* to, int wave) const {
+        : loader((unsigned)(s.ld * 2), DOWN ? (unsigned)min(ROWS, s.len - i0) * 2 : BK * 2), tail(attn::TileLoader<P, LINES>((unsigned)(s.ld * 2), DOWN ? 0 : (unsigned)(s.k % BK) * 2).first),
+          base(reinterpret_cast<const OP*>(s.p) + (DOWN ? i0 : i0 * s.ld)), ld(s.ld), lines(DOWN ? s.k : s.len - i0), last(DOWN ? 1 << 30 : s.k - BK),
+          useful(DOWN ? (unsigned)min(ROWS, s.len - i0) * 2 : BK * 2) {}
+    __device__ __forceinline__ void load(int k, long plane, char* to, int wave) {
         const OP* p = base + plane + (DOWN ? k * ld : k);
-        loader.load(p, DOWN ? lines - k : lines, (unsigned)(ld * 2), useful, to, wave);
+        if constexpr (TAIL && !DOWN) {
+            if (k > last) loader.first = tail;                    // (what lies behind is the next row; k only grows)
+            loader.load(p, k < last + BK ? lines : 0, (unsigned)(ld * 2), k <= last ? useful : (unsigned)(last + BK - k) * 2, to, wave);
+        } else loader.load(p, DOWN ? lines - k : lines, (unsigned)(ld * 2), useful, to, wave);
     }
     // operand fragment: 32 rows at i0, sixteen contraction elements at 16 s
     static __device__ __forceinline__ u32x4 fragment(const char* tile, int i0, int s, int lane) {
@@ -182,7 +188,7 @@ template <typename OP, int BK, int ROWS, bool DOWN> struct Operand {
 };
 
 // what happens to a finished tile: C (m, n), column n = lane % 32 of a 32 x 32 tile
-enum { E_LSE, E_DZ, E_OUT, E_PART };
+enum { E_LSE, E_DZ, E_GRAD };
 struct Epi {
     const float* parts;                          // maxima: x, W, dloss
     const elt* bias;
@@ -191,9 +197,9 @@ struct Epi {
     float *pm, *pl, *zl;                         // E_LSE: (m tiles, Rp) maxima and sums, label logits
     bwd16* dz; long dz_plane; int dz_ld;         // E_DZ
     float* db;                                   // E_DZ: (n tiles, dz_ld) column sums, or NULL
-    void* out; long ldo; int accumulate;         // E_OUT: elements of elt; E_PART: fp32 (slice, m, n)
+    void* out; long ldo; int accumulate;         // E_GRAD: elements of elt, or, with `part`, fp32 (slice, m, n)
     long slice;
-    int R, V, v0, Rp, label_bytes, with_w;       // with_w: dz W^T (dx), else x^T dz (dW)
+    int R, V, v0, Rp, label_bytes, part, with_w, pad_;      // with_w: dz W^T (dx), else x^T dz (dW)
 };
 __device__ __forceinline__ long label_of(const Epi& e, int r) {
     return e.label_bytes == 8 ? (long)reinterpret_cast<const long long*>(e.labels)[r] : (long)reinterpret_cast<const int*>(e.labels)[r];
@@ -202,13 +208,33 @@ __device__ __forceinline__ long label_of(const Epi& e, int r) {
 // C = A B^T over k, four waves as 2 x 2, each MT x NT tiles of 32 x 32.  ST stages of LDS, loads ST - 1 steps ahead.
 // What bounds it: the LDS reads of 64 x 64 per wave (four 16-byte fragments for four matrix instructions) plus the stages' writes come to 1.5 times the
 // matrix instructions' cycles at the peak rate; several blocks per CU keep both busy.
-template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> __global__ __launch_bounds__(256, (NPL == 1 && BK == 32 ? 3 : 2)) void product_kernel(Side A, Side B, Epi e, int mtiles, int ntiles, int ksteps, int slices) {
-    constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * 2, SB = BN * BK * 2, STAGE = NPL * (SA + SB), ST = 49152 / STAGE < 4 ? (49152 / STAGE > 2 ? 49152 / STAGE : 2) : 4;
-    typedef Operand<OP, BK, BM, AD> OA;
-    typedef Operand<OP, BK, BN, BD> OB;
+struct Job { Side A, B; Epi e; int mtiles, ntiles, ksteps, slices; };
+template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> struct Product {
+    static constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * 2, SB = BN * BK * 2, STAGE = NPL * (SA + SB), ST = 49152 / STAGE < 4 ? (49152 / STAGE > 2 ? 49152 / STAGE : 2) : 4;
+    static constexpr int LDS = ST * STAGE;
+    static __device__ __forceinline__ void run(char* lds, int block, const Job& job);
+};
+template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> __global__ __launch_bounds__(256, (NPL == 1 && BK == 32 ? 3 : 2)) void product_kernel(Job job) {
+    typedef Product<OP, BK, MT, NT, AD, BD, EPI, SCALED> P;
+    __shared__ __attribute__((aligned(1024))) char lds[P::LDS];
+    P::run(lds, blockIdx.x, job);
+}
+// dW and dx of a piece in one launch, 64 x 64 tiles: neither fills the chip by itself
+template <typename OP, int BKW, int BKX, bool SCALED> __global__ __launch_bounds__(256, 2) void grads_kernel(Job dw, Job dx, int first) {
+    typedef Product<OP, BKW, 1, 1, true, true, E_GRAD, SCALED> W;
+    typedef Product<OP, BKX, 1, 1, false, false, E_GRAD, SCALED> X;
+    __shared__ __attribute__((aligned(1024))) char lds[W::LDS > X::LDS ? W::LDS : X::LDS];
+    if ((int)blockIdx.x < first) W::run(lds, blockIdx.x, dw);
+    else X::run(lds, blockIdx.x - first, dx);
+}
+template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED>::run(char* lds, int block, const Job& job) {
+    const Side &A = job.A, &B = job.B;
+    const Epi& e = job.e;
+    const int mtiles = job.mtiles, ntiles = job.ntiles, ksteps = job.ksteps, slices = job.slices;
+    typedef Operand<OP, BK, BM, AD, MT == 1> OA;
+    typedef Operand<OP, BK, BN, BD, MT == 1> OB;
     constexpr int LOADS = NPL * (OA::N + OB::N);
-    __shared__ __attribute__((aligned(1024))) char lds[ST * STAGE];
-    const int item = attn::xcd_item(mtiles * ntiles * slices);
+    const int item = attn::xcd_item(mtiles * ntiles * slices, block);
     if (item < 0) return;
     // eight m tiles by all n tiles, m fastest: the tiles in flight on an XCD share both operands in its L2
     const int sl = item / (mtiles * ntiles), tile = item - sl * mtiles * ntiles, band = tile / (8 * ntiles), high = min(8, mtiles - 8 * band);
@@ -223,8 +249,8 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.f;
-    const OA oa(A, m0);
-    const OB ob(B, n0);
+    OA oa(A, m0);
+    OB ob(B, n0);
     const auto load = [&](int s, char* to) {
         const int k = (k_lo + s) * BK;
 #pragma unroll
@@ -405,26 +431,27 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
         int ex = g_exp(max_of(e.parts + 2 * PARTS)) - DZ_BITS;
         if constexpr (SCALED) ex -= up_exp(max_of(e.with_w ? e.parts + PARTS : e.parts));
         const float f = ldexpf(1.f, ex);
+        // every row and column that exists (R, V)
+        const auto each = [&](auto&& put) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int n = n0 + nw + 32 * j + (lane & 31);
-            if (n >= e.V) continue;                               // (V, R: the columns and rows that exist)
+            for (int j = 0; j < NT; ++j) {
+                const int n = n0 + nw + 32 * j + (lane & 31);
+                if (n >= e.V) continue;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const int m = m0 + mw + 32 * i + 8 * (x >> 2) + 4 * h + (x & 3);
-                    if (m >= e.R) continue;
-                    const float v = acc[i][j][x] * f;
-                    if constexpr (EPI == E_OUT) {
-                        elt* o = reinterpret_cast<elt*>(e.out) + m * e.ldo + n;
-                        *o = (elt)(e.accumulate ? (float)*o + v : v);
-                    } else {
-                        float* o = reinterpret_cast<float*>(e.out) + sl * e.slice + m * e.ldo + n;
-                        *o = e.accumulate ? *o + v : v;
+                    for (int x = 0; x < 16; ++x) {
+                        const int m = m0 + mw + 32 * i + 8 * (x >> 2) + 4 * h + (x & 3);
+                        if (m < e.R) put(m * e.ldo + n, acc[i][j][x] * f);
                     }
-                }
-        }
+            }
+        };
+        float* po = reinterpret_cast<float*>(e.out) + sl * e.slice;
+        elt* eo = reinterpret_cast<elt*>(e.out);
+        if (e.part && e.accumulate) each([&](long at, float v) { po[at] += v; });
+        else if (e.part) each([&](long at, float v) { po[at] = v; });
+        else if (e.accumulate) each([&](long at, float v) { eo[at] = (elt)((float)eo[at] + v); });
+        else each([&](long at, float v) { eo[at] = (elt)v; });
     }
 }
 
@@ -516,20 +543,10 @@ static bool bad(const sarVocabCe* a) {
 static Plan plan(const sarVocabCe* a, bool grad) {
     Plan p = {};
     p.Rp = up64(a->R); p.Dp = up64(a->D); p.Vp = up64(a->V);
-    // operands are read where they lie when they have the products' type, their rows are 16-byte aligned and no row ends inside a contraction step
-    const bool scaled = grad ? BWD_SCALED : FWD_SCALED;
-    p.pack_x = scaled || a->D % 64 || a->ldx % 8 || (uintptr_t)a->x % 16;
-    p.pack_w = scaled || a->V % 64 || a->ldk % 8 || (uintptr_t)a->kernel % 16;
-    size_t at = 0;
-    const auto take = [&](size_t n) { const size_t o = at; at += up(n); return o; };
-    p.parts = take(3 * PARTS * 4);
-    if (p.pack_x) p.xo = take((size_t)a->R * p.Dp * 2 * NPL);
-    if (p.pack_w) p.wo = take((size_t)a->D * p.Vp * 2 * NPL);
+    int cols = p.Vp;
     if (!grad) {
         p.small_z = small(a->V, a->R);
         p.lse_slices = cdiv(a->V, p.small_z ? 64 : 128);
-        p.a = take((size_t)p.lse_slices * p.Rp * 4); p.b = take((size_t)p.lse_slices * p.Rp * 4);
-        p.zl = take((size_t)p.Rp * 4);
     } else {
         // a piece's dz: about 128 MB, which the 256 MB last-level cache holds between its writer and its two readers
         long w = (128L << 20) / ((long)p.Rp * 2 * NPL) / 256 * 256;
@@ -537,12 +554,27 @@ static Plan plan(const sarVocabCe* a, bool grad) {
         p.pieces = cdiv(a->V, w);
         p.piece = (int)(p.pieces == 1 ? p.Vp : cdiv(cdiv(a->V, p.pieces), 256) * 256L);
         p.pieces = cdiv(a->V, p.piece);
-        const int cols = p.piece < p.Vp ? p.piece : p.Vp;
+        cols = p.piece < p.Vp ? p.piece : p.Vp;
         p.small_z = small(cols, p.Rp); p.small_dx = small(a->R, a->D); p.small_dw = small(a->D, cols);
         p.dx_slices = cut(tiles(a->R, a->D, p.small_dx ? 64 : 128), cols / 32);
         p.dw_slices = cut(tiles(a->D, cols, p.small_dw ? 64 : 128), p.Rp / 32);
         p.db_slices = cdiv(p.Rp, p.small_z ? 64 : 128);
         p.dx_parts = p.dx_slices > 1 || p.pieces > 1;
+    }
+    // operands are read where they lie when they have the products' type, their rows start on 4-byte boundaries (what a load into LDS needs) and
+    // end with a whole 16-byte piece, or a whole step (Operand: TAIL), where they are read along the contraction (x, and W for dx)
+    const bool scaled = grad ? BWD_SCALED : FWD_SCALED;
+    p.pack_x = scaled || a->D % (p.small_z ? 8 : 64) || a->ldx % 2 || (uintptr_t)a->x % 4;
+    p.pack_w = scaled || a->V % (!grad ? 2 : p.small_dx ? 8 : 64) || a->ldk % 2 || (uintptr_t)a->kernel % 4;
+    size_t at = 0;
+    const auto take = [&](size_t n) { const size_t o = at; at += up(n); return o; };
+    p.parts = take(3 * PARTS * 4);
+    if (p.pack_x) p.xo = take((size_t)a->R * p.Dp * 2 * NPL);
+    if (p.pack_w) p.wo = take((size_t)a->D * p.Vp * 2 * NPL);
+    if (!grad) {
+        p.a = take((size_t)p.lse_slices * p.Rp * 4); p.b = take((size_t)p.lse_slices * p.Rp * 4);
+        p.zl = take((size_t)p.Rp * 4);
+    } else {
         p.dz = take((size_t)p.Rp * cols * 2 * NPL);
         if (p.dx_parts) p.dxp = take((size_t)p.dx_slices * a->R * a->D * 4);
         if (p.dw_slices > 1) p.dwp = take((size_t)p.dw_slices * a->D * cols * 4);
@@ -579,13 +611,15 @@ template <typename OP, bool SCALED> static void operands(const sarVocabCe* a, co
     if (p.pack_w) pack(w, p.wo, a->D, a->V, p.Vp, parts + PARTS);
     if (n) hipLaunchKernelGGL((pack_kernel<OP, SCALED>), dim3(some_blocks(blocks), n), dim3(256), 0, st, jobs);
 }
-template <typename OP, bool AD, bool BD, int EPI, bool SCALED> static void product(Side A, Side B, const Epi& e, int m, int n, int k, int slices, bool small_tiles, hipStream_t st) {
+template <bool AD, bool BD> static Job job_of(Side A, Side B, const Epi& e, int m, int n, int k, int slices, bool small_tiles) {
+    const int t = small_tiles ? 64 : 128;
+    return {A, B, e, cdiv(m, t), cdiv(n, t), cdiv(k, step_of(AD, BD)), slices};
+}
+static unsigned blocks_of(const Job& j) { return (unsigned)attn::xcd_grid((long)j.mtiles * j.ntiles * j.slices); }
+template <typename OP, bool AD, bool BD, int EPI, bool SCALED> static void product(const Job& j, bool small_tiles, hipStream_t st) {
     constexpr int BK = step_of(AD, BD);
-    const int ksteps = k / BK;
-    const int t = small_tiles ? 64 : 128, mt = cdiv(m, t), nt = cdiv(n, t);
-    const dim3 grid((unsigned)attn::xcd_grid((long)mt * nt * slices));
-    if (small_tiles) hipLaunchKernelGGL((product_kernel<OP, BK, 1, 1, AD, BD, EPI, SCALED>), grid, dim3(256), 0, st, A, B, e, mt, nt, ksteps, slices);
-    else hipLaunchKernelGGL((product_kernel<OP, BK, 2, 2, AD, BD, EPI, SCALED>), grid, dim3(256), 0, st, A, B, e, mt, nt, ksteps, slices);
+    if (small_tiles) hipLaunchKernelGGL((product_kernel<OP, BK, 1, 1, AD, BD, EPI, SCALED>), dim3(blocks_of(j)), dim3(256), 0, st, j);
+    else hipLaunchKernelGGL((product_kernel<OP, BK, 2, 2, AD, BD, EPI, SCALED>), dim3(blocks_of(j)), dim3(256), 0, st, j);
 }
 
 }
@@ -602,13 +636,13 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     Side x, w;
     operands<fwd16, FWD_SCALED>(a, p, false, x, w, st);
     w.len = p.pack_w ? p.Vp : a->V; w.k = a->D;
-    x.len = a->R; x.k = p.Dp;
+    x.len = a->R; x.k = p.pack_x ? p.Dp : a->D;
     Epi e = {};
     e.parts = reinterpret_cast<float*>(ws + p.parts);
     e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = a->labels; e.label_bytes = a->label_bytes;
     e.pm = reinterpret_cast<float*>(ws + p.a); e.pl = reinterpret_cast<float*>(ws + p.b); e.zl = reinterpret_cast<float*>(ws + p.zl);
     e.R = a->R; e.V = a->V; e.Rp = p.Rp;
-    product<fwd16, true, false, E_LSE, FWD_SCALED>(w, x, e, a->V, a->R, p.Dp, 1, p.small_z, st);
+    product<fwd16, true, false, E_LSE, FWD_SCALED>(job_of<true, false>(w, x, e, a->V, a->R, p.Dp, 1, p.small_z), p.small_z, st);
     hipLaunchKernelGGL(finish_kernel, dim3((unsigned)cdiv(a->R, 16)), dim3(256), 0, st, e.pm, e.pl, e.zl, a->labels, a->label_bytes, a->loss, a->lse, a->R, p.Rp, a->V, p.lse_slices);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
@@ -634,8 +668,8 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         e.R = a->R; e.V = a->V; e.v0 = v0; e.Rp = p.Rp;
         Side wz = from(w, v0), xz = x;
         wz.len = (p.pack_w ? p.Vp : a->V) - v0; wz.k = a->D;
-        xz.len = a->R; xz.k = p.Dp;
-        product<bwd16, true, false, E_DZ, BWD_SCALED>(wz, xz, e, ld, p.Rp, p.Dp, 1, p.small_z, st);
+        xz.len = a->R; xz.k = p.pack_x ? p.Dp : a->D;
+        product<bwd16, true, false, E_DZ, BWD_SCALED>(job_of<true, false>(wz, xz, e, ld, p.Rp, p.Dp, 1, p.small_z), p.small_z, st);
         SumJobs sums = {};
         int ns = 0;
         long blocks = 0;
@@ -644,34 +678,36 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
             const long b = rows * cdiv(cols_, 256);
             blocks = b > blocks ? b : blocks;
         };
+        Job dw = {}, dx = {};
         if (a->dkernel) {
             Epi o = e;
-            o.R = a->D; o.V = cols; o.with_w = 0;
+            o.R = a->D; o.V = cols; o.with_w = 0; o.part = p.dw_slices > 1;
             const Side A = {x.p, x.plane, x.ld, p.pack_x ? p.Dp : a->D, a->R}, B = {dz, plane, ld, ld, p.Rp};
             elt* out = reinterpret_cast<elt*>(a->dkernel) + v0;
-            if (p.dw_slices > 1) {
+            if (o.part) {
                 o.out = ws + p.dwp; o.slice = (long)a->D * ld; o.ldo = ld;
-                product<bwd16, true, true, E_PART, BWD_SCALED>(A, B, o, a->D, cols, p.Rp, p.dw_slices, p.small_dw, st);
                 sum(p.dwp, p.dw_slices, o.slice, a->D, cols, ld, out, a->V, a->accumulate);
-            } else {
-                o.out = out; o.ldo = a->V; o.accumulate = a->accumulate;
-                product<bwd16, true, true, E_OUT, BWD_SCALED>(A, B, o, a->D, cols, p.Rp, 1, p.small_dw, st);
-            }
+            } else { o.out = out; o.ldo = a->V; o.accumulate = a->accumulate; }
+            dw = job_of<true, true>(A, B, o, a->D, cols, p.Rp, p.dw_slices, p.small_dw);
         }
-        if (a->dbias) sum(p.dbp, p.db_slices, ld, 1, cols, ld, reinterpret_cast<elt*>(a->dbias) + v0, cols, a->accumulate);
         if (a->dx) {
             Epi o = e;
-            o.R = a->R; o.V = a->D; o.with_w = 1; o.ldo = a->D;
-            const Side A = {dz, plane, ld, p.Rp, ld}, B0 = from(w, v0), B = {B0.p, w.plane, w.ld, a->D, ld};
-            if (p.dx_parts) {
+            o.R = a->R; o.V = a->D; o.with_w = 1; o.ldo = a->D; o.part = p.dx_parts;
+            const Side A = {dz, plane, ld, p.Rp, ld}, B = {from(w, v0).p, w.plane, w.ld, a->D, p.pack_w ? ld : cols};
+            if (o.part) {
                 o.out = ws + p.dxp; o.slice = (long)a->R * a->D; o.accumulate = i > 0;
-                product<bwd16, false, false, E_PART, BWD_SCALED>(A, B, o, a->R, a->D, ld, p.dx_slices, p.small_dx, st);
                 if (i == p.pieces - 1) sum(p.dxp, p.dx_slices, o.slice, a->R, a->D, a->D, reinterpret_cast<elt*>(a->dx), a->D, 0);
-            } else {
-                o.out = a->dx;
-                product<bwd16, false, false, E_OUT, BWD_SCALED>(A, B, o, a->R, a->D, ld, 1, p.small_dx, st);
-            }
+            } else o.out = a->dx;
+            dx = job_of<false, false>(A, B, o, a->R, a->D, ld, p.dx_slices, p.small_dx);
         }
+        if (a->dkernel && a->dx && p.small_dw && p.small_dx) {
+            const unsigned first = blocks_of(dw);
+            hipLaunchKernelGGL((grads_kernel<bwd16, step_of(true, true), step_of(false, false), BWD_SCALED>), dim3(first + blocks_of(dx)), dim3(256), 0, st, dw, dx, (int)first);
+        } else {
+            if (a->dkernel) product<bwd16, true, true, E_GRAD, BWD_SCALED>(dw, p.small_dw, st);
+            if (a->dx) product<bwd16, false, false, E_GRAD, BWD_SCALED>(dx, p.small_dx, st);
+        }
+        if (a->dbias) sum(p.dbp, p.db_slices, ld, 1, cols, ld, reinterpret_cast<elt*>(a->dbias) + v0, cols, a->accumulate);
         if (ns) hipLaunchKernelGGL(sum_slices_kernel, dim3(some_blocks(blocks), ns), dim3(256), 0, st, sums);
     }
     SAR_CHECK_LAUNCH();

@@ -60,11 +60,13 @@ static inline bool wide_rows(int elt_bytes, std::initializer_list<long> strides)
     return false;
 }
 static inline bool few_rows(const sarXattn* a) { return (long)a->Tq * (a->Hq / a->Hkv) <= 32; }
-// key slices: as many as bring the grid to `blocks`, of 256 keys at least, 64 at most (one lane each in the joining kernel)
+// key slices: as many as give every CU a block, of 256 keys at least; more (up to `blocks` blocks, which evens out ragged lengths) only of 1024 keys,
+// eight tiles a wave, below which a block's start costs more than its work; 64 at most (one lane each in the joining kernel)
 static inline int key_splits(const sarXattn* a, int rows_per_block, int blocks) {
-    const long R = (long)a->Tq * (a->Hq / a->Hkv), tiles = (R + rows_per_block - 1) / rows_per_block * a->B * a->Hkv, keys = (a->Tk + 255L) / 256;
-    long s = (blocks + tiles - 1) / tiles;
-    if (s > keys) s = keys;
+    const long R = (long)a->Tq * (a->Hq / a->Hkv), tiles = (R + rows_per_block - 1) / rows_per_block * a->B * a->Hkv;
+    const auto least = [](long x, long y) { return x < y ? x : y; };
+    const long few = least((256 + tiles - 1) / tiles, (a->Tk + 255L) / 256), many = least((blocks + tiles - 1) / tiles, (a->Tk + 1023L) / 1024);
+    const long s = few > many ? few : many;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 // a few rows: `waves` waves of a block can take eight 32-key tiles each before a second launch (joining slices: 5 us) costs less than going on

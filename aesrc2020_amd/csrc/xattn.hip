@@ -177,9 +177,14 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
 
 // ---- dQ (and delta): as the forward, a wave holds 32 rows as columns n, the keys and values stream through LDS.  It also leaves {lse log2 e,
 // delta} of every row in `stats` (B, Hq, Tq, 2) for the dK, dV kernel.
-template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dq_kernel(sarXattn a, float2* __restrict__ stats, int row_tiles) {
+// delta = do . o takes o as the forward rounded it, an error of half a step of |do . o| that is lost among many keys but not among few (bf16, 10
+// keys: the gradients 1.7 times as far from float64 as their own rounding; now 1.4).  SUMMED: a first pass over the keys sums p dp instead, used up to
+// SUMMED_KEYS keys of a 16-bit type.
+constexpr int SUMMED_KEYS = 256;
+template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dq_kernel(sarXattn a, float2* __restrict__ stats, int row_tiles) {
     constexpr int KT = step_rows<T, WN>(), P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, WM = 4 / WN, NS = KT / 32 / WM, TILE = KT * P;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
+    __shared__ float joined[SUMMED ? WM : 1][WN][64];
     const int item = xcd_item(a.B * a.Hkv * row_tiles);
     if (item < 0) return;
     const int rt = item % row_tiles, bh = item / row_tiles, b = bh / a.Hkv, hk = bh % a.Hkv;
@@ -211,14 +216,28 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
 #pragma unroll
             for (int i = 0; i < Num<T>::PER; ++i) dl = fmaf((float)as16<T>(gf[c])[i], (float)as16<T>(of[c])[i], dl);
         dl = half_sum(dl);
-        if (wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
     }
+    const bool summed = SUMMED && len > 0;
+    if (!summed && wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
     f32x16 dq[ND];
     clear(dq);
+    float sum = 0.f;
     int cur = 0;
-    for (int j = 0; j < len; j += KT, cur ^= 2 * TILE) {
+    for (int step = 0, steps = (len + KT - 1) / KT, all = summed ? 2 * steps : steps; step < all; ++step, cur ^= 2 * TILE) {
+        const bool first = summed && step < steps;                // the pass that sums p dp
+        const int j = (step < steps ? step : step - steps) * KT;
         tile_barrier();
-        if (j + KT < len) load(j + KT, lds + (cur ^ (2 * TILE)));
+        if (step + 1 < all) load((step + 1 < steps ? step + 1 : step + 1 - steps) % steps * KT, lds + (cur ^ (2 * TILE)));
+        if (summed && step == steps) {                            // the first pass is over: delta from all keys
+            sum = half_sum(sum);
+            if constexpr (SUMMED && WM > 1) {
+                joined[wm][wn][lane] = sum;
+                __syncthreads();
+                sum = joined[0][wn][lane] + joined[1][wn][lane];
+            }
+            dl = sum;
+            if (wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
+        }
         if (row0 >= rl || (WM > 1 && j + 32 * wm >= len)) continue;
         const char *lk = lds + cur, *lv = lds + cur + TILE;
 #pragma unroll
@@ -237,7 +256,14 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
                 for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], sl, -e);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dp[i] = __builtin_amdgcn_exp2f(s[i]) * (dp[i] - dl);
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]);
+            if (first) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum = fmaf(s[i], dp[i], sum);
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] = s[i] * (dp[i] - dl);
             u32x4 df[4];
             pack<T>(dp, df);
 #pragma unroll
@@ -377,10 +403,15 @@ template <int DP> static void launch_bwd(const sarXattn& a, float2* stats, hipSt
     const bool few_q = paired<DP>() && (R <= 64 || cdiv(R, 128) * bh < 512), few_k = paired<DP>() && (a.Tk <= 64 || cdiv(a.Tk, 128) * bh < 512);
     const int rt = cdiv(R, few_q ? 64 : 128), kt = cdiv(a.Tk, few_k ? 64 : 128);
     const dim3 gq((unsigned)xcd_grid(rt * bh)), gk((unsigned)xcd_grid(kt * bh));
+    const bool summed = sizeof(elt) == 2 && a.Tk <= SUMMED_KEYS;
     if constexpr (paired<DP>()) {
-        if (few_q) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2>), gq, dim3(256), 0, st, a, stats, rt);
+        if (few_q && !summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2, false>), gq, dim3(256), 0, st, a, stats, rt);
     }
-    if (!few_q) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4>), gq, dim3(256), 0, st, a, stats, rt);
+    if (!few_q && !summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4, false>), gq, dim3(256), 0, st, a, stats, rt);
+    if constexpr (sizeof(elt) == 2) {
+        if (few_q && summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2, true>), gq, dim3(256), 0, st, a, stats, rt);
+        if (!few_q && summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4, true>), gq, dim3(256), 0, st, a, stats, rt);
+    }
     if (!kt) return;
     if constexpr (paired<DP>()) {
         if (few_k) hipLaunchKernelGGL((xattn_dkv_kernel<elt, DP, 2>), gk, dim3(256), 0, st, a, stats, kt);

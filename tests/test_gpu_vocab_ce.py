@@ -166,6 +166,33 @@ def test_large_logits_no_labels_and_zero_gradients():
     assert torch.equal(bad[ok], loss[ok]) and (torch.isnan(bad[5]) or lab[5] < 0)
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("R,D,V", [(40, 72, 202), (40, 50, 201), (40, 64, 192), (300, 136, 20010)])
+def test_a_bad_row_stays_alone(R, D, V, dt):
+    """NaN in one row of x (its neighbours end inside a contraction step) and in one column of the kernel: only what reads them is NaN; rows that are
+    4-byte but not 16-byte aligned."""
+    from aesrc2020_amd.losses import vocab_crossentropy, vocab_crossentropy_grad
+    t = DT[dt]
+    x, w, lab, b, dl = make(R, D, V, t, seed=D)
+    loss, lse = vocab_crossentropy(x, w, lab, b, return_lse=True)
+    step = 4 // t.itemsize
+    raw = torch.zeros(x.numel() + step, device="cuda", dtype=t); raw[step:] = x.flatten()
+    rw = torch.zeros(w.numel() + step, device="cuda", dtype=t); rw[step:] = w.flatten()
+    x2, w2 = raw[step:].view(R, D), rw[step:].view(D, V)
+    l2, s2 = vocab_crossentropy(x2, w2, lab, b, return_lse=True)
+    assert torch.equal(l2, loss) and torch.equal(s2, lse)
+    for p, q in zip(vocab_crossentropy_grad(dl, x2, w2, lab, s2, b), vocab_crossentropy_grad(dl, x, w, lab, lse, b)):
+        assert torch.equal(p, q)
+    y = x.clone(); y[20, 0] = math.nan
+    bad = vocab_crossentropy(y, w, lab, b)
+    ok = torch.ones(R, dtype=torch.bool, device="cuda"); ok[20] = False
+    assert torch.equal(bad[ok], loss[ok]) and torch.isnan(bad[20])
+    y = x.clone(); y[20] = 0; y[20, 0] = math.inf                  # its row without a label: nothing of it in the gradients but 0 * inf in dkernel's first row
+    l3 = lab.clone(); l3[20] = -1
+    dx, dw, _ = vocab_crossentropy_grad(dl, y, w, l3, lse, b)
+    assert torch.isfinite(dx).all() and torch.isfinite(dw[1:]).all()
+
+
 def test_accumulate_empty_and_graph():
     from aesrc2020_amd.losses import vocab_crossentropy, vocab_crossentropy_grad
     x, w, lab, b, dl = make(100, 64, 330, torch.float32, seed=4)
