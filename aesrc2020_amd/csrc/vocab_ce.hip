@@ -187,6 +187,9 @@ template <typename OP, int BK, int ROWS, bool DOWN, bool TAIL> struct Operand {
     }
 };
 
+// where the scale of dz comes from: bf16 planes need none; few rows are looked through by every wave, more by a launch of their own
+enum { G_ONE, G_ROWS, G_PARTS };
+constexpr int G_FEW = 1024;
 // what happens to a finished tile: C (m, n), column n = lane % 32 of a 32 x 32 tile
 enum { E_LSE, E_DZ, E_GRAD };
 struct Epi {
@@ -195,11 +198,13 @@ struct Epi {
     const void* labels;
     const float *dloss, *lse;
     float *pm, *pl, *zl;                         // E_LSE: (m tiles, Rp) maxima and sums, label logits
-    bwd16* dz; long dz_plane; int dz_ld;         // E_DZ
+    float *loss, *lse_out;                       // E_LSE, one m tile: the results themselves
+    void* dz; long dz_plane; int dz_ld, g_from;  // E_DZ
     float* db;                                   // E_DZ: (n tiles, dz_ld) column sums, or NULL
+    elt* db_out; int db_accumulate;              // E_DZ, one n tile: the sums themselves
     void* out; long ldo; int accumulate;         // E_GRAD: elements of elt, or, with `part`, fp32 (slice, m, n)
     long slice;
-    int R, V, v0, Rp, label_bytes, part, with_w, pad_;      // with_w: dz W^T (dx), else x^T dz (dW)
+    int R, V, v0, Rp, R_all, label_bytes, part, with_w;      // with_w: dz W^T (dx), else x^T dz (dW)
 };
 __device__ __forceinline__ long label_of(const Epi& e, int r) {
     return e.label_bytes == 8 ? (long)reinterpret_cast<const long long*>(e.labels)[r] : (long)reinterpret_cast<const int*>(e.labels)[r];
@@ -208,32 +213,49 @@ __device__ __forceinline__ long label_of(const Epi& e, int r) {
 // C = A B^T over k, four waves as 2 x 2, each MT x NT tiles of 32 x 32.  ST stages of LDS, loads ST - 1 steps ahead.
 // What bounds it: the LDS reads of 64 x 64 per wave (four 16-byte fragments for four matrix instructions) plus the stages' writes come to 1.5 times the
 // matrix instructions' cycles at the peak rate; several blocks per CU keep both busy.
+// a row's results from its maximum, sum and label logit (all in powers of two)
+__device__ __forceinline__ void finish_row(float* loss, float* lse, int r, float m, float l, float own, long lab, int V) {
+    if (lse) lse[r] = (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (loss) loss[r] = lab >= 0 && lab < V ? (m - own + __builtin_amdgcn_logf(l)) * LN2 : 0.f;
+}
+__device__ __forceinline__ int dz_exp(const Epi& e) {             // dz is held times 2^this
+    if (e.g_from == G_ONE) return DZ_BITS;
+    if (e.g_from == G_PARTS) return DZ_BITS - g_exp(max_of(e.parts + 2 * PARTS));
+    float m = 0.f;
+    for (int r = threadIdx.x & 63; r < e.R_all; r += 64) {
+        const float v = fabsf(e.dloss[r]);
+        if (v < INFINITY) m = fmaxf(m, v);
+    }
+    return DZ_BITS - g_exp(wave_max(m));
+}
+
 struct Job { Side A, B; Epi e; int mtiles, ntiles, ksteps, slices; };
-template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> struct Product {
-    static constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * 2, SB = BN * BK * 2, STAGE = NPL * (SA + SB), ST = 49152 / STAGE < 4 ? (49152 / STAGE > 2 ? 49152 / STAGE : 2) : 4;
+// PA, PB: planes of the operands (1, or 2: hi, lo); PZ: planes of the dz that E_DZ writes
+template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED, int PA, int PB, int PZ> struct Product {
+    static constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * 2, SB = BN * BK * 2, STAGE = PA * SA + PB * SB, ST = 49152 / STAGE < 4 ? (49152 / STAGE > 2 ? 49152 / STAGE : 2) : 4;
     static constexpr int LDS = ST * STAGE;
     static __device__ __forceinline__ void run(char* lds, int block, const Job& job);
 };
-template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> __global__ __launch_bounds__(256, (NPL == 1 && BK == 32 ? 3 : 2)) void product_kernel(Job job) {
-    typedef Product<OP, BK, MT, NT, AD, BD, EPI, SCALED> P;
+template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED, int PA, int PB, int PZ> __global__ __launch_bounds__(256, (PA * PB == 1 && BK == 32 ? 3 : 2)) void product_kernel(Job job) {
+    typedef Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA, PB, PZ> P;
     __shared__ __attribute__((aligned(1024))) char lds[P::LDS];
     P::run(lds, blockIdx.x, job);
 }
 // dW and dx of a piece in one launch, 64 x 64 tiles: neither fills the chip by itself
-template <typename OP, int BKW, int BKX, bool SCALED> __global__ __launch_bounds__(256, 2) void grads_kernel(Job dw, Job dx, int first) {
-    typedef Product<OP, BKW, 1, 1, true, true, E_GRAD, SCALED> W;
-    typedef Product<OP, BKX, 1, 1, false, false, E_GRAD, SCALED> X;
+template <typename OP, int BKW, int BKX, bool SCALED, int PO, int PZ> __global__ __launch_bounds__(256, 2) void grads_kernel(Job dw, Job dx, int first) {
+    typedef Product<OP, BKW, 1, 1, true, true, E_GRAD, SCALED, PO, PZ, PZ> W;
+    typedef Product<OP, BKX, 1, 1, false, false, E_GRAD, SCALED, PZ, PO, PZ> X;
     __shared__ __attribute__((aligned(1024))) char lds[W::LDS > X::LDS ? W::LDS : X::LDS];
     if ((int)blockIdx.x < first) W::run(lds, blockIdx.x, dw);
     else X::run(lds, blockIdx.x - first, dx);
 }
-template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED> __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED>::run(char* lds, int block, const Job& job) {
+template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED, int PA, int PB, int PZ> __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA, PB, PZ>::run(char* lds, int block, const Job& job) {
     const Side &A = job.A, &B = job.B;
     const Epi& e = job.e;
     const int mtiles = job.mtiles, ntiles = job.ntiles, ksteps = job.ksteps, slices = job.slices;
     typedef Operand<OP, BK, BM, AD, MT == 1> OA;
     typedef Operand<OP, BK, BN, BD, MT == 1> OB;
-    constexpr int LOADS = NPL * (OA::N + OB::N);
+    constexpr int LOADS = PA * OA::N + PB * OB::N;
     const int item = attn::xcd_item(mtiles * ntiles * slices, block);
     if (item < 0) return;
     // eight m tiles by all n tiles, m fastest: the tiles in flight on an XCD share both operands in its L2
@@ -254,10 +276,9 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
     const auto load = [&](int s, char* to) {
         const int k = (k_lo + s) * BK;
 #pragma unroll
-        for (int p = 0; p < NPL; ++p) {
-            oa.load(k, p * A.plane, to + p * SA, w);
-            ob.load(k, p * B.plane, to + NPL * SA + p * SB, w);
-        }
+        for (int p = 0; p < PA; ++p) oa.load(k, p * A.plane, to + p * SA, w);
+#pragma unroll
+        for (int p = 0; p < PB; ++p) ob.load(k, p * B.plane, to + PA * SA + p * SB, w);
     };
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s)
@@ -267,24 +288,27 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
         if (s + ST - 1 <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * LOADS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (s + ST - 1 < steps) load(s + ST - 1, lds + (cur == 0 ? ST - 1 : cur - 1) * STAGE);
-        const char *ta = lds + cur * STAGE, *tb = ta + NPL * SA;
+        const char *ta = lds + cur * STAGE, *tb = ta + PA * SA;
 #pragma unroll
         for (int q = 0; q < BK / 16; ++q) {
-            u32x4 a[NPL][MT], b[NPL][NT];
+            u32x4 a[PA][MT], b[PB][NT];
 #pragma unroll
-            for (int p = 0; p < NPL; ++p) {
+            for (int p = 0; p < PA; ++p)
 #pragma unroll
                 for (int i = 0; i < MT; ++i) a[p][i] = OA::fragment(ta + p * SA, (wm * MT + i) * 32, q, lane);
 #pragma unroll
-                for (int j = 0; j < NT; ++j) b[p][j] = OB::fragment(tb + p * SB, (wn * NT + j) * 32, q, lane);
-            }
-            // fp32: the small products first
+            for (int p = 0; p < PB; ++p)
 #pragma unroll
-            for (int c = NPL == 2 ? 0 : 2; c < 3; ++c)
+                for (int j = 0; j < NT; ++j) b[p][j] = OB::fragment(tb + p * SB, (wn * NT + j) * 32, q, lane);
+            // the small products first; lo lo is left out
+#pragma unroll
+            for (int c = 0; c < 3; ++c) {
+                if (c == 0 ? PA < 2 : c == 1 ? PB < 2 : false) continue;
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = attn::mma<OP>(a[c == 0 ? NPL - 1 : 0][i], b[c == 1 ? NPL - 1 : 0][j], acc[i][j]);
+                    for (int j = 0; j < NT; ++j) acc[i][j] = attn::mma<OP>(a[c == 0 ? PA - 1 : 0][i], b[c == 1 ? PB - 1 : 0][j], acc[i][j]);
+            }
         }
         cur = cur == ST - 1 ? 0 : cur + 1;
     }
@@ -328,14 +352,21 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
                 if (at == 32 * i + 8 * (x >> 2) + 4 * h + (x & 3)) f(i, x);
     };
     if constexpr (EPI == E_LSE) {                                 // m: vocabulary entries, n: rows of x
-        float* join = reinterpret_cast<float*>(lds);              // (2, BN) maxima and sums of the lower waves
-        float top[NT], l[NT];
+        float* join = reinterpret_cast<float*>(lds);              // (3, BN): maxima, sums and label logits of the lower waves
+        float top[NT], l[NT], own[NT];
         logits(0);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int r = n0 + nw + 32 * j + (lane & 31);
             const long lab = r < e.R ? label_of(e, r) : -1, at = lab - m0 - mw;
-            if (__any(at >= 0 && at < 32 * MT && lab < e.V)) place(lab < e.V ? at : -1, [&](int i, int x) { e.zl[r] = acc[i][j][x]; });
+            own[j] = -INFINITY;                                   // the label's logit, where the wave has it
+            if (__any(at >= 0 && at < 32 * MT && lab < e.V)) {
+                place(lab < e.V ? at : -1, [&](int i, int x) {
+                    own[j] = acc[i][j][x];
+                    if (mtiles > 1) e.zl[r] = own[j];
+                });
+            }
+            own[j] = attn::half_max(own[j]);
             top[j] = -INFINITY;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
@@ -353,18 +384,21 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-            if (wm && h == 0) { join[nw + 32 * j + lane] = top[j]; join[BN + nw + 32 * j + lane] = l[j]; }
+            if (wm && h == 0) { join[nw + 32 * j + lane] = top[j]; join[BN + nw + 32 * j + lane] = l[j]; join[2 * BN + nw + 32 * j + lane] = own[j]; }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int r = n0 + nw + 32 * j + lane;
             if (wm || h || r >= e.Rp) continue;
             const float t2 = join[nw + 32 * j + lane], l2 = join[BN + nw + 32 * j + lane], M = fmaxf(top[j], t2), base = M == -INFINITY ? 0.f : M;
-            e.pm[(long)mt * e.Rp + r] = M;
-            e.pl[(long)mt * e.Rp + r] = l[j] * __builtin_amdgcn_exp2f(top[j] - base) + l2 * __builtin_amdgcn_exp2f(t2 - base);
+            const float L = l[j] * __builtin_amdgcn_exp2f(top[j] - base) + l2 * __builtin_amdgcn_exp2f(t2 - base);
+            if (mtiles > 1) {
+                e.pm[(long)mt * e.Rp + r] = M;
+                e.pl[(long)mt * e.Rp + r] = L;
+            } else if (r < e.R) finish_row(e.loss, e.lse_out, r, M, L, fmaxf(own[j], join[2 * BN + nw + 32 * j + lane]), label_of(e, r), e.V);
         }
     } else if constexpr (EPI == E_DZ) {                           // m: vocabulary entries from v0 on, n: rows of x
-        const float gs = ldexpf(1.f, DZ_BITS - g_exp(max_of(e.parts + 2 * PARTS)));
+        const float gs = ldexpf(1.f, dz_exp(e));
         logits(e.v0);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -387,7 +421,7 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum[k] = 0.f;
 #pragma unroll
-        for (int p = 0; p < NPL; ++p) {
+        for (int p = 0; p < PZ; ++p) {
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < NT; ++j)
@@ -395,26 +429,26 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
                     for (int a = 0; a < 4; ++a) {
-                        typename Num<bwd16>::x4 q;
+                        typename Num<OP>::x4 q;
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            q[x] = (bwd16)acc[i][j][4 * a + x];
-                            if constexpr (NPL == 2) acc[i][j][4 * a + x] -= (float)q[x];
+                            q[x] = (OP)acc[i][j][4 * a + x];
+                            if constexpr (PZ == 2) acc[i][j][4 * a + x] -= (float)q[x];
                         }
                         const int c = mw + 32 * i + 8 * a + 4 * h;
-                        *reinterpret_cast<typename Num<bwd16>::x4*>(lds + chunk_at<BM * 2>(nw + 32 * j + (lane & 31), c >> 3) + (c & 4) * 2) = q;
+                        *reinterpret_cast<typename Num<OP>::x4*>(lds + chunk_at<BM * 2>(nw + 32 * j + (lane & 31), c >> 3) + (c & 4) * 2) = q;
                     }
             __syncthreads();
 #pragma unroll
             for (int t = 0; t < REP; ++t) {
                 const int row = (threadIdx.x + 256 * t) / CH, ch = threadIdx.x % CH, r = n0 + row, c = m0 + ch * 8;
-                const auto q = *reinterpret_cast<const typename Num<bwd16>::x16*>(lds + chunk_at<BM * 2>(row, ch));
-                if (r < e.Rp && c < e.dz_ld) *reinterpret_cast<typename Num<bwd16>::x16*>(e.dz + p * e.dz_plane + (long)r * e.dz_ld + c) = q;
+                const auto q = *reinterpret_cast<const typename Num<OP>::x16*>(lds + chunk_at<BM * 2>(row, ch));
+                if (r < e.Rp && c < e.dz_ld) *reinterpret_cast<typename Num<OP>::x16*>(reinterpret_cast<OP*>(e.dz) + p * e.dz_plane + (long)r * e.dz_ld + c) = q;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) sum[k] += (float)q[k];
             }
         }
-        if (e.db) {
+        if (e.db || e.db_out) {
             float* red = reinterpret_cast<float*>(lds);           // (256 / CH, BM)
             __syncthreads();
 #pragma unroll
@@ -424,11 +458,14 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
                 float v = 0.f;
 #pragma unroll
                 for (int k = 0; k < 256 / CH; ++k) v += red[k * BM + threadIdx.x];
-                e.db[(long)nt * e.dz_ld + m0 + threadIdx.x] = v * (1.f / gs);
+                v *= 1.f / gs;
+                const int c = m0 + threadIdx.x;
+                if (!e.db_out) e.db[(long)nt * e.dz_ld + c] = v;
+                else if (e.v0 + c < e.V) e.db_out[c] = (elt)(e.db_accumulate ? (float)e.db_out[c] + v : v);
             }
         }
     } else {
-        int ex = g_exp(max_of(e.parts + 2 * PARTS)) - DZ_BITS;
+        int ex = -dz_exp(e);
         if constexpr (SCALED) ex -= up_exp(max_of(e.with_w ? e.parts + PARTS : e.parts));
         const float f = ldexpf(1.f, ex);
         // every row and column that exists (R, V)
@@ -482,10 +519,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ p
     if (g || r >= R) return;
 #pragma unroll
     for (int x = 1; x < 16; ++x) join(m, l, sm[x][c], ss[x][c]);
-    const float s = (m + __builtin_amdgcn_logf(l)) * LN2;         // (maxima, sums and label logits are in powers of two)
-    const long lab = label_bytes == 8 ? (long)reinterpret_cast<const long long*>(labels)[r] : (long)reinterpret_cast<const int*>(labels)[r];
-    if (lse) lse[r] = s;
-    if (loss) loss[r] = lab >= 0 && lab < V ? (m - zl[r] + __builtin_amdgcn_logf(l)) * LN2 : 0.f;
+    finish_row(loss, lse, r, m, l, zl[r], label_bytes == 8 ? (long)reinterpret_cast<const long long*>(labels)[r] : (long)reinterpret_cast<const int*>(labels)[r], V);
 }
 
 // out (rows, cols) (+)= sum of the slices, for up to three results (blockIdx.y)
@@ -520,6 +554,8 @@ struct Plan {
     bool pack_x, pack_w;
     int piece, pieces;
     bool small_z, small_dx, small_dw;   // 64 x 64 tiles instead of 128 x 128
+    bool light;                         // bf16, all small: bf16 operands as they are and dz in two bf16 planes -- more products, but neither maxima nor packing
+    int dz_planes, g_from;
     int dx_slices, dw_slices, lse_slices, db_slices;
     bool dx_parts;
     size_t parts, xo, wo, a, b, zl, dz, dxp, dwp, dbp, bytes;      // offsets
@@ -560,10 +596,13 @@ static Plan plan(const sarVocabCe* a, bool grad) {
         p.dw_slices = cut(tiles(a->D, cols, p.small_dw ? 64 : 128), p.Rp / 32);
         p.db_slices = cdiv(p.Rp, p.small_z ? 64 : 128);
         p.dx_parts = p.dx_slices > 1 || p.pieces > 1;
+        p.light = SAR_ELT == 1 && p.small_z && p.small_dx && p.small_dw;
+        p.dz_planes = p.light ? 2 : NPL;
+        p.g_from = p.light ? G_ONE : BWD_SCALED || a->R > G_FEW ? G_PARTS : G_ROWS;
     }
     // operands are read where they lie when they have the products' type, their rows start on 4-byte boundaries (what a load into LDS needs) and
     // end with a whole 16-byte piece, or a whole step (Operand: TAIL), where they are read along the contraction (x, and W for dx)
-    const bool scaled = grad ? BWD_SCALED : FWD_SCALED;
+    const bool scaled = grad ? BWD_SCALED && !p.light : FWD_SCALED;
     p.pack_x = scaled || a->D % (p.small_z ? 8 : 64) || a->ldx % 2 || (uintptr_t)a->x % 4;
     p.pack_w = scaled || a->V % (!grad ? 2 : p.small_dx ? 8 : 64) || a->ldk % 2 || (uintptr_t)a->kernel % 4;
     size_t at = 0;
@@ -575,10 +614,10 @@ static Plan plan(const sarVocabCe* a, bool grad) {
         p.a = take((size_t)p.lse_slices * p.Rp * 4); p.b = take((size_t)p.lse_slices * p.Rp * 4);
         p.zl = take((size_t)p.Rp * 4);
     } else {
-        p.dz = take((size_t)p.Rp * cols * 2 * NPL);
+        p.dz = take((size_t)p.Rp * cols * 2 * p.dz_planes);
         if (p.dx_parts) p.dxp = take((size_t)p.dx_slices * a->R * a->D * 4);
         if (p.dw_slices > 1) p.dwp = take((size_t)p.dw_slices * a->D * cols * 4);
-        if (a->dbias) p.dbp = take((size_t)p.db_slices * cols * 4);
+        if (a->dbias && p.db_slices > 1) p.dbp = take((size_t)p.db_slices * cols * 4);
     }
     p.bytes = at;
     return p;
@@ -587,7 +626,7 @@ static Plan plan(const sarVocabCe* a, bool grad) {
 // contraction elements per LDS stage.  64 (two stages) where an operand is read along the contraction on both sides -- whole 128-byte lines -- or on
 // neither: dx 189 -> 159 us, dW 158 -> 141 us for an 8192 x 8192 piece against 1024; 32 (three stages, three blocks per CU) for the logits:
 // 595 against 614 us for 8192 x 32000 x 1024.  fp32 (two planes): 32.
-constexpr int step_of(bool ad, bool bd) { return NPL == 2 || ad != bd ? 32 : 64; }
+constexpr int step_of(bool ad, bool bd, bool planes = NPL == 2) { return planes || ad != bd ? 32 : 64; }
 static unsigned some_blocks(long n) { return (unsigned)(n < 1 ? 1 : n < 4096 ? n : 4096); }
 // the operands as the products read them
 template <typename OP, bool SCALED> static void operands(const sarVocabCe* a, const Plan& p, bool grad, Side& x, Side& w, hipStream_t st) {
@@ -595,7 +634,7 @@ template <typename OP, bool SCALED> static void operands(const sarVocabCe* a, co
     float* parts = reinterpret_cast<float*>(ws + p.parts);
     const MaxJobs all = {{{a->x, a->R, a->ldx, a->D, 0}, {a->kernel, a->D, a->ldk, a->V, 0}, {a->dloss, 1, a->R, a->R, 1}}}, gradient = {{all.j[2]}};
     if (SCALED) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, grad ? 3 : 2), dim3(1024), 0, st, all, parts);
-    else if (grad) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, 1), dim3(1024), 0, st, gradient, parts + 2 * PARTS);
+    else if (grad && p.g_from == G_PARTS) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, 1), dim3(1024), 0, st, gradient, parts + 2 * PARTS);
     x = {a->x, 0, a->ldx, 0, 0};
     w = {a->kernel, 0, a->ldk, 0, 0};
     PackJobs jobs = {};
@@ -611,15 +650,15 @@ template <typename OP, bool SCALED> static void operands(const sarVocabCe* a, co
     if (p.pack_w) pack(w, p.wo, a->D, a->V, p.Vp, parts + PARTS);
     if (n) hipLaunchKernelGGL((pack_kernel<OP, SCALED>), dim3(some_blocks(blocks), n), dim3(256), 0, st, jobs);
 }
-template <bool AD, bool BD> static Job job_of(Side A, Side B, const Epi& e, int m, int n, int k, int slices, bool small_tiles) {
+static Job job_of(Side A, Side B, const Epi& e, int m, int n, int k, int step, int slices, bool small_tiles) {
     const int t = small_tiles ? 64 : 128;
-    return {A, B, e, cdiv(m, t), cdiv(n, t), cdiv(k, step_of(AD, BD)), slices};
+    return {A, B, e, cdiv(m, t), cdiv(n, t), cdiv(k, step), slices};
 }
 static unsigned blocks_of(const Job& j) { return (unsigned)attn::xcd_grid((long)j.mtiles * j.ntiles * j.slices); }
 template <typename OP, bool AD, bool BD, int EPI, bool SCALED> static void product(const Job& j, bool small_tiles, hipStream_t st) {
     constexpr int BK = step_of(AD, BD);
-    if (small_tiles) hipLaunchKernelGGL((product_kernel<OP, BK, 1, 1, AD, BD, EPI, SCALED>), dim3(blocks_of(j)), dim3(256), 0, st, j);
-    else hipLaunchKernelGGL((product_kernel<OP, BK, 2, 2, AD, BD, EPI, SCALED>), dim3(blocks_of(j)), dim3(256), 0, st, j);
+    if (small_tiles) hipLaunchKernelGGL((product_kernel<OP, BK, 1, 1, AD, BD, EPI, SCALED, NPL, NPL, NPL>), dim3(blocks_of(j)), dim3(256), 0, st, j);
+    else hipLaunchKernelGGL((product_kernel<OP, BK, 2, 2, AD, BD, EPI, SCALED, NPL, NPL, NPL>), dim3(blocks_of(j)), dim3(256), 0, st, j);
 }
 
 }
@@ -642,8 +681,10 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = a->labels; e.label_bytes = a->label_bytes;
     e.pm = reinterpret_cast<float*>(ws + p.a); e.pl = reinterpret_cast<float*>(ws + p.b); e.zl = reinterpret_cast<float*>(ws + p.zl);
     e.R = a->R; e.V = a->V; e.Rp = p.Rp;
-    product<fwd16, true, false, E_LSE, FWD_SCALED>(job_of<true, false>(w, x, e, a->V, a->R, p.Dp, 1, p.small_z), p.small_z, st);
-    hipLaunchKernelGGL(finish_kernel, dim3((unsigned)cdiv(a->R, 16)), dim3(256), 0, st, e.pm, e.pl, e.zl, a->labels, a->label_bytes, a->loss, a->lse, a->R, p.Rp, a->V, p.lse_slices);
+    e.loss = a->loss; e.lse_out = a->lse;
+    const Job z = job_of(w, x, e, a->V, a->R, p.Dp, step_of(true, false), 1, p.small_z);
+    product<fwd16, true, false, E_LSE, FWD_SCALED>(z, p.small_z, st);
+    if (z.mtiles > 1) hipLaunchKernelGGL(finish_kernel, dim3((unsigned)cdiv(a->R, 16)), dim3(256), 0, st, e.pm, e.pl, e.zl, a->labels, a->label_bytes, a->loss, a->lse, a->R, p.Rp, a->V, p.lse_slices);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
 }
@@ -653,9 +694,10 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
     const Plan p = plan(a, true);
     if (a->ws_bytes < 0 || (size_t)a->ws_bytes < p.bytes) return SAR_EINVAL;
     char* ws = reinterpret_cast<char*>(a->ws);
-    bwd16* dz = reinterpret_cast<bwd16*>(ws + p.dz);
+    void* dz = ws + p.dz;
     Side x, w;
-    operands<bwd16, BWD_SCALED>(a, p, true, x, w, st);
+    if (p.light) operands<fwd16, false>(a, p, true, x, w, st);
+    else operands<bwd16, BWD_SCALED>(a, p, true, x, w, st);
     const auto from = [](const Side& s, int v) { Side t = s; t.p = reinterpret_cast<const bwd16*>(s.p) + v; return t; };
     for (int i = 0; i < p.pieces; ++i) {
         const int v0 = i * p.piece, cols = a->V - v0 < p.piece ? a->V - v0 : p.piece, ld = up64(cols);
@@ -664,12 +706,18 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         e.parts = reinterpret_cast<float*>(ws + p.parts);
         e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = a->labels; e.label_bytes = a->label_bytes; e.dloss = a->dloss; e.lse = a->lse;
         e.dz = dz; e.dz_plane = plane; e.dz_ld = ld;
-        e.db = a->dbias ? reinterpret_cast<float*>(ws + p.dbp) : nullptr;
+        if (a->dbias && p.db_slices > 1) e.db = reinterpret_cast<float*>(ws + p.dbp);
+        else if (a->dbias) { e.db_out = reinterpret_cast<elt*>(a->dbias) + v0; e.db_accumulate = a->accumulate; }
+        e.g_from = p.g_from; e.R_all = a->R;
         e.R = a->R; e.V = a->V; e.v0 = v0; e.Rp = p.Rp;
         Side wz = from(w, v0), xz = x;
         wz.len = (p.pack_w ? p.Vp : a->V) - v0; wz.k = a->D;
         xz.len = a->R; xz.k = p.pack_x ? p.Dp : a->D;
-        product<bwd16, true, false, E_DZ, BWD_SCALED>(job_of<true, false>(wz, xz, e, ld, p.Rp, p.Dp, 1, p.small_z), p.small_z, st);
+        const Job z = job_of(wz, xz, e, ld, p.Rp, p.Dp, step_of(true, false), 1, p.small_z);
+        if constexpr (SAR_ELT == 1) {
+            if (p.light) hipLaunchKernelGGL((product_kernel<fwd16, step_of(true, false), 1, 1, true, false, E_DZ, false, 1, 1, 2>), dim3(blocks_of(z)), dim3(256), 0, st, z);
+        }
+        if (!p.light) product<bwd16, true, false, E_DZ, BWD_SCALED>(z, p.small_z, st);
         SumJobs sums = {};
         int ns = 0;
         long blocks = 0;
@@ -688,7 +736,7 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
                 o.out = ws + p.dwp; o.slice = (long)a->D * ld; o.ldo = ld;
                 sum(p.dwp, p.dw_slices, o.slice, a->D, cols, ld, out, a->V, a->accumulate);
             } else { o.out = out; o.ldo = a->V; o.accumulate = a->accumulate; }
-            dw = job_of<true, true>(A, B, o, a->D, cols, p.Rp, p.dw_slices, p.small_dw);
+            dw = job_of(A, B, o, a->D, cols, p.Rp, step_of(true, true, p.dz_planes == 2), p.dw_slices, p.small_dw);
         }
         if (a->dx) {
             Epi o = e;
@@ -698,16 +746,19 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
                 o.out = ws + p.dxp; o.slice = (long)a->R * a->D; o.accumulate = i > 0;
                 if (i == p.pieces - 1) sum(p.dxp, p.dx_slices, o.slice, a->R, a->D, a->D, reinterpret_cast<elt*>(a->dx), a->D, 0);
             } else o.out = a->dx;
-            dx = job_of<false, false>(A, B, o, a->R, a->D, ld, p.dx_slices, p.small_dx);
+            dx = job_of(A, B, o, a->R, a->D, ld, step_of(false, false, p.dz_planes == 2), p.dx_slices, p.small_dx);
         }
-        if (a->dkernel && a->dx && p.small_dw && p.small_dx) {
-            const unsigned first = blocks_of(dw);
-            hipLaunchKernelGGL((grads_kernel<bwd16, step_of(true, true), step_of(false, false), BWD_SCALED>), dim3(first + blocks_of(dx)), dim3(256), 0, st, dw, dx, (int)first);
+        const unsigned first = a->dkernel ? blocks_of(dw) : 0, both = first + (a->dx ? blocks_of(dx) : 0);
+        if (p.light) {
+            if constexpr (SAR_ELT == 1)
+                if (both) hipLaunchKernelGGL((grads_kernel<fwd16, step_of(true, true, true), step_of(false, false, true), false, 1, 2>), dim3(both), dim3(256), 0, st, dw, dx, (int)first);
+        } else if (a->dkernel && a->dx && p.small_dw && p.small_dx) {
+            hipLaunchKernelGGL((grads_kernel<bwd16, step_of(true, true), step_of(false, false), BWD_SCALED, NPL, NPL>), dim3(both), dim3(256), 0, st, dw, dx, (int)first);
         } else {
             if (a->dkernel) product<bwd16, true, true, E_GRAD, BWD_SCALED>(dw, p.small_dw, st);
             if (a->dx) product<bwd16, false, false, E_GRAD, BWD_SCALED>(dx, p.small_dx, st);
         }
-        if (a->dbias) sum(p.dbp, p.db_slices, ld, 1, cols, ld, reinterpret_cast<elt*>(a->dbias) + v0, cols, a->accumulate);
+        if (a->dbias && p.db_slices > 1) sum(p.dbp, p.db_slices, ld, 1, cols, ld, reinterpret_cast<elt*>(a->dbias) + v0, cols, a->accumulate);
         if (ns) hipLaunchKernelGGL(sum_slices_kernel, dim3(some_blocks(blocks), ns), dim3(256), 0, st, sums);
     }
     SAR_CHECK_LAUNCH();

@@ -190,7 +190,8 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
     const int rt = item % row_tiles, bh = item / row_tiles, b = bh / a.Hkv, hk = bh % a.Hkv;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31, wn = w % WN, wm = w / WN;
     const int R = a.Tq * (a.Hq / a.Hkv), row0 = (rt * WN + wn) * 32, r = row0 + n;
-    const int rl = live_rows(a, b), len = rt * 32 * WN < rl ? live_keys(a, b) : 0;
+    // (one key: its probability is 1 whatever the score, so nothing flows to the queries)
+    const int rl = live_rows(a, b), keys = live_keys(a, b), len = rt * 32 * WN < rl && keys > 1 ? keys : 0;
     const Row me = row_of(a, hk, min(r, R - 1));
     const float sl = a.scale * LOG2E;
     const unsigned ks = (unsigned)(a.k_st * sizeof(T)), vs = (unsigned)(a.v_st * sizeof(T)), db = (unsigned)(a.D * sizeof(T));
@@ -342,6 +343,9 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
             for (int x = 0; x < 4; ++x)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) s[4 * x + c] = __builtin_amdgcn_exp2f(fmaf(s[4 * x + c], sl, -st[2 * (8 * x + 4 * h + c)]));
+            if (len == 1)                                         // p = 1 exactly, and ds = 0 below
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = 1.f;
             u32x4 pf[4];
             pack<T>(s, pf);
 #pragma unroll
@@ -352,6 +356,7 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
             for (int x = 0; x < 4; ++x)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) dp[4 * x + c] = s[4 * x + c] * (dp[4 * x + c] - st[2 * (8 * x + 4 * h + c) + 1]);
+            if (len == 1) dp = zero16();
             pack<T>(dp, pf);
 #pragma unroll
             for (int d = 0; d < ND; ++d) dk[d] = mma_down<T, P>(lq, 32 * wm, d, pf, dk[d], lane);

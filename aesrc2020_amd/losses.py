@@ -5,6 +5,7 @@ SphereFace / CosFace / ArcFace keep the reference constructor (n_classes, s, m, 
 glorot_uniform (losses.py:22-26).  circle_loss(y_true, y_pred, gamma, margin) -> per-sample loss (losses.py:157-172).
 """
 import ctypes
+import struct
 
 import torch
 
@@ -152,6 +153,9 @@ class _VocabCe(ctypes.Structure):
                [(n, ctypes.c_long) for n in ("ws_bytes", "ldx", "ldk")] + [(n, ctypes.c_int) for n in ("R", "D", "V", "label_bytes", "accumulate", "pad_")]
 
 
+_VOCAB_CE = struct.Struct("11Q3l6i")                                        # the same fields as bytes
+
+
 def _vocab_args(x, kernel, labels, bias):
     """-> x, kernel (rows contiguous), bias, labels as the kernels take them."""
     if x.dim() != 2 or kernel.dim() != 2 or x.shape[1] != kernel.shape[0] or kernel.shape[1] < 1 or kernel.shape[0] < 1:
@@ -172,20 +176,19 @@ def _vocab_args(x, kernel, labels, bias):
     return x, kernel, bias
 
 
-def _vocab_launch(direction, a, x):
+def _vocab_launch(direction, x, kernel, labels, ptrs, sizes):
+    """ptrs: dloss .. dbias; sizes: R, D, V, bytes of a label, accumulate."""
     name = "sar_vocab_ce_%s_%s" % (direction, _SFX[x.dtype])
-    n = _lib.lib().fn[name + "_workspace_bytes"](ctypes.byref(a))
+    R, D, V = sizes[:3]
+    args = (x.stride(0) if R > 1 else D, kernel.stride(0) if D > 1 else V, *sizes, 0)
+    ptrs = (x.data_ptr(), kernel.data_ptr(), ptrs[0], labels.data_ptr(), *ptrs[1:])
+    n = _lib.lib().fn[name + "_workspace_bytes"](_VOCAB_CE.pack(*ptrs, 0, 0, *args))
     ws = torch.empty(n, dtype=torch.uint8, device=x.device)                  # (torch's blocks are 512-byte aligned)
-    a.ws, a.ws_bytes = ws.data_ptr(), n
-    _launch(name, x.device, ctypes.byref(a))
+    _launch(name, x.device, _VOCAB_CE.pack(*ptrs, ws.data_ptr(), n, *args))
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _rowstride(t, width):
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    return 0 if t is None else t.data_ptr()
 
 
 def vocab_crossentropy(x, kernel, labels, bias=None, return_lse=False, loss=None, lse=None):
@@ -199,8 +202,7 @@ def vocab_crossentropy(x, kernel, labels, bias=None, return_lse=False, loss=None
     if return_lse or lse is not None:
         lse = _result("lse", lse, (R,), torch.float32, x.device)
     if R:
-        _vocab_launch("fwd", _VocabCe(x.data_ptr(), kernel.data_ptr(), _ptr(bias), labels.data_ptr(), None, loss.data_ptr(), _ptr(lse), None, None, None, None, 0,
-                                      _rowstride(x, D), _rowstride(kernel, V), R, D, V, labels.element_size(), 0, 0), x)
+        _vocab_launch("fwd", x, kernel, labels, (_ptr(bias), 0, loss.data_ptr(), _ptr(lse), 0, 0, 0), (R, D, V, labels.element_size(), 0))
     return (loss, lse) if return_lse else loss
 
 
@@ -217,8 +219,8 @@ def vocab_crossentropy_grad(dloss, x, kernel, labels, lse, bias=None, dx=None, d
     dkernel = _result("dkernel", dkernel, (D, V), x.dtype, x.device)
     dbias = None if bias is None else _result("dbias", dbias, (V,), x.dtype, x.device)
     if R:
-        _vocab_launch("bwd", _VocabCe(x.data_ptr(), kernel.data_ptr(), _ptr(bias), labels.data_ptr(), dloss.data_ptr(), None, lse.data_ptr(), _ptr(dx), dkernel.data_ptr(), _ptr(dbias), None, 0,
-                                      _rowstride(x, D), _rowstride(kernel, V), R, D, V, labels.element_size(), 1 if accumulate else 0, 0), x)
+        _vocab_launch("bwd", x, kernel, labels, (_ptr(bias), dloss.data_ptr(), 0, lse.data_ptr(), _ptr(dx), dkernel.data_ptr(), _ptr(dbias)),
+                      (R, D, V, labels.element_size(), 1 if accumulate else 0))
     elif not accumulate:
         dkernel.zero_()
         if dbias is not None:

@@ -131,6 +131,23 @@ def test_forward_and_gradients(shape, dt):
 
 
 @pytest.mark.parametrize("dt", DT)
+def test_one_key_gives_exact_results(dt):
+    """One frame (of one, or of many with a length of 1): its probability is 1, the output is v, nothing flows to q and k, dv sums dout.
+    The forward takes p = exp2(fma(s, f, -m)) and divides by the sum: with one key p = l = 1 + d, d a few 2^-24, and out = fl(fl(p v) fl(1 / l)): three
+    roundings of 2^-24 whatever d is -- fp32 is that near v, and a 16-bit result, whose half step is far wider, is v itself."""
+    A = _att()
+    q, k, v, g = make(2, 70, 40, 4, 2, 48, DT[dt], seed=12)
+    for kk, vv, kl in ((k[:, :1], v[:, :1], None), (k, v, lens(1, 1))):
+        out, lse = A.cross_attention(q, kk, vv, k_lens=kl, return_lse=True)
+        dq, dk, dv = A.cross_attention_grad(g, q, kk, vv, out, lse, k_lens=kl)
+        vv = v[:, :1].repeat_interleave(2, 2).expand(2, 70, 4, 48)
+        assert ((out.double() - vv.double()).abs() <= 3.01 * 2.0 ** -24 * vv.double().abs()).all() if dt == "f32" else torch.equal(out, vv)
+        assert (dq == 0).all() and (dk == 0).all() and (dv[:, 1:] == 0).all()
+        want = g.double().view(2, 70, 2, 2, 48).sum((1, 3))
+        assert ((dv[:, 0].double() - want).abs() <= u(DT[dt]) * want.abs() * 1.01 + 2.0 ** -24 * 140 * g.double().abs().view(2, 70, 2, 2, 48).sum((1, 3))).all()
+
+
+@pytest.mark.parametrize("dt", DT)
 def test_gradients_against_differences(dt):
     """d/dt of sum(out * g) along a direction, by central differences of the float64 forward, against the kernels' gradients."""
     A = _att()

@@ -193,9 +193,10 @@ def test_a_bad_row_stays_alone(R, D, V, dt):
     assert torch.isfinite(dx).all() and torch.isfinite(dw[1:]).all()
 
 
-def test_accumulate_empty_and_graph():
+@pytest.mark.parametrize("R", [20, 100])
+def test_accumulate_empty_and_graph(R):
     from aesrc2020_amd.losses import vocab_crossentropy, vocab_crossentropy_grad
-    x, w, lab, b, dl = make(100, 64, 330, torch.float32, seed=4)
+    x, w, lab, b, dl = make(R, 64, 330, torch.float32, seed=4)
     _, lse = vocab_crossentropy(x, w, lab, b, return_lse=True)
     _, dw, db = vocab_crossentropy_grad(dl, x, w, lab, lse, b)
     aw, ab = torch.ones_like(dw), torch.full_like(db, 2.0)
@@ -211,7 +212,7 @@ def test_accumulate_empty_and_graph():
         l1, s1 = vocab_crossentropy(x, w, lab, b, return_lse=True)
         g1 = vocab_crossentropy_grad(dl, x, w, lab, s1, b)
     for i in range(4):
-        x.copy_(make(100, 64, 330, torch.float32, seed=30 + i)[0]); lab.copy_((lab + 17) % 330)
+        x.copy_(make(R, 64, 330, torch.float32, seed=30 + i)[0]); lab.copy_((lab + 17) % 330)
         gr.replay()
         l2, s2 = vocab_crossentropy(x, w, lab, b, return_lse=True)
         g2 = vocab_crossentropy_grad(dl, x, w, lab, s2, b)
