@@ -79,6 +79,28 @@ static inline FwdPlan fwd_plan(const sarXattn* a) {
     if (R > 64 && (R + 127) / 128 * bh >= 512) return {4, 1};
     return {2, (R + 63) / 64 * bh >= 192 ? 1 : key_splits(a, 64, 384)};
 }
+// The backward: four waves on 128 columns where those blocks fill the chip twice, else two pairs on 64 -- and where 64 are all there are.  Where the
+// blocks are fewer than the CUs, the streamed axis (keys for dQ, the rows of all the group's heads for dK, dV) is cut into slices of eight steps
+// of 64 at least, whose fp32 sums a further launch adds.
+constexpr int SUMMED_KEYS = 256;
+struct BwdPlan { bool few_q, few_k; int dq_slices, dkv_slices; size_t dq_at, dkv_at, bytes; };
+static inline int cut_slices(long blocks, long steps) {
+    const long want = (512 + blocks - 1) / blocks, most = steps / 8;
+    return blocks >= 256 || most < 2 ? 1 : (int)(want < most ? want : most);
+}
+static inline BwdPlan bwd_plan(const sarXattn* a) {
+    BwdPlan p = {};
+    const long R = (long)a->Tq * (a->Hq / a->Hkv), bh = (long)a->B * a->Hkv;
+    p.few_q = R <= 64 || (R + 127) / 128 * bh < 512;
+    p.few_k = a->Tk <= 64 || (a->Tk + 127) / 128 * bh < 512;
+    p.dq_slices = a->Tk <= SUMMED_KEYS ? 1 : cut_slices((R + 63) / 64 * bh, (a->Tk + 63) / 64);
+    p.dkv_slices = cut_slices((a->Tk + 63) / 64 * bh, (a->Tq + 63) / 64 * (long)(a->Hq / a->Hkv));
+    const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    p.dq_at = up(8 * (size_t)a->B * a->Hq * a->Tq);
+    p.dkv_at = p.dq_at + (p.dq_slices > 1 ? up(4 * (size_t)p.dq_slices * a->B * a->Tq * a->Hq * a->D) : 0);
+    p.bytes = p.dkv_at + (p.dkv_slices > 1 ? 8 * (size_t)p.dkv_slices * a->B * a->Tk * a->Hkv * a->D : 0);
+    return p;
+}
 static inline size_t part_bytes(const sarXattn* a, int splits) {
     return splits > 1 ? 4 * (size_t)part_floats((long)a->B * a->Hq * a->Tq, a->D, splits) : 0;
 }

@@ -179,25 +179,25 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
 // delta} of every row in `stats` (B, Hq, Tq, 2) for the dK, dV kernel.
 // delta = do . o takes o as the forward rounded it, an error of half a step of |do . o| that is lost among many keys but not among few (bf16, 10
 // keys: the gradients 1.7 times as far from float64 as their own rounding; now 1.4).  SUMMED: a first pass over the keys sums p dp instead, used up to
-// SUMMED_KEYS keys of a 16-bit type.
-constexpr int SUMMED_KEYS = 256;
-template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dq_kernel(sarXattn a, float2* __restrict__ stats, int row_tiles) {
+// SUMMED_KEYS keys of a 16-bit type (one slice).
+template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dq_kernel(sarXattn a, float2* __restrict__ stats, float* __restrict__ part, int row_tiles, int slices) {
     constexpr int KT = step_rows<T, WN>(), P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, WM = 4 / WN, NS = KT / 32 / WM, TILE = KT * P;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
     __shared__ float joined[SUMMED ? WM : 1][WN][64];
-    const int item = xcd_item(a.B * a.Hkv * row_tiles);
+    const int item = xcd_item(a.B * a.Hkv * slices * row_tiles);
     if (item < 0) return;
-    const int rt = item % row_tiles, bh = item / row_tiles, b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int rt = item % row_tiles, sp = item / row_tiles % slices, bh = item / row_tiles / slices, b = bh / a.Hkv, hk = bh % a.Hkv;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31, wn = w % WN, wm = w / WN;
     const int R = a.Tq * (a.Hq / a.Hkv), row0 = (rt * WN + wn) * 32, r = row0 + n;
     // (one key: its probability is 1 whatever the score, so nothing flows to the queries)
-    const int rl = live_rows(a, b), keys = live_keys(a, b), len = rt * 32 * WN < rl && keys > 1 ? keys : 0;
+    const int rl = live_rows(a, b), keys = live_keys(a, b), all_keys = rt * 32 * WN < rl && keys > 1 ? keys : 0;
+    const int per = ((all_keys + KT - 1) / KT + slices - 1) / slices * KT, k0 = min(sp * per, all_keys), len = min(per, all_keys - k0);      // this slice's keys
     const Row me = row_of(a, hk, min(r, R - 1));
     const float sl = a.scale * LOG2E;
     const unsigned ks = (unsigned)(a.k_st * sizeof(T)), vs = (unsigned)(a.v_st * sizeof(T)), db = (unsigned)(a.D * sizeof(T));
     const TileLoader<P, KT> tk(ks, db), tv(vs, db);
-    const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
-    const T* vb = reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
+    const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh + k0 * a.k_st;
+    const T* vb = reinterpret_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh + k0 * a.v_st;
     const auto load = [&](int j, char* to) {
         tk.load(kb + j * a.k_st, len - j, ks, db, to, w);
         tv.load(vb + j * a.v_st, len - j, vs, db, to + TILE, w);
@@ -219,7 +219,7 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
         dl = half_sum(dl);
     }
     const bool summed = SUMMED && len > 0;
-    if (!summed && wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
+    if (!summed && sp == 0 && wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
     f32x16 dq[ND];
     clear(dq);
     float sum = 0.f;
@@ -281,23 +281,28 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
         if (wm) return;
         add(join, dq, lane);
     }
-    if (r < R) store_column<T, ND>(reinterpret_cast<T*>(a.dq) + (((long)b * a.Tq + me.t) * a.Hq + me.h) * a.D, dq, a.scale, r < rl, a.D, h);
+    if (r >= R) return;
+    const long at = (((long)b * a.Tq + me.t) * a.Hq + me.h) * a.D;
+    if (slices == 1) store_column<T, ND>(reinterpret_cast<T*>(a.dq) + at, dq, a.scale, r < rl, a.D, h);
+    else store_column<float, ND>(part + sp * ((long)a.B * a.Tq * a.Hq * a.D) + at, dq, a.scale, r < rl, a.D, h);
 }
 
 // ---- dK, dV: a wave holds 32 keys as columns n; the rows of one query head after the other stream through LDS
-template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dkv_kernel(sarXattn a, const float2* __restrict__ stats, int key_tiles) {
+template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dkv_kernel(sarXattn a, const float2* __restrict__ stats, float* __restrict__ part, int key_tiles, int slices) {
     constexpr int WM = 4 / WN, RT = 32 * WM, P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, TILE = RT * P, BUF = 2 * TILE;
     __shared__ __attribute__((aligned(1024))) char lds[2 * BUF];                 // Q, dO; two of each
     __shared__ __attribute__((aligned(16))) float2 row_stats[2][RT];
     // 128 wide, both fragments and both sums do not fit 256 registers: the K fragments stay in the wave's own piece of LDS, in lane order
     constexpr bool KL = sizeof(T) == 2 && DP == 128;
     __shared__ __attribute__((aligned(16))) u32x4 k_frags[KL ? 4 : 1][KL ? NC : 1][KL ? 64 : 1];
-    const int item = xcd_item(a.B * a.Hkv * key_tiles);
+    const int item = xcd_item(a.B * a.Hkv * slices * key_tiles);
     if (item < 0) return;
-    const int kt = item % key_tiles, bh = item / key_tiles, b = bh / a.Hkv, hk = bh % a.Hkv, G = a.Hq / a.Hkv;
+    const int kt = item % key_tiles, sp = item / key_tiles % slices, bh = item / key_tiles / slices, b = bh / a.Hkv, hk = bh % a.Hkv, G = a.Hq / a.Hkv;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31, wn = w % WN, wm = w / WN;
     const int len = live_keys(a, b), key0 = (kt * WN + wn) * 32, key = key0 + n;
     const int tl = kt * 32 * WN < len ? live_rows(a, b) / G : 0;                 // tokens
+    // the row tiles of all heads, one after the other, cut into slices
+    const int across = (tl + RT - 1) / RT, tiles = across * G, per = (tiles + slices - 1) / slices, i0 = min(sp * per, tiles), i1 = min(i0 + per, tiles);
     const float sl = a.scale * LOG2E;
     const unsigned qs = (unsigned)(a.q_st * sizeof(T)), gs = (unsigned)(a.g_st * sizeof(T)), db = (unsigned)(a.D * sizeof(T));
     const TileLoader<P, RT> tq(qs, db), tg(gs, db);
@@ -313,9 +318,10 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
         const int i = t + (int)threadIdx.x;
         return threadIdx.x < RT && i < tl ? sb[(long)g * a.Tq + i] : make_float2(0.f, 0.f);
     };
-    if (tl > 0) {
-        load(0, 0, lds);
-        if (threadIdx.x < RT) row_stats[0][threadIdx.x] = load_stats(0, 0);
+    int g = i0 < i1 ? i0 / across : 0, t = i0 < i1 ? (i0 - g * across) * RT : 0;
+    if (i0 < i1) {
+        load(g, t, lds);
+        if (threadIdx.x < RT) row_stats[0][threadIdx.x] = load_stats(g, t);
     }
     u32x4 kf[NC], vf[NC];
     load_row<T, DP>(reinterpret_cast<const T*>(a.k) + b * a.k_sb + min(key, a.Tk - 1) * a.k_st + hk * a.k_sh, key < len, a.D, h, kf);
@@ -326,13 +332,13 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     load_row<T, DP>(reinterpret_cast<const T*>(a.v) + b * a.v_sb + min(key, a.Tk - 1) * a.v_st + hk * a.v_sh, key < len, a.D, h, vf);
     f32x16 dk[ND], dv[ND];
     clear(dk); clear(dv);
-    int g = 0, t = 0, cur = 0, par = 0;
-    while (g < G && tl > 0) {
+    int cur = 0, par = 0;
+    for (int i = i0; i < i1; ++i) {
         tile_barrier();
         int gn = g, tn = t + RT;
         if (tn >= tl) { ++gn; tn = 0; }
         float2 next = make_float2(0.f, 0.f);
-        if (gn < G) { next = load_stats(gn, tn); load(gn, tn, lds + (cur ^ BUF)); }
+        if (i + 1 < i1) { next = load_stats(gn, tn); load(gn, tn, lds + (cur ^ BUF)); }
         if (key0 < len && (WM == 1 || t + 32 * wm < tl)) {
             const char *lq = lds + cur, *lg = lds + cur + TILE;
             const float* st = reinterpret_cast<const float*>(row_stats[par]) + wm * 64;
@@ -376,8 +382,27 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     }
     if (key >= a.Tk) return;
     const long at = (((long)b * a.Tk + key) * a.Hkv + hk) * a.D;  // frames behind the length: their gradient is zero
-    store_column<T, ND>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, key < len, a.D, h);
-    store_column<T, ND>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, key < len, a.D, h);
+    if (slices == 1) {
+        store_column<T, ND>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, key < len, a.D, h);
+        store_column<T, ND>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, key < len, a.D, h);
+    } else {
+        const long n = (long)a.B * a.Tk * a.Hkv * a.D;
+        store_column<float, ND>(part + sp * n + at, dk, a.scale, key < len, a.D, h);
+        store_column<float, ND>(part + (slices + sp) * n + at, dv, 1.f, key < len, a.D, h);
+    }
+}
+
+// the sliced gradients: out = sum over the slices, in their order
+struct SumJob { const float* part; void* out; long n; int slices; };
+struct SumJobs { SumJob j[3]; };
+template <typename T> __global__ __launch_bounds__(256) void xattn_sum_kernel(SumJobs jobs) {
+    const SumJob j = jobs.j[blockIdx.y];
+    for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4; i < j.n; i += (long)gridDim.x * 1024) {
+        f32x4 v = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int s = 0; s < j.slices; ++s) v += *reinterpret_cast<const f32x4*>(j.part + s * j.n + i);
+        store4<T>(reinterpret_cast<T*>(j.out) + i, v[0], v[1], v[2], v[3]);
+    }
 }
 
 }  // namespace attn
@@ -402,31 +427,45 @@ template <int DP> static void launch_fwd(const sarXattn& a, hipStream_t st) {
     }
     if (!two) hipLaunchKernelGGL((xattn_fwd_kernel<elt, DP, 4>), grid, dim3(256), 0, st, a, rt, p.splits);
 }
-template <int DP> static void launch_bwd(const sarXattn& a, float2* stats, hipStream_t st) {
-    const long R = (long)a.Tq * (a.Hq / a.Hkv), bh = (long)a.B * a.Hkv;
-    // four waves on 128 columns where those blocks fill the chip twice, else two pairs on 64 -- and where 64 are all there are
-    const bool few_q = paired<DP>() && (R <= 64 || cdiv(R, 128) * bh < 512), few_k = paired<DP>() && (a.Tk <= 64 || cdiv(a.Tk, 128) * bh < 512);
-    const int rt = cdiv(R, few_q ? 64 : 128), kt = cdiv(a.Tk, few_k ? 64 : 128);
-    const dim3 gq((unsigned)xcd_grid(rt * bh)), gk((unsigned)xcd_grid(kt * bh));
+template <int DP> static void launch_bwd(const sarXattn& a, hipStream_t st) {
+    const BwdPlan p = bwd_plan(&a);
+    const long bh = (long)a.B * a.Hkv, nq = (long)a.B * a.Tq * a.Hq * a.D, nk = (long)a.B * a.Tk * a.Hkv * a.D;
+    float2* stats = reinterpret_cast<float2*>(a.ws);
+    float* pq = reinterpret_cast<float*>(reinterpret_cast<char*>(a.ws) + p.dq_at);
+    float* pk = reinterpret_cast<float*>(reinterpret_cast<char*>(a.ws) + p.dkv_at);
+    const bool few_q = paired<DP>() && p.few_q, few_k = paired<DP>() && p.few_k;
+    const int rt = cdiv((long)a.Tq * (a.Hq / a.Hkv), few_q ? 64 : 128), kt = cdiv(a.Tk, few_k ? 64 : 128);
+    const dim3 gq((unsigned)xcd_grid(rt * bh * p.dq_slices)), gk((unsigned)xcd_grid(kt * bh * p.dkv_slices));
     const bool summed = sizeof(elt) == 2 && a.Tk <= SUMMED_KEYS;
     if constexpr (paired<DP>()) {
-        if (few_q && !summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2, false>), gq, dim3(256), 0, st, a, stats, rt);
+        if (few_q && !summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2, false>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
     }
-    if (!few_q && !summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4, false>), gq, dim3(256), 0, st, a, stats, rt);
+    if (!few_q && !summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4, false>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
     if constexpr (sizeof(elt) == 2) {
-        if (few_q && summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2, true>), gq, dim3(256), 0, st, a, stats, rt);
-        if (!few_q && summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4, true>), gq, dim3(256), 0, st, a, stats, rt);
+        if (few_q && summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2, true>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
+        if (!few_q && summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4, true>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
     }
-    if (!kt) return;
-    if constexpr (paired<DP>()) {
-        if (few_k) hipLaunchKernelGGL((xattn_dkv_kernel<elt, DP, 2>), gk, dim3(256), 0, st, a, stats, kt);
+    if (kt) {
+        if constexpr (paired<DP>()) {
+            if (few_k) hipLaunchKernelGGL((xattn_dkv_kernel<elt, DP, 2>), gk, dim3(256), 0, st, a, stats, pk, kt, p.dkv_slices);
+        }
+        if (!few_k) hipLaunchKernelGGL((xattn_dkv_kernel<elt, DP, 4>), gk, dim3(256), 0, st, a, stats, pk, kt, p.dkv_slices);
     }
-    if (!few_k) hipLaunchKernelGGL((xattn_dkv_kernel<elt, DP, 4>), gk, dim3(256), 0, st, a, stats, kt);
+    SumJobs sums = {};
+    int n = 0;
+    long most = 0;
+    const auto sum = [&](const float* part, void* out, long count, int slices) {
+        sums.j[n++] = {part, out, count, slices};
+        most = count > most ? count : most;
+    };
+    if (p.dq_slices > 1) sum(pq, a.dq, nq, p.dq_slices);
+    if (kt && p.dkv_slices > 1) { sum(pk, a.dk, nk, p.dkv_slices); sum(pk + p.dkv_slices * nk, a.dv, nk, p.dkv_slices); }
+    if (n) hipLaunchKernelGGL((xattn_sum_kernel<elt>), dim3((unsigned)(most < 2048 * 1024 ? cdiv(most, 1024) : 2048), n), dim3(256), 0, st, sums);
 }
 
 #if SAR_ELT == 0      // the same for every type
 extern "C" size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, few_rows(a) ? step_splits(a, a->D <= 32 ? 8 : a->D <= 64 ? 4 : 2) : fwd_plan(a).splits); }   // (the widest type's waves)
-extern "C" size_t sar_xattn_bwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : 8 * (size_t)a->B * a->Hq * a->Tq; }
+extern "C" size_t sar_xattn_bwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : bwd_plan(a).bytes; }
 #endif
 
 extern "C" int SAR_FN(sar_xattn_fwd)(const sarXattn* a, hipStream_t stream) {
@@ -446,12 +485,11 @@ extern "C" int SAR_FN(sar_xattn_bwd)(const sarXattn* a, hipStream_t stream) {
     if (bad(a) || !a->lse || !a->dout || !a->dq || !a->dk || !a->dv || !a->ws) return SAR_EINVAL;
     for (const void* p : {a->dout, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
         if ((uintptr_t)p % 16) return SAR_EINVAL;
-    if (bad_strides(sizeof(elt), &a->g_sb, 3) || wide_rows(sizeof(elt), {a->g_st}) || bad_workspace(a, 8 * (size_t)a->B * a->Hq * a->Tq)) return SAR_EINVAL;
-    float2* stats = reinterpret_cast<float2*>(a->ws);
-    if (a->D <= 32) launch_bwd<32>(*a, stats, stream);
-    else if (a->D <= 64) launch_bwd<64>(*a, stats, stream);
-    else if (a->D <= 96) launch_bwd<96>(*a, stats, stream);
-    else launch_bwd<128>(*a, stats, stream);
+    if (bad_strides(sizeof(elt), &a->g_sb, 3) || wide_rows(sizeof(elt), {a->g_st}) || bad_workspace(a, bwd_plan(a).bytes)) return SAR_EINVAL;
+    if (a->D <= 32) launch_bwd<32>(*a, stream);
+    else if (a->D <= 64) launch_bwd<64>(*a, stream);
+    else if (a->D <= 96) launch_bwd<96>(*a, stream);
+    else launch_bwd<128>(*a, stream);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
 }

@@ -99,7 +99,10 @@ SHAPES = [(1, 1, 1, 1, 1, 8, None, None),
           (2, 129, 257, 3, 1, 40, (257, 256), (129, 128)),
           (2, 50, 1030, 4, 2, 96, (1030, 700), None),
           (1, 16, 2100, 2, 1, 104, None, None),
-          (3, 200, 7, 2, 2, 16, (7, 6, 0), None)]
+          (3, 200, 7, 2, 2, 16, (7, 6, 0), None),
+          (1, 9, 1500, 2, 1, 64, None, None),                      # few rows, many keys: dQ in key slices
+          (2, 600, 5, 8, 1, 48, (5, 1), (600, 577)),               # few keys, many rows of shared heads: dK, dV in row slices
+          (1, 300, 1300, 6, 3, 128, None, None)]
 
 
 @pytest.mark.parametrize("dt", DT)
