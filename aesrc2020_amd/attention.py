@@ -173,7 +173,7 @@ class EncoderCache8:
 
     def store(self, k, v, k_lens=None, first=0):
         """Write frames [first, first + T) of every utterance from k, v (batch, T, heads, dim) (fp32, bf16 or fp16); `first` is a multiple of 64:
-        a streaming encoder appends whole blocks.  k_lens: how many of these T frames each utterance has (int32 (batch,); None: all) -- the
+        a streaming encoder appends chunks, all but an utterance's last of whole blocks.  k_lens: how many of these T frames each utterance has (int32 (batch,); None: all) -- the
         rest is stored as zeros.  The cache's lens become first + k_lens; with first > 0 an utterance without new frames keeps its length."""
         k, v = _rows("k", k), _rows("v", v, k)
         B, T, H, D = k.shape

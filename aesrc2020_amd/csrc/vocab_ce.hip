@@ -407,6 +407,12 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
             const bool has = lab >= 0 && lab < e.V;
             // a row that is left out: p = exp2(-inf) = 0 and g = 0
             const float g = has ? e.dloss[r] * gs : 0.f, lse = has ? e.lse[r] * LOG2E : INFINITY;
+            // (lse is rounded: where it is large an exponent can come out above 0, which no probability's is; a NaN stays one)
+            if (__any(has && fabsf(lse) > 1048576.f))
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) acc[i][j][x] = acc[i][j][x] > lse ? lse : acc[i][j][x];
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll

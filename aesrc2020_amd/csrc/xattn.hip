@@ -97,6 +97,7 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     f32x16 o[ND];
     clear(o);
     float m = NO_MAX, l = 0.f;
+    bool large = false;
     int cur = 0;
     for (int j = k0; j < k1; j += KT, cur ^= 2 * TILE) {
         tile_barrier();
@@ -127,15 +128,17 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
         if (__any(top > m + 8.f)) {
             const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
             m = mn; l *= f;
+            large = __any(fabsf(m) > LARGE && m != NO_MAX);
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
         }
+        exponents(s, sl, m, large);
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) { s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], sl, -m)); l += s[u][i]; }
+            for (int i = 0; i < 16; ++i) { s[u][i] = __builtin_amdgcn_exp2f(s[u][i]); l += s[u][i]; }
             u32x4 p[4];
             pack<T>(s[u], p);
 #pragma unroll
@@ -222,6 +225,7 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
     if (!summed && sp == 0 && wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
     f32x16 dq[ND];
     clear(dq);
+    const bool large = __any(fabsf(e) > LARGE);
     float sum = 0.f;
     int cur = 0;
     for (int step = 0, steps = (len + KT - 1) / KT, all = summed ? 2 * steps : steps; step < all; ++step, cur ^= 2 * TILE) {
@@ -256,6 +260,7 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], sl, -e);
             }
+            if (large) at_most_zero(s);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]);
             if (first) {
@@ -292,6 +297,7 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     constexpr int WM = 4 / WN, RT = 32 * WM, P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, TILE = RT * P, BUF = 2 * TILE;
     __shared__ __attribute__((aligned(1024))) char lds[2 * BUF];                 // Q, dO; two of each
     __shared__ __attribute__((aligned(16))) float2 row_stats[2][RT];
+    __shared__ int large[2];                                      // whether a row of the tile has a large lse
     // 128 wide, both fragments and both sums do not fit 256 registers: the K fragments stay in the wave's own piece of LDS, in lane order
     constexpr bool KL = sizeof(T) == 2 && DP == 128;
     __shared__ __attribute__((aligned(16))) u32x4 k_frags[KL ? 4 : 1][KL ? NC : 1][KL ? 64 : 1];
@@ -318,10 +324,16 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
         const int i = t + (int)threadIdx.x;
         return threadIdx.x < RT && i < tl ? sb[(long)g * a.Tq + i] : make_float2(0.f, 0.f);
     };
+    const auto put_stats = [&](int to, float2 v) {               // (RT <= 64: the first wave's lanes)
+        if (w) return;
+        if (lane < RT) row_stats[to][lane] = v;
+        const int any = __any(fabsf(v.x) > LARGE);
+        if (lane == 0) large[to] = any;
+    };
     int g = i0 < i1 ? i0 / across : 0, t = i0 < i1 ? (i0 - g * across) * RT : 0;
     if (i0 < i1) {
         load(g, t, lds);
-        if (threadIdx.x < RT) row_stats[0][threadIdx.x] = load_stats(g, t);
+        put_stats(0, load_stats(g, t));
     }
     u32x4 kf[NC], vf[NC];
     load_row<T, DP>(reinterpret_cast<const T*>(a.k) + b * a.k_sb + min(key, a.Tk - 1) * a.k_st + hk * a.k_sh, key < len, a.D, h, kf);
@@ -348,7 +360,10 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
 #pragma unroll
             for (int x = 0; x < 4; ++x)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s[4 * x + c] = __builtin_amdgcn_exp2f(fmaf(s[4 * x + c], sl, -st[2 * (8 * x + 4 * h + c)]));
+                for (int c = 0; c < 4; ++c) s[4 * x + c] = fmaf(s[4 * x + c], sl, -st[2 * (8 * x + 4 * h + c)]);
+            if (__builtin_amdgcn_readfirstlane(large[par])) at_most_zero(s);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]);
             if (len == 1)                                         // p = 1 exactly, and ds = 0 below
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = 1.f;
@@ -368,7 +383,7 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
             for (int d = 0; d < ND; ++d) dk[d] = mma_down<T, P>(lq, 32 * wm, d, pf, dk[d], lane);
         }
         g = gn; t = tn; cur ^= BUF; par ^= 1;
-        if (threadIdx.x < RT) row_stats[par][threadIdx.x] = next;
+        put_stats(par, next);
     }
     if constexpr (WM > 1) {
         static_assert(WM == 2, "");

@@ -137,6 +137,7 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = NO_MAX, l = 0.f, unit = 1.f;                        // o holds sums in units of `unit` (a power of two; 1 without a cache)
     if (S8 && t0 + w < t1) unit = vs[(t0 + w) * 32 / KV_BLOCK];
+    bool large = false;
     int cur = 0;
     for (int t = t0 + w; t < t1; t += NW, cur ^= 2 * TILE) {
         if (t + NW < t1) {
@@ -145,7 +146,7 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Loader::N) : "memory");
         } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         const char *tk = mine + cur, *tv = tk + TILE;
-        f32x16 s;
+        f32x16 tile_s[1], &s = tile_s[0];
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = 0.f;
         if constexpr (S8) {
@@ -176,14 +177,16 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
         if (__any(top > m + 8.f) || (S8 && nu != unit)) {
             const float mn = fmaxf(m, top), e = __builtin_amdgcn_exp2f(m - mn), eo = S8 ? e * (unit / nu) : e;
             m = mn; l *= e;
+            large = __any(fabsf(m) > LARGE && m != NO_MAX);
             if (S8) unit = nu;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= eo;
         }
+        exponents(tile_s, f, m, large);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], f, -m)); l += s[i]; }
+        for (int i = 0; i < 16; ++i) { s[i] = __builtin_amdgcn_exp2f(s[i]); l += s[i]; }
         u32x4 p[NPL][4];
         pack_planes<C, NPL>(s, p);
 #pragma unroll

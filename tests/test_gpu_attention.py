@@ -206,6 +206,47 @@ def test_large_scores_given_scale_and_out_buffers(dt):
         check(out, want[0], bounds(q, k, v, None, None, scale), "out", DT[dt])
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("Tq,Tk", [(6, 50), (90, 600)])
+def test_lengths_outside_the_range_and_garbage_behind_them(Tq, Tk, dt):
+    """Lengths below 0 and above the time axis count as its ends; rows of q and dout behind a length (NaN, inf, the type's lowest value) leave no trace."""
+    A = _att()
+    t = DT[dt]
+    q, k, v, g = make(4, Tq, Tk, 4, 2, 32, t, seed=Tk)
+    ql, kl = lens(Tq + 9, 3, -2, 5), lens(Tk, Tk + 100, 7, -1)
+    clean = [x.clone() for x in (q, k, v, g)]
+    for x, n in ((q, ql), (g, ql), (k, kl), (v, kl)):
+        for i, junk in enumerate((math.nan, math.inf, -math.inf, torch.finfo(t).min)):
+            x[i, max(0, int(n[i])):] = junk
+    res = []
+    for a, b, c, d in ((q, k, v, g), clean):
+        o, l = A.cross_attention(a, b, c, k_lens=kl, q_lens=ql, return_lse=True)
+        res.append((o, l) + A.cross_attention_grad(d, a, b, c, o, l, k_lens=kl, q_lens=ql))
+    assert all(torch.equal(x, y) and not torch.isnan(x).any() for x, y in zip(*res))
+    o, l, dq, dk, dv = res[0]
+    for i, (m, n) in enumerate(((Tq, Tk), (3, Tk), (0, 7), (5, 0))):
+        assert (o[i, m:] == 0).all() and torch.isneginf(l[i, :, m:]).all() and (dq[i, m:] == 0).all() and (dk[i, n:] == 0).all() and (dv[i, n:] == 0).all()
+    assert (dk[2] == 0).all() and (o[3] == 0).all() and (dq[3] == 0).all()
+
+
+def test_scores_of_any_size():
+    """fp32 scores around +-1e32 and -1e36 on every key: the softmax is that of their differences (0 or not of this world)."""
+    A = _att()
+    k = torch.ones(1, 40, 1, 8, device="cuda"); v = torch.randn(1, 40, 1, 8, device="cuda")
+    for Tq in (1, 50):
+        for s in (1e32, -1e32, -1e36):
+            q = torch.full((1, Tq, 1, 8), s / 8, device="cuda")
+            out, lse = A.cross_attention(q, k, v, scale=1.0, return_lse=True)
+            assert torch.allclose(out, v.mean(1, keepdim=True).expand_as(out), rtol=0, atol=40 * 2.0 ** -23) and torch.isfinite(lse).all()
+            for d in A.cross_attention_grad(torch.ones_like(out), q, k, v, out, lse, scale=1.0):
+                assert not torch.isnan(d).any()
+    q = torch.zeros(1, 70, 1, 16, device="cuda", dtype=torch.float16); q[..., 0] = 60000.0      # fp16: scores to 6e8, one key ahead of the others
+    k = torch.zeros(1, 90, 1, 16, device="cuda", dtype=torch.float16); k[0, :, 0, 0] = torch.linspace(0, 10000, 90).half()
+    v = torch.randn(1, 90, 1, 16, device="cuda").half()
+    for n in (1, 70):
+        assert torch.equal(A.cross_attention(q[:, :n], k, v, scale=1.0), v[:, 89:].expand(1, n, 1, 16))
+
+
 def test_scores_that_are_not_finite():
     """An infinite key: rows whose score is +inf are NaN as softmax has it; a row that meets only -inf has nothing to attend to."""
     A = _att()

@@ -156,6 +156,16 @@ def test_large_logits_no_labels_and_zero_gradients():
     want, bd = reference(x, w, lab, b, dl)
     loss, lse = vocab_crossentropy(x, w, lab, b, return_lse=True)
     check(loss, want[0], bd[0], "loss")
+    for big in (1e9, 1e13):                                        # logits whose rounding is whole units: one-hot, finite, the sum rules hold
+        hx = torch.zeros(3, 64, device="cuda"); hx[:, 0] = big
+        hw = torch.zeros(64, 200, device="cuda"); hw[0] = torch.linspace(0, 1, 200, device="cuda")
+        hl = torch.tensor([199, 5, 0], dtype=torch.int32, device="cuda")
+        l2, s2 = vocab_crossentropy(hx, hw, hl, return_lse=True)
+        gx, gw, _ = vocab_crossentropy_grad(torch.ones(3, device="cuda"), hx, hw, hl, s2)
+        assert torch.allclose(l2.double(), big * (1 - hw[0, hl.long()].double()), rtol=2.0 ** -21, atol=0) and torch.isfinite(gx).all() and torch.isfinite(gw).all()
+        p = gw[0].double() / big                                   # sum over the rows of softmax - onehot: the last entry, minus the labels
+        want = torch.zeros(200, device="cuda", dtype=torch.float64); want[199] = 2.0; want[5] = want[0] = -1.0
+        assert torch.allclose(p, want, rtol=0, atol=1e-5)
     none = torch.full_like(lab, -1)
     assert (vocab_crossentropy(x, w, none, b) == 0).all()
     for d, lb in ((dl, none), (torch.zeros_like(dl), lab)):
