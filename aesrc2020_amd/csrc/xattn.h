@@ -49,10 +49,11 @@ template <int N> __device__ __forceinline__ void exponents(f32x16 (&s)[N], float
             for (int i = 0; i < 16; ++i) s[u][i] = fmaf(s[u][i], f, -m);
     }
 }
-// the backward's exponents s f - lse: lse is rounded too, so where it is large they can come out above 0, which no probability's is (a NaN stays one)
-__device__ __forceinline__ void at_most_zero(f32x16& s) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = s[i] > 0.f ? 0.f : s[i];
+// lse in powers of two for the backward's p = exp2(s f - e).  It is rounded too: past 2^22 by whole units, which decide what p comes out as.  There it is
+// moved up by its rounding, so that no p is above 1 and the gradients stay finite.  A row that met no score (lse -inf) gets 0.
+__device__ __forceinline__ float backward_exponent(float lse) {
+    const float e = lse * LOG2E, a = fabsf(e);
+    return e == -INFINITY ? 0.f : a > 4194304.f ? fmaf(a, 2.384185791015625e-7f, e) : e;
 }
 
 struct Row { int t, h; };

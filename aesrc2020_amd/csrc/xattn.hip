@@ -213,8 +213,7 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
         load_row<T, DP>(reinterpret_cast<const T*>(a.q) + b * a.q_sb + me.t * a.q_st + me.h * a.q_sh, r < rl, a.D, h, qf);
         load_row<T, DP>(reinterpret_cast<const T*>(a.dout) + b * a.g_sb + me.t * a.g_st + me.h * a.g_sh, r < rl, a.D, h, gf);
         load_row<T, DP>(reinterpret_cast<const T*>(a.out) + b * a.o_sb + me.t * a.o_st + me.h * a.o_sh, r < rl, a.D, h, of);
-        if (r < rl) e = a.lse[stat_at(a, b, me)] * LOG2E;
-        if (e == -INFINITY) e = 0.f;                              // a row without keys meets no key
+        if (r < rl) e = backward_exponent(a.lse[stat_at(a, b, me)]);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -225,15 +224,18 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
     if (!summed && sp == 0 && wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
     f32x16 dq[ND];
     clear(dq);
-    const bool large = __any(fabsf(e) > LARGE);
     float sum = 0.f;
     int cur = 0;
-    for (int step = 0, steps = (len + KT - 1) / KT, all = summed ? 2 * steps : steps; step < all; ++step, cur ^= 2 * TILE) {
-        const bool first = summed && step < steps;                // the pass that sums p dp
-        const int j = (step < steps ? step : step - steps) * KT;
+    bool first = summed;                                          // the pass that sums p dp
+    for (int j = 0; j < len; cur ^= 2 * TILE) {
+        const int next = SUMMED && first && j + KT >= len ? 0 : j + KT;
         tile_barrier();
-        if (step + 1 < all) load((step + 1 < steps ? step + 1 : step + 1 - steps) % steps * KT, lds + (cur ^ (2 * TILE)));
-        if (summed && step == steps) {                            // the first pass is over: delta from all keys
+        if (next < len) load(next, lds + (cur ^ (2 * TILE)));
+        const int at_key = j;
+        const bool summing = first;
+        j = next;
+        if (SUMMED && next == 0) first = false;
+        if (SUMMED && summed && !summing && at_key == 0) {        // the first pass is over: delta from all keys
             sum = half_sum(sum);
             if constexpr (SUMMED && WM > 1) {
                 joined[wm][wn][lane] = sum;
@@ -243,7 +245,7 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
             dl = sum;
             if (wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
         }
-        if (row0 >= rl || (WM > 1 && j + 32 * wm >= len)) continue;
+        if (row0 >= rl || (WM > 1 && at_key + 32 * wm >= len)) continue;
         const char *lk = lds + cur, *lv = lds + cur + TILE;
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
@@ -253,17 +255,16 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
             for (int c = 0; c < NC; ++c) s = mma<T>(frag<P>(lk, at + n, c, h), qf[c], s);
 #pragma unroll
             for (int c = 0; c < NC; ++c) dp = mma<T>(frag<P>(lv, at + n, c, h), gf[c], dp);
-            if (j + KT > len) {                                   // (a key behind the length is a zero row: its p is no number to be trusted)
+            if (at_key + KT > len) {                              // (a key behind the length is a zero row: its p is no number to be trusted)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = j + at + 8 * (i >> 2) + 4 * h + (i & 3) < len ? fmaf(s[i], sl, -e) : -INFINITY;
+                for (int i = 0; i < 16; ++i) s[i] = at_key + at + 8 * (i >> 2) + 4 * h + (i & 3) < len ? fmaf(s[i], sl, -e) : -INFINITY;
             } else {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], sl, -e);
             }
-            if (large) at_most_zero(s);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]);
-            if (first) {
+            if (SUMMED && summing) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum = fmaf(s[i], dp[i], sum);
                 continue;
@@ -297,7 +298,6 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     constexpr int WM = 4 / WN, RT = 32 * WM, P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, TILE = RT * P, BUF = 2 * TILE;
     __shared__ __attribute__((aligned(1024))) char lds[2 * BUF];                 // Q, dO; two of each
     __shared__ __attribute__((aligned(16))) float2 row_stats[2][RT];
-    __shared__ int large[2];                                      // whether a row of the tile has a large lse
     // 128 wide, both fragments and both sums do not fit 256 registers: the K fragments stay in the wave's own piece of LDS, in lane order
     constexpr bool KL = sizeof(T) == 2 && DP == 128;
     __shared__ __attribute__((aligned(16))) u32x4 k_frags[KL ? 4 : 1][KL ? NC : 1][KL ? 64 : 1];
@@ -324,11 +324,10 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
         const int i = t + (int)threadIdx.x;
         return threadIdx.x < RT && i < tl ? sb[(long)g * a.Tq + i] : make_float2(0.f, 0.f);
     };
-    const auto put_stats = [&](int to, float2 v) {               // (RT <= 64: the first wave's lanes)
-        if (w) return;
-        if (lane < RT) row_stats[to][lane] = v;
-        const int any = __any(fabsf(v.x) > LARGE);
-        if (lane == 0) large[to] = any;
+    // one key: p = 1 whatever the score (s 0 - 0), and ds = 0 (dK is stored as zero)
+    const float sk = len == 1 ? 0.f : sl;
+    const auto put_stats = [&](int to, float2 v) {
+        if (threadIdx.x < RT) row_stats[to][threadIdx.x] = make_float2(len == 1 ? 0.f : v.x, v.y);
     };
     int g = i0 < i1 ? i0 / across : 0, t = i0 < i1 ? (i0 - g * across) * RT : 0;
     if (i0 < i1) {
@@ -360,13 +359,9 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
 #pragma unroll
             for (int x = 0; x < 4; ++x)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s[4 * x + c] = fmaf(s[4 * x + c], sl, -st[2 * (8 * x + 4 * h + c)]);
-            if (__builtin_amdgcn_readfirstlane(large[par])) at_most_zero(s);
+                for (int c = 0; c < 4; ++c) s[4 * x + c] = fmaf(s[4 * x + c], sk, -st[2 * (8 * x + 4 * h + c)]);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]);
-            if (len == 1)                                         // p = 1 exactly, and ds = 0 below
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = 1.f;
             u32x4 pf[4];
             pack<T>(s, pf);
 #pragma unroll
@@ -377,7 +372,6 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
             for (int x = 0; x < 4; ++x)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) dp[4 * x + c] = s[4 * x + c] * (dp[4 * x + c] - st[2 * (8 * x + 4 * h + c) + 1]);
-            if (len == 1) dp = zero16();
             pack<T>(dp, pf);
 #pragma unroll
             for (int d = 0; d < ND; ++d) dk[d] = mma_down<T, P>(lq, 32 * wm, d, pf, dk[d], lane);
@@ -398,11 +392,11 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     if (key >= a.Tk) return;
     const long at = (((long)b * a.Tk + key) * a.Hkv + hk) * a.D;  // frames behind the length: their gradient is zero
     if (slices == 1) {
-        store_column<T, ND>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, key < len, a.D, h);
+        store_column<T, ND>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, key < len && len > 1, a.D, h);
         store_column<T, ND>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, key < len, a.D, h);
     } else {
         const long n = (long)a.B * a.Tk * a.Hkv * a.D;
-        store_column<float, ND>(part + sp * n + at, dk, a.scale, key < len, a.D, h);
+        store_column<float, ND>(part + sp * n + at, dk, a.scale, key < len && len > 1, a.D, h);
         store_column<float, ND>(part + (slices + sp) * n + at, dv, 1.f, key < len, a.D, h);
     }
 }
