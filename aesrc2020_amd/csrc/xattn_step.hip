@@ -4,8 +4,8 @@
 // loads the next tile straight into one (whole rows, coalesced) while it computes from the other.
 //
 // The same kernel reads the 8-bit cache (include/sarnet.h: sarKv8): e4m3 values are converted exactly into the 16-bit operand type (bf16 for
-// bf16 and fp32 queries, fp16 for fp16 ones); the scale of a 64-key block multiplies the fp32 scores (K), and the fp32 sums as a ratio of
-// powers of two (V).  fp32 queries and probabilities enter as three bf16 planes (8 + 8 + 8 bits hold an fp32 mantissa): products are exact, sums fp32,
+// bf16 and fp32 queries, fp16 for fp16 ones); the scale of a 64-key block multiplies the fp32 scores (K); V's goes into the bf16 values (a bf16 has
+// an fp32's range), and beside fp16 ones into the fp32 sums as a ratio of powers of two.  fp32 queries and probabilities enter as three bf16 planes (8 + 8 + 8 bits hold an fp32 mantissa): products are exact, sums fp32,
 // at a third of the bf16 rate instead of the fp32 MFMA's sixteenth.
 // Compiled once per element type: SAR_ELT 0 = fp32, 1 = bf16, 2 = fp16.
 #include "xattn.h"
@@ -30,28 +30,28 @@ constexpr int KV_BLOCK = 64;            // frames that share a scale
 
 struct Kv8 { const unsigned char *k8, *v8; const float *ks, *vs; long frames; };   // (B, Hkv, frames, D), (B, Hkv, frames / 64)
 
-// eight e4m3 values -> eight 16-bit ones, exactly
-template <typename C> __device__ __forceinline__ u32x4 widen8(u32x2 w) {
+// eight e4m3 values times a power of two -> eight 16-bit ones, exactly
+template <typename C> __device__ __forceinline__ u32x4 widen8(u32x2 w, float scale) {
     u32x4 o;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int src = (int)w[i >> 1];
         if constexpr (__is_same(C, __bf16)) {
-            const auto v = (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, 1.f, false);
+            const auto v = (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, scale, false);
             o[i] = __builtin_bit_cast(unsigned, v);
         } else {
-            const auto v = (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(src, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(src, 1.f, false);
+            const auto v = (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(src, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(src, scale, false);
             o[i] = __builtin_bit_cast(unsigned, v);
         }
     }
     return o;
 }
 // mma_down (attn_tiles.h) over a tile of e4m3 rows: the transposing read hands a lane eight rows of one column as bytes
-template <typename C, int PITCH> __device__ __forceinline__ u32x4 down8(const char* tile, int dt, int s, int lane) {
+template <typename C, int PITCH> __device__ __forceinline__ u32x4 down8(const char* tile, int dt, int s, int lane, float scale) {
     const int i = lane & 15, slot = i >> 1, r = 16 * s + 4 * (lane >> 5) + (slot & 3) + 8 * (slot >> 2);
     typedef __attribute__((ext_vector_type(2))) int i32x2;
     const i32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(tile + chunk_at<PITCH>(r, 2 * dt + ((lane >> 4) & 1)) + (i & 1) * 8));
-    return widen8<C>(__builtin_bit_cast(u32x2, v));
+    return widen8<C>(__builtin_bit_cast(u32x2, v), scale);
 }
 
 // a 32 x 32 fp32 result as operand planes of the 16-bit type: one (rounded), or three whose sum is the value
@@ -135,8 +135,12 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-    float m = NO_MAX, l = 0.f, unit = 1.f;                        // o holds sums in units of `unit` (a power of two; 1 without a cache)
-    if (S8 && t0 + w < t1) unit = vs[(t0 + w) * 32 / KV_BLOCK];
+    // fp16 values of a cache: o holds sums in units of V's scale, `unit`, else 1.  (A block whose values end below 2^-31 counts as one of that size:
+    // no fp16 result shows it.)
+    constexpr bool UNITS = S8 && __is_same(C, _Float16);
+    const auto unit_of = [&](int t) { return fmaxf(vs[t * 32 / KV_BLOCK], 9.094947017729282e-13f); };
+    float m = NO_MAX, l = 0.f, unit = 1.f;
+    if (UNITS && t0 + w < t1) unit = unit_of(t0 + w);
     bool large = false;
     int cur = 0;
     for (int t = t0 + w; t < t1; t += NW, cur ^= 2 * TILE) {
@@ -157,7 +161,7 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
                     const bool half = 32 * c + 16 * h + 8 >= a.D;
                     x[2] = half ? 0 : x[2]; x[3] = half ? 0 : x[3];
                 }
-                const u32x4 lo = widen8<C>(u32x2{x[0], x[1]}), hi = widen8<C>(u32x2{x[2], x[3]});
+                const u32x4 lo = widen8<C>(u32x2{x[0], x[1]}, 1.f), hi = widen8<C>(u32x2{x[2], x[3]}, 1.f);
 #pragma unroll
                 for (int k = NPL - 1; k >= 0; --k) { s = mma<C>(lo, qf[k][2 * c], s); s = mma<C>(hi, qf[k][2 * c + 1], s); }
             }
@@ -165,7 +169,7 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
 #pragma unroll
             for (int c = 0; c < NC; ++c) s = mma<T>(frag<P>(tk, n, c, h), qf[0][c], s);
         }
-        const float f = S8 ? sl * ks[t * 32 / KV_BLOCK] : sl, nu = S8 ? vs[t * 32 / KV_BLOCK] : 1.f;
+        const float f = S8 ? sl * ks[t * 32 / KV_BLOCK] : sl, nu = UNITS ? unit_of(t) : 1.f, v_scale = S8 && !UNITS ? vs[t * 32 / KV_BLOCK] : 1.f;
         float top = NO_MAX;
         if (t * 32 + 32 > len) {
 #pragma unroll
@@ -174,11 +178,11 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
         top = half_max(top) * f;
-        if (__any(top > m + 8.f) || (S8 && nu != unit)) {
-            const float mn = fmaxf(m, top), e = __builtin_amdgcn_exp2f(m - mn), eo = S8 ? e * (unit / nu) : e;
+        if (__any(top > m + 8.f) || (UNITS && nu != unit)) {
+            const float mn = fmaxf(m, top), e = __builtin_amdgcn_exp2f(m - mn), eo = UNITS ? e * unit / nu : e;     // (in this order: no power of two passes the range before e has taken it back)
             m = mn; l *= e;
             large = __any(fabsf(m) > LARGE && m != NO_MAX);
-            if (S8) unit = nu;
+            if (UNITS) unit = nu;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -194,7 +198,7 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
             if constexpr (S8) {
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const u32x4 v = down8<C, P>(tv, d, x, lane);
+                    const u32x4 v = down8<C, P>(tv, d, x, lane, v_scale);
 #pragma unroll
                     for (int k = NPL - 1; k >= 0; --k) o[d] = mma<C>(v, p[k][x], o[d]);
                 }

@@ -348,6 +348,27 @@ def test_cache_attention(B, Tq, Tk, Hq, H, D, kl, dt):
     check(c.attend(q), want[0], bounds(q, kd, vd, kl, None, None), "out", DT[dt])
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("Tk", [256, 1100])
+def test_cache_blocks_of_very_different_size(dt, Tk):
+    """V's blocks from the largest numbers to the smallest a result can show; columns that only small blocks reach; keys that pick one block."""
+    A = _att()
+    q, k, v, _ = make(1, 3, Tk, 2, 1, 32, torch.float32, seed=Tk)
+    size = (6e4, 1e-7, 1.0, 1e-12) if dt == "f16" else (1e25, 1e-25, 1.0, 1e12)
+    blocks = torch.arange(Tk, device="cuda") // 64 % 4
+    v = torch.sign(v) * torch.tensor(size, device="cuda")[blocks][None, :, None, None]
+    v[:, :, :, 8:16] *= (blocks != 0)[None, :, None, None]
+    v[:, :, :, 16:24] *= (blocks == 1)[None, :, None, None]
+    k[:, :, :, 0] = torch.tensor((-40.0, 0.0, 40.0, 0.0), device="cuda")[blocks][None, :, None]
+    q = q.to(DT[dt])
+    q[:, 0, :, 0] = 4.0; q[:, 1, :, 0] = -4.0; q[:, 2, :, 0] = 0.0                             # block 2 decides; block 0 does; all alike
+    c = A.EncoderCache8(1, Tk, 1, 32)
+    c.store(k, v)
+    wide = lambda y, s: (y.float().double() * s.double().repeat_interleave(64, 2)[..., None])[:, :, :Tk].transpose(1, 2)  # noqa: E731
+    kd, vd = wide(c.k8, c.k_scale), wide(c.v8, c.v_scale)
+    check(c.attend(q), R.attend(q, kd, vd)[0], bounds(q, kd, vd, None, None, None), "out", DT[dt])
+
+
 def test_cache_appends_blocks_and_replays():
     """A streaming encoder's chunks, an utterance that ends early, queries of another type than the stored one, and a captured step over later stores."""
     A = _att()
