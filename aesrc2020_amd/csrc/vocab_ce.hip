@@ -219,7 +219,7 @@ __device__ __forceinline__ void finish_row(float* loss, float* lse, int r, float
     if (loss) loss[r] = lab >= 0 && lab < V ? (m - own + __builtin_amdgcn_logf(l)) * LN2 : 0.f;
 }
 __device__ __forceinline__ int dz_exp(const Epi& e) {             // dz is held times 2^this
-    if (e.g_from == G_ONE) return DZ_BITS;
+    if (e.g_from == G_ONE) return 0;                              // (a bf16 has an fp32's range)
     if (e.g_from == G_PARTS) return DZ_BITS - g_exp(max_of(e.parts + 2 * PARTS));
     float m = 0.f;
     for (int r = threadIdx.x & 63; r < e.R_all; r += 64) {

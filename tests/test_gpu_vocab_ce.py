@@ -125,6 +125,19 @@ def test_gradients_against_differences(dt):
         assert abs(num - ana) <= (v.abs() * 1.05 * bd[2 + i]).sum().item() + 1e-8, (i, num, ana)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("R,D,V", [(20, 48, 130), (1100, 640, 4000)])
+@pytest.mark.parametrize("e", [100, -60])
+def test_gradients_follow_the_size_of_dloss(e, R, D, V, dt):
+    """A power of two on dloss is one on the gradients, whatever held dz in between (tiny probabilities may come out as zeros: a quarter of a rounding)."""
+    from aesrc2020_amd.losses import vocab_crossentropy, vocab_crossentropy_grad
+    x, w, lab, b, dl = make(R, D, V, DT[dt], seed=8)
+    _, lse = vocab_crossentropy(x, w, lab, b, return_lse=True)
+    for g, h in zip(vocab_crossentropy_grad(dl, x, w, lab, lse, b), vocab_crossentropy_grad(dl * 2.0 ** e, x, w, lab, lse, b)):
+        g, h = g.double(), h.double() * 2.0 ** -e
+        assert torch.isfinite(h).all() and ((g - h).abs() <= torch.finfo(DT[dt]).eps * g.abs() + 2.0 ** -40 * g.abs().max()).all()
+
+
 @pytest.mark.parametrize("dt", DT)
 def test_strides_scales_and_wide_ranges(dt):
     """Strided and unaligned rows and kernels; tensors far from 1 in size; upstream gradients of one row a million times another's."""
