@@ -104,20 +104,21 @@ static inline FwdPlan fwd_plan(const sarXattn* a) {
     if (R > 64 && (R + 127) / 128 * bh >= 512) return {4, 1};
     return {2, (R + 63) / 64 * bh >= 192 ? 1 : key_splits(a, 64, 384)};
 }
-// The backward: four waves on 128 columns where those blocks fill the chip twice, else two pairs on 64 -- and where 64 are all there are.  Where the
-// blocks are fewer than the CUs, the streamed axis (keys for dQ, the rows of all the group's heads for dK, dV) is cut into slices of eight steps
-// of 64 at least, whose fp32 sums a further launch adds.
-constexpr int SUMMED_KEYS = 256;
+// The backward of up to SMALL_KEYS keys is one kernel (xattn.hip).  Else four waves on 128 columns where those blocks fill the chip twice, two pairs on
+// 64 where not.  Where the blocks are fewer than half the CUs, the streamed axis (keys for dQ, the rows of all the group's heads for dK, dV) is cut
+// into slices of two steps of 64 at least, up to a block per CU, whose fp32 sums a further launch adds: bf16 1 x 400 x 400, 4 heads of 64: 19.3 ->
+// 17.6 us, fp32 64 -> 38; slices for two blocks per CU gained nothing (32 x 16 steps of 128-wide heads 42 -> 52 us).
+constexpr int SUMMED_KEYS = 256, SMALL_KEYS = 64;
 struct BwdPlan { bool few_q, few_k; int dq_slices, dkv_slices; size_t dq_at, dkv_at, bytes; };
 static inline int cut_slices(long blocks, long steps) {
-    const long want = (512 + blocks - 1) / blocks, most = steps / 8;
-    return blocks >= 256 || most < 2 ? 1 : (int)(want < most ? want : most);
+    const long want = blocks < 1 ? 1 : 256 / blocks, most = steps / 2;         // (no blocks: no keys)
+    return want < 2 || most < 2 ? 1 : (int)(want < most ? want : most);
 }
 static inline BwdPlan bwd_plan(const sarXattn* a) {
     BwdPlan p = {};
     const long R = (long)a->Tq * (a->Hq / a->Hkv), bh = (long)a->B * a->Hkv;
     p.few_q = R <= 64 || (R + 127) / 128 * bh < 512;
-    p.few_k = a->Tk <= 64 || (a->Tk + 127) / 128 * bh < 512;
+    p.few_k = (a->Tk + 127) / 128 * bh < 512;
     p.dq_slices = a->Tk <= SUMMED_KEYS ? 1 : cut_slices((R + 63) / 64 * bh, (a->Tk + 63) / 64);
     p.dkv_slices = cut_slices((a->Tk + 63) / 64 * bh, (a->Tq + 63) / 64 * (long)(a->Hq / a->Hkv));
     const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };

@@ -55,6 +55,15 @@ template <int N> __device__ __forceinline__ void add(const float* p, f32x16 (&o)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] += p[(d * 16 + i) * 64 + lane];
 }
+// Loads that a loop uses are waited for before it: inside, the wait would be for the tiles that the loop has under way too (the compiler counts
+// its own loads only).
+template <int N> __device__ __forceinline__ void settle(u32x4 (&f)[N]) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) asm volatile("" : "+v"(f[c]));
+}
+// the row tiles of a group's heads, one head after the other
+struct RowTile { int g, t; };
+__device__ __forceinline__ RowTile after(RowTile r, int rows, int tl) { return r.t + rows >= tl ? RowTile{r.g + 1, 0} : RowTile{r.g, r.t + rows}; }
 // a wave's column of D values: lane holds column n, values 32 d + 8 i + 4 h + (0..3)
 template <typename T, int ND> __device__ __forceinline__ void store_column(T* p, const f32x16 (&o)[ND], float f, bool in, int D, int h) {
 #pragma unroll
@@ -315,24 +324,29 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     const T* qb = reinterpret_cast<const T*>(a.q) + b * a.q_sb + (long)hk * G * a.q_sh;
     const T* gb = reinterpret_cast<const T*>(a.dout) + b * a.g_sb + (long)hk * G * a.g_sh;
     const float2* sb = stats + ((long)b * a.Hq + hk * G) * a.Tq;
-    const auto load = [&](int g, int t, char* to) {
-        tq.load(qb + g * a.q_sh + t * a.q_st, tl - t, qs, db, to, w);
-        tg.load(gb + g * a.g_sh + t * a.g_st, tl - t, gs, db, to + TILE, w);
+    const auto load = [&](RowTile r, char* to) {
+        tq.load(qb + r.g * a.q_sh + r.t * a.q_st, tl - r.t, qs, db, to, w);
+        tg.load(gb + r.g * a.g_sh + r.t * a.g_st, tl - r.t, gs, db, to + TILE, w);
     };
     // {lse log2 e, delta} of the tile's rows.  Rows behind the last one get zeros as their Q and dO do: p = exp2(0), which meets zero rows.
-    const auto load_stats = [&](int g, int t) {
-        const int i = t + (int)threadIdx.x;
-        return threadIdx.x < RT && i < tl ? sb[(long)g * a.Tq + i] : make_float2(0.f, 0.f);
+    const auto load_stats = [&](RowTile r) {
+        return sb[(long)r.g * a.Tq + min(r.t + (int)threadIdx.x % RT, tl - 1)];
     };
     // one key: p = 1 whatever the score (s 0 - 0), and ds = 0 (dK is stored as zero)
     const float sk = len == 1 ? 0.f : sl;
-    const auto put_stats = [&](int to, float2 v) {
-        if (threadIdx.x < RT) row_stats[to][threadIdx.x] = make_float2(len == 1 ? 0.f : v.x, v.y);
+    const auto put_stats = [&](int to, RowTile r, float2 v) {
+        const bool in = r.t + (int)threadIdx.x < tl;
+        if (threadIdx.x < RT) row_stats[to][threadIdx.x] = make_float2(in && len > 1 ? v.x : 0.f, in ? v.y : 0.f);
     };
-    int g = i0 < i1 ? i0 / across : 0, t = i0 < i1 ? (i0 - g * across) * RT : 0;
+    // (statistics are fetched two steps ahead and put right behind a barrier, where nothing has to be waited for)
+    RowTile at_row = {0, 0}, next_row = {0, 0};
+    float2 next = make_float2(0.f, 0.f);
     if (i0 < i1) {
-        load(g, t, lds);
-        put_stats(0, load_stats(g, t));
+        at_row = {i0 / across, (i0 - i0 / across * across) * RT};
+        next_row = after(at_row, RT, tl);
+        load(at_row, lds);
+        put_stats(0, at_row, load_stats(at_row));
+        next = load_stats(i0 + 1 < i1 ? next_row : at_row);
     }
     u32x4 kf[NC], vf[NC];
     load_row<T, DP>(reinterpret_cast<const T*>(a.k) + b * a.k_sb + min(key, a.Tk - 1) * a.k_st + hk * a.k_sh, key < len, a.D, h, kf);
@@ -341,15 +355,21 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
         for (int c = 0; c < NC; ++c) k_frags[w][c][lane] = kf[c];
     }
     load_row<T, DP>(reinterpret_cast<const T*>(a.v) + b * a.v_sb + min(key, a.Tk - 1) * a.v_st + hk * a.v_sh, key < len, a.D, h, vf);
+    if constexpr (!KL) settle(kf);
+    settle(vf);
     f32x16 dk[ND], dv[ND];
     clear(dk); clear(dv);
     int cur = 0, par = 0;
     for (int i = i0; i < i1; ++i) {
         tile_barrier();
-        int gn = g, tn = t + RT;
-        if (tn >= tl) { ++gn; tn = 0; }
-        float2 next = make_float2(0.f, 0.f);
-        if (i + 1 < i1) { next = load_stats(gn, tn); load(gn, tn, lds + (cur ^ BUF)); }
+        const int t = at_row.t;
+        at_row = next_row;
+        if (i + 1 < i1) {
+            put_stats(par ^ 1, at_row, next);
+            load(at_row, lds + (cur ^ BUF));
+            next_row = after(at_row, RT, tl);
+            next = load_stats(i + 2 < i1 ? next_row : at_row);
+        }
         if (key0 < len && (WM == 1 || t + 32 * wm < tl)) {
             const char *lq = lds + cur, *lg = lds + cur + TILE;
             const float* st = reinterpret_cast<const float*>(row_stats[par]) + wm * 64;
@@ -376,8 +396,7 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
 #pragma unroll
             for (int d = 0; d < ND; ++d) dk[d] = mma_down<T, P>(lq, 32 * wm, d, pf, dk[d], lane);
         }
-        g = gn; t = tn; cur ^= BUF; par ^= 1;
-        put_stats(par, next);
+        cur ^= BUF; par ^= 1;
     }
     if constexpr (WM > 1) {
         static_assert(WM == 2, "");
@@ -391,6 +410,192 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     }
     if (key >= a.Tk) return;
     const long at = (((long)b * a.Tk + key) * a.Hkv + hk) * a.D;  // frames behind the length: their gradient is zero
+    if (slices == 1) {
+        store_column<T, ND>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, key < len && len > 1, a.D, h);
+        store_column<T, ND>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, key < len, a.D, h);
+    } else {
+        const long n = (long)a.B * a.Tk * a.Hkv * a.D;
+        store_column<float, ND>(part + sp * n + at, dk, a.scale, key < len && len > 1, a.D, h);
+        store_column<float, ND>(part + (slices + sp) * n + at, dv, 1.f, key < len, a.D, h);
+    }
+}
+
+// ---- dQ, dK, dV in one launch where 64 keys are all there are: a block holds a key head's keys as two pairs of waves' columns (as above), so S and dP
+// are computed once for all three gradients, and ds, through LDS, meets the keys again for dQ.  Five products a tile instead of seven, one launch
+// instead of two: what fp32 (whose matrix instructions bound it) and small calls (which latency does) both need.  64 x 72 x 39, 8 heads of 64: fp32 45 ->
+// 34 us, bf16 18 -> 14; 2 x 20 x 39, 4 heads, bf16: 11 -> 7; 8 x 1000 x 64, 8 heads of 128, bf16: 54 -> 43.
+// delta is the sum of p dp over the keys (see xattn_dq_kernel).
+template <typename T, int DP> struct Small {
+    static constexpr int P = pitch<T, DP>(), TILE = 64 * P, BUFS = P <= 128 ? 2 : 1;             // (two blocks a CU in either case)
+    static constexpr int DS_PITCH = 68, DS_AT = TILE + BUFS * 2 * TILE, LDS = DS_AT + 64 * DS_PITCH * 4;
+};
+// sums of 2 N values over the 32 lanes of a half, the values shared out on the way: lane n ends with value (n & 1) 8 + (n & 2) 2 + (n & 4) / 2 + (n & 8) / 8
+template <int N> __device__ __forceinline__ float shared_sums(const float (&x)[2 * N], int lane) {
+    float y[N];
+    const bool up = lane & (8 / N);
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = (up ? x[i + N] : x[i]) + __shfl_xor(up ? x[i] : x[i + N], 8 / N, 64);
+    if constexpr (N > 1) return shared_sums<N / 2>(y, lane);
+    else return y[0] + __shfl_xor(y[0], 16, 64);
+}
+template <typename T, int DP> __global__ __launch_bounds__(256, 2) void xattn_small_bwd_kernel(sarXattn a, float* __restrict__ part, int slices) {
+    typedef Small<T, DP> S;
+    constexpr int P = S::P, NC = DP * (int)sizeof(T) / 32, ND = DP / 32, TILE = S::TILE, RT = 64, BUFS = S::BUFS;
+    constexpr bool KL = P == 256;       // KL: the K fragments are read from the tile (they do not fit the registers as well)
+    extern __shared__ __attribute__((aligned(1024))) char lds[];                                 // K; Q, dO (BUFS of each); ds (keys, rows) fp32
+    __shared__ __attribute__((aligned(16))) float exponent[2][RT];
+    __shared__ __attribute__((aligned(16))) float sums[2][RT];
+    const int item = xcd_item(a.B * a.Hkv * slices);
+    if (item < 0) return;
+    const int sp = item % slices, bh = item / slices, b = bh / a.Hkv, hk = bh % a.Hkv, G = a.Hq / a.Hkv;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31, wn = w & 1, wm = w >> 1;
+    const int len = live_keys(a, b), key0 = wn * 32, key = key0 + n;
+    const int tl = len ? live_rows(a, b) / G : 0;
+    const int across = (tl + RT - 1) / RT, tiles = across * G, per = (tiles + slices - 1) / slices, i0 = min(sp * per, tiles), i1 = min(i0 + per, tiles);
+    const unsigned ks = (unsigned)(a.k_st * sizeof(T)), qs = (unsigned)(a.q_st * sizeof(T)), gs = (unsigned)(a.g_st * sizeof(T)), db = (unsigned)(a.D * sizeof(T));
+    const T* qb = reinterpret_cast<const T*>(a.q) + b * a.q_sb + (long)hk * G * a.q_sh;
+    const T* gb = reinterpret_cast<const T*>(a.dout) + b * a.g_sb + (long)hk * G * a.g_sh;
+    const float* lse = a.lse + ((long)b * a.Hq + hk * G) * a.Tq;
+    const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
+    const TileLoader<P, RT> tq(qs, db), tg(gs, db);
+    const auto load = [&](RowTile r, char* to) {
+        tq.load(qb + r.g * a.q_sh + r.t * a.q_st, tl - r.t, qs, db, to, w);
+        tg.load(gb + r.g * a.g_sh + r.t * a.g_st, tl - r.t, gs, db, to + TILE, w);
+    };
+    // lse log2 e of the tile's rows.  One key: p = 1 whatever the score, and ds = 0 (dQ, dK are stored as zero).
+    // A key behind the length is a zero row: its p, which dQ and delta would meet, is made 0.
+    const float sk = len == 1 ? 0.f : a.scale * LOG2E, none = key < len ? 0.f : -INFINITY;
+    const auto load_lse = [&](RowTile r) {
+        return lse[(long)r.g * a.Tq + min(r.t + (int)threadIdx.x % RT, tl - 1)];
+    };
+    const auto put_lse = [&](int to, RowTile r, float v) {
+        if (threadIdx.x < RT) exponent[to][threadIdx.x] = len > 1 && r.t + (int)threadIdx.x < tl ? backward_exponent(v) : 0.f;
+    };
+    char* const tiles_at = lds + TILE;
+    float* const ds_at = reinterpret_cast<float*>(lds + S::DS_AT);
+    RowTile at_row = {0, 0}, next_row = {0, 0};
+    float next = 0.f;
+    if (i0 < i1) {
+        at_row = {i0 / across, (i0 - i0 / across * across) * RT};
+        next_row = after(at_row, RT, tl);
+        TileLoader<P, RT>(ks, db).load(kb, len, ks, db, lds, w);
+        load(at_row, tiles_at);
+        put_lse(0, at_row, load_lse(at_row));
+        next = load_lse(i0 + 1 < i1 ? next_row : at_row);
+    }
+    u32x4 kf[NC], vf[NC];
+    if constexpr (!KL) load_row<T, DP>(kb + min(key, a.Tk - 1) * a.k_st, key < len, a.D, h, kf);
+    load_row<T, DP>(reinterpret_cast<const T*>(a.v) + b * a.v_sb + min(key, a.Tk - 1) * a.v_st + hk * a.v_sh, key < len, a.D, h, vf);
+    if constexpr (!KL) settle(kf);
+    settle(vf);
+    f32x16 dk[ND], dv[ND];
+    clear(dk); clear(dv);
+    int cur = 0, par = 0;
+    for (int i = i0; i < i1; ++i) {
+        tile_barrier();
+        const int t = at_row.t, g = at_row.g;
+        at_row = next_row;
+        if (i + 1 < i1) {
+            put_lse(par ^ 1, at_row, next);
+            if constexpr (BUFS == 2) load(at_row, tiles_at + (cur ^ (2 * TILE)));
+            next_row = after(at_row, RT, tl);
+            next = load_lse(i + 2 < i1 ? next_row : at_row);
+        }
+        const bool live = key0 < len && t + 32 * wm < tl;
+        const char *lq = tiles_at + cur, *lg = tiles_at + cur + TILE;
+        const float* ex = exponent[par] + 32 * wm;
+        f32x16 s = zero16(), dp = zero16();
+        if (live) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s = mma<T>(frag<P>(lq, 32 * wm + n, c, h), KL ? frag<P>(lds, key, c, h) : kf[c], s);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[4 * x + c] = __builtin_amdgcn_exp2f(fmaf(s[4 * x + c], sk, none - ex[8 * x + 4 * h + c]));
+            u32x4 pf[4];
+            pack<T>(s, pf);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) dv[d] = mma_down<T, P>(lg, 32 * wm, d, pf, dv[d], lane);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) dp = mma<T>(frag<P>(lg, 32 * wm + n, c, h), vf[c], dp);
+        }
+        float pdp[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pdp[i] = s[i] * dp[i];       // (a wave without keys: 0)
+        const float sum = shared_sums<8>(pdp, lane);
+        const int place = (lane & 1) * 8 + (lane & 2) * 2 + (lane & 4) / 2 + (lane & 8) / 8;
+        if (n < 16) sums[wn][32 * wm + 8 * (place >> 2) + 4 * h + (place & 3)] = sum;
+        lds_barrier();
+        if (live) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                f32x4 v;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int row = 8 * x + 4 * h + c;
+                    const float dl = sums[0][32 * wm + row] + sums[1][32 * wm + row];
+                    v[c] = dp[4 * x + c] = s[4 * x + c] * (dp[4 * x + c] - dl);
+                }
+                *reinterpret_cast<f32x4*>(ds_at + key * S::DS_PITCH + 32 * wm + 8 * x + 4 * h) = v;
+            }
+            u32x4 pf[4];
+            pack<T>(dp, pf);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) dk[d] = mma_down<T, P>(lq, 32 * wm, d, pf, dk[d], lane);
+        }
+        lds_barrier();                                            // ds is there; the reads of Q and dO are done
+        if constexpr (BUFS == 1) {
+            if (i + 1 < i1) load(at_row, tiles_at);
+        }
+        // dQ of the wave's 32 rows, every second 32 of the width
+        if (t + 32 * wm < tl) {
+            const int row = t + 32 * wm + n;
+            T* to = reinterpret_cast<T*>(a.dq) + (((long)b * a.Tq + row) * a.Hq + hk * G + g) * a.D;
+            u32x4 df[2][4];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (32 * k < len) {
+                    f32x16 x;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = ds_at[(32 * k + 8 * (i >> 2) + 4 * h + (i & 3)) * S::DS_PITCH + 32 * wm + n];
+                    pack<T>(x, df[k]);
+                }
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                if ((d & 1) != wn) continue;
+                f32x16 q = zero16();
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (32 * k < len) q = mma_down<T, P>(lds, 32 * k, d, df[k], q, lane);
+                if (row < tl) {
+                    const bool in = len > 1;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int dd = 32 * d + 8 * i + 4 * h;
+                        if (dd < a.D) store4<T>(to + dd, in ? q[4 * i] * a.scale : 0.f, in ? q[4 * i + 1] * a.scale : 0.f, in ? q[4 * i + 2] * a.scale : 0.f, in ? q[4 * i + 3] * a.scale : 0.f);
+                    }
+                }
+            }
+        }
+        par ^= 1;
+        if (BUFS == 2) cur ^= 2 * TILE;
+    }
+    if (sp == 0) {                                                // rows behind the length: zeros
+        const int wide = G * a.D / 4;
+        for (long i = threadIdx.x; i < (long)(a.Tq - tl) * wide; i += 256) {
+            const long row = i / wide;
+            store4<T>(reinterpret_cast<T*>(a.dq) + (((long)b * a.Tq + tl + row) * a.Hq + hk * G) * a.D + (i - row * wide) * 4, 0.f, 0.f, 0.f, 0.f);
+        }
+    }
+    float* join = reinterpret_cast<float*>(lds) + wn * 2 * ND * 1024;
+    static_assert(2 * 2 * ND * 1024 * 4 <= S::LDS, "");
+    __syncthreads();
+    if (wm) { put(join, dk, lane); put(join + ND * 1024, dv, lane); }
+    __syncthreads();
+    if (wm) return;
+    add(join, dk, lane); add(join + ND * 1024, dv, lane);
+    if (key >= a.Tk) return;
+    const long at = (((long)b * a.Tk + key) * a.Hkv + hk) * a.D;
     if (slices == 1) {
         store_column<T, ND>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, key < len && len > 1, a.D, h);
         store_column<T, ND>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, key < len, a.D, h);
@@ -436,7 +641,7 @@ template <int DP> static void launch_fwd(const sarXattn& a, hipStream_t st) {
     }
     if (!two) hipLaunchKernelGGL((xattn_fwd_kernel<elt, DP, 4>), grid, dim3(256), 0, st, a, rt, p.splits);
 }
-template <int DP> static void launch_bwd(const sarXattn& a, hipStream_t st) {
+template <int DP> static int launch_bwd(const sarXattn& a, hipStream_t st) {
     const BwdPlan p = bwd_plan(&a);
     const long bh = (long)a.B * a.Hkv, nq = (long)a.B * a.Tq * a.Hq * a.D, nk = (long)a.B * a.Tk * a.Hkv * a.D;
     float2* stats = reinterpret_cast<float2*>(a.ws);
@@ -445,16 +650,25 @@ template <int DP> static void launch_bwd(const sarXattn& a, hipStream_t st) {
     const bool few_q = paired<DP>() && p.few_q, few_k = paired<DP>() && p.few_k;
     const int rt = cdiv((long)a.Tq * (a.Hq / a.Hkv), few_q ? 64 : 128), kt = cdiv(a.Tk, few_k ? 64 : 128);
     const dim3 gq((unsigned)xcd_grid(rt * bh * p.dq_slices)), gk((unsigned)xcd_grid(kt * bh * p.dkv_slices));
-    const bool summed = sizeof(elt) == 2 && a.Tk <= SUMMED_KEYS;
+    const bool small = paired<DP>() && a.Tk > 0 && a.Tk <= SMALL_KEYS, summed = sizeof(elt) == 2 && a.Tk <= SUMMED_KEYS;
     if constexpr (paired<DP>()) {
-        if (few_q && !summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2, false>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
+        if (small) {
+            typedef Small<elt, DP> S;
+            static PerDeviceFlag raised;
+            if (S::LDS > 60 * 1024 && !raised) {
+                if (hipFuncSetAttribute(reinterpret_cast<const void*>(&xattn_small_bwd_kernel<elt, DP>), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess) return SAR_ELAUNCH;
+                raised = true;
+            }
+            hipLaunchKernelGGL((xattn_small_bwd_kernel<elt, DP>), dim3((unsigned)xcd_grid(bh * p.dkv_slices)), dim3(256), S::LDS, st, a, pk, p.dkv_slices);
+        }
+        if (!small && few_q && !summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2, false>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
     }
-    if (!few_q && !summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4, false>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
+    if (!small && !few_q && !summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4, false>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
     if constexpr (sizeof(elt) == 2) {
-        if (few_q && summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2, true>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
-        if (!few_q && summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4, true>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
+        if (!small && few_q && summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 2, true>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
+        if (!small && !few_q && summed) hipLaunchKernelGGL((xattn_dq_kernel<elt, DP, 4, true>), gq, dim3(256), 0, st, a, stats, pq, rt, p.dq_slices);
     }
-    if (kt) {
+    if (kt && !small) {
         if constexpr (paired<DP>()) {
             if (few_k) hipLaunchKernelGGL((xattn_dkv_kernel<elt, DP, 2>), gk, dim3(256), 0, st, a, stats, pk, kt, p.dkv_slices);
         }
@@ -470,6 +684,8 @@ template <int DP> static void launch_bwd(const sarXattn& a, hipStream_t st) {
     if (p.dq_slices > 1) sum(pq, a.dq, nq, p.dq_slices);
     if (kt && p.dkv_slices > 1) { sum(pk, a.dk, nk, p.dkv_slices); sum(pk + p.dkv_slices * nk, a.dv, nk, p.dkv_slices); }
     if (n) hipLaunchKernelGGL((xattn_sum_kernel<elt>), dim3((unsigned)(most < 2048 * 1024 ? cdiv(most, 1024) : 2048), n), dim3(256), 0, st, sums);
+    SAR_CHECK_LAUNCH();
+    return SAR_OK;
 }
 
 #if SAR_ELT == 0      // the same for every type
@@ -495,10 +711,5 @@ extern "C" int SAR_FN(sar_xattn_bwd)(const sarXattn* a, hipStream_t stream) {
     for (const void* p : {a->dout, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
         if ((uintptr_t)p % 16) return SAR_EINVAL;
     if (bad_strides(sizeof(elt), &a->g_sb, 3) || wide_rows(sizeof(elt), {a->g_st}) || bad_workspace(a, bwd_plan(a).bytes)) return SAR_EINVAL;
-    if (a->D <= 32) launch_bwd<32>(*a, stream);
-    else if (a->D <= 64) launch_bwd<64>(*a, stream);
-    else if (a->D <= 96) launch_bwd<96>(*a, stream);
-    else launch_bwd<128>(*a, stream);
-    SAR_CHECK_LAUNCH();
-    return SAR_OK;
+    return a->D <= 32 ? launch_bwd<32>(*a, stream) : a->D <= 64 ? launch_bwd<64>(*a, stream) : a->D <= 96 ? launch_bwd<96>(*a, stream) : launch_bwd<128>(*a, stream);
 }

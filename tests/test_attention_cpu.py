@@ -52,6 +52,17 @@ def test_c_refuses_missing_and_small_workspaces(sfx):
     assert L["sar_xattn_fwd_workspace_bytes"](ctypes.byref(_args(D=7))) == 0
 
 
+def test_c_workspace_sizes():
+    """No keys, one key, the largest calls: sizes that hold every slice and overflow nothing."""
+    from aesrc2020_amd import _lib
+    L = _lib.lib().fn
+    size = lambda **kw: L["sar_xattn_bwd_workspace_bytes"](ctypes.byref(_args(**kw)))  # noqa: E731
+    assert size(Tk=0) == 256 and size(Tk=1) == 256                 # {lse, delta} of 2 x 4 x 3 rows
+    assert size(B=1, Tq=1000, Tk=0) == 8 * 4000
+    assert size(B=1, Tq=100, Tk=4000, Hq=2) > 8 * 200 + 4 * 100 * 2 * 64                   # dQ in slices
+    assert size(B=1024, Hq=32, Hkv=32, Tq=4096, Tk=4096, D=128) == 8 * 1024 * 32 * 4096
+
+
 @pytest.mark.parametrize("sfx", ["f32", "bf16", "f16"])
 def test_c_cache_refuses(sfx):
     from aesrc2020_amd import _lib

@@ -102,7 +102,9 @@ SHAPES = [(1, 1, 1, 1, 1, 8, None, None),
           (3, 200, 7, 2, 2, 16, (7, 6, 0), None),
           (1, 9, 1500, 2, 1, 64, None, None),                      # few rows, many keys: dQ in key slices
           (2, 600, 5, 8, 1, 48, (5, 1), (600, 577)),               # few keys, many rows of shared heads: dK, dV in row slices
-          (1, 300, 1300, 6, 3, 128, None, None)]
+          (1, 300, 1300, 6, 3, 128, None, None),
+          (2, 130, 64, 4, 2, 128, (33, 32), (130, 64)), (3, 65, 33, 2, 2, 96, (33, 0, 2), (0, 65, 64)), (1, 300, 64, 3, 1, 24, None, None),
+          (1, 700, 64, 2, 1, 64, None, None)]
 
 
 @pytest.mark.parametrize("dt", DT)
