@@ -8,7 +8,7 @@
 // Backward, in pieces of the vocabulary: the piece's logits are computed again, turned into dz in the epilogue and written once in the
 // operand type; two more products read that piece (it stays in the last-level cache) for dx and dW.
 //
-// All products run on the 32x32x16 matrix instructions.  fp32 operands are two fp16 planes under one power-of-two scale per tensor that puts its
+// The products run on the 32x32x16 matrix instructions (small fp32 ones on the fp32 ones: direct()).  fp32 operands are two fp16 planes under one power-of-two scale per tensor that puts its
 // largest element in [2^13, 2^14): hi + lo hold 22 bits, hi hi + hi lo + lo hi is the product to 2^-22 or so of |a| |b|, at a third of the fp16 rate
 // (the fp32 matrix instructions run at a sixteenth).  dz is held in fp16: scaled by the power of two that puts the largest |g| in [1/2, 1), times
 // 2^14, every probability down to 2^-28 is a normal number with 11 bits; for bf16 the backward therefore takes x and W in fp16 too (under a scale as
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(1024) void absmax_kernel(MaxJobs jobs, float* __res
 
 struct PackJob { const elt* x; void* y; long rows, ld, plane; int cols, pitch; const float* part; };
 struct PackJobs { PackJob j[2]; };
-// rows of `cols` elements -> rows of `pitch` operand elements, zeros behind (planes hi, lo for fp32), for x and W (blockIdx.y)
+// rows of `cols` elements -> rows of `pitch` operand elements, zeros behind (planes hi, lo of scaled fp32), for x and W (blockIdx.y)
 template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_kernel(PackJobs jobs) {
     const PackJob j = jobs.j[blockIdx.y];
     const float f = SCALED ? ldexpf(1.f, up_exp(max_of(j.part))) : 1.f;
@@ -140,15 +140,19 @@ template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? p[k] : (elt)0.f;
         }
-        typename Num<OP>::x16 hi, lo;
+        constexpr int PER = Num<OP>::PER;
+        typename Num<OP>::x16 hi[8 / PER], lo[8 / PER];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const float s = SCALED ? (float)v[k] * f : (float)v[k];
-            hi[k] = (OP)s;
-            if constexpr (NPL == 2) lo[k] = (OP)(s - (float)hi[k]);
+            hi[k / PER][k % PER] = (OP)s;
+            if constexpr (SCALED && NPL == 2) lo[k / PER][k % PER] = (OP)(s - (float)hi[k / PER][k % PER]);
         }
-        *reinterpret_cast<typename Num<OP>::x16*>(y + r * j.pitch + c) = hi;
-        if constexpr (NPL == 2) *reinterpret_cast<typename Num<OP>::x16*>(y + j.plane + r * j.pitch + c) = lo;
+#pragma unroll
+        for (int q = 0; q < 8 / PER; ++q) {
+            *reinterpret_cast<typename Num<OP>::x16*>(y + r * j.pitch + c + q * PER) = hi[q];
+            if constexpr (SCALED && NPL == 2) *reinterpret_cast<typename Num<OP>::x16*>(y + j.plane + r * j.pitch + c + q * PER) = lo[q];
+        }
     }
 }
 
@@ -159,7 +163,7 @@ struct Side { const void* p; long plane, ld; int len, k; };
 // an operand's LDS tile of one stage: ROWS of the output's side, BK of the contraction; everything outside the tensor arrives as zeros
 // TAIL: the contraction may end inside a step (64 x 64 tiles; the larger ones' loads are 3 % slower with it and take packed operands instead)
 template <typename OP, int BK, int ROWS, bool DOWN, bool TAIL> struct Operand {
-    static constexpr int P = DOWN ? ROWS * 2 : BK * 2, LINES = DOWN ? BK : ROWS, BYTES = ROWS * BK * 2, N = attn::TileLoader<P, LINES>::N;
+    static constexpr int E = sizeof(OP), P = DOWN ? ROWS * E : BK * E, LINES = DOWN ? BK : ROWS, N = attn::TileLoader<P, LINES>::N;
     attn::TileLoader<P, LINES> loader;
     unsigned tail;                               // the loader's offsets for the last, shorter step along the contraction
     const OP* base;
@@ -167,19 +171,25 @@ template <typename OP, int BK, int ROWS, bool DOWN, bool TAIL> struct Operand {
     int lines, last;
     unsigned useful;
     __device__ __forceinline__ Operand(const Side& s, int i0)
-        : loader((unsigned)(s.ld * 2), DOWN ? (unsigned)min(ROWS, s.len - i0) * 2 : BK * 2), tail(attn::TileLoader<P, LINES>((unsigned)(s.ld * 2), DOWN ? 0 : (unsigned)(s.k % BK) * 2).first),
+        : loader((unsigned)(s.ld * E), DOWN ? (unsigned)min(ROWS, s.len - i0) * E : BK * E), tail(attn::TileLoader<P, LINES>((unsigned)(s.ld * E), DOWN ? 0 : (unsigned)(s.k % BK) * E).first),
           base(reinterpret_cast<const OP*>(s.p) + (DOWN ? i0 : i0 * s.ld)), ld(s.ld), lines(DOWN ? s.k : s.len - i0), last(DOWN ? 1 << 30 : s.k - BK),
-          useful(DOWN ? (unsigned)min(ROWS, s.len - i0) * 2 : BK * 2) {}
+          useful(DOWN ? (unsigned)min(ROWS, s.len - i0) * E : BK * E) {}
     __device__ __forceinline__ void load(int k, long plane, char* to, int wave) {
         const OP* p = base + plane + (DOWN ? k * ld : k);
         if constexpr (TAIL && !DOWN) {
             if (k > last) loader.first = tail;                    // (what lies behind is the next row; k only grows)
-            loader.load(p, k < last + BK ? lines : 0, (unsigned)(ld * 2), k <= last ? useful : (unsigned)(last + BK - k) * 2, to, wave);
-        } else loader.load(p, DOWN ? lines - k : lines, (unsigned)(ld * 2), useful, to, wave);
+            loader.load(p, k < last + BK ? lines : 0, (unsigned)(ld * E), k <= last ? useful : (unsigned)(last + BK - k) * E, to, wave);
+        } else loader.load(p, DOWN ? lines - k : lines, (unsigned)(ld * E), useful, to, wave);
     }
-    // operand fragment: 32 rows at i0, sixteen contraction elements at 16 s
+    // operand fragment: 32 rows at i0, sixteen (fp32: eight) contraction elements from the s-th such group on
     static __device__ __forceinline__ u32x4 fragment(const char* tile, int i0, int s, int lane) {
-        if constexpr (DOWN) {
+        if constexpr (DOWN && E == 4) {
+            const int i = i0 + (lane & 31), k = 8 * s + 4 * (lane >> 5);
+            u32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const unsigned*>(tile + chunk_at<P>(k + j, i >> 2) + (i & 3) * 4);
+            return v;
+        } else if constexpr (DOWN) {
             const int i = lane & 15, k = 16 * s + 8 * (lane >> 5) + (i >> 2), ch = (i0 >> 3) + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1), off = (i & 1) * 8;
             const u32x2 a = attn::tr16(tile + chunk_at<P>(k, ch) + off), b = attn::tr16(tile + chunk_at<P>(k + 4, ch) + off);
             return u32x4{a[0], a[1], b[0], b[1]};
@@ -232,7 +242,7 @@ __device__ __forceinline__ int dz_exp(const Epi& e) {             // dz is held 
 struct Job { Side A, B; Epi e; int mtiles, ntiles, ksteps, slices; };
 // PA, PB: planes of the operands (1, or 2: hi, lo); PZ: planes of the dz that E_DZ writes
 template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED, int PA, int PB, int PZ> struct Product {
-    static constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * 2, SB = BN * BK * 2, STAGE = PA * SA + PB * SB, ST = 49152 / STAGE < 4 ? (49152 / STAGE > 2 ? 49152 / STAGE : 2) : 4;
+    static constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * (int)sizeof(OP), SB = BN * BK * (int)sizeof(OP), STAGE = PA * SA + PB * SB, ST = 49152 / STAGE < 4 ? (49152 / STAGE > 2 ? 49152 / STAGE : 2) : 4;
     static constexpr int LDS = ST * STAGE;
     static __device__ __forceinline__ void run(char* lds, int block, const Job& job);
 };
@@ -290,7 +300,7 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
         if (s + ST - 1 < steps) load(s + ST - 1, lds + (cur == 0 ? ST - 1 : cur - 1) * STAGE);
         const char *ta = lds + cur * STAGE, *tb = ta + PA * SA;
 #pragma unroll
-        for (int q = 0; q < BK / 16; ++q) {
+        for (int q = 0; q < BK * (int)sizeof(OP) / 32; ++q) {
             u32x4 a[PA][MT], b[PB][NT];
 #pragma unroll
             for (int p = 0; p < PA; ++p)
@@ -424,11 +434,11 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
             if (__any(has && at >= 0 && at < 32 * MT)) place(has ? at : -1, [&](int i, int x) { acc[i][j][x] -= g; });
         }
         // through LDS into whole row pieces of the (rows, piece) array; the column sums (db) on the way
-        constexpr int CH = BM / 8, REP = BN * CH / 256;
-        static_assert(BN * BM * 2 <= ST * STAGE && 256 / CH * BM * 4 <= ST * STAGE, "");
-        float sum[8];
+        constexpr int E = sizeof(OP), PER = 16 / E, CH = BM / PER, REP = BN * CH / 256;
+        static_assert(BN * BM * E <= ST * STAGE && 256 / CH * BM * 4 <= ST * STAGE, "");
+        float sum[PER];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum[k] = 0.f;
+        for (int k = 0; k < PER; ++k) sum[k] = 0.f;
 #pragma unroll
         for (int p = 0; p < PZ; ++p) {
             __syncthreads();
@@ -445,23 +455,23 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
                             if constexpr (PZ == 2) acc[i][j][4 * a + x] -= (float)q[x];
                         }
                         const int c = mw + 32 * i + 8 * a + 4 * h;
-                        *reinterpret_cast<typename Num<OP>::x4*>(lds + chunk_at<BM * 2>(nw + 32 * j + (lane & 31), c >> 3) + (c & 4) * 2) = q;
+                        *reinterpret_cast<typename Num<OP>::x4*>(lds + chunk_at<BM * E>(nw + 32 * j + (lane & 31), c / PER) + c % PER * E) = q;
                     }
             __syncthreads();
 #pragma unroll
             for (int t = 0; t < REP; ++t) {
-                const int row = (threadIdx.x + 256 * t) / CH, ch = threadIdx.x % CH, r = n0 + row, c = m0 + ch * 8;
-                const auto q = *reinterpret_cast<const typename Num<OP>::x16*>(lds + chunk_at<BM * 2>(row, ch));
+                const int row = (threadIdx.x + 256 * t) / CH, ch = threadIdx.x % CH, r = n0 + row, c = m0 + ch * PER;
+                const auto q = *reinterpret_cast<const typename Num<OP>::x16*>(lds + chunk_at<BM * E>(row, ch));
                 if (r < e.Rp && c < e.dz_ld) *reinterpret_cast<typename Num<OP>::x16*>(reinterpret_cast<OP*>(e.dz) + p * e.dz_plane + (long)r * e.dz_ld + c) = q;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) sum[k] += (float)q[k];
+                for (int k = 0; k < PER; ++k) sum[k] += (float)q[k];
             }
         }
         if (e.db || e.db_out) {
             float* red = reinterpret_cast<float*>(lds);           // (256 / CH, BM)
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < 8; ++k) red[threadIdx.x / CH * BM + threadIdx.x % CH * 8 + k] = sum[k];
+            for (int k = 0; k < PER; ++k) red[threadIdx.x / CH * BM + threadIdx.x % CH * PER + k] = sum[k];
             __syncthreads();
             if ((int)threadIdx.x < BM && m0 + (int)threadIdx.x < e.dz_ld) {
                 float v = 0.f;
@@ -563,8 +573,10 @@ struct Plan {
     bool pack_x, pack_w;
     int piece, pieces;
     bool small_z, small_dx, small_dw;   // 64 x 64 tiles instead of 128 x 128
-    bool light;                         // bf16, all small: bf16 operands as they are and dz in two bf16 planes -- more products, but neither maxima nor packing
-    int dz_planes, g_from;
+    // operands of the inputs' type, as they are: more matrix cycles, but neither maxima nor packing.  bf16 where all tiles are small: dz in two bf16
+    // planes.  fp32 where the products are small (direct()): the fp32 matrix instructions.
+    bool light;
+    int dz_planes, g_from;              // (planes of two bytes)
     int dx_slices, dw_slices, lse_slices, db_slices;
     bool dx_parts;
     size_t parts, xo, wo, a, b, zl, dz, dxp, dwp, dbp, bytes;      // offsets
@@ -580,6 +592,14 @@ static int cut(long t, int ksteps) {
     return (int)(s < 1 || most < 1 ? 1 : s < most ? s : most);
 }
 
+// fp32: whether the fp32 matrix instructions on the operands as they are cost less than two more launches (maxima, packing) and the bytes those move, 12 for
+// each element of x and W.  R x D x V, us direct / packed.  Forward: 20 x 256 x 1000 12 / 16, 2496 x 256 x 1000 21 / 25, 1 x 512 x 20000 27 / 41, 256 x 512 x
+// 20000 54 / 54.  Backward, with three products: 20 x 256 x 1000 21 / 24, 500 x 256 x 1000 25 / 29, 2496 x 256 x 1000 58 / 50, 64 x 512 x 20000 64 / 73,
+// 128 rows 95 / 89; where W has to be copied all the same (its rows end inside a 16-byte piece), 16 x 512 x 20001: 78 / 70.
+static bool direct(const sarVocabCe* a, bool grad) {
+    const long work = (a->R + 63L) / 64 * 64 * a->D * a->V, elements = ((long)a->R + a->V) * a->D;
+    return SAR_ELT == 0 && work <= (grad ? (1L << 27) + (a->V % 4 ? 0 : 80 * elements) : (1L << 29) + 160 * elements);
+}
 constexpr int MOST = 1 << 22;
 static bool bad(const sarVocabCe* a) {
     return !a || a->R < 1 || a->D < 1 || a->V < 1 || a->R > MOST || a->D > (1 << 16) || a->V > MOST || (a->label_bytes != 4 && a->label_bytes != 8) || a->ldx < a->D || a->ldk < a->V ||
@@ -589,8 +609,9 @@ static Plan plan(const sarVocabCe* a, bool grad) {
     Plan p = {};
     p.Rp = up64(a->R); p.Dp = up64(a->D); p.Vp = up64(a->V);
     int cols = p.Vp;
+    p.light = direct(a, grad);                                    // (64 x 64 tiles in any case)
     if (!grad) {
-        p.small_z = small(a->V, a->R);
+        p.small_z = p.light || small(a->V, a->R);
         p.lse_slices = cdiv(a->V, p.small_z ? 64 : 128);
     } else {
         // a piece's dz: about 128 MB, which the 256 MB last-level cache holds between its writer and its two readers (8192 x 32000 x 1024: 2384 us;
@@ -601,20 +622,21 @@ static Plan plan(const sarVocabCe* a, bool grad) {
         p.piece = (int)(p.pieces == 1 ? p.Vp : cdiv(cdiv(a->V, p.pieces), 256) * 256L);
         p.pieces = cdiv(a->V, p.piece);
         cols = p.piece < p.Vp ? p.piece : p.Vp;
-        p.small_z = small(cols, p.Rp); p.small_dx = small(a->R, a->D); p.small_dw = small(a->D, cols);
+        p.small_z = p.light || small(cols, p.Rp); p.small_dx = p.light || small(a->R, a->D); p.small_dw = p.light || small(a->D, cols);
         p.dx_slices = cut(tiles(a->R, a->D, p.small_dx ? 64 : 128), cols / 32);
         p.dw_slices = cut(tiles(a->D, cols, p.small_dw ? 64 : 128), p.Rp / 32);
         p.db_slices = cdiv(p.Rp, p.small_z ? 64 : 128);
         p.dx_parts = p.dx_slices > 1 || p.pieces > 1;
-        p.light = SAR_ELT == 1 && p.small_z && p.small_dx && p.small_dw;
+        p.light |= SAR_ELT == 1 && p.small_z && p.small_dx && p.small_dw;
         p.dz_planes = p.light ? 2 : NPL;
         p.g_from = p.light ? G_ONE : BWD_SCALED || a->R > G_FEW ? G_PARTS : G_ROWS;
     }
     // operands are read where they lie when they have the products' type, their rows start on 4-byte boundaries (what a load into LDS needs) and
     // end with a whole 16-byte piece, or a whole step (Operand: TAIL), where they are read along the contraction (x, and W for dx)
-    const bool scaled = grad ? BWD_SCALED && !p.light : FWD_SCALED;
-    p.pack_x = scaled || a->D % (p.small_z ? 8 : 64) || a->ldx % 2 || (uintptr_t)a->x % 4;
-    p.pack_w = scaled || a->V % (!grad ? 2 : p.small_dx ? 8 : 64) || a->ldk % 2 || (uintptr_t)a->kernel % 4;
+    const bool scaled = !p.light && (grad ? BWD_SCALED : FWD_SCALED);
+    constexpr int PIECE = 16 / sizeof(elt), WORD = SAR_ELT == 0 ? 1 : 2;         // elements of 16 bytes, of 4
+    p.pack_x = scaled || a->D % (p.small_z ? PIECE : 64) || a->ldx % WORD || (uintptr_t)a->x % 4;
+    p.pack_w = scaled || a->V % (!grad ? WORD : p.small_dx ? PIECE : 64) || a->ldk % WORD || (uintptr_t)a->kernel % 4;
     size_t at = 0;
     const auto take = [&](size_t n) { const size_t o = at; at += up(n); return o; };
     p.parts = take(3 * PARTS * 4);
@@ -683,7 +705,8 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     if (a->ws_bytes < 0 || (size_t)a->ws_bytes < p.bytes) return SAR_EINVAL;
     char* ws = reinterpret_cast<char*>(a->ws);
     Side x, w;
-    operands<fwd16, FWD_SCALED>(a, p, false, x, w, st);
+    if (p.light) operands<elt, false>(a, p, false, x, w, st);
+    else operands<fwd16, FWD_SCALED>(a, p, false, x, w, st);
     w.len = p.pack_w ? p.Vp : a->V; w.k = a->D;
     x.len = a->R; x.k = p.pack_x ? p.Dp : a->D;
     Epi e = {};
@@ -693,7 +716,10 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     e.R = a->R; e.V = a->V; e.Rp = p.Rp;
     e.loss = a->loss; e.lse_out = a->lse;
     const Job z = job_of(w, x, e, a->V, a->R, p.Dp, step_of(true, false), 1, p.small_z);
-    product<fwd16, true, false, E_LSE, FWD_SCALED>(z, p.small_z, st);
+    if constexpr (SAR_ELT == 0) {
+        if (p.light) hipLaunchKernelGGL((product_kernel<elt, 32, 1, 1, true, false, E_LSE, false, 1, 1, 1>), dim3(blocks_of(z)), dim3(256), 0, st, z);
+    }
+    if (!p.light) product<fwd16, true, false, E_LSE, FWD_SCALED>(z, p.small_z, st);
     if (z.mtiles > 1) hipLaunchKernelGGL(finish_kernel, dim3((unsigned)cdiv(a->R, 16)), dim3(256), 0, st, e.pm, e.pl, e.zl, a->labels, a->label_bytes, a->loss, a->lse, a->R, p.Rp, a->V, p.lse_slices);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
@@ -706,9 +732,9 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
     char* ws = reinterpret_cast<char*>(a->ws);
     void* dz = ws + p.dz;
     Side x, w;
-    if (p.light) operands<fwd16, false>(a, p, true, x, w, st);
+    if (p.light) operands<elt, false>(a, p, true, x, w, st);
     else operands<bwd16, BWD_SCALED>(a, p, true, x, w, st);
-    const auto from = [](const Side& s, int v) { Side t = s; t.p = reinterpret_cast<const bwd16*>(s.p) + v; return t; };
+    const auto from = [&](const Side& s, int v) { Side t = s; t.p = reinterpret_cast<const char*>(s.p) + (long)v * (p.light ? (long)sizeof(elt) : 2); return t; };
     for (int i = 0; i < p.pieces; ++i) {
         const int v0 = i * p.piece, cols = a->V - v0 < p.piece ? a->V - v0 : p.piece, ld = up64(cols);
         const long plane = (long)p.Rp * ld;
@@ -724,8 +750,9 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         wz.len = (p.pack_w ? p.Vp : a->V) - v0; wz.k = a->D;
         xz.len = a->R; xz.k = p.pack_x ? p.Dp : a->D;
         const Job z = job_of(wz, xz, e, ld, p.Rp, p.Dp, step_of(true, false), 1, p.small_z);
-        if constexpr (SAR_ELT == 1) {
-            if (p.light) hipLaunchKernelGGL((product_kernel<fwd16, step_of(true, false), 1, 1, true, false, E_DZ, false, 1, 1, 2>), dim3(blocks_of(z)), dim3(256), 0, st, z);
+        constexpr int PZ = SAR_ELT == 1 ? 2 : 1;                  // planes of the light form's dz
+        if constexpr (SAR_ELT != 2) {
+            if (p.light) hipLaunchKernelGGL((product_kernel<elt, step_of(true, false), 1, 1, true, false, E_DZ, false, 1, 1, PZ>), dim3(blocks_of(z)), dim3(256), 0, st, z);
         }
         if (!p.light) product<bwd16, true, false, E_DZ, BWD_SCALED>(z, p.small_z, st);
         SumJobs sums = {};
@@ -760,8 +787,8 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         }
         const unsigned first = a->dkernel ? blocks_of(dw) : 0, both = first + (a->dx ? blocks_of(dx) : 0);
         if (p.light) {
-            if constexpr (SAR_ELT == 1)
-                if (both) hipLaunchKernelGGL((grads_kernel<fwd16, step_of(true, true, true), step_of(false, false, true), false, 1, 2>), dim3(both), dim3(256), 0, st, dw, dx, (int)first);
+            if constexpr (SAR_ELT != 2)
+                if (both) hipLaunchKernelGGL((grads_kernel<elt, step_of(true, true, true), step_of(false, false, true), false, 1, PZ>), dim3(both), dim3(256), 0, st, dw, dx, (int)first);
         } else if (a->dkernel && a->dx && p.small_dw && p.small_dx) {
             hipLaunchKernelGGL((grads_kernel<bwd16, step_of(true, true), step_of(false, false), BWD_SCALED, NPL, NPL>), dim3(both), dim3(256), 0, st, dw, dx, (int)first);
         } else {

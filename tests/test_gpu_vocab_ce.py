@@ -71,7 +71,7 @@ def check(got, want, bound, what):
     assert r.max().item() <= 1.0, (what, r.max().item(), (got.double() - want).abs().max().item())
 
 
-SHAPES = [(1, 1, 1), (1, 256, 1000), (5, 40, 11), (33, 32, 32), (64, 96, 257), (130, 131, 300), (300, 256, 1000), (77, 512, 4099), (700, 64, 5003), (2, 1024, 20000)]
+SHAPES = [(1, 1, 1), (1, 256, 1000), (5, 40, 11), (33, 32, 32), (64, 96, 257), (130, 131, 300), (300, 256, 1000), (77, 512, 4099), (700, 64, 5003), (2, 1024, 20000), (2600, 264, 1000), (40, 72, 30001), (4000, 36, 12), (65, 30, 999)]
 
 
 @pytest.mark.parametrize("dt", DT)
