@@ -51,10 +51,16 @@ template <typename T, int DP> constexpr int pitch() {
     return b <= 64 ? 64 : b <= 128 ? 128 : b <= 256 ? 256 : 512;
 }
 // 16-byte chunk `ch` of row `row`: eight consecutive rows put one chunk into eight different bank groups of 16 bytes (row-wise 16-byte
-// reads), four consecutive rows put a PAIR of chunks into four different ones (the transposing reads)
+// reads), four consecutive rows put a PAIR of chunks into four different ones (the transposing reads).  LDS hands out sixteen such groups a cycle, so
+// this costs twice the fewest cycles.  SIXTEEN (rows of 64 to 256 bytes): sixteen rows, and four rows a run of FOUR chunks, in different groups, no
+// conflict left -- for more address arithmetic: the vocabulary products gain 2 % by it; attention's loops, which need the registers, do not (8 x 1024
+// x 4096: dQ 391 -> 385 us, dK, dV 565 -> 595; fp32 64 x 72 x 39 28 -> 33).
 // (every bit of the swizzle is one bit of the row: the swizzle of a sum of rows without common bits is the two swizzles' xor)
-template <int PITCH> __device__ __forceinline__ constexpr int swizzle(int row) { return PITCH == 64 ? (row & 2) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1); }
-template <int PITCH> __device__ __forceinline__ int chunk_at(int row, int ch) { return row * PITCH + ((ch ^ swizzle<PITCH>(row)) << 4); }
+template <int PITCH, bool SIXTEEN = false> __device__ __forceinline__ constexpr int swizzle(int row) {
+    if constexpr (SIXTEEN) return PITCH == 64 ? (row >> 2) & 3 : PITCH == 128 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+    return PITCH == 64 ? (row & 2) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1);
+}
+template <int PITCH, bool SIXTEEN = false> __device__ __forceinline__ int chunk_at(int row, int ch) { return row * PITCH + ((ch ^ swizzle<PITCH, SIXTEEN>(row)) << 4); }
 // fragment of chunk c: row `row`
 template <int PITCH> __device__ __forceinline__ u32x4 frag(const char* tile, int row, int c, int h) {
     return *reinterpret_cast<const u32x4*>(tile + chunk_at<PITCH>(row, 2 * c + h));
@@ -149,12 +155,13 @@ __device__ __forceinline__ void dma16(u32x4 rsrc, unsigned offset, unsigned lds)
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // ROWS rows of `bytes` useful bytes each, `stride` bytes apart, by the block's four waves
-template <int PITCH, int ROWS> struct TileLoader {
+template <int PITCH, int ROWS, bool SIXTEEN = false> struct TileLoader {
+    static_assert(!SIXTEEN || PITCH <= 256, "a step of the loader is sixteen rows at least");
     static constexpr int CPR = PITCH / 16, ALL = ROWS * PITCH / 1024, N = (ALL + 3) / 4;
     unsigned first, step;
     __device__ __forceinline__ TileLoader(unsigned stride, unsigned bytes) {
         const int slot = threadIdx.x, row = slot / CPR, pos = slot % CPR;
-        const unsigned ch = pos ^ swizzle<PITCH>(row);            // the piece that belongs at `pos`
+        const unsigned ch = pos ^ swizzle<PITCH, SIXTEEN>(row);   // the piece that belongs at `pos`
         first = ch * 16 < bytes ? row * stride + ch * 16 : 0x80000000u;                        // behind the row: out of any range
         step = 256 / CPR * stride;
     }

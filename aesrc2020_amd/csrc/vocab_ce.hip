@@ -51,7 +51,7 @@ struct sarVocabCe {
 // one namespace per build: the templates below differ from build to build under the same arguments
 namespace SAR_FN(vce) {
 using attn::Num;
-using attn::chunk_at;
+template <int PITCH> __device__ __forceinline__ int chunk_at(int row, int ch) { return attn::chunk_at<PITCH, true>(row, ch); }
 using attn::as16;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -163,15 +163,15 @@ struct Side { const void* p; long plane, ld; int len, k; };
 // an operand's LDS tile of one stage: ROWS of the output's side, BK of the contraction; everything outside the tensor arrives as zeros
 // TAIL: the contraction may end inside a step (64 x 64 tiles; the larger ones' loads are 3 % slower with it and take packed operands instead)
 template <typename OP, int BK, int ROWS, bool DOWN, bool TAIL> struct Operand {
-    static constexpr int E = sizeof(OP), P = DOWN ? ROWS * E : BK * E, LINES = DOWN ? BK : ROWS, N = attn::TileLoader<P, LINES>::N;
-    attn::TileLoader<P, LINES> loader;
+    static constexpr int E = sizeof(OP), P = DOWN ? ROWS * E : BK * E, LINES = DOWN ? BK : ROWS, N = attn::TileLoader<P, LINES, true>::N;
+    attn::TileLoader<P, LINES, true> loader;
     unsigned tail;                               // the loader's offsets for the last, shorter step along the contraction
     const OP* base;
     long ld;
     int lines, last;
     unsigned useful;
     __device__ __forceinline__ Operand(const Side& s, int i0)
-        : loader((unsigned)(s.ld * E), DOWN ? (unsigned)min(ROWS, s.len - i0) * E : BK * E), tail(attn::TileLoader<P, LINES>((unsigned)(s.ld * E), DOWN ? 0 : (unsigned)(s.k % BK) * E).first),
+        : loader((unsigned)(s.ld * E), DOWN ? (unsigned)min(ROWS, s.len - i0) * E : BK * E), tail(attn::TileLoader<P, LINES, true>((unsigned)(s.ld * E), DOWN ? 0 : (unsigned)(s.k % BK) * E).first),
           base(reinterpret_cast<const OP*>(s.p) + (DOWN ? i0 : i0 * s.ld)), ld(s.ld), lines(DOWN ? s.k : s.len - i0), last(DOWN ? 1 << 30 : s.k - BK),
           useful(DOWN ? (unsigned)min(ROWS, s.len - i0) * E : BK * E) {}
     __device__ __forceinline__ void load(int k, long plane, char* to, int wave) {

@@ -61,6 +61,12 @@ template <int N> __device__ __forceinline__ void settle(u32x4 (&f)[N]) {
 #pragma unroll
     for (int c = 0; c < N; ++c) asm volatile("" : "+v"(f[c]));
 }
+// The lane's number as a value the compiler knows nothing of: what depends on it (the tile reads' addresses) is computed again in every step instead of
+// being held in registers, where those are short.
+template <bool SHORT> __device__ __forceinline__ int again(int lane) {
+    if constexpr (SHORT) asm volatile("" : "+v"(lane));
+    return lane;
+}
 // the row tiles of a group's heads, one head after the other
 struct RowTile { int g, t; };
 __device__ __forceinline__ RowTile after(RowTile r, int rows, int tl) { return r.t + rows >= tl ? RowTile{r.g + 1, 0} : RowTile{r.g, r.t + rows}; }
@@ -259,6 +265,7 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
             const int at = 32 * (u * WM + wm);
+            const int lane = again<SUMMED && DP == 128>(threadIdx.x & 63), h = lane >> 5, n = lane & 31;
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
             for (int c = 0; c < NC; ++c) s = mma<T>(frag<P>(lk, at + n, c, h), qf[c], s);
@@ -501,6 +508,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256, 2) void xattn_sm
             next_row = after(at_row, RT, tl);
             next = load_lse(i + 2 < i1 ? next_row : at_row);
         }
+        const int lane = again<sizeof(T) == 2 && DP == 128>(threadIdx.x & 63), h = lane >> 5, n = lane & 31, key = key0 + n;
         const bool live = key0 < len && t + 32 * wm < tl;
         const char *lq = tiles_at + cur, *lg = tiles_at + cur + TILE;
         const float* ex = exponent[par] + 32 * wm;
