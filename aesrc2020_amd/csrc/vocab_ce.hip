@@ -655,10 +655,11 @@ static Plan plan(const sarVocabCe* a, bool grad) {
     return p;
 }
 
-// contraction elements per LDS stage.  64 (two stages) where an operand is read along the contraction on both sides -- whole 128-byte lines -- or on
-// neither: dx 189 -> 159 us, dW 158 -> 141 us for an 8192 x 8192 piece against 1024; 32 (three stages, three blocks per CU) for the logits:
-// 595 against 614 us for 8192 x 32000 x 1024.  fp32 (two planes): 32.
-constexpr int step_of(bool ad, bool bd, bool planes = NPL == 2) { return planes || ad != bd ? 32 : 64; }
+// contraction elements per LDS stage: 64, two stages (whole 128-byte lines where an operand is read along the contraction; half the barriers) -- an 8192 x
+// 8192 piece against 1024, us with 64 / with 32: dx 147 / 183, dW 128 / 143, dz 158 / 160, the logits of 8192 x 32000 525 / 548.  fp32 (two planes): 32.
+// Logits of a shorter contraction on 128 x 128 tiles: 32 with three stages, whose blocks start and end beside two others (777 x 512 x 40001: 57 / 53).
+constexpr int step_of(bool planes = NPL == 2) { return planes ? 32 : 64; }
+static int logits_step(const sarVocabCe* a, bool small_tiles) { return small_tiles || a->D > 768 ? step_of() : 32; }
 static unsigned some_blocks(long n) { return (unsigned)(n < 1 ? 1 : n < 4096 ? n : 4096); }
 // the operands as the products read them
 template <typename OP, bool SCALED> static void operands(const sarVocabCe* a, const Plan& p, bool grad, Side& x, Side& w, hipStream_t st) {
@@ -687,10 +688,11 @@ static Job job_of(Side A, Side B, const Epi& e, int m, int n, int k, int step, i
     return {A, B, e, cdiv(m, t), cdiv(n, t), cdiv(k, step), slices};
 }
 static unsigned blocks_of(const Job& j) { return (unsigned)attn::xcd_grid((long)j.mtiles * j.ntiles * j.slices); }
-template <typename OP, bool AD, bool BD, int EPI, bool SCALED> static void product(const Job& j, bool small_tiles, hipStream_t st) {
-    constexpr int BK = step_of(AD, BD);
+template <typename OP, bool AD, bool BD, int EPI, bool SCALED> static void product(const Job& j, bool small_tiles, int step, hipStream_t st) {
+    constexpr int BK = step_of();
     if (small_tiles) hipLaunchKernelGGL((product_kernel<OP, BK, 1, 1, AD, BD, EPI, SCALED, NPL, NPL, NPL>), dim3(blocks_of(j)), dim3(256), 0, st, j);
-    else hipLaunchKernelGGL((product_kernel<OP, BK, 2, 2, AD, BD, EPI, SCALED, NPL, NPL, NPL>), dim3(blocks_of(j)), dim3(256), 0, st, j);
+    else if (EPI == E_GRAD || step == BK) hipLaunchKernelGGL((product_kernel<OP, BK, 2, 2, AD, BD, EPI, SCALED, NPL, NPL, NPL>), dim3(blocks_of(j)), dim3(256), 0, st, j);
+    else if constexpr (EPI != E_GRAD) hipLaunchKernelGGL((product_kernel<OP, 32, 2, 2, AD, BD, EPI, SCALED, NPL, NPL, NPL>), dim3(blocks_of(j)), dim3(256), 0, st, j);
 }
 
 }
@@ -715,11 +717,12 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     e.pm = reinterpret_cast<float*>(ws + p.a); e.pl = reinterpret_cast<float*>(ws + p.b); e.zl = reinterpret_cast<float*>(ws + p.zl);
     e.R = a->R; e.V = a->V; e.Rp = p.Rp;
     e.loss = a->loss; e.lse_out = a->lse;
-    const Job z = job_of(w, x, e, a->V, a->R, p.Dp, step_of(true, false), 1, p.small_z);
+    const int step = logits_step(a, p.small_z);
+    const Job z = job_of(w, x, e, a->V, a->R, p.Dp, p.light ? 32 : step, 1, p.small_z);
     if constexpr (SAR_ELT == 0) {
         if (p.light) hipLaunchKernelGGL((product_kernel<elt, 32, 1, 1, true, false, E_LSE, false, 1, 1, 1>), dim3(blocks_of(z)), dim3(256), 0, st, z);
     }
-    if (!p.light) product<fwd16, true, false, E_LSE, FWD_SCALED>(z, p.small_z, st);
+    if (!p.light) product<fwd16, true, false, E_LSE, FWD_SCALED>(z, p.small_z, step, st);
     if (z.mtiles > 1) hipLaunchKernelGGL(finish_kernel, dim3((unsigned)cdiv(a->R, 16)), dim3(256), 0, st, e.pm, e.pl, e.zl, a->labels, a->label_bytes, a->loss, a->lse, a->R, p.Rp, a->V, p.lse_slices);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
@@ -749,12 +752,13 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         Side wz = from(w, v0), xz = x;
         wz.len = (p.pack_w ? p.Vp : a->V) - v0; wz.k = a->D;
         xz.len = a->R; xz.k = p.pack_x ? p.Dp : a->D;
-        const Job z = job_of(wz, xz, e, ld, p.Rp, p.Dp, step_of(true, false), 1, p.small_z);
+        const int step = logits_step(a, p.small_z);
+        const Job z = job_of(wz, xz, e, ld, p.Rp, p.Dp, step, 1, p.small_z);
         constexpr int PZ = SAR_ELT == 1 ? 2 : 1;                  // planes of the light form's dz
         if constexpr (SAR_ELT != 2) {
-            if (p.light) hipLaunchKernelGGL((product_kernel<elt, step_of(true, false), 1, 1, true, false, E_DZ, false, 1, 1, PZ>), dim3(blocks_of(z)), dim3(256), 0, st, z);
+            if (p.light) hipLaunchKernelGGL((product_kernel<elt, step_of(), 1, 1, true, false, E_DZ, false, 1, 1, PZ>), dim3(blocks_of(z)), dim3(256), 0, st, z);
         }
-        if (!p.light) product<bwd16, true, false, E_DZ, BWD_SCALED>(z, p.small_z, st);
+        if (!p.light) product<bwd16, true, false, E_DZ, BWD_SCALED>(z, p.small_z, step, st);
         SumJobs sums = {};
         int ns = 0;
         long blocks = 0;
@@ -773,7 +777,7 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
                 o.out = ws + p.dwp; o.slice = (long)a->D * ld; o.ldo = ld;
                 sum(p.dwp, p.dw_slices, o.slice, a->D, cols, ld, out, a->V, a->accumulate);
             } else { o.out = out; o.ldo = a->V; o.accumulate = a->accumulate; }
-            dw = job_of(A, B, o, a->D, cols, p.Rp, step_of(true, true, p.dz_planes == 2), p.dw_slices, p.small_dw);
+            dw = job_of(A, B, o, a->D, cols, p.Rp, step_of(p.dz_planes == 2), p.dw_slices, p.small_dw);
         }
         if (a->dx) {
             Epi o = e;
@@ -783,17 +787,17 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
                 o.out = ws + p.dxp; o.slice = (long)a->R * a->D; o.accumulate = i > 0;
                 if (i == p.pieces - 1) sum(p.dxp, p.dx_slices, o.slice, a->R, a->D, a->D, reinterpret_cast<elt*>(a->dx), a->D, 0);
             } else o.out = a->dx;
-            dx = job_of(A, B, o, a->R, a->D, ld, step_of(false, false, p.dz_planes == 2), p.dx_slices, p.small_dx);
+            dx = job_of(A, B, o, a->R, a->D, ld, step_of(p.dz_planes == 2), p.dx_slices, p.small_dx);
         }
         const unsigned first = a->dkernel ? blocks_of(dw) : 0, both = first + (a->dx ? blocks_of(dx) : 0);
         if (p.light) {
             if constexpr (SAR_ELT != 2)
-                if (both) hipLaunchKernelGGL((grads_kernel<elt, step_of(true, true, true), step_of(false, false, true), false, 1, PZ>), dim3(both), dim3(256), 0, st, dw, dx, (int)first);
+                if (both) hipLaunchKernelGGL((grads_kernel<elt, step_of(true), step_of(true), false, 1, PZ>), dim3(both), dim3(256), 0, st, dw, dx, (int)first);
         } else if (a->dkernel && a->dx && p.small_dw && p.small_dx) {
-            hipLaunchKernelGGL((grads_kernel<bwd16, step_of(true, true), step_of(false, false), BWD_SCALED, NPL, NPL>), dim3(both), dim3(256), 0, st, dw, dx, (int)first);
+            hipLaunchKernelGGL((grads_kernel<bwd16, step_of(), step_of(), BWD_SCALED, NPL, NPL>), dim3(both), dim3(256), 0, st, dw, dx, (int)first);
         } else {
-            if (a->dkernel) product<bwd16, true, true, E_GRAD, BWD_SCALED>(dw, p.small_dw, st);
-            if (a->dx) product<bwd16, false, false, E_GRAD, BWD_SCALED>(dx, p.small_dx, st);
+            if (a->dkernel) product<bwd16, true, true, E_GRAD, BWD_SCALED>(dw, p.small_dw, step_of(), st);
+            if (a->dx) product<bwd16, false, false, E_GRAD, BWD_SCALED>(dx, p.small_dx, step_of(), st);
         }
         if (a->dbias && p.db_slices > 1) sum(p.dbp, p.db_slices, ld, 1, cols, ld, reinterpret_cast<elt*>(a->dbias) + v0, cols, a->accumulate);
         if (ns) hipLaunchKernelGGL(sum_slices_kernel, dim3(some_blocks(blocks), ns), dim3(256), 0, st, sums);
