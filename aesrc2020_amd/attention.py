@@ -5,7 +5,6 @@ is the single-token form, EncoderCache8 holds an utterance's keys and values in 
 Everything runs on the current HIP stream of the tensors' device, allocates through torch (so calls can be captured into a HIP graph) and
 raises ValueError for arguments it does not take.  layers.CrossAttention is the Layer over the same calls."""
 import ctypes
-import math
 import struct
 
 import torch
@@ -24,6 +23,8 @@ class Xattn(ctypes.Structure):
 
 
 _XATTN = struct.Struct("12Ql15l6ifi")                                  # the same fields: packing bytes costs a fifth of filling the Structure
+_WS, _WS_AT = struct.Struct("Ql"), Xattn.ws.offset
+_NAMES = {n: {d: "sar_%s_%s" % (n, s) for d, s in _SFX.items()} for n in ("xattn_fwd", "xattn_bwd", "kv8_attend")}
 
 
 def _rows(name, x, like=None):
@@ -71,15 +72,13 @@ def _launch(name, device, *args):
         raise RuntimeError("%s failed with status %d" % (name, rc))
 
 
-def _xattn(query, device, ptrs, strides, sizes, scale, may_need):
-    """sarXattn as bytes, with a workspace where the call needs one -> (bytes, workspace to keep until the launch)."""
-    scale = 1.0 / math.sqrt(sizes[5]) if scale is None else float(scale)
-    a = _XATTN.pack(*ptrs, 0, 0, *strides, *sizes, scale, 0)
-    n = _lib.lib().fn[query](a) if may_need else 0
+def _with_workspace(query, device, a):
+    """sarXattn as bytes -> the same with a workspace where the call needs one, and the workspace to keep until the launch."""
+    n = _lib.lib().fn[query](a)
     if not n:
         return a, None
     ws = torch.empty(n, dtype=torch.uint8, device=device)
-    return _XATTN.pack(*ptrs, ws.data_ptr(), n, *strides, *sizes, scale, 0), ws
+    return a[:_WS_AT] + _WS.pack(ws.data_ptr(), n) + a[_WS_AT + _WS.size:], ws
 
 
 def _result(name, t, shape, dtype, device):
@@ -88,6 +87,15 @@ def _result(name, t, shape, dtype, device):
     if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device or not t.is_contiguous() or t.data_ptr() % 16:
         raise ValueError("%s has to be a contiguous, 16-byte aligned %s tensor of shape %r on %s" % (name, dtype, tuple(shape), device))
     return t
+
+
+def _result_like(name, t, q):
+    """`t`, or a new tensor, of q's shape and type, contiguous (empty_like is the faster call; q's rows are aligned: _rows)."""
+    return torch.empty_like(q) if t is None and q.is_contiguous() else _result(name, t, q.shape, q.dtype, q.device)
+
+
+def _scale(scale, D):
+    return D ** -0.5 if scale is None else float(scale)
 
 
 def _check_kv(q, k, v):
@@ -109,17 +117,19 @@ def cross_attention(q, k, v, k_lens=None, q_lens=None, scale=None, return_lse=Fa
     q = _rows("q", q)
     k, v = _check_kv(q, k, v)
     B, Tq, Hq, D = q.shape
-    Tk, Hkv = k.shape[1], k.shape[2]
-    out = _result("out", out, (B, Tq, Hq, D), q.dtype, q.device)
+    Tk, Hkv, device = k.shape[1], k.shape[2], q.device
+    out = _result_like("out", out, q)
     if return_lse or lse is not None:
-        lse = _result("lse", lse, (B, Hq, Tq), torch.float32, q.device)
-    kl, ql = _lens("k_lens", k_lens, B, q.device), _lens("q_lens", q_lens, B, q.device)
-    if out.numel():
-        qp = q.data_ptr()
-        ptrs = (qp, k.data_ptr() if Tk else qp, v.data_ptr() if Tk else qp, 0, out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, kl, ql)      # (no frames: never read)
-        a, ws = _xattn("sar_xattn_fwd_workspace_bytes", q.device, ptrs, q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + out.stride()[:3] + (0, 0, 0),
-                       (B, Tq, Tk, Hq, Hkv, D), scale, Tk > 256)       # (sarnet.h: 256 keys never need one)
-        _launch("sar_xattn_fwd_" + _SFX[q.dtype], q.device, a)
+        lse = _result("lse", lse, (B, Hq, Tq), torch.float32, device)
+    kl = 0 if k_lens is None else _lens("k_lens", k_lens, B, device)
+    ql = 0 if q_lens is None else _lens("q_lens", q_lens, B, device)
+    if B and Tq:
+        qp, sq, sk, sv, so = q.data_ptr(), q.stride(), k.stride(), v.stride(), out.stride()
+        a = _XATTN.pack(qp, k.data_ptr() if Tk else qp, v.data_ptr() if Tk else qp, 0, out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, kl, ql, 0, 0,      # (no frames: never read)
+                        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], so[0], so[1], so[2], 0, 0, 0, B, Tq, Tk, Hq, Hkv, D, _scale(scale, D), 0)
+        if Tk > 256:                                                   # (sarnet.h: 256 keys never need a workspace)
+            a, ws = _with_workspace("sar_xattn_fwd_workspace_bytes", device, a)
+        _launch(_NAMES["xattn_fwd"][q.dtype], device, a)
     return (out, lse) if return_lse else out
 
 
@@ -131,22 +141,23 @@ def cross_attention_grad(dout, q, k, v, out, lse, k_lens=None, q_lens=None, scal
     k, v = _check_kv(q, k, v)
     dout, out = _rows("dout", dout, q), _rows("out", out, q)
     B, Tq, Hq, D = q.shape
-    Tk, Hkv = k.shape[1], k.shape[2]
+    Tk, Hkv, device = k.shape[1], k.shape[2], q.device
     if dout.shape != q.shape or out.shape != q.shape:
         raise ValueError("dout %r and out %r have to have the shape of q %r" % (tuple(dout.shape), tuple(out.shape), tuple(q.shape)))
-    lse = _result("lse", lse, (B, Hq, Tq), torch.float32, q.device)
-    dq = _result("dq", dq, q.shape, q.dtype, q.device)
-    dk, dv = _result("dk", dk, k.shape, q.dtype, q.device), _result("dv", dv, v.shape, q.dtype, q.device)
-    kl, ql = _lens("k_lens", k_lens, B, q.device), _lens("q_lens", q_lens, B, q.device)
+    lse = _result("lse", lse, (B, Hq, Tq), torch.float32, device)
+    dq = _result_like("dq", dq, q) if B and Tq else _result("dq", dq, q.shape, q.dtype, device)
+    dk, dv = _result("dk", dk, k.shape, q.dtype, device), _result("dv", dv, v.shape, q.dtype, device)
+    kl = 0 if k_lens is None else _lens("k_lens", k_lens, B, device)
+    ql = 0 if q_lens is None else _lens("q_lens", q_lens, B, device)
     if Tq == 0:
         dk.zero_(); dv.zero_()
-    elif q.numel():
-        qp = q.data_ptr()
-        ptrs = (qp, k.data_ptr() if Tk else qp, v.data_ptr() if Tk else qp, dout.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(),
-                dk.data_ptr() if Tk else qp, dv.data_ptr() if Tk else qp, kl, ql)                # (no frames: never read or written)
-        a, ws = _xattn("sar_xattn_bwd_workspace_bytes", q.device, ptrs, q.stride()[:3] + k.stride()[:3] + v.stride()[:3] + out.stride()[:3] + dout.stride()[:3],
-                       (B, Tq, Tk, Hq, Hkv, D), scale, True)
-        _launch("sar_xattn_bwd_" + _SFX[q.dtype], q.device, a)
+    elif B:
+        qp, sq, sk, sv, so, sg = q.data_ptr(), q.stride(), k.stride(), v.stride(), out.stride(), dout.stride()
+        a = _XATTN.pack(qp, k.data_ptr() if Tk else qp, v.data_ptr() if Tk else qp, dout.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(),
+                        dk.data_ptr() if Tk else qp, dv.data_ptr() if Tk else qp, kl, ql, 0, 0,  # (no frames: never read or written)
+                        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], so[0], so[1], so[2], sg[0], sg[1], sg[2], B, Tq, Tk, Hq, Hkv, D, _scale(scale, D), 0)
+        a, ws = _with_workspace("sar_xattn_bwd_workspace_bytes", device, a)
+        _launch(_NAMES["xattn_bwd"][q.dtype], device, a)
     return dq, dk, dv
 
 
@@ -192,13 +203,18 @@ class EncoderCache8:
         -> out of q's type.  Made for a few rows (Tq Hq / heads); each 32 of them read the cache once."""
         q = _rows("q", q)
         B, Tq, Hq, D = q.shape
-        if B != self.batch or D != self.dim or q.device != self.device:
-            raise ValueError("q %r on %s does not fit a cache of %d utterances, %d heads of %d on %s" % (tuple(q.shape), q.device, self.batch, self.heads, self.dim, self.device))
-        _heads(Hq, self.heads, D)
-        out = _result("out", out, q.shape, q.dtype, q.device)
-        if out.numel():
-            ptrs = (q.data_ptr(), 0, 0, 0, out.data_ptr(), 0, 0, 0, 0, self.lens.data_ptr(), _lens("q_lens", q_lens, B, q.device))
-            a, ws = _xattn("sar_kv8_attend_workspace_bytes", q.device, ptrs, q.stride()[:3] + (0,) * 6 + out.stride()[:3] + (0, 0, 0),
-                           (B, Tq, self.frames, Hq, self.heads, D), scale, self.frames > 256)
-            _launch("sar_kv8_attend_" + _SFX[q.dtype], q.device, a, self.k8.data_ptr(), self.k_scale.data_ptr(), self.v8.data_ptr(), self.v_scale.data_ptr(), self.k8.shape[2])
+        device = q.device
+        if B != self.batch or D != self.dim or device != self.device:
+            raise ValueError("q %r on %s does not fit a cache of %d utterances, %d heads of %d on %s" % (tuple(q.shape), device, self.batch, self.heads, self.dim, self.device))
+        if Hq < 1 or Hq % self.heads:
+            _heads(Hq, self.heads, D)
+        out = _result_like("out", out, q)
+        ql = 0 if q_lens is None else _lens("q_lens", q_lens, B, device)
+        if Tq:
+            s, so = q.stride(), out.stride()
+            a = _XATTN.pack(q.data_ptr(), 0, 0, 0, out.data_ptr(), 0, 0, 0, 0, self.lens.data_ptr(), ql, 0, 0, s[0], s[1], s[2], 0, 0, 0, 0, 0, 0, so[0], so[1], so[2], 0, 0, 0,
+                            B, Tq, self.frames, Hq, self.heads, D, _scale(scale, D), 0)
+            if self.frames > 256:
+                a, ws = _with_workspace("sar_kv8_attend_workspace_bytes", device, a)
+            _launch(_NAMES["kv8_attend"][q.dtype], device, a, self.k8.data_ptr(), self.k_scale.data_ptr(), self.v8.data_ptr(), self.v_scale.data_ptr(), self.k8.shape[2])
         return out
