@@ -8,8 +8,8 @@
 // Backward, in pieces of the vocabulary: the piece's logits are computed again, turned into dz in the epilogue and written once in the
 // operand type; two more products read that piece (it stays in the last-level cache) for dx and dW.
 //
-// The products run on the 32x32x16 matrix instructions (small fp32 ones on the fp32 ones: direct()).  fp32 operands are two fp16 planes under one power-of-two scale per tensor that puts its
-// largest element in [2^13, 2^14): hi + lo hold 22 bits, hi hi + hi lo + lo hi is the product to 2^-22 or so of |a| |b|, at a third of the fp16 rate
+// The products run on the 32x32x16 matrix instructions (small fp32 ones on the fp32 ones: direct()).
+// fp32 operands are two fp16 planes under one power-of-two scale per tensor that puts its largest element in [2^13, 2^14): hi + lo hold 22 bits, hi hi + hi lo + lo hi is the product to 2^-22 or so of |a| |b|, at a third of the fp16 rate
 // (the fp32 matrix instructions run at a sixteenth).  dz is held in fp16: scaled by the power of two that puts the largest |g| in [1/2, 1), times
 // 2^14, every probability down to 2^-28 is a normal number with 11 bits; for bf16 the backward therefore takes x and W in fp16 too (under a scale as
 // above their 8 bits are exact), which leaves the gradients the accuracy of their own rounding.

@@ -10,7 +10,7 @@ import struct
 import torch
 
 from . import _lib
-from .attention import _SFX, _launch, _result
+from .attention import _SFX, _WS, _launch, _result
 from .engine import glorot_uniform
 from .layers import Layer
 
@@ -154,37 +154,45 @@ class _VocabCe(ctypes.Structure):
 
 
 _VOCAB_CE = struct.Struct("11Q3l6i")                                        # the same fields as bytes
+_WS_AT = _VocabCe.ws.offset
+_LABELS = {torch.int32: 4, torch.int64: 8}
 
 
 def _vocab_args(x, kernel, labels, bias):
-    """-> x, kernel (rows contiguous), bias, labels as the kernels take them."""
-    if x.dim() != 2 or kernel.dim() != 2 or x.shape[1] != kernel.shape[0] or kernel.shape[1] < 1 or kernel.shape[0] < 1:
-        raise ValueError("x %r and kernel %r have to be (rows, D) and (D, vocabulary)" % (tuple(x.shape), tuple(kernel.shape)))
-    if x.dtype not in _SFX or not x.is_cuda:
-        raise ValueError("x has to be a float32, bfloat16 or float16 tensor on a HIP device, got %s on %s" % (x.dtype, x.device))
-    if kernel.dtype != x.dtype or kernel.device != x.device:
-        raise ValueError("kernel is %s on %s, x is %s on %s" % (kernel.dtype, kernel.device, x.dtype, x.device))
-    R, (D, V) = x.shape[0], kernel.shape
-    if bias is not None and (tuple(bias.shape) != (V,) or bias.dtype != x.dtype or bias.device != x.device or not bias.is_contiguous()):
-        raise ValueError("bias has to be a contiguous %s tensor of %d values on %s" % (x.dtype, V, x.device))
-    if tuple(labels.shape) != (R,) or labels.dtype not in (torch.int32, torch.int64) or labels.device != x.device or not labels.is_contiguous():
-        raise ValueError("labels have to be a contiguous int32 or int64 tensor of %d values on %s" % (R, x.device))
+    """-> x, kernel (rows contiguous), R, D, V: as the kernels take them."""
+    xs, ks = x.shape, kernel.shape
+    if len(xs) != 2 or len(ks) != 2 or xs[1] != ks[0] or ks[0] < 1 or ks[1] < 1:
+        raise ValueError("x %r and kernel %r have to be (rows, D) and (D, vocabulary)" % (tuple(xs), tuple(ks)))
+    R, D, V = xs[0], ks[0], ks[1]
+    dtype, device = x.dtype, x.device
+    if dtype not in _SFX or not x.is_cuda:
+        raise ValueError("x has to be a float32, bfloat16 or float16 tensor on a HIP device, got %s on %s" % (dtype, device))
+    if kernel.dtype != dtype or kernel.device != device:
+        raise ValueError("kernel is %s on %s, x is %s on %s" % (kernel.dtype, kernel.device, dtype, device))
+    if bias is not None and (bias.shape != (V,) or bias.dtype != dtype or bias.device != device or not bias.is_contiguous()):
+        raise ValueError("bias has to be a contiguous %s tensor of %d values on %s" % (dtype, V, device))
+    if labels.shape != (R,) or labels.dtype not in _LABELS or labels.device != device or not labels.is_contiguous():
+        raise ValueError("labels have to be a contiguous int32 or int64 tensor of %d values on %s" % (R, device))
     if R > 1 << 22 or V > 1 << 22 or D > 1 << 16 or (R // 64 + 1) * (V // 64 + 1) > 1 << 28:
         raise ValueError("%d rows, %d wide, over %d classes: at most 2^22, 2^16 and 2^22 are taken, and 2^40 logits" % (R, D, V))
-    x = x if x.stride(1) == 1 and D <= x.stride(0) <= 1 << 22 or R == 0 else x.clone(memory_format=torch.contiguous_format)
-    kernel = kernel if kernel.stride(1) == 1 and V <= kernel.stride(0) <= 1 << 22 else kernel.clone(memory_format=torch.contiguous_format)
-    return x, kernel, bias
+    step, one = x.stride()
+    if R and (one != 1 or not D <= step <= 1 << 22):
+        x = x.clone(memory_format=torch.contiguous_format)
+    step, one = kernel.stride()
+    if one != 1 or not V <= step <= 1 << 22:
+        kernel = kernel.clone(memory_format=torch.contiguous_format)
+    return x, kernel, R, D, V
 
 
-def _vocab_launch(direction, x, kernel, labels, ptrs, sizes):
-    """ptrs: dloss .. dbias; sizes: R, D, V, bytes of a label, accumulate."""
-    name = "sar_vocab_ce_%s_%s" % (direction, _SFX[x.dtype])
-    R, D, V = sizes[:3]
-    args = (x.stride(0) if R > 1 else D, kernel.stride(0) if D > 1 else V, *sizes, 0)
-    ptrs = (x.data_ptr(), kernel.data_ptr(), ptrs[0], labels.data_ptr(), *ptrs[1:])
-    n = _lib.lib().fn[name + "_workspace_bytes"](_VOCAB_CE.pack(*ptrs, 0, 0, *args))
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device)                  # (torch's blocks are 512-byte aligned)
-    _launch(name, x.device, _VOCAB_CE.pack(*ptrs, ws.data_ptr(), n, *args))
+def _vocab_launch(direction, x, kernel, labels, bias, dloss, loss, lse, dx, dkernel, dbias, R, D, V, accumulate=0):
+    dtype, device = x.dtype, x.device
+    name = "sar_vocab_ce_%s_%s" % (direction, _SFX[dtype])
+    args = (x.data_ptr(), kernel.data_ptr(), _ptr(bias), labels.data_ptr(), _ptr(dloss), _ptr(loss), _ptr(lse), _ptr(dx), _ptr(dkernel), _ptr(dbias), 0, 0,
+            x.stride(0) if R > 1 else D, kernel.stride(0) if D > 1 else V, R, D, V, _LABELS[labels.dtype], accumulate, 0)
+    a = _VOCAB_CE.pack(*args)
+    n = _lib.lib().fn[name + "_workspace_bytes"](a)
+    ws = torch.empty(n, dtype=torch.uint8, device=device)                    # (torch's blocks are 512-byte aligned)
+    _launch(name, device, a[:_WS_AT] + _WS.pack(ws.data_ptr(), n) + a[_WS_AT + _WS.size:])
 
 
 def _ptr(t):
@@ -196,23 +204,22 @@ def vocab_crossentropy(x, kernel, labels, bias=None, return_lse=False, loss=None
 
     x (R, D) hidden rows, kernel (D, V) in the Dense layout, bias (V) or None: all fp32, bf16 or fp16; labels (R) int32 or int64, a label outside
     [0, V) leaves its row out (loss 0).  -> loss (R) fp32, and with return_lse the rows' log-sum-exp (R) fp32 that vocab_crossentropy_grad needs."""
-    x, kernel, bias = _vocab_args(x, kernel, labels, bias)
-    R, (D, V) = x.shape[0], kernel.shape
+    x, kernel, R, D, V = _vocab_args(x, kernel, labels, bias)
     loss = _result("loss", loss, (R,), torch.float32, x.device)
     if return_lse or lse is not None:
         lse = _result("lse", lse, (R,), torch.float32, x.device)
     if R:
-        _vocab_launch("fwd", x, kernel, labels, (_ptr(bias), 0, loss.data_ptr(), _ptr(lse), 0, 0, 0), (R, D, V, labels.element_size(), 0))
+        _vocab_launch("fwd", x, kernel, labels, bias, None, loss, lse, None, None, None, R, D, V)
     return (loss, lse) if return_lse else loss
 
 
 def vocab_crossentropy_grad(dloss, x, kernel, labels, lse, bias=None, dx=None, dkernel=None, dbias=None, accumulate=False, need_dx=True):
     """Gradients of vocab_crossentropy: dloss (R) fp32 -> (dx, dkernel, dbias | None) of the inputs' type, each element rounded once from an fp32
-    sum.  softmax - onehot is held in 16 bits (fp32: about twice that) relative to the largest |dloss|, so rows of very different dloss (2^20 and more)
-    belong in different calls.  x has to be finite in rows that are left out too.  accumulate (fp32 only): add to the `dkernel`, `dbias` given, as parameter gradients of this package are.  need_dx=False: dx is None.
+    sum.  accumulate (fp32 only): add to the `dkernel`, `dbias` given, as parameter gradients of this package are.  need_dx=False: dx is None.
+    softmax - onehot is held in 16 bits (fp32: about twice that) relative to the largest |dloss|, so rows of very different dloss (2^20 and more) belong
+    in different calls.  x has to be finite in rows that are left out too.
     No atomics: the same inputs give the same bits."""
-    x, kernel, bias = _vocab_args(x, kernel, labels, bias)
-    R, (D, V) = x.shape[0], kernel.shape
+    x, kernel, R, D, V = _vocab_args(x, kernel, labels, bias)
     if accumulate and (x.dtype != torch.float32 or dkernel is None or (bias is not None and dbias is None)):
         raise ValueError("accumulate needs fp32 and the buffers to add to")
     dloss, lse = _result("dloss", dloss, (R,), torch.float32, x.device), _result("lse", lse, (R,), torch.float32, x.device)
@@ -220,8 +227,7 @@ def vocab_crossentropy_grad(dloss, x, kernel, labels, lse, bias=None, dx=None, d
     dkernel = _result("dkernel", dkernel, (D, V), x.dtype, x.device)
     dbias = None if bias is None else _result("dbias", dbias, (V,), x.dtype, x.device)
     if R:
-        _vocab_launch("bwd", x, kernel, labels, (_ptr(bias), dloss.data_ptr(), 0, lse.data_ptr(), _ptr(dx), dkernel.data_ptr(), _ptr(dbias)),
-                      (R, D, V, labels.element_size(), 1 if accumulate else 0))
+        _vocab_launch("bwd", x, kernel, labels, bias, dloss, None, lse, dx, dkernel, dbias, R, D, V, 1 if accumulate else 0)
     elif not accumulate:
         dkernel.zero_()
         if dbias is not None:
