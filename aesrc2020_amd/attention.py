@@ -19,7 +19,7 @@ class Xattn(ctypes.Structure):
     """include/sarnet.h: sarXattn."""
     _fields_ = [(n, _P) for n in ("q", "k", "v", "dout", "out", "lse", "dq", "dk", "dv", "k_lens", "q_lens", "ws")] + [("ws_bytes", _L)] + \
                [(n, _L) for n in ("q_sb", "q_st", "q_sh", "k_sb", "k_st", "k_sh", "v_sb", "v_st", "v_sh", "o_sb", "o_st", "o_sh", "g_sb", "g_st", "g_sh")] + \
-               [(n, _I) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "D")] + [("scale", ctypes.c_float), ("pad_", _I)]
+               [(n, _I) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "D")] + [("scale", ctypes.c_float), ("elt_bytes", _I)]
 
 
 _XATTN = struct.Struct("12Ql15l6ifi")                                  # the same fields: packing bytes costs a fifth of filling the Structure
@@ -126,7 +126,7 @@ def cross_attention(q, k, v, k_lens=None, q_lens=None, scale=None, return_lse=Fa
     if B and Tq:
         qp, sq, sk, sv, so = q.data_ptr(), q.stride(), k.stride(), v.stride(), out.stride()
         a = _XATTN.pack(qp, k.data_ptr() if Tk else qp, v.data_ptr() if Tk else qp, 0, out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, kl, ql, 0, 0,      # (no frames: never read)
-                        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], so[0], so[1], so[2], 0, 0, 0, B, Tq, Tk, Hq, Hkv, D, _scale(scale, D), 0)
+                        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], so[0], so[1], so[2], 0, 0, 0, B, Tq, Tk, Hq, Hkv, D, _scale(scale, D), q.element_size())
         if Tk > 256:                                                   # (sarnet.h: 256 keys never need a workspace)
             a, ws = _with_workspace("sar_xattn_fwd_workspace_bytes", device, a)
         _launch(_NAMES["xattn_fwd"][q.dtype], device, a)
@@ -155,7 +155,7 @@ def cross_attention_grad(dout, q, k, v, out, lse, k_lens=None, q_lens=None, scal
         qp, sq, sk, sv, so, sg = q.data_ptr(), q.stride(), k.stride(), v.stride(), out.stride(), dout.stride()
         a = _XATTN.pack(qp, k.data_ptr() if Tk else qp, v.data_ptr() if Tk else qp, dout.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(),
                         dk.data_ptr() if Tk else qp, dv.data_ptr() if Tk else qp, kl, ql, 0, 0,  # (no frames: never read or written)
-                        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], so[0], so[1], so[2], sg[0], sg[1], sg[2], B, Tq, Tk, Hq, Hkv, D, _scale(scale, D), 0)
+                        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], so[0], so[1], so[2], sg[0], sg[1], sg[2], B, Tq, Tk, Hq, Hkv, D, _scale(scale, D), q.element_size())
         a, ws = _with_workspace("sar_xattn_bwd_workspace_bytes", device, a)
         _launch(_NAMES["xattn_bwd"][q.dtype], device, a)
     return dq, dk, dv
@@ -213,7 +213,7 @@ class EncoderCache8:
         if Tq:
             s, so = q.stride(), out.stride()
             a = _XATTN.pack(q.data_ptr(), 0, 0, 0, out.data_ptr(), 0, 0, 0, 0, self.lens.data_ptr(), ql, 0, 0, s[0], s[1], s[2], 0, 0, 0, 0, 0, 0, so[0], so[1], so[2], 0, 0, 0,
-                            B, Tq, self.frames, Hq, self.heads, D, _scale(scale, D), 0)
+                            B, Tq, self.frames, Hq, self.heads, D, _scale(scale, D), q.element_size())
             if self.frames > 256:
                 a, ws = _with_workspace("sar_kv8_attend_workspace_bytes", device, a)
             _launch(_NAMES["kv8_attend"][q.dtype], device, a, self.k8.data_ptr(), self.k_scale.data_ptr(), self.v8.data_ptr(), self.v_scale.data_ptr(), self.k8.shape[2])

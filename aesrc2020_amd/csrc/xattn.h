@@ -15,7 +15,7 @@ struct sarXattn {
     long q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, o_sb, o_st, o_sh, g_sb, g_st, g_sh;
     int B, Tq, Tk, Hq, Hkv, D;
     float scale;
-    int pad_;
+    int elt_bytes;
 };
 
 namespace attn {
@@ -94,8 +94,13 @@ static inline int key_splits(const sarXattn* a, int rows_per_block, int blocks) 
     const long s = few > many ? few : many;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
-// a few rows: `waves` waves of a block can take eight 32-key tiles each before a second launch (joining slices: 5 us) costs less than going on
-static inline int step_splits(const sarXattn* a, int waves) { return a->Tk <= waves * 256 ? 1 : key_splits(a, 32, 1024); }
+// a few rows: a second launch (joining slices: 5 us) costs more than going on until each of a block's `waves` has six 32-key tiles (three of fp32, whose
+// products take longer), or eight where the blocks fill the chip by themselves.  8-bit, 4 x 2000, 4 heads of 64: bf16 10.4 in one slice, 9.4 in eight,
+// fp32 16.2 and 10.8; bf16 64 x 1140, 8 heads: 16 and 19; fp32 keys, 1 x 450, 8 heads of 128: 39 and 25
+static inline int step_splits(const sarXattn* a, int waves, bool fp32) {
+    const long tiles = ((long)a->Tq * (a->Hq / a->Hkv) + 31) / 32 * a->B * a->Hkv;
+    return a->Tk <= waves * (tiles >= 256 ? 256 : fp32 ? 96 : 192) ? 1 : key_splits(a, 32, 1024);
+}
 // the forward for many rows: four waves on 128 rows where those blocks fill the chip's 256 CUs twice; else two pairs of waves on 64; the key axis
 // is cut only where even those are fewer than the CUs (partial results cost their writing and reading)
 struct FwdPlan { int waves, splits; };

@@ -697,7 +697,7 @@ template <int DP> static int launch_bwd(const sarXattn& a, hipStream_t st) {
 }
 
 #if SAR_ELT == 0      // the same for every type
-extern "C" size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, few_rows(a) ? step_splits(a, a->D <= 32 ? 8 : a->D <= 64 ? 4 : 2) : fwd_plan(a).splits); }   // (the widest type's waves)
+extern "C" size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, few_rows(a) ? step_splits(a, a->elt_bytes == 2 ? (a->D <= 64 ? 8 : 4) : a->D <= 32 ? 8 : a->D <= 64 ? 4 : 2, a->elt_bytes != 2) : fwd_plan(a).splits); }   // (most_waves(); fp32 has the fewest)
 extern "C" size_t sar_xattn_bwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : bwd_plan(a).bytes; }
 #endif
 

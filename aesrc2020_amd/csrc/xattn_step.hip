@@ -362,7 +362,7 @@ template <typename C, bool S8, int DP, int NW> static int launch_waves(const sar
 // without key slices, the wider block where the keys are many for four waves
 template <typename C, bool S8, int DP> static int launch_step(const sarXattn& a, const Kv8& kv, hipStream_t st) {
     constexpr int NW = step_waves<elt, S8, DP>(), MW = most_waves<elt, S8, DP>();
-    const int splits = step_splits(&a, MW);
+    const int splits = step_splits(&a, MW, SAR_ELT == 0);
     if (bad_workspace(&a, part_bytes(&a, splits))) return SAR_EINVAL;
     if constexpr (MW > NW) {
         if (splits == 1 && a.Tk > 256) return launch_waves<C, S8, DP, MW>(a, kv, 1, st);
@@ -386,7 +386,7 @@ int SAR_FN(xattn_step)(const sarXattn* a, hipStream_t stream) { return step<elt,
 // ---- the 8-bit cache
 static bool bad8(const sarXattn* a, long frames) { return bad_shape(a) || frames < a->Tk || frames % KV_BLOCK || frames > (1L << 30); }
 #if SAR_ELT == 0      // the same for every type
-extern "C" size_t sar_kv8_attend_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, step_splits(a, 8)); }   // (its rows are at most 128 bytes: eight waves)
+extern "C" size_t sar_kv8_attend_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, step_splits(a, 8, a->elt_bytes != 2)); }   // (its rows are at most 128 bytes: eight waves)
 #endif
 extern "C" int SAR_FN(sar_kv8_attend)(const sarXattn* a, const void* k8, const float* k_scale, const void* v8, const float* v_scale, long frames, hipStream_t stream) {
     if (bad8(a, frames) || bad_strides(sizeof(elt), &a->q_sb, 3) || bad_strides(sizeof(elt), &a->o_sb, 3) || !a->q || !a->out || !k8 || !v8 || !k_scale || !v_scale) return SAR_EINVAL;

@@ -604,7 +604,7 @@ typedef struct {
     long q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, o_sb, o_st, o_sh, g_sb, g_st, g_sh;
     int B, Tq, Tk, Hq, Hkv, D;
     float scale;
-    int pad_;
+    int elt_bytes;                 /* read by the workspace queries only: 2, 4, or 0 for the most that any type needs */
 } sarXattn;
 size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a);
 size_t sar_xattn_bwd_workspace_bytes(const sarXattn* a);

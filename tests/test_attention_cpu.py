@@ -60,6 +60,10 @@ def test_c_workspace_sizes():
     assert size(Tk=0) == 256 and size(Tk=1) == 256                 # {lse, delta} of 2 x 4 x 3 rows
     assert size(B=1, Tq=1000, Tk=0) == 8 * 4000
     assert size(B=1, Tq=100, Tk=4000, Hq=2) > 8 * 200 + 4 * 100 * 2 * 64                   # dQ in slices
+    for kw in (dict(B=1, Tq=1, Tk=t, D=d) for t in (256, 257, 700, 1100, 1700, 5000) for d in (32, 64, 128)):
+        for q in ("sar_xattn_fwd_workspace_bytes", "sar_kv8_attend_workspace_bytes"):
+            most, two, four = (L[q](ctypes.byref(_args(elt_bytes=e, **kw))) for e in (0, 2, 4))
+            assert two <= four == most and (kw["Tk"] > 256 or most == 0), (kw, q)
     assert size(B=1024, Hq=32, Hkv=32, Tq=4096, Tk=4096, D=128) == 8 * 1024 * 32 * 4096
 
 
