@@ -77,16 +77,28 @@ __device__ __forceinline__ int g_exp(float v) {                   // v 2^-e in [
     return v == 0.f ? 0 : min(max(e, -110), 110);
 }
 
+// labels (R) of 4 or 8 bytes; a row whose label lies outside [0, V) is left out
+struct Labels { const void* p; int bytes, V; };
+__device__ __forceinline__ long label_of(const Labels& l, long r) {
+    return l.bytes == 8 ? (long)reinterpret_cast<const long long*>(l.p)[r] : (long)reinterpret_cast<const int*>(l.p)[r];
+}
+__device__ __forceinline__ bool counts(const Labels& l, long r) {
+    const long v = label_of(l, r);
+    return v >= 0 && v < l.V;
+}
+
 struct MaxJob { const void* x; long rows, ld; int cols, f32; };
-struct MaxJobs { MaxJob j[3]; };
-// partial maxima of the finite |values| of up to three tensors (blockIdx.y): PARTS places each
+struct MaxJobs { MaxJob j[3]; Labels labels; };
+// partial maxima of the finite |values| of up to three tensors (blockIdx.y): PARTS places each.  dloss (f32): of the rows that have a label -- what a
+// row that is left out holds must not decide how finely the others' dz is held.
 __global__ __launch_bounds__(1024) void absmax_kernel(MaxJobs jobs, float* __restrict__ part) {
     __shared__ float red[16];
     const MaxJob j = jobs.j[blockIdx.y];
     float m = 0.f;
     const auto see = [&](float v) { v = fabsf(v); if (v < INFINITY) m = fmaxf(m, v); };
     if (j.f32) {
-        for (long c = blockIdx.x * 1024 + threadIdx.x; c < j.cols; c += PARTS * 1024) see(reinterpret_cast<const float*>(j.x)[c]);
+        for (long c = blockIdx.x * 1024 + threadIdx.x; c < j.cols; c += PARTS * 1024)
+            if (counts(jobs.labels, c)) see(reinterpret_cast<const float*>(j.x)[c]);
     } else {
         // sixteen bytes a thread where rows are aligned for it; whole tensors without gaps as one row
         constexpr int V = Num<elt>::PER;
@@ -205,7 +217,7 @@ enum { E_LSE, E_DZ, E_GRAD };
 struct Epi {
     const float* parts;                          // maxima: x, W, dloss
     const elt* bias;
-    const void* labels;
+    Labels labels;
     const float *dloss, *lse;
     float *pm, *pl, *zl;                         // E_LSE: (m tiles, Rp) maxima and sums, label logits
     float *loss, *lse_out;                       // E_LSE, one m tile: the results themselves
@@ -214,11 +226,8 @@ struct Epi {
     elt* db_out; int db_accumulate;              // E_DZ, one n tile: the sums themselves
     void* out; long ldo; int accumulate;         // E_GRAD: elements of elt, or, with `part`, fp32 (slice, m, n)
     long slice;
-    int R, V, v0, Rp, R_all, label_bytes, part, with_w;      // with_w: dz W^T (dx), else x^T dz (dW)
+    int R, V, v0, Rp, R_all, part, with_w;       // with_w: dz W^T (dx), else x^T dz (dW)
 };
-__device__ __forceinline__ long label_of(const Epi& e, int r) {
-    return e.label_bytes == 8 ? (long)reinterpret_cast<const long long*>(e.labels)[r] : (long)reinterpret_cast<const int*>(e.labels)[r];
-}
 
 // a row's results from its maximum, sum and label logit (all in powers of two)
 __device__ __forceinline__ void finish_row(float* loss, float* lse, int r, float m, float l, float own, long lab, int V) {
@@ -231,7 +240,7 @@ __device__ __forceinline__ int dz_exp(const Epi& e) {             // dz is held 
     float m = 0.f;
     for (int r = threadIdx.x & 63; r < e.R_all; r += 64) {
         const float v = fabsf(e.dloss[r]);
-        if (v < INFINITY) m = fmaxf(m, v);
+        if (counts(e.labels, r) && v < INFINITY) m = fmaxf(m, v);
     }
     return DZ_BITS - g_exp(wave_max(m));
 }
@@ -372,7 +381,7 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int r = n0 + nw + 32 * j + (lane & 31);
-            const long lab = r < e.R ? label_of(e, r) : -1, at = lab - m0 - mw;
+            const long lab = r < e.R ? label_of(e.labels, r) : -1, at = lab - m0 - mw;
             own[j] = -INFINITY;                                   // the label's logit, where the wave has it
             if (__any(at >= 0 && at < 32 * MT && lab < e.V)) {
                 place(lab < e.V ? at : -1, [&](int i, int x) {
@@ -409,7 +418,7 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
             if (mtiles > 1) {
                 e.pm[(long)mt * e.Rp + r] = M;
                 e.pl[(long)mt * e.Rp + r] = L;
-            } else if (r < e.R) finish_row(e.loss, e.lse_out, r, M, L, fmaxf(own[j], join[2 * BN + nw + 32 * j + lane]), label_of(e, r), e.V);
+            } else if (r < e.R) finish_row(e.loss, e.lse_out, r, M, L, fmaxf(own[j], join[2 * BN + nw + 32 * j + lane]), label_of(e.labels, r), e.V);
         }
     } else if constexpr (EPI == E_DZ) {                           // m: vocabulary entries from v0 on, n: rows of x
         const float gs = ldexpf(1.f, dz_exp(e));
@@ -417,7 +426,7 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int r = n0 + nw + 32 * j + (lane & 31);
-            const long lab = r < e.R ? label_of(e, r) : -1;
+            const long lab = r < e.R ? label_of(e.labels, r) : -1;
             const bool has = lab >= 0 && lab < e.V;
             // a row that is left out: p = exp2(-inf) = 0 and g = 0
             const float g = has ? e.dloss[r] * gs : 0.f, lse = has ? e.lse[r] * LOG2E : INFINITY;
@@ -513,8 +522,8 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
 }
 
 // lse and loss of a row from its slices' maxima and sums: 16 rows x 16 groups of slices a block
-__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ pm, const float* __restrict__ pl, const float* __restrict__ zl, const void* __restrict__ labels, int label_bytes,
-                                                     float* __restrict__ loss, float* __restrict__ lse, int R, int Rp, int V, int slices) {
+__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ pm, const float* __restrict__ pl, const float* __restrict__ zl, Labels labels,
+                                                     float* __restrict__ loss, float* __restrict__ lse, int R, int Rp, int slices) {
     __shared__ float sm[16][17], ss[16][17];
     const int c = threadIdx.x & 15, g = threadIdx.x >> 4, r = blockIdx.x * 16 + c;
     const auto join = [](float& m, float& l, float m2, float l2) {
@@ -539,7 +548,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ p
     if (g || r >= R) return;
 #pragma unroll
     for (int x = 1; x < 16; ++x) join(m, l, sm[x][c], ss[x][c]);
-    finish_row(loss, lse, r, m, l, zl[r], label_bytes == 8 ? (long)reinterpret_cast<const long long*>(labels)[r] : (long)reinterpret_cast<const int*>(labels)[r], V);
+    finish_row(loss, lse, r, m, l, zl[r], label_of(labels, r), labels.V);
 }
 
 // out (rows, cols) (+)= sum of the slices, for up to three results (blockIdx.y)
@@ -666,7 +675,7 @@ static unsigned some_blocks(long n) { return (unsigned)(n < 1 ? 1 : n < 4096 ? n
 template <typename OP, bool SCALED> static void operands(const sarVocabCe* a, const Plan& p, bool grad, Side& x, Side& w, hipStream_t st) {
     char* ws = reinterpret_cast<char*>(a->ws);
     float* parts = reinterpret_cast<float*>(ws + p.parts);
-    const MaxJobs all = {{{a->x, a->R, a->ldx, a->D, 0}, {a->kernel, a->D, a->ldk, a->V, 0}, {a->dloss, 1, a->R, a->R, 1}}}, gradient = {{all.j[2]}};
+    const MaxJobs all = {{{a->x, a->R, a->ldx, a->D, 0}, {a->kernel, a->D, a->ldk, a->V, 0}, {a->dloss, 1, a->R, a->R, 1}}, {a->labels, a->label_bytes, a->V}}, gradient = {{all.j[2]}, all.labels};
     if (SCALED) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, grad ? 3 : 2), dim3(1024), 0, st, all, parts);
     else if (grad && p.g_from == G_PARTS) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, 1), dim3(1024), 0, st, gradient, parts + 2 * PARTS);
     x = {a->x, 0, a->ldx, 0, 0};
@@ -714,7 +723,7 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     x.len = a->R; x.k = p.pack_x ? p.Dp : a->D;
     Epi e = {};
     e.parts = reinterpret_cast<float*>(ws + p.parts);
-    e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = a->labels; e.label_bytes = a->label_bytes;
+    e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = {a->labels, a->label_bytes, a->V};
     e.pm = reinterpret_cast<float*>(ws + p.a); e.pl = reinterpret_cast<float*>(ws + p.b); e.zl = reinterpret_cast<float*>(ws + p.zl);
     e.R = a->R; e.V = a->V; e.Rp = p.Rp;
     e.loss = a->loss; e.lse_out = a->lse;
@@ -724,7 +733,7 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
         if (p.light) hipLaunchKernelGGL((product_kernel<elt, 32, 1, 1, true, false, E_LSE, false, 1, 1, 1>), dim3(blocks_of(z)), dim3(256), 0, st, z);
     }
     if (!p.light) product<fwd16, true, false, E_LSE, FWD_SCALED>(z, p.small_z, step, st);
-    if (z.mtiles > 1) hipLaunchKernelGGL(finish_kernel, dim3((unsigned)cdiv(a->R, 16)), dim3(256), 0, st, e.pm, e.pl, e.zl, a->labels, a->label_bytes, a->loss, a->lse, a->R, p.Rp, a->V, p.lse_slices);
+    if (z.mtiles > 1) hipLaunchKernelGGL(finish_kernel, dim3((unsigned)cdiv(a->R, 16)), dim3(256), 0, st, e.pm, e.pl, e.zl, e.labels, a->loss, a->lse, a->R, p.Rp, p.lse_slices);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
 }
@@ -744,7 +753,7 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         const long plane = (long)p.Rp * ld;
         Epi e = {};
         e.parts = reinterpret_cast<float*>(ws + p.parts);
-        e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = a->labels; e.label_bytes = a->label_bytes; e.dloss = a->dloss; e.lse = a->lse;
+        e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = {a->labels, a->label_bytes, a->V}; e.dloss = a->dloss; e.lse = a->lse;
         e.dz = dz; e.dz_plane = plane; e.dz_ld = ld;
         if (a->dbias && p.db_slices > 1) e.db = reinterpret_cast<float*>(ws + p.dbp);
         else if (a->dbias) { e.db_out = reinterpret_cast<elt*>(a->dbias) + v0; e.db_accumulate = a->accumulate; }

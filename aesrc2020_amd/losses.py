@@ -216,8 +216,8 @@ def vocab_crossentropy(x, kernel, labels, bias=None, return_lse=False, loss=None
 def vocab_crossentropy_grad(dloss, x, kernel, labels, lse, bias=None, dx=None, dkernel=None, dbias=None, accumulate=False, need_dx=True):
     """Gradients of vocab_crossentropy: dloss (R) fp32 -> (dx, dkernel, dbias | None) of the inputs' type, each element rounded once from an fp32
     sum.  accumulate (fp32 only): add to the `dkernel`, `dbias` given, as parameter gradients of this package are.  need_dx=False: dx is None.
-    softmax - onehot is held in 16 bits (fp32: about twice that) relative to the largest |dloss|, so rows of very different dloss (2^20 and more) belong
-    in different calls.  x has to be finite in rows that are left out too.
+    softmax - onehot is held in 16 bits (fp32: about twice that) relative to the largest |dloss| of a row with a label, so such rows of very different
+    dloss (2^20 and more) belong in different calls.  x has to be finite in rows that are left out too.
     No atomics: the same inputs give the same bits."""
     x, kernel, R, D, V = _vocab_args(x, kernel, labels, bias)
     if accumulate and (x.dtype != torch.float32 or dkernel is None or (bias is not None and dbias is None)):

@@ -639,7 +639,7 @@ int sar_kv8_attend_f16(const sarXattn* a, const void* k8, const float* k_scale, 
  * Suffix = type of x, kernel, bias and their gradients: f32 | bf16 | f16.
  *   z = x W + b;  lse_r = log sum_v exp z_rv;  loss_r = lse_r - z_{r, label_r};  dz = dloss_r (softmax(z) - onehot);  dx = dz W^T, dkernel = x^T dz, dbias = sum_r dz
  * x (R, D) with row stride ldx, kernel (D, V) with row stride ldk (elements; the Keras Dense layout), bias (V) or NULL, labels (R) of
- * label_bytes 4 or 8; a label outside [0, V) leaves its row out: loss 0, no gradient (its x has to be finite all the same: dkernel meets it as 0 x).  loss, lse, dloss (R) fp32 (forward: either may be NULL; backward:
+ * label_bytes 4 or 8; a label outside [0, V) leaves its row out: loss 0, no gradient (its dloss is not looked at; its x has to be finite all the same: dkernel meets it as 0 x).  loss, lse, dloss (R) fp32 (forward: either may be NULL; backward:
  * lse of the forward).  dx (R, D), dkernel (D, V), dbias (V) contiguous, each may be NULL; accumulate (f32 only): dkernel and dbias are added to.
  * ws: the matching _workspace_bytes of the same struct, 256-byte aligned; nothing in it has to be initialised, nothing is kept there. */
 typedef struct {
