@@ -9,10 +9,13 @@
 // operand type; two more products read that piece (it stays in the last-level cache) for dx and dW.
 //
 // The products run on the 32x32x16 matrix instructions (small fp32 ones on the fp32 ones: direct()).
-// fp32 operands are two fp16 planes under one power-of-two scale per tensor that puts its largest element in [2^13, 2^14): hi + lo hold 22 bits, hi hi + hi lo + lo hi is the product to 2^-22 or so of |a| |b|, at a third of the fp16 rate
-// (the fp32 matrix instructions run at a sixteenth).  dz is held in fp16: scaled by the power of two that puts the largest |g| in [1/2, 1), times
-// 2^14, every probability down to 2^-28 is a normal number with 11 bits; for bf16 the backward therefore takes x and W in fp16 too (under a scale as
-// above their 8 bits are exact), which leaves the gradients the accuracy of their own rounding.
+// fp32 operands are two fp16 planes under a power of two that puts the largest element in [2^13, 2^14): hi + lo hold 22 bits of elements down to 2^-16
+// of that one (below, 2^-38 of it), hi hi + hi lo + lo hi is the product to 2^-22 or so of |a| |b|, at a third of the fp16 rate (the fp32 matrix
+// instructions run at a sixteenth).  For the logits every row of x has its own scale, so that no row reaches another's results; W has one.
+// dz is held in fp16: scaled by the power of two that puts the largest |g| in [1/2, 1), times 2^14, every probability down to 2^-28 is a normal number
+// with 11 bits; for bf16 the backward therefore takes x and W in fp16 too (their 8 bits are exact down to 2^-31 of the largest), which leaves the
+// gradients the accuracy of their own rounding.  dW = x^T dz sums over the rows, so there x is packed a second time, under one scale, of the rows
+// with a label: an element of dW is good to 2^-38 of the largest |x| among them.
 // Compiled once per element type: SAR_ELT 0 = fp32, 1 = bf16, 2 = fp16.
 #include "attn_tiles.h"
 
@@ -56,11 +59,12 @@ using attn::as16;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int NPL = SAR_ELT == 0 ? 2 : 1;
-constexpr bool FWD_SCALED = SAR_ELT == 0, BWD_SCALED = SAR_ELT != 2;           // operands packed under a power of two per tensor
+constexpr bool FWD_SCALED = SAR_ELT == 0, BWD_SCALED = SAR_ELT != 2;           // operands packed under powers of two
 constexpr int DZ_BITS = 14;
 
-// Device scalars of a call: maxima of |x|, |W| (fp32 only) and |dloss|, reduced from 256 partial maxima each by whoever reads them
+// Device scalars of a call: maxima of |x| (rows with a label), |W| and |dloss| (the same rows), reduced from 256 partial maxima each by whoever reads them
 constexpr int PARTS = 256;
+enum { PART_X, PART_W, PART_G };
 __device__ __forceinline__ float max_of(const float* part) {
     const int l = threadIdx.x & 63;
     return wave_max(fmaxf(fmaxf(part[l], part[l + 64]), fmaxf(part[l + 128], part[l + 192])));
@@ -87,64 +91,62 @@ __device__ __forceinline__ bool counts(const Labels& l, long r) {
     return v >= 0 && v < l.V;
 }
 
-struct MaxJob { const void* x; long rows, ld; int cols, f32; };
+enum { MAX_ALL, MAX_ROWS, MAX_G };       // of a whole tensor, of its rows with a label, of dloss
+struct MaxJob { const void* x; long rows, ld; int cols, kind, part; };
 struct MaxJobs { MaxJob j[3]; Labels labels; };
-// partial maxima of the finite |values| of up to three tensors (blockIdx.y): PARTS places each.  dloss (f32): of the rows that have a label -- what a
-// row that is left out holds must not decide how finely the others' dz is held.
+// partial maxima of the finite |values| of up to three tensors (blockIdx.y): PARTS places each.  What a row that is left out holds must not decide how
+// finely the others' x and dz are held.
 __global__ __launch_bounds__(1024) void absmax_kernel(MaxJobs jobs, float* __restrict__ part) {
     __shared__ float red[16];
     const MaxJob j = jobs.j[blockIdx.y];
+    constexpr int V = Num<elt>::PER;
     float m = 0.f;
     const auto see = [&](float v) { v = fabsf(v); if (v < INFINITY) m = fmaxf(m, v); };
-    if (j.f32) {
+    // n elements at p, by threads `first`, first + step, ...: sixteen bytes each where p and n allow it
+    const auto row = [&](const elt* p, long n, bool wide, long first, long step) {
+        if (wide) {
+            const auto* q = reinterpret_cast<const typename Num<elt>::x16*>(p);
+            long c = first;
+            n /= V;
+            for (; c + 3 * step < n; c += 4 * step) {             // four loads in flight
+                const auto a = q[c], b = q[c + step], d = q[c + 2 * step], e = q[c + 3 * step];
+#pragma unroll
+                for (int k = 0; k < V; ++k) { see((float)a[k]); see((float)b[k]); see((float)d[k]); see((float)e[k]); }
+            }
+            for (; c < n; c += step) {
+                const auto a = q[c];
+#pragma unroll
+                for (int k = 0; k < V; ++k) see((float)a[k]);
+            }
+        } else
+            for (long c = first; c < n; c += step) see((float)p[c]);
+    };
+    const elt* x = reinterpret_cast<const elt*>(j.x);
+    const bool aligned = (uintptr_t)j.x % 16 == 0, wide = aligned && j.cols % V == 0 && j.ld % V == 0;
+    if (j.kind == MAX_G) {
         for (long c = blockIdx.x * 1024 + threadIdx.x; c < j.cols; c += PARTS * 1024)
             if (counts(jobs.labels, c)) see(reinterpret_cast<const float*>(j.x)[c]);
+    } else if (j.kind == MAX_ROWS) {                              // a wave per row
+        for (long r = blockIdx.x * 16 + (threadIdx.x >> 6); r < j.rows; r += PARTS * 16)
+            if (counts(jobs.labels, r)) row(x + r * j.ld, j.cols, wide, threadIdx.x & 63, 64);
+    } else if (j.ld == j.cols) {                                  // no gaps: as one row
+        row(x, j.rows * j.cols, aligned && j.rows * j.cols % V == 0, (long)blockIdx.x * 1024 + threadIdx.x, PARTS * 1024);
     } else {
-        // sixteen bytes a thread where rows are aligned for it; whole tensors without gaps as one row
-        constexpr int V = Num<elt>::PER;
-        const bool flat = j.ld == j.cols, wide = (flat ? j.rows * j.cols : j.cols) % V == 0 && (flat || j.ld % V == 0) && (uintptr_t)j.x % 16 == 0;
-        const elt* x = reinterpret_cast<const elt*>(j.x);
-        const long rows = flat ? 1 : j.rows, cols = flat ? j.rows * j.cols : j.cols, n = wide ? cols / V : cols;
-        const long first = flat ? (long)blockIdx.x * 1024 + threadIdx.x : threadIdx.x, step = flat ? PARTS * 1024 : 1024;
-        for (long r = flat ? 0 : blockIdx.x; r < rows; r += PARTS) {
-            const elt* p = x + r * j.ld;
-            if (wide) {
-                const auto* q = reinterpret_cast<const typename Num<elt>::x16*>(p);
-                long c = first;
-                for (; c + 3 * step < n; c += 4 * step) {         // four loads in flight
-                    const auto a = q[c], b = q[c + step], d = q[c + 2 * step], e = q[c + 3 * step];
-#pragma unroll
-                    for (int k = 0; k < V; ++k) { see((float)a[k]); see((float)b[k]); see((float)d[k]); see((float)e[k]); }
-                }
-                for (; c < n; c += step) {
-                    const auto a = q[c];
-#pragma unroll
-                    for (int k = 0; k < V; ++k) see((float)a[k]);
-                }
-            } else
-                for (long c = first; c < n; c += step) see((float)p[c]);
-        }
+        for (long r = blockIdx.x; r < j.rows; r += PARTS) row(x + r * j.ld, j.cols, wide, threadIdx.x, 1024);
     }
     m = block_max(m, red);
-    if (threadIdx.x == 0) part[blockIdx.y * PARTS + blockIdx.x] = m;
+    if (threadIdx.x == 0) part[j.part * PARTS + blockIdx.x] = m;
 }
 
-struct PackJob { const elt* x; void* y; long rows, ld, plane; int cols, pitch; const float* part; };
-struct PackJobs { PackJob j[2]; };
-// rows of `cols` elements -> rows of `pitch` operand elements, zeros behind (planes hi, lo of scaled fp32), for x and W (blockIdx.y)
+// rows of `cols` elements -> rows of `pitch` operand elements, zeros behind (SCALED: planes hi, lo of fp32), for x and W (blockIdx.y).  The scale comes from
+// `part`'s maxima; or, with row_f, every row has its own, whose inverse is left there, and with `all` the rows go there too under the scale of `part`,
+// those without a label as zeros.
+struct PackJob { const elt* x; void* y; long rows, ld, plane; int cols, pitch; const float* part; float* row_f; void* all; };
+struct PackJobs { PackJob j[2]; Labels labels; };
 template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_kernel(PackJobs jobs) {
     const PackJob j = jobs.j[blockIdx.y];
-    const float f = SCALED ? ldexpf(1.f, up_exp(max_of(j.part))) : 1.f;
-    const int per = j.pitch / 8;
-    OP* y = reinterpret_cast<OP*>(j.y);
-    // a block takes 256 pieces of eight of one row, then the next block's
-    const int across = (per + 255) / 256;
-    for (long i = blockIdx.x; i < j.rows * across; i += gridDim.x) {
-        const long r = i / across;
-        const int c = ((int)(i - r * across) * 256 + threadIdx.x) * 8;
-        if (c >= j.pitch) continue;
+    const auto fetch = [&](long r, int c, elt (&v)[8]) {
         const elt* p = j.x + r * j.ld + c;
-        elt v[8];
         if (c + 8 <= j.cols) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = p[k];
@@ -152,19 +154,53 @@ template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? p[k] : (elt)0.f;
         }
+    };
+    const auto put = [&](void* to, long r, int c, const elt (&v)[8], float f, bool none) {
         constexpr int PER = Num<OP>::PER;
+        OP* y = reinterpret_cast<OP*>(to) + r * j.pitch + c;
         typename Num<OP>::x16 hi[8 / PER], lo[8 / PER];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float s = SCALED ? (float)v[k] * f : (float)v[k];
+            const float s = none ? 0.f : SCALED ? (float)v[k] * f : (float)v[k];
             hi[k / PER][k % PER] = (OP)s;
             if constexpr (SCALED && NPL == 2) lo[k / PER][k % PER] = (OP)(s - (float)hi[k / PER][k % PER]);
         }
 #pragma unroll
         for (int q = 0; q < 8 / PER; ++q) {
-            *reinterpret_cast<typename Num<OP>::x16*>(y + r * j.pitch + c + q * PER) = hi[q];
-            if constexpr (SCALED && NPL == 2) *reinterpret_cast<typename Num<OP>::x16*>(y + j.plane + r * j.pitch + c + q * PER) = lo[q];
+            *reinterpret_cast<typename Num<OP>::x16*>(y + q * PER) = hi[q];
+            if constexpr (SCALED && NPL == 2) *reinterpret_cast<typename Num<OP>::x16*>(y + j.plane + q * PER) = lo[q];
         }
+    };
+    const float f = SCALED && j.part ? ldexpf(1.f, up_exp(max_of(j.part))) : 1.f;
+    elt v[8];
+    if (SCALED && j.row_f) {                                      // a wave per row, which it reads twice if it is wider than 512
+        const int lane = threadIdx.x & 63;
+        for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < j.rows; r += (long)gridDim.x * 4) {
+            float m = 0.f;
+            const bool in = j.all && counts(jobs.labels, r);
+            for (int c = lane * 8; c < j.pitch; c += 512) {
+                fetch(r, c, v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) { const float a = fabsf((float)v[k]); if (a < INFINITY) m = fmaxf(m, a); }
+            }
+            const int e = up_exp(wave_max(m));
+            if (lane == 0) j.row_f[r] = ldexpf(1.f, -e);
+            for (int c = lane * 8; c < j.pitch; c += 512) {
+                if (j.pitch > 512) fetch(r, c, v);
+                put(j.y, r, c, v, ldexpf(1.f, e), false);
+                if (j.all) put(j.all, r, c, v, f, !in);
+            }
+        }
+        return;
+    }
+    // a block takes 256 pieces of eight of one row, then the next block's
+    const int across = (j.pitch / 8 + 255) / 256;
+    for (long i = blockIdx.x; i < j.rows * across; i += gridDim.x) {
+        const long r = i / across;
+        const int c = ((int)(i - r * across) * 256 + threadIdx.x) * 8;
+        if (c >= j.pitch) continue;
+        fetch(r, c, v);
+        put(j.y, r, c, v, f, false);
     }
 }
 
@@ -215,7 +251,8 @@ constexpr int G_FEW = 1024;
 // what happens to a finished tile: C (m, n), column n = lane % 32 of a 32 x 32 tile
 enum { E_LSE, E_DZ, E_GRAD };
 struct Epi {
-    const float* parts;                          // maxima: x, W, dloss
+    const float* parts;                          // maxima: PART_X, PART_W, PART_G
+    const float* row_f;                          // the inverses of x's scales, a row each
     const elt* bias;
     Labels labels;
     const float *dloss, *lse;
@@ -236,7 +273,7 @@ __device__ __forceinline__ void finish_row(float* loss, float* lse, int r, float
 }
 __device__ __forceinline__ int dz_exp(const Epi& e) {             // dz is held times 2^this
     if (e.g_from == G_ONE) return 0;                              // (a bf16 has an fp32's range)
-    if (e.g_from == G_PARTS) return DZ_BITS - g_exp(max_of(e.parts + 2 * PARTS));
+    if (e.g_from == G_PARTS) return DZ_BITS - g_exp(max_of(e.parts + PART_G * PARTS));
     float m = 0.f;
     for (int r = threadIdx.x & 63; r < e.R_all; r += 64) {
         const float v = fabsf(e.dloss[r]);
@@ -256,7 +293,8 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
     static constexpr int LDS = ST * STAGE;
     static __device__ __forceinline__ void run(char* lds, int block, const Job& job);
 };
-template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED, int PA, int PB, int PZ> __global__ __launch_bounds__(256, (PA * PB == 1 && BK == 32 ? 3 : 2)) void product_kernel(Job job) {
+template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED, int PA, int PB, int PZ>
+__global__ __launch_bounds__(256, (PA * PB == 1 && BK == 32 ? 3 : 2)) void product_kernel(Job job) {
     typedef Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA, PB, PZ> P;
     __shared__ __attribute__((aligned(1024))) char lds[P::LDS];
     P::run(lds, blockIdx.x, job);
@@ -269,7 +307,8 @@ template <typename OP, int BKW, int BKX, bool SCALED, int PO, int PZ> __global__
     if ((int)blockIdx.x < first) W::run(lds, blockIdx.x, dw);
     else X::run(lds, blockIdx.x - first, dx);
 }
-template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED, int PA, int PB, int PZ> __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA, PB, PZ>::run(char* lds, int block, const Job& job) {
+template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED, int PA, int PB, int PZ>
+__device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA, PB, PZ>::run(char* lds, int block, const Job& job) {
     const Side &A = job.A, &B = job.B;
     const Epi& e = job.e;
     const int mtiles = job.mtiles, ntiles = job.ntiles, ksteps = job.ksteps, slices = job.slices;
@@ -338,7 +377,14 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
     const int mw = wm * MT * 32, nw = wn * NT * 32;               // the wave's corner of the tile
     // logits in powers of two: y = (acc f + b) log2 e, entries behind the vocabulary -inf
     const auto logits = [&](int v0) {
-        const float f = LOG2E * (SCALED ? ldexpf(1.f, -up_exp(max_of(e.parts)) - up_exp(max_of(e.parts + PARTS))) : 1.f);
+        float f[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) f[j] = LOG2E;
+        if constexpr (SCALED) {
+            const float fw = LOG2E * ldexpf(1.f, -up_exp(max_of(e.parts + PART_W * PARTS)));
+#pragma unroll
+            for (int j = 0; j < NT; ++j) f[j] = fw * e.row_f[min(n0 + nw + 32 * j + (lane & 31), e.R_all - 1)];
+        }
         const int first = v0 + m0 + mw + 4 * h;
         if (v0 + m0 + BM <= e.V) {
 #pragma unroll
@@ -352,7 +398,7 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) acc[i][j][4 * a + x] = fmaf(acc[i][j][4 * a + x], f, b[x]);
+                        for (int x = 0; x < 4; ++x) acc[i][j][4 * a + x] = fmaf(acc[i][j][4 * a + x], f[j], b[x]);
                 }
         } else {
 #pragma unroll
@@ -362,7 +408,7 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
                     const int v = first + 32 * i + 8 * (x >> 2) + (x & 3);
                     const float b = e.bias && v < e.V ? (float)e.bias[v] * LOG2E : 0.f;
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j][x] = v < e.V ? fmaf(acc[i][j][x], f, b) : -INFINITY;
+                    for (int j = 0; j < NT; ++j) acc[i][j][x] = v < e.V ? fmaf(acc[i][j][x], f[j], b) : -INFINITY;
                 }
         }
     };
@@ -495,7 +541,7 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
         }
     } else {
         int ex = -dz_exp(e);
-        if constexpr (SCALED) ex -= up_exp(max_of(e.with_w ? e.parts + PARTS : e.parts));
+        if constexpr (SCALED) ex -= up_exp(max_of(e.parts + (e.with_w ? PART_W : PART_X) * PARTS));
         const float f = ldexpf(1.f, ex);
         // every row and column that exists (R, V)
         const auto each = [&](auto&& put) {
@@ -580,7 +626,7 @@ __global__ __launch_bounds__(256) void sum_slices_kernel(SumJobs jobs) {
 // ---- plan of a call: what is packed, the pieces, the tiles, the workspace
 struct Plan {
     int Rp, Dp, Vp;                     // rows, hidden width and vocabulary rounded up to the contraction steps
-    bool pack_x, pack_w;
+    bool pack_x, pack_w, own_x;         // own_x: dW reads a packing of x of its own
     int piece, pieces;
     bool small_z, small_dx, small_dw;   // 64 x 64 tiles instead of 128 x 128
     // operands of the inputs' type, as they are: more matrix cycles, but neither maxima nor packing.  bf16 where all tiles are small: dz in two bf16
@@ -589,7 +635,7 @@ struct Plan {
     int dz_planes, g_from;              // (planes of two bytes)
     int dx_slices, dw_slices, lse_slices, db_slices;
     bool dx_parts;
-    size_t parts, xo, wo, a, b, zl, dz, dxp, dwp, dbp, bytes;      // offsets
+    size_t parts, rows, xo, wo, xg, a, b, zl, dz, dxp, dwp, dbp, bytes;      // offsets
 };
 static size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 static int up64(int n) { return (n + 63) & ~63; }
@@ -640,6 +686,7 @@ static Plan plan(const sarVocabCe* a, bool grad) {
         p.light |= SAR_ELT == 1 && p.small_z && p.small_dx && p.small_dw;
         p.dz_planes = p.light ? 2 : NPL;
         p.g_from = p.light ? G_ONE : BWD_SCALED || a->R > G_FEW ? G_PARTS : G_ROWS;
+        p.own_x = !p.light && BWD_SCALED && a->dkernel;
     }
     // operands are read where they lie when they have the products' type, their rows start on 4-byte boundaries (what a load into LDS needs) and
     // end with a whole 16-byte piece, or a whole step (Operand: TAIL), where they are read along the contraction (x, and W for dx)
@@ -650,6 +697,8 @@ static Plan plan(const sarVocabCe* a, bool grad) {
     size_t at = 0;
     const auto take = [&](size_t n) { const size_t o = at; at += up(n); return o; };
     p.parts = take(3 * PARTS * 4);
+    if (scaled) p.rows = take((size_t)a->R * 4);
+    if (p.own_x) p.xg = take((size_t)a->R * p.Dp * 2 * NPL);
     if (p.pack_x) p.xo = take((size_t)a->R * p.Dp * 2 * NPL);
     if (p.pack_w) p.wo = take((size_t)a->D * p.Vp * 2 * NPL);
     if (!grad) {
@@ -671,27 +720,33 @@ static Plan plan(const sarVocabCe* a, bool grad) {
 constexpr int step_of(bool planes = NPL == 2) { return planes ? 32 : 64; }
 static int logits_step(const sarVocabCe* a, bool small_tiles) { return small_tiles || a->D > 768 ? step_of() : 32; }
 static unsigned some_blocks(long n) { return (unsigned)(n < 1 ? 1 : n < 4096 ? n : 4096); }
-// the operands as the products read them
-template <typename OP, bool SCALED> static void operands(const sarVocabCe* a, const Plan& p, bool grad, Side& x, Side& w, hipStream_t st) {
+// the operands as the products read them; xg: x as dW reads it
+struct Operands { Side x, w, xg; };
+template <typename OP, bool SCALED> static Operands operands(const sarVocabCe* a, const Plan& p, bool grad, hipStream_t st) {
     char* ws = reinterpret_cast<char*>(a->ws);
     float* parts = reinterpret_cast<float*>(ws + p.parts);
-    const MaxJobs all = {{{a->x, a->R, a->ldx, a->D, 0}, {a->kernel, a->D, a->ldk, a->V, 0}, {a->dloss, 1, a->R, a->R, 1}}, {a->labels, a->label_bytes, a->V}}, gradient = {{all.j[2]}, all.labels};
-    if (SCALED) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, grad ? 3 : 2), dim3(1024), 0, st, all, parts);
-    else if (grad && p.g_from == G_PARTS) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, 1), dim3(1024), 0, st, gradient, parts + 2 * PARTS);
-    x = {a->x, 0, a->ldx, 0, 0};
-    w = {a->kernel, 0, a->ldk, 0, 0};
-    PackJobs jobs = {};
+    MaxJobs max = {{}, {a->labels, a->label_bytes, a->V}};
     int n = 0;
+    if (p.own_x) max.j[n++] = {a->x, a->R, a->ldx, a->D, MAX_ROWS, PART_X};
+    if (SCALED) max.j[n++] = {a->kernel, a->D, a->ldk, a->V, MAX_ALL, PART_W};
+    if (grad && p.g_from == G_PARTS) max.j[n++] = {a->dloss, 1, a->R, a->R, MAX_G, PART_G};
+    if (n) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, n), dim3(1024), 0, st, max, parts);
+    Operands o = {{a->x, 0, a->ldx, 0, 0}, {a->kernel, 0, a->ldk, 0, 0}, {}};
+    PackJobs jobs = {{}, max.labels};
+    n = 0;
     long blocks = 0;
-    const auto pack = [&](Side& s, size_t to, int rows, int cols, int pitch, const float* part) {
-        jobs.j[n++] = {reinterpret_cast<const elt*>(s.p), ws + to, rows, s.ld, (long)rows * pitch, cols, pitch, part};
+    const auto pack = [&](Side& s, size_t to, int rows, int cols, int pitch, const float* part, float* row_f, void* all) {
+        jobs.j[n++] = {reinterpret_cast<const elt*>(s.p), ws + to, rows, s.ld, (long)rows * pitch, cols, pitch, part, row_f, all};
         s = {ws + to, (long)rows * pitch, pitch, 0, 0};
-        const long b = (long)rows * cdiv(pitch, 2048);
+        const long b = row_f ? cdiv(rows, 4) : (long)rows * cdiv(pitch, 2048);
         blocks = b > blocks ? b : blocks;
     };
-    if (p.pack_x) pack(x, p.xo, a->R, a->D, p.Dp, parts);
-    if (p.pack_w) pack(w, p.wo, a->D, a->V, p.Vp, parts + PARTS);
+    if (p.pack_x) pack(o.x, p.xo, a->R, a->D, p.Dp, p.own_x ? parts + PART_X * PARTS : nullptr, SCALED ? reinterpret_cast<float*>(ws + p.rows) : nullptr, p.own_x ? ws + p.xg : nullptr);
+    if (p.pack_w) pack(o.w, p.wo, a->D, a->V, p.Vp, SCALED ? parts + PART_W * PARTS : nullptr, nullptr, nullptr);
     if (n) hipLaunchKernelGGL((pack_kernel<OP, SCALED>), dim3(some_blocks(blocks), n), dim3(256), 0, st, jobs);
+    o.xg = o.x;
+    if (p.own_x) o.xg.p = ws + p.xg;
+    return o;
 }
 static Job job_of(Side A, Side B, const Epi& e, int m, int n, int k, int step, int slices, bool small_tiles) {
     const int t = small_tiles ? 64 : 128;
@@ -700,9 +755,10 @@ static Job job_of(Side A, Side B, const Epi& e, int m, int n, int k, int step, i
 static unsigned blocks_of(const Job& j) { return (unsigned)attn::xcd_grid((long)j.mtiles * j.ntiles * j.slices); }
 template <typename OP, bool AD, bool BD, int EPI, bool SCALED> static void product(const Job& j, bool small_tiles, int step, hipStream_t st) {
     constexpr int BK = step_of();
-    if (small_tiles) hipLaunchKernelGGL((product_kernel<OP, BK, 1, 1, AD, BD, EPI, SCALED, NPL, NPL, NPL>), dim3(blocks_of(j)), dim3(256), 0, st, j);
-    else if (EPI == E_GRAD || step == BK) hipLaunchKernelGGL((product_kernel<OP, BK, 2, 2, AD, BD, EPI, SCALED, NPL, NPL, NPL>), dim3(blocks_of(j)), dim3(256), 0, st, j);
-    else if constexpr (EPI != E_GRAD) hipLaunchKernelGGL((product_kernel<OP, 32, 2, 2, AD, BD, EPI, SCALED, NPL, NPL, NPL>), dim3(blocks_of(j)), dim3(256), 0, st, j);
+    const dim3 grid(blocks_of(j)), block(256);
+    if (small_tiles) hipLaunchKernelGGL((product_kernel<OP, BK, 1, 1, AD, BD, EPI, SCALED, NPL, NPL, NPL>), grid, block, 0, st, j);
+    else if (EPI == E_GRAD || step == BK) hipLaunchKernelGGL((product_kernel<OP, BK, 2, 2, AD, BD, EPI, SCALED, NPL, NPL, NPL>), grid, block, 0, st, j);
+    else if constexpr (EPI != E_GRAD) hipLaunchKernelGGL((product_kernel<OP, 32, 2, 2, AD, BD, EPI, SCALED, NPL, NPL, NPL>), grid, block, 0, st, j);
 }
 
 }
@@ -716,13 +772,12 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     const Plan p = plan(a, false);
     if (a->ws_bytes < 0 || (size_t)a->ws_bytes < p.bytes) return SAR_EINVAL;
     char* ws = reinterpret_cast<char*>(a->ws);
-    Side x, w;
-    if (p.light) operands<elt, false>(a, p, false, x, w, st);
-    else operands<fwd16, FWD_SCALED>(a, p, false, x, w, st);
+    Operands in = p.light ? operands<elt, false>(a, p, false, st) : operands<fwd16, FWD_SCALED>(a, p, false, st);
+    Side &x = in.x, &w = in.w;
     w.len = p.pack_w ? p.Vp : a->V; w.k = a->D;
     x.len = a->R; x.k = p.pack_x ? p.Dp : a->D;
     Epi e = {};
-    e.parts = reinterpret_cast<float*>(ws + p.parts);
+    e.parts = reinterpret_cast<float*>(ws + p.parts); e.row_f = reinterpret_cast<float*>(ws + p.rows); e.R_all = a->R;
     e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = {a->labels, a->label_bytes, a->V};
     e.pm = reinterpret_cast<float*>(ws + p.a); e.pl = reinterpret_cast<float*>(ws + p.b); e.zl = reinterpret_cast<float*>(ws + p.zl);
     e.R = a->R; e.V = a->V; e.Rp = p.Rp;
@@ -744,22 +799,20 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
     if (a->ws_bytes < 0 || (size_t)a->ws_bytes < p.bytes) return SAR_EINVAL;
     char* ws = reinterpret_cast<char*>(a->ws);
     void* dz = ws + p.dz;
-    Side x, w;
-    if (p.light) operands<elt, false>(a, p, true, x, w, st);
-    else operands<bwd16, BWD_SCALED>(a, p, true, x, w, st);
+    const Operands in = p.light ? operands<elt, false>(a, p, true, st) : operands<bwd16, BWD_SCALED>(a, p, true, st);
     const auto from = [&](const Side& s, int v) { Side t = s; t.p = reinterpret_cast<const char*>(s.p) + (long)v * (p.light ? (long)sizeof(elt) : 2); return t; };
     for (int i = 0; i < p.pieces; ++i) {
         const int v0 = i * p.piece, cols = a->V - v0 < p.piece ? a->V - v0 : p.piece, ld = up64(cols);
         const long plane = (long)p.Rp * ld;
         Epi e = {};
-        e.parts = reinterpret_cast<float*>(ws + p.parts);
+        e.parts = reinterpret_cast<float*>(ws + p.parts); e.row_f = reinterpret_cast<float*>(ws + p.rows);
         e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = {a->labels, a->label_bytes, a->V}; e.dloss = a->dloss; e.lse = a->lse;
         e.dz = dz; e.dz_plane = plane; e.dz_ld = ld;
         if (a->dbias && p.db_slices > 1) e.db = reinterpret_cast<float*>(ws + p.dbp);
         else if (a->dbias) { e.db_out = reinterpret_cast<elt*>(a->dbias) + v0; e.db_accumulate = a->accumulate; }
         e.g_from = p.g_from; e.R_all = a->R;
         e.R = a->R; e.V = a->V; e.v0 = v0; e.Rp = p.Rp;
-        Side wz = from(w, v0), xz = x;
+        Side wz = from(in.w, v0), xz = in.x;
         wz.len = (p.pack_w ? p.Vp : a->V) - v0; wz.k = a->D;
         xz.len = a->R; xz.k = p.pack_x ? p.Dp : a->D;
         const int step = logits_step(a, p.small_z);
@@ -781,7 +834,7 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         if (a->dkernel) {
             Epi o = e;
             o.R = a->D; o.V = cols; o.with_w = 0; o.part = p.dw_slices > 1;
-            const Side A = {x.p, x.plane, x.ld, p.pack_x ? p.Dp : a->D, a->R}, B = {dz, plane, ld, ld, p.Rp};
+            const Side A = {in.xg.p, in.xg.plane, in.xg.ld, p.pack_x ? p.Dp : a->D, a->R}, B = {dz, plane, ld, ld, p.Rp};
             elt* out = reinterpret_cast<elt*>(a->dkernel) + v0;
             if (o.part) {
                 o.out = ws + p.dwp; o.slice = (long)a->D * ld; o.ldo = ld;
@@ -792,7 +845,7 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         if (a->dx) {
             Epi o = e;
             o.R = a->R; o.V = a->D; o.with_w = 1; o.ldo = a->D; o.part = p.dx_parts;
-            const Side A = {dz, plane, ld, p.Rp, ld}, B = {from(w, v0).p, w.plane, w.ld, a->D, p.pack_w ? ld : cols};
+            const Side A = {dz, plane, ld, p.Rp, ld}, B = {from(in.w, v0).p, in.w.plane, in.w.ld, a->D, p.pack_w ? ld : cols};
             if (o.part) {
                 o.out = ws + p.dxp; o.slice = (long)a->R * a->D; o.accumulate = i > 0;
                 if (i == p.pieces - 1) sum(p.dxp, p.dx_slices, o.slice, a->R, a->D, a->D, reinterpret_cast<elt*>(a->dx), a->D, 0);

@@ -31,3 +31,50 @@ def test_dloss_of_rows_without_a_label_is_not_looked_at(R, D, V, dt):
         for labels in (lab, lab.long()):
             got = run(torch.where(out, torch.full_like(dl, junk), dl), x, w, labels, b)
             assert all(torch.equal(g, w_) for g, w_ in zip(got, want)), junk
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("R,D,V", SIZES)
+def test_a_large_row_without_a_label_leaves_no_trace(R, D, V, dt):
+    """x of left-out rows up to what the type holds: every result of the others, and the kernel's and the bias's gradients, bit for bit."""
+    x, w, lab, b, dl = make(R, D, V, DT[dt], seed=R)
+    out = (lab < 0) | (lab >= V)
+    want = run(dl, torch.where(out[:, None], torch.zeros_like(x), x), w, lab, b)
+    for size in (6e4,) if dt == "f16" else (1e6, 1e12, 1e20, 1e37):
+        got = run(dl, torch.where(out[:, None], torch.full_like(x, size) * torch.sign(x), x), w, lab, b)
+        for i, (g, w_) in enumerate(zip(got, want)):
+            assert torch.equal(g[~out], w_[~out]) if i in (1, 2) else torch.equal(g, w_), (size, i)
+        assert (got[2][out] == 0).all()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("R,D,V", SIZES)
+def test_a_large_row_leaves_the_other_rows_alone(R, D, V, dt):
+    """A labelled row far larger than the others: their loss, log-sum-exp and dx do not change by a bit."""
+    x, w, lab, b, dl = make(R, D, V, DT[dt], seed=R)
+    others = torch.arange(R, device="cuda") != 2
+    want = run(dl, x, w, lab, b)
+    for size in (1e4,) if dt == "f16" else (1e4, 1e6, 1e10, 1e20, 1e30):
+        y = x.clone(); y[2] *= size
+        got = run(dl, y, w, lab, b)
+        assert torch.isfinite(got[0]).all() and torch.isfinite(got[2]).all()
+        assert all(torch.equal(g[others], w_[others]) for g, w_ in zip(got[:3], want)), size
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("R,D,V", SIZES[1:])
+def test_rows_of_many_sizes(R, D, V, dt):
+    """Rows of x over eight orders of magnitude (fp16: five), each held to its own.
+
+    The logits of a row: fp32 sums of D products, |dz| <= 2^-24 (D + 4) sum |x W|; packed fp32 operands add 2^-21 sum |x W| and, for elements far below
+    their maxima, 2^-37 D max|x_r| max|W| with x_r THIS row.  lse and loss: as derived in test_gpu_vocab_ce.py.  dx: dz's steps (ed there) met by W."""
+    from tests.test_gpu_vocab_ce import check, reference
+    x, w, lab, b, dl = make(R, D, V, DT[dt], seed=R + 1)
+    e = torch.linspace(-3, 2 if dt == "f16" else 5, R, device="cuda")[torch.randperm(R, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")]
+    x = (x.float() * 10.0 ** e[:, None]).to(x.dtype)
+    got = run(dl, x, w, lab, b)
+    for i in range(0, R, 97):                                      # one row at a time: reference() takes maxima over its rows
+        s = slice(i, i + 1)
+        want, bd = reference(x[s], w, lab[s], b, dl[s])
+        check(got[0][s], want[0], bd[0], "loss"); check(got[1][s], want[1], bd[1], "lse")
+        check(got[2][s], want[2], bd[2] + 2.0 ** -38 * dl.abs().max().item() * w.double().abs().sum(1), "dx")
