@@ -50,10 +50,11 @@ template <int N> __device__ __forceinline__ void exponents(f32x16 (&s)[N], float
     }
 }
 // lse in powers of two for the backward's p = exp2(s f - e).  It is rounded too: past 2^22 by whole units, which decide what p comes out as.  There it is
-// moved up by its rounding, so that no p is above 1 and the gradients stay finite.  A row that met no score (lse -inf) gets 0.
-__device__ __forceinline__ float backward_exponent(float lse) {
-    const float e = lse * LOG2E, a = fabsf(e);
-    return e == -INFINITY ? 0.f : a > 4194304.f ? fmaf(a, 2.384185791015625e-7f, e) : e;
+// moved up by its roundings, so that no p is above 1 and the gradients stay finite.  A row that met no score (lse -inf) gets 0.
+// up: p is wanted times 2^up (below 2^22 that costs nothing of e: up is a multiple of its last place).
+__device__ __forceinline__ float backward_exponent(float lse, float up = 0.f) {
+    const float e = lse * LOG2E, a = fabsf(e), r = e - up;
+    return e == -INFINITY ? 0.f : a > 4194304.f ? fmaf(a, 2.384185791015625e-7f, r) : r;
 }
 
 struct Row { int t, h; };

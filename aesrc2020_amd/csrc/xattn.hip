@@ -81,6 +81,57 @@ template <typename T, int ND> __device__ __forceinline__ void store_column(T* p,
         }
 }
 
+// ---- fp16 operands of the gradients' second products.  ds of a mean over a batch (p of 1 / Tk, dout of 1e-4) is far below fp16's normal numbers, and the
+// largest ds lies above the largest dq: as they are, dout of 1e-4 cost dq 1.4 % at 1140 keys, and ds past 65504 was infinite.  So p, 1 at most, is
+// held times 2^15 (its exponent says so), and ds under a power of two of its column (a row for dQ, a key for dK) besides: as a softmax's maximum that
+// follows the largest |ds| so far, puts it into [2^4, 2^15], and takes the sums along when it changes, which hardly a tile makes it do.
+// bf16 and fp32 have the range.  It costs 16-bit training 0 to 5 % (8 x 1024 x 4096 of 128: forward and backward 1204 -> 1235 us; 4 x 300 x 2000 of 64:
+// 70.5 -> 73.5), 8 % where 128-wide heads spill (8 x 1000 x 200: 97 -> 105); with the maximum kept within 2^2 of the limit twice that.
+template <typename T> constexpr bool narrow() { return __is_same(T, _Float16); }
+template <typename T> constexpr float p_bits() { return narrow<T>() ? 15.f : 0.f; }
+template <typename T> constexpr float p_down() { return narrow<T>() ? 1.f / 32768.f : 1.f; }
+constexpr float DS_MOST = 32768.f, DS_UP = 1.152921504606846976e18f;            // 2^60, above what any ds that reaches a result needs; |ds| < 2^56 of fp16 inputs
+__device__ __forceinline__ float largest(const f32x16& x) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, fabsf(x[i])), fabsf(x[i + 1]));
+    return top;
+}
+// the power of two that puts `top` into [2^(bits - 1), 2^bits), DS_UP at most
+__device__ __forceinline__ float raise(float top, int bits) {
+    int e = 0;
+    (void)frexpf(top, &e);
+    return top == 0.f ? DS_UP : fminf(ldexpf(1.f, bits - e), DS_UP);
+}
+template <typename T, int N> __device__ __forceinline__ void times(f32x16 (&o)[N], float f) {
+    if constexpr (narrow<T>()) {
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= f;
+    }
+}
+// pack (attn_tiles.h) of s f (fp16; the others: of s)
+template <typename T> __device__ __forceinline__ void pack_times(const f32x16& s, float f, u32x4* p) {
+    if constexpr (narrow<T>()) {
+        f32x16 up;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) up[i] = s[i] * f;
+        pack<T>(up, p);
+    } else pack<T>(s, p);
+}
+template <typename T> struct ColumnScale {
+    float f = narrow<T>() ? DS_UP : 1.f;
+    // room for ds f, of which `top` is the largest that the lane has; the sums come along.  -> what to multiply ds f with once more
+    template <int N> __device__ __forceinline__ float fit(float top, f32x16 (&sums)[N]) {
+        top = half_max(top);
+        const float g = top > DS_MOST ? fminf(raise(top, 5), 1.f) : 1.f;
+        times<T>(sums, g);
+        f *= g;
+        return g;
+    }
+};
+
 // ---- forward: a block takes 32 WN rows (as columns n) against one slice of the keys
 template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_fwd_kernel(sarXattn a, int row_tiles, int splits) {
     constexpr int KT = step_rows<T, WN>(), P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, WM = 4 / WN, NS = KT / 32 / WM, TILE = KT * P;
@@ -228,7 +279,7 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
         load_row<T, DP>(reinterpret_cast<const T*>(a.q) + b * a.q_sb + me.t * a.q_st + me.h * a.q_sh, r < rl, a.D, h, qf);
         load_row<T, DP>(reinterpret_cast<const T*>(a.dout) + b * a.g_sb + me.t * a.g_st + me.h * a.g_sh, r < rl, a.D, h, gf);
         load_row<T, DP>(reinterpret_cast<const T*>(a.out) + b * a.o_sb + me.t * a.o_st + me.h * a.o_sh, r < rl, a.D, h, of);
-        if (r < rl) e = backward_exponent(a.lse[stat_at(a, b, me)]);
+        if (r < rl) e = backward_exponent(a.lse[stat_at(a, b, me)], p_bits<T>());
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -239,6 +290,7 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
     if (!summed && sp == 0 && wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
     f32x16 dq[ND];
     clear(dq);
+    ColumnScale<T> up;
     float sum = 0.f;
     int cur = 0;
     bool first = summed;                                          // the pass that sums p dp
@@ -257,7 +309,7 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
                 __syncthreads();
                 sum = joined[0][wn][lane] + joined[1][wn][lane];
             }
-            dl = sum;
+            dl = sum * p_down<T>();
             if (wm == 0 && h == 0 && r < R) stats[stat_at(a, b, me)] = make_float2(e, dl);
         }
         if (row0 >= rl || (WM > 1 && at_key + 32 * wm >= len)) continue;
@@ -286,13 +338,22 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
                 continue;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dp[i] = s[i] * (dp[i] - dl);
+            for (int i = 0; i < 16; ++i) dp[i] = s[i] * (narrow<T>() ? fmaf(dp[i], up.f, -dl * up.f) : dp[i] - dl);
+            if constexpr (narrow<T>()) {
+                const float top = largest(dp);
+                if (__builtin_expect(__any(top > DS_MOST), 0)) {
+                    const float g = up.fit(top, dq);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dp[i] *= g;
+                }
+            }
             u32x4 df[4];
             pack<T>(dp, df);
 #pragma unroll
             for (int d = 0; d < ND; ++d) dq[d] = mma_down<T, P>(lk, at, d, df, dq[d], lane);
         }
     }
+    times<T>(dq, p_down<T>() / up.f);
     if constexpr (WM > 1) {
         static_assert(WM == 2, "");
         float* join = reinterpret_cast<float*>(lds) + wn * ND * 1024;
@@ -339,11 +400,11 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     const auto load_stats = [&](RowTile r) {
         return sb[(long)r.g * a.Tq + min(r.t + (int)threadIdx.x % RT, tl - 1)];
     };
-    // one key: p = 1 whatever the score (s 0 - 0), and ds = 0 (dK is stored as zero)
+    // one key: p = 1 whatever the score (s 0 - 0, or times 2^p_bits), and ds = 0 (dK is stored as zero)
     const float sk = len == 1 ? 0.f : sl;
     const auto put_stats = [&](int to, RowTile r, float2 v) {
         const bool in = r.t + (int)threadIdx.x < tl;
-        if (threadIdx.x < RT) row_stats[to][threadIdx.x] = make_float2(in && len > 1 ? v.x : 0.f, in ? v.y : 0.f);
+        if (threadIdx.x < RT) row_stats[to][threadIdx.x] = make_float2(in && len > 1 ? v.x : -p_bits<T>(), in ? v.y : 0.f);
     };
     // (statistics are fetched two steps ahead and put right behind a barrier, where nothing has to be waited for)
     RowTile at_row = {0, 0}, next_row = {0, 0};
@@ -366,6 +427,7 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
     settle(vf);
     f32x16 dk[ND], dv[ND];
     clear(dk); clear(dv);
+    ColumnScale<T> up;
     int cur = 0, par = 0;
     for (int i = i0; i < i1; ++i) {
         tile_barrier();
@@ -399,12 +461,18 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
             for (int x = 0; x < 4; ++x)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) dp[4 * x + c] = s[4 * x + c] * (dp[4 * x + c] - st[2 * (8 * x + 4 * h + c) + 1]);
-            pack<T>(dp, pf);
+            if constexpr (narrow<T>()) {
+                const float top = key < len ? largest(dp) * up.f : 0.f;
+                if (__builtin_expect(__any(top > DS_MOST), 0)) up.fit(top, dk);
+            }
+            pack_times<T>(dp, up.f, pf);
 #pragma unroll
             for (int d = 0; d < ND; ++d) dk[d] = mma_down<T, P>(lq, 32 * wm, d, pf, dk[d], lane);
         }
         cur ^= BUF; par ^= 1;
     }
+    times<T>(dk, p_down<T>() / up.f);
+    times<T>(dv, p_down<T>());
     if constexpr (WM > 1) {
         static_assert(WM == 2, "");
         float* join = reinterpret_cast<float*>(lds) + wn * 2 * ND * 1024;
@@ -476,7 +544,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256, 2) void xattn_sm
         return lse[(long)r.g * a.Tq + min(r.t + (int)threadIdx.x % RT, tl - 1)];
     };
     const auto put_lse = [&](int to, RowTile r, float v) {
-        if (threadIdx.x < RT) exponent[to][threadIdx.x] = len > 1 && r.t + (int)threadIdx.x < tl ? backward_exponent(v) : 0.f;
+        if (threadIdx.x < RT) exponent[to][threadIdx.x] = len > 1 && r.t + (int)threadIdx.x < tl ? backward_exponent(v, p_bits<T>()) : -p_bits<T>();
     };
     char* const tiles_at = lds + TILE;
     float* const ds_at = reinterpret_cast<float*>(lds + S::DS_AT);
@@ -497,6 +565,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256, 2) void xattn_sm
     settle(vf);
     f32x16 dk[ND], dv[ND];
     clear(dk); clear(dv);
+    ColumnScale<T> up;
     int cur = 0, par = 0;
     for (int i = i0; i < i1; ++i) {
         tile_barrier();
@@ -541,13 +610,17 @@ template <typename T, int DP> __global__ __launch_bounds__(256, 2) void xattn_sm
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int row = 8 * x + 4 * h + c;
-                    const float dl = sums[0][32 * wm + row] + sums[1][32 * wm + row];
+                    const float dl = (sums[0][32 * wm + row] + sums[1][32 * wm + row]) * p_down<T>();
                     v[c] = dp[4 * x + c] = s[4 * x + c] * (dp[4 * x + c] - dl);
                 }
                 *reinterpret_cast<f32x4*>(ds_at + key * S::DS_PITCH + 32 * wm + 8 * x + 4 * h) = v;
             }
+            if constexpr (narrow<T>()) {
+                const float top = key < len ? largest(dp) * up.f : 0.f;
+                if (__builtin_expect(__any(top > DS_MOST), 0)) up.fit(top, dk);
+            }
             u32x4 pf[4];
-            pack<T>(dp, pf);
+            pack_times<T>(dp, up.f, pf);
 #pragma unroll
             for (int d = 0; d < ND; ++d) dk[d] = mma_down<T, P>(lq, 32 * wm, d, pf, dk[d], lane);
         }
@@ -560,14 +633,27 @@ template <typename T, int DP> __global__ __launch_bounds__(256, 2) void xattn_sm
             const int row = t + 32 * wm + n;
             T* to = reinterpret_cast<T*>(a.dq) + (((long)b * a.Tq + row) * a.Hq + hk * G + g) * a.D;
             u32x4 df[2][4];
+            const auto ds_of = [&](int k, int i) { return ds_at[(32 * k + 8 * (i >> 2) + 4 * h + (i & 3)) * S::DS_PITCH + 32 * wm + n]; };
+            float f = 1.f;
+            if constexpr (narrow<T>()) {                          // all keys are here: the row's scale is known.  (Read twice: the registers are short.)
+                float top = 0.f;
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (32 * k < len) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(ds_of(k, i)));
+                    }
+                f = raise(half_max(top), 14);
+            }
 #pragma unroll
             for (int k = 0; k < 2; ++k)
                 if (32 * k < len) {
                     f32x16 x;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = ds_at[(32 * k + 8 * (i >> 2) + 4 * h + (i & 3)) * S::DS_PITCH + 32 * wm + n];
-                    pack<T>(x, df[k]);
+                    for (int i = 0; i < 16; ++i) x[i] = ds_of(k, i);
+                    pack_times<T>(x, f, df[k]);
                 }
+            const float back = a.scale * (p_down<T>() / f);
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 if ((d & 1) != wn) continue;
@@ -580,7 +666,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256, 2) void xattn_sm
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int dd = 32 * d + 8 * i + 4 * h;
-                        if (dd < a.D) store4<T>(to + dd, in ? q[4 * i] * a.scale : 0.f, in ? q[4 * i + 1] * a.scale : 0.f, in ? q[4 * i + 2] * a.scale : 0.f, in ? q[4 * i + 3] * a.scale : 0.f);
+                        if (dd < a.D) store4<T>(to + dd, in ? q[4 * i] * back : 0.f, in ? q[4 * i + 1] * back : 0.f, in ? q[4 * i + 2] * back : 0.f, in ? q[4 * i + 3] * back : 0.f);
                     }
                 }
             }
@@ -595,6 +681,8 @@ template <typename T, int DP> __global__ __launch_bounds__(256, 2) void xattn_sm
             store4<T>(reinterpret_cast<T*>(a.dq) + (((long)b * a.Tq + tl + row) * a.Hq + hk * G) * a.D + (i - row * wide) * 4, 0.f, 0.f, 0.f, 0.f);
         }
     }
+    times<T>(dk, p_down<T>() / up.f);
+    times<T>(dv, p_down<T>());
     float* join = reinterpret_cast<float*>(lds) + wn * 2 * ND * 1024;
     static_assert(2 * 2 * ND * 1024 * 4 <= S::LDS, "");
     __syncthreads();
