@@ -29,6 +29,8 @@ _NAMES = {n: {d: "sar_%s_%s" % (n, s) for d, s in _SFX.items()} for n in ("xattn
 
 def _rows(name, x, like=None):
     """x as the kernels take it: 4-D, last axis contiguous, rows on 16-byte boundaries and at most 16 MB apart -- a view that is not is copied."""
+    if x is None:
+        raise ValueError("%s is missing" % name)
     if x.dim() != 4:
         raise ValueError("%s has to be (batch, time, heads, dim), got shape %r" % (name, tuple(x.shape)))
     if like is None:
@@ -89,6 +91,14 @@ def _result(name, t, shape, dtype, device):
     return t
 
 
+def _given(name, t, shape, dtype, device):
+    """An fp32 vector that a gradient reads as it is: lse, dloss."""
+    if t is None or tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError("%s has to be a contiguous %s tensor of shape %r on %s, got %s" %
+                         (name, dtype, tuple(shape), device, "None" if t is None else "%s %r on %s" % (t.dtype, tuple(t.shape), t.device)))
+    return t
+
+
 def _result_like(name, t, q):
     """`t`, or a new tensor, of q's shape and type, contiguous (empty_like is the faster call; q's rows are aligned: _rows)."""
     return torch.empty_like(q) if t is None and q.is_contiguous() else _result(name, t, q.shape, q.dtype, q.device)
@@ -144,7 +154,7 @@ def cross_attention_grad(dout, q, k, v, out, lse, k_lens=None, q_lens=None, scal
     Tk, Hkv, device = k.shape[1], k.shape[2], q.device
     if dout.shape != q.shape or out.shape != q.shape:
         raise ValueError("dout %r and out %r have to have the shape of q %r" % (tuple(dout.shape), tuple(out.shape), tuple(q.shape)))
-    lse = _result("lse", lse, (B, Hq, Tq), torch.float32, device)
+    lse = _given("lse", lse, (B, Hq, Tq), torch.float32, device)
     dq = _result_like("dq", dq, q) if B and Tq else _result("dq", dq, q.shape, q.dtype, device)
     dk, dv = _result("dk", dk, k.shape, q.dtype, device), _result("dv", dv, v.shape, q.dtype, device)
     kl = 0 if k_lens is None else _lens("k_lens", k_lens, B, device)

@@ -10,7 +10,7 @@ import struct
 import torch
 
 from . import _lib
-from .attention import _SFX, _WS, _launch, _result
+from .attention import _SFX, _WS, _given, _launch, _result
 from .engine import glorot_uniform
 from .layers import Layer
 
@@ -160,6 +160,8 @@ _LABELS = {torch.int32: 4, torch.int64: 8}
 
 def _vocab_args(x, kernel, labels, bias):
     """-> x, kernel (rows contiguous), R, D, V: as the kernels take them."""
+    if x is None or kernel is None or labels is None:
+        raise ValueError("x, kernel and labels have to be given")
     xs, ks = x.shape, kernel.shape
     if len(xs) != 2 or len(ks) != 2 or xs[1] != ks[0] or ks[0] < 1 or ks[1] < 1:
         raise ValueError("x %r and kernel %r have to be (rows, D) and (D, vocabulary)" % (tuple(xs), tuple(ks)))
@@ -223,7 +225,7 @@ def vocab_crossentropy_grad(dloss, x, kernel, labels, lse, bias=None, dx=None, d
     x, kernel, R, D, V = _vocab_args(x, kernel, labels, bias)
     if accumulate and (x.dtype != torch.float32 or dkernel is None or (bias is not None and dbias is None)):
         raise ValueError("accumulate needs fp32 and the buffers to add to")
-    dloss, lse = _result("dloss", dloss, (R,), torch.float32, x.device), _result("lse", lse, (R,), torch.float32, x.device)
+    dloss, lse = _given("dloss", dloss, (R,), torch.float32, x.device), _given("lse", lse, (R,), torch.float32, x.device)
     dx = _result("dx", dx, (R, D), x.dtype, x.device) if need_dx else None
     dkernel = _result("dkernel", dkernel, (D, V), x.dtype, x.device)
     dbias = None if bias is None else _result("dbias", dbias, (V,), x.dtype, x.device)

@@ -1,0 +1,27 @@
+"""Arguments of the decoder operators that only a device shows: what is missing, what lies where."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def test_gradients_need_the_forwards_statistics():
+    """lse and dloss are inputs: None is refused, a view that starts off a 16-byte boundary is taken."""
+    from aesrc2020_amd.attention import cross_attention, cross_attention_grad
+    from aesrc2020_amd.losses import vocab_crossentropy, vocab_crossentropy_grad
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, do = (torch.randn(2, n, 2, 16, generator=g, device="cuda") for n in (5, 9, 9, 5))
+    out, lse = cross_attention(q, k, v, return_lse=True)
+    x, w = torch.randn(6, 32, generator=g, device="cuda"), torch.randn(32, 64, generator=g, device="cuda")
+    lab, dl = torch.arange(6, device="cuda"), torch.rand(6, generator=g, device="cuda")
+    _, zl = vocab_crossentropy(x, w, lab, return_lse=True)
+    for f in (lambda: cross_attention_grad(do, q, k, v, out, None), lambda: cross_attention_grad(do, q, k, v, None, lse), lambda: cross_attention_grad(None, q, k, v, out, lse),
+              lambda: vocab_crossentropy_grad(dl, x, w, lab, None), lambda: vocab_crossentropy_grad(None, x, w, lab, zl), lambda: vocab_crossentropy_grad(dl, x, w, None, zl)):
+        with pytest.raises(ValueError):
+            f()
+    off = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)  # noqa: E731
+    assert off(lse).data_ptr() % 16 == 4
+    for a, b in zip(cross_attention_grad(do, q, k, v, out, off(lse)), cross_attention_grad(do, q, k, v, out, lse)):
+        assert torch.equal(a, b)
+    for a, b in zip(vocab_crossentropy_grad(off(dl), x, w, lab, off(zl))[:2], vocab_crossentropy_grad(dl, x, w, lab, zl)[:2]):
+        assert torch.equal(a, b)
