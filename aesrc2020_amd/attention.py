@@ -134,9 +134,9 @@ def cross_attention(q, k, v, k_lens=None, q_lens=None, scale=None, return_lse=Fa
     kl = 0 if k_lens is None else _lens("k_lens", k_lens, B, device)
     ql = 0 if q_lens is None else _lens("q_lens", q_lens, B, device)
     if B and Tq:
-        qp, sq, sk, sv, so = q.data_ptr(), q.stride(), k.stride(), v.stride(), out.stride()
+        qp, sq, sk, sv = q.data_ptr(), q.stride(), k.stride(), v.stride()
         a = _XATTN.pack(qp, k.data_ptr() if Tk else qp, v.data_ptr() if Tk else qp, 0, out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, kl, ql, 0, 0,      # (no frames: never read)
-                        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], so[0], so[1], so[2], 0, 0, 0, B, Tq, Tk, Hq, Hkv, D, _scale(scale, D), q.element_size())
+                        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], Tq * Hq * D, Hq * D, D, 0, 0, 0, B, Tq, Tk, Hq, Hkv, D, _scale(scale, D), q.element_size())
         if Tk > 256:                                                   # (sarnet.h: 256 keys never need a workspace)
             a, ws = _with_workspace("sar_xattn_fwd_workspace_bytes", device, a)
         _launch(_NAMES["xattn_fwd"][q.dtype], device, a)
@@ -221,8 +221,8 @@ class EncoderCache8:
         out = _result_like("out", out, q)
         ql = 0 if q_lens is None else _lens("q_lens", q_lens, B, device)
         if Tq:
-            s, so = q.stride(), out.stride()
-            a = _XATTN.pack(q.data_ptr(), 0, 0, 0, out.data_ptr(), 0, 0, 0, 0, self.lens.data_ptr(), ql, 0, 0, s[0], s[1], s[2], 0, 0, 0, 0, 0, 0, so[0], so[1], so[2], 0, 0, 0,
+            s = q.stride()
+            a = _XATTN.pack(q.data_ptr(), 0, 0, 0, out.data_ptr(), 0, 0, 0, 0, self.lens.data_ptr(), ql, 0, 0, s[0], s[1], s[2], 0, 0, 0, 0, 0, 0, Tq * Hq * D, Hq * D, D, 0, 0, 0,
                             B, Tq, self.frames, Hq, self.heads, D, _scale(scale, D), q.element_size())
             if self.frames > 256:
                 a, ws = _with_workspace("sar_kv8_attend_workspace_bytes", device, a)

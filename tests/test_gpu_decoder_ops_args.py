@@ -25,3 +25,22 @@ def test_gradients_need_the_forwards_statistics():
         assert torch.equal(a, b)
     for a, b in zip(vocab_crossentropy_grad(off(dl), x, w, lab, off(zl))[:2], vocab_crossentropy_grad(dl, x, w, lab, zl)[:2]):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("Tq", [3, 90])
+def test_results_go_into_any_contiguous_buffer(Tq):
+    """An axis of length 1 may have any stride in a contiguous tensor (a transposed or sliced buffer)."""
+    from aesrc2020_amd.attention import EncoderCache8, cross_attention, cross_attention_grad
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v, do = (torch.randn(1, n, 1, 64, generator=g, device="cuda") for n in (Tq, 70, 70, Tq))
+    cache = EncoderCache8(1, 70, 1, 64)
+    cache.store(k, v)
+    want, lse = cross_attention(q, k, v, return_lse=True)
+    held = cache.attend(q)
+    grads = cross_attention_grad(do, q, k, v, want, lse)
+    for make in (lambda n: torch.empty(1, n, 64, 1, device="cuda").transpose(2, 3), lambda n: torch.empty(1 * n * 64, device="cuda").as_strided((1, n, 1, 64), (3, 64, 7, 1))):
+        out = make(Tq)
+        assert out.is_contiguous() and cross_attention(q, k, v, out=out) is out and torch.equal(out, want)
+        assert cache.attend(q, out=out) is out and torch.equal(out, held)
+        got = cross_attention_grad(do, q, k, v, out.copy_(want), lse, dq=make(Tq), dk=make(70), dv=make(70))
+        assert all(torch.equal(a, b) for a, b in zip(got, grads))
