@@ -70,6 +70,8 @@ def _launch(name, device, *args):
             rc = fn(*args, torch.cuda.current_stream().cuda_stream)
     else:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))      # (torch.cuda.current_stream().cuda_stream without the Stream object: 2 us less)
+    if rc == -1:
+        raise ValueError("%s does not take these arguments: include/sarnet.h states its limits" % name)
     if rc != 0:
         raise RuntimeError("%s failed with status %d" % (name, rc))
 

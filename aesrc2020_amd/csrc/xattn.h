@@ -72,7 +72,8 @@ __device__ __host__ __forceinline__ long part_floats(long rows, int D, int split
 static inline bool bad_shape(const sarXattn* a) {
     if (!a || a->B < 1 || a->Tq < 1 || a->Tk < 0 || a->Hkv < 1 || a->Hq < 1 || a->Hq % a->Hkv || a->D < 8 || a->D > 128 || a->D % 8) return true;
     const long R = (long)a->Tq * (a->Hq / a->Hkv);
-    return R > (1L << 30) || a->Tk > (1 << 30) || (R + 31) / 32 * a->B * a->Hkv > (1L << 24) || (a->Tk + 127L) / 128 * a->B * a->Hkv > (1L << 24);
+    // a launch has fewer than 2^32 threads: 512 for 32 rows at most, 256 for 128 keys
+    return R > (1L << 30) || a->Tk > (1 << 30) || (R + 31) / 32 * a->B * a->Hkv > (1L << 23) - 8 || (a->Tk + 127L) / 128 * a->B * a->Hkv > (1L << 24) - 8;
 }
 static inline bool bad_strides(int elt_bytes, const long* s, int n) {
     for (int i = 0; i < n; ++i)

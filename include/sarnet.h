@@ -592,7 +592,8 @@ int sar_adam_l2_update_f32(float* params, const float* grads, float* m, float* v
  * [0, T] count as the nearer end.  Rows of K and V behind a length are not used, whatever they hold.  A row behind its q_len, and a
  * row without keys, gets out = 0, lse = -inf and no gradient.  lse (B, Hq, Tq) fp32: optional in the forward, needed (with out) by the backward.
  * ws: sar_xattn_fwd_workspace_bytes / _bwd_workspace_bytes of the same arguments, 16-byte aligned (0: none; a forward over at most 256 keys never
- * needs one); nothing in it has to be initialised.  Time strides: at most 16 MB. */
+ * needs one); nothing in it has to be initialised.  Time strides: at most 16 MB.  B Hkv times the 32s in Tq Hq / Hkv: below 2^23; times the 128s in Tk:
+ * below 2^24. */
 typedef struct {
     const void *q, *k, *v, *dout;
     void* out;
