@@ -297,7 +297,7 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
 __global__ __launch_bounds__(256, (PA * PB == 1 && BK == 32 ? 3 : 2)) void product_kernel(Job job) {
     typedef Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA, PB, PZ> P;
     __shared__ __attribute__((aligned(1024))) char lds[P::LDS];
-    P::run(lds, blockIdx.x, job);
+    P::run(lds, blockIdx.x + gridDim.x * blockIdx.y, job);
 }
 // dW and dx of a piece in one launch, 64 x 64 tiles: neither fills the chip by itself
 template <typename OP, int BKW, int BKX, bool SCALED, int PO, int PZ> __global__ __launch_bounds__(256, 2) void grads_kernel(Job dw, Job dx, int first) {
@@ -753,9 +753,14 @@ static Job job_of(Side A, Side B, const Epi& e, int m, int n, int k, int step, i
     return {A, B, e, cdiv(m, t), cdiv(n, t), cdiv(k, step), slices};
 }
 static unsigned blocks_of(const Job& j) { return (unsigned)attn::xcd_grid((long)j.mtiles * j.ntiles * j.slices); }
+// a launch has fewer than 2^32 threads along an axis: in rows of 2^22 blocks (a multiple of the XCDs; surplus blocks find no item)
+static dim3 grid_of(const Job& j) {
+    const unsigned n = blocks_of(j), row = 1u << 22;
+    return n <= row ? dim3(n) : dim3(row, (n + row - 1) / row);
+}
 template <typename OP, bool AD, bool BD, int EPI, bool SCALED> static void product(const Job& j, bool small_tiles, int step, hipStream_t st) {
     constexpr int BK = step_of();
-    const dim3 grid(blocks_of(j)), block(256);
+    const dim3 grid = grid_of(j), block(256);
     if (small_tiles) hipLaunchKernelGGL((product_kernel<OP, BK, 1, 1, AD, BD, EPI, SCALED, NPL, NPL, NPL>), grid, block, 0, st, j);
     else if (EPI == E_GRAD || step == BK) hipLaunchKernelGGL((product_kernel<OP, BK, 2, 2, AD, BD, EPI, SCALED, NPL, NPL, NPL>), grid, block, 0, st, j);
     else if constexpr (EPI != E_GRAD) hipLaunchKernelGGL((product_kernel<OP, 32, 2, 2, AD, BD, EPI, SCALED, NPL, NPL, NPL>), grid, block, 0, st, j);
