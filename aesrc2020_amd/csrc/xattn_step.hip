@@ -282,13 +282,15 @@ template <typename T> __global__ __launch_bounds__(256) void xattn_combine_kerne
 // ---- writing the cache: one block per (K or V, utterance, head, 64 frames): maximum, scale, conversion in one pass over its 64 D values
 struct Kv8Side { const void* x; long sb, st, sh; unsigned char* y; float* scale; };
 template <typename T> __global__ __launch_bounds__(256) void kv8_store_kernel(Kv8Side sk, Kv8Side sv, const int* __restrict__ lens, int* __restrict__ lens_out, int T_in, int H, int D,
-                                                                              long frames, int first, int blocks) {
+                                                                              long frames, int first, int blocks, int total) {
     __shared__ float red[4];
     constexpr int V = 8;                                          // values a thread and step; D is a multiple of 8
     const Kv8Side& sd = blockIdx.y ? sv : sk;
     const T* x = reinterpret_cast<const T*>(sd.x);
     const long sb = sd.sb, st = sd.st, sh = sd.sh;
-    const int j = blockIdx.x % blocks, bh = blockIdx.x / blocks, b = bh / H, hh = bh % H;
+    const int item = blockIdx.x + gridDim.x * blockIdx.z;
+    if (item >= total) return;
+    const int j = item % blocks, bh = item / blocks, b = bh / H, hh = bh % H;
     const int per = D / V, n = KV_BLOCK * per;                    // <= 1024: four steps
     const int live = lens ? min(max(lens[b], 0), T_in) : T_in;
     // the cache's length: an utterance without new frames keeps the one it has
@@ -404,8 +406,9 @@ extern "C" int SAR_FN(sar_kv8_store)(const void* k, long k_sb, long k_st, long k
         if (!p || (uintptr_t)p % 16) return SAR_EINVAL;
     const int blocks = cdiv(T, KV_BLOCK);
     if ((long)B * H > (1L << 30) / blocks) return SAR_EINVAL;
-    hipLaunchKernelGGL((kv8_store_kernel<elt>), dim3((unsigned)(B * H * blocks), 2), dim3(256), 0, stream, Kv8Side{k, k_sb, k_st, k_sh, (unsigned char*)k8, k_scale},
-                       Kv8Side{v, v_sb, v_st, v_sh, (unsigned char*)v8, v_scale}, lens, lens_out, T, H, D, frames, first, blocks);
+    const int total = B * H * blocks, row = total < (1 << 22) ? total : 1 << 22;     // (fewer than 2^32 threads along an axis)
+    hipLaunchKernelGGL((kv8_store_kernel<elt>), dim3((unsigned)row, 2, (unsigned)cdiv(total, row)), dim3(256), 0, stream, Kv8Side{k, k_sb, k_st, k_sh, (unsigned char*)k8, k_scale},
+                       Kv8Side{v, v_sb, v_st, v_sh, (unsigned char*)v8, v_scale}, lens, lens_out, T, H, D, frames, first, blocks, total);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
 }
