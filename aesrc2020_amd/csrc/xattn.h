@@ -28,8 +28,9 @@ constexpr float NO_MAX = -3.402823e38f; // the running maximum before any key: f
 __device__ __forceinline__ int live_keys(const sarXattn& a, int b) { return a.k_lens ? min(max(a.k_lens[b], 0), a.Tk) : a.Tk; }
 __device__ __forceinline__ int live_rows(const sarXattn& a, int b) { return (a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq) * (a.Hq / a.Hkv); }
 
-// |scale| log2 e; for a scale of 0 a number that makes any finite product 0 and leaves -inf what it is
-__device__ __forceinline__ float score_factor(const sarXattn& a) { return fmaxf(fabsf(a.scale) * LOG2E, 1e-37f); }
+// |scale| log2 e; for a scale of 0 the smallest number, which makes nothing of any finite product and leaves -inf what it is
+constexpr float LEAST = 1.401298464324817e-45f;
+__device__ __forceinline__ float score_factor(const sarXattn& a) { return fmaxf(fabsf(a.scale) * LOG2E, LEAST); }
 
 // exp2(s f - m), m = the largest s f, rounded: one fma, whose product is exact; the rounding of m comes back as a factor that p and its sum share --
 // until m passes LARGE, where the factor itself would do harm: then the product is rounded as m's was, and the difference is exact.  (A branch per

@@ -169,7 +169,7 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
 #pragma unroll
             for (int c = 0; c < NC; ++c) s = mma<T>(frag<P>(tk, n, c, h), qf[0][c], s);
         }
-        const float f = S8 ? sl * ks[t * 32 / KV_BLOCK] : sl, nu = UNITS ? unit_of(t) : 1.f, v_scale = S8 && !UNITS ? vs[t * 32 / KV_BLOCK] : 1.f;
+        const float f = S8 ? fmaxf(fabsf(a.scale) * LOG2E * ks[t * 32 / KV_BLOCK], LEAST) : sl, nu = UNITS ? unit_of(t) : 1.f, v_scale = S8 && !UNITS ? vs[t * 32 / KV_BLOCK] : 1.f;
         float top = NO_MAX;
         if (t * 32 + 32 > len) {
 #pragma unroll

@@ -25,3 +25,33 @@ def test_more_blocks_than_one_row_of_a_launch():
             assert (w[:n] == row).all() and (w[n:] == 0).all()
         assert (s == 1).all()
     assert c.lens.tolist() == [T, T - 1, 0, 64]
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("Tq", [1, 3])
+def test_scores_of_no_size(Tq, dt):
+    """A scale of 0, and keys so small that their scores' factor leaves fp32's range: every frame weighs the same, those behind the length nothing."""
+    from aesrc2020_amd.attention import EncoderCache8
+    q, k, v, _ = make(2, Tq, 150, 4, 2, 32, torch.float32, seed=9)
+    kl = lens(150, 37)
+    c = EncoderCache8(2, 150, 2, 32)
+    for size, scale in ((1.0, 0.0), (2.0 ** -60, 0.0), (2.0 ** -125, 0.0), (2.0 ** 100, 0.0), (2.0 ** -120, 1e-20), (2.0 ** -125, 1.0)):
+        c.store(k * size, v, kl)
+        out = c.attend(q.to(DT[dt]), scale=scale)
+        held = (c.v8.float() * c.v_scale.repeat_interleave(64, 2)[..., None])[:, :, :150].transpose(1, 2).double()
+        for b, n in enumerate((150, 37)):
+            want = held[b, :n].mean(0).repeat_interleave(2, 0).expand(Tq, 4, 32)
+            # all p are 1 (or share one rounding), n + 3 fp32 sums of them and of v, the result's rounding
+            lim = 2.0 ** -24 * (2 * n + 8) * held[b, :n].abs().mean(0).repeat_interleave(2, 0) + torch.finfo(DT[dt]).eps / 2 * want.abs()
+            assert ((out[b].double() - want).abs() <= lim + (2.0 ** -25 if dt == "f16" else 0.0)).all(), (size, scale, b)
+
+
+def test_a_scale_of_zero_makes_nothing_of_large_scores():
+    """q . k of 2^120 on some keys, of -2^120 on others."""
+    from aesrc2020_amd.attention import cross_attention
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.ones(1, 70, 1, 16, device="cuda") * torch.where(torch.arange(70, device="cuda") % 3 == 0, -1.0, 1.0)[None, :, None, None]
+    v = torch.randn(1, 70, 1, 16, generator=g, device="cuda")
+    for n in (1, 50):
+        out = cross_attention(torch.full((1, n, 1, 16), 2.0 ** 116, device="cuda"), k, v, scale=0.0)
+        assert torch.allclose(out.double(), v.double().mean(1, keepdim=True).expand(1, n, 1, 16), rtol=0, atol=80 * 2.0 ** -23)
