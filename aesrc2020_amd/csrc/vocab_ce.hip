@@ -283,6 +283,8 @@ __device__ __forceinline__ int dz_exp(const Epi& e) {             // dz is held 
 }
 
 struct Job { Side A, B; Epi e; int mtiles, ntiles, ksteps, slices; };
+// a launch has fewer than 2^32 threads along an axis: blocks in rows of so many (a multiple of the XCDs; surplus blocks find no item)
+constexpr unsigned LAUNCH_ROW = 1u << 22;
 // C = A B^T over k, four waves as 2 x 2, each MT x NT tiles of 32 x 32.  ST stages of LDS, loads ST - 1 steps ahead.
 // What bounds it (16 bits, 128 x 128 tiles): LDS hands out four 16-byte fragments for four matrix instructions of a wave and takes the stages' loads,
 // about as many cycles as the matrix instructions need; with two blocks a CU those are busy 45 (dz) to 68 % (dW) of the time, at the 1.8 GHz that the
@@ -297,7 +299,7 @@ template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool S
 __global__ __launch_bounds__(256, (PA * PB == 1 && BK == 32 ? 3 : 2)) void product_kernel(Job job) {
     typedef Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA, PB, PZ> P;
     __shared__ __attribute__((aligned(1024))) char lds[P::LDS];
-    P::run(lds, blockIdx.x + gridDim.x * blockIdx.y, job);
+    P::run(lds, blockIdx.x + LAUNCH_ROW * blockIdx.y, job);
 }
 // dW and dx of a piece in one launch, 64 x 64 tiles: neither fills the chip by itself
 template <typename OP, int BKW, int BKX, bool SCALED, int PO, int PZ> __global__ __launch_bounds__(256, 2) void grads_kernel(Job dw, Job dx, int first) {
@@ -753,10 +755,9 @@ static Job job_of(Side A, Side B, const Epi& e, int m, int n, int k, int step, i
     return {A, B, e, cdiv(m, t), cdiv(n, t), cdiv(k, step), slices};
 }
 static unsigned blocks_of(const Job& j) { return (unsigned)attn::xcd_grid((long)j.mtiles * j.ntiles * j.slices); }
-// a launch has fewer than 2^32 threads along an axis: in rows of 2^22 blocks (a multiple of the XCDs; surplus blocks find no item)
 static dim3 grid_of(const Job& j) {
-    const unsigned n = blocks_of(j), row = 1u << 22;
-    return n <= row ? dim3(n) : dim3(row, (n + row - 1) / row);
+    const unsigned n = blocks_of(j);
+    return n <= LAUNCH_ROW ? dim3(n) : dim3(LAUNCH_ROW, (n + LAUNCH_ROW - 1) / LAUNCH_ROW);
 }
 template <typename OP, bool AD, bool BD, int EPI, bool SCALED> static void product(const Job& j, bool small_tiles, int step, hipStream_t st) {
     constexpr int BK = step_of();

@@ -138,6 +138,7 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
     // fp16 values of a cache: o holds sums in units of V's scale, `unit`, else 1.  (A block whose values end below 2^-31 counts as one of that size:
     // no fp16 result shows it.)
     constexpr bool UNITS = S8 && __is_same(C, _Float16);
+    constexpr float MOST = 3.4028235e38f;
     const auto unit_of = [&](int t) { return fmaxf(vs[t * 32 / KV_BLOCK], 9.094947017729282e-13f); };
     float m = NO_MAX, l = 0.f, unit = 1.f;
     if (UNITS && t0 + w < t1) unit = unit_of(t0 + w);
@@ -179,7 +180,8 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
         top = half_max(top) * f;
         if (__any(top > m + 8.f) || (UNITS && nu != unit)) {
-            const float mn = fmaxf(m, top), e = __builtin_amdgcn_exp2f(m - mn), eo = UNITS ? e * unit / nu : e;     // (in this order: no power of two passes the range before e has taken it back)
+            const float mn = fmaxf(m, top), e = __builtin_amdgcn_exp2f(m - mn), eo = UNITS ? fminf(e * unit / nu, MOST) : e;     // (in this order: no power of two passes the range before e has taken it back)
+            const bool beyond = UNITS && unit > nu * 1.2089258196146292e24f;     // by 2^80: sums other than 0 are past fp16's range, and stay finite here
             m = mn; l *= e;
             large = __any(fabsf(m) > LARGE && m != NO_MAX);
             if (UNITS) unit = nu;
@@ -187,6 +189,12 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= eo;
+            if (UNITS && __builtin_expect(beyond, 0)) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] = fabsf(o[d][i]) == INFINITY ? copysignf(MOST, o[d][i]) : o[d][i];
+            }
         }
         exponents(tile_s, f, m, large);
 #pragma unroll
@@ -279,17 +287,18 @@ template <typename T> __global__ __launch_bounds__(256) void xattn_combine_kerne
     if (a.lse && lane == 0) a.lse[i] = in ? M * LN2 + logf(L) : -INFINITY;
 }
 
+// a launch has fewer than 2^32 threads along an axis: blocks in rows of so many
+constexpr int LAUNCH_ROW = 1 << 22;
 // ---- writing the cache: one block per (K or V, utterance, head, 64 frames): maximum, scale, conversion in one pass over its 64 D values
 struct Kv8Side { const void* x; long sb, st, sh; unsigned char* y; float* scale; };
 template <typename T> __global__ __launch_bounds__(256) void kv8_store_kernel(Kv8Side sk, Kv8Side sv, const int* __restrict__ lens, int* __restrict__ lens_out, int T_in, int H, int D,
-                                                                              long frames, int first, int blocks, int total) {
+                                                                              long frames, int first, unsigned blocks, unsigned total) {
     __shared__ float red[4];
     constexpr int V = 8;                                          // values a thread and step; D is a multiple of 8
     const Kv8Side& sd = blockIdx.y ? sv : sk;
     const T* x = reinterpret_cast<const T*>(sd.x);
     const long sb = sd.sb, st = sd.st, sh = sd.sh;
-    const int item = blockIdx.x + gridDim.x * blockIdx.z;
-    if (item >= total) return;
+    const unsigned item = min(blockIdx.x + LAUNCH_ROW * blockIdx.z, total - 1);    // (the last row's surplus blocks write the last item's values again)
     const int j = item % blocks, bh = item / blocks, b = bh / H, hh = bh % H;
     const int per = D / V, n = KV_BLOCK * per;                    // <= 1024: four steps
     const int live = lens ? min(max(lens[b], 0), T_in) : T_in;
@@ -406,9 +415,11 @@ extern "C" int SAR_FN(sar_kv8_store)(const void* k, long k_sb, long k_st, long k
         if (!p || (uintptr_t)p % 16) return SAR_EINVAL;
     const int blocks = cdiv(T, KV_BLOCK);
     if ((long)B * H > (1L << 30) / blocks) return SAR_EINVAL;
-    const int total = B * H * blocks, row = total < (1 << 22) ? total : 1 << 22;     // (fewer than 2^32 threads along an axis)
-    hipLaunchKernelGGL((kv8_store_kernel<elt>), dim3((unsigned)row, 2, (unsigned)cdiv(total, row)), dim3(256), 0, stream, Kv8Side{k, k_sb, k_st, k_sh, (unsigned char*)k8, k_scale},
-                       Kv8Side{v, v_sb, v_st, v_sh, (unsigned char*)v8, v_scale}, lens, lens_out, T, H, D, frames, first, blocks, total);
+    const int total = B * H * blocks;
+    const Kv8Side ks = {k, k_sb, k_st, k_sh, (unsigned char*)k8, k_scale}, vs = {v, v_sb, v_st, v_sh, (unsigned char*)v8, v_scale};
+    const int row = total < LAUNCH_ROW ? total : LAUNCH_ROW;
+    hipLaunchKernelGGL((kv8_store_kernel<elt>), dim3((unsigned)row, 2, (unsigned)cdiv(total, row)), dim3(256), 0, stream, ks, vs, lens, lens_out, T, H, D, frames, first, (unsigned)blocks,
+                       (unsigned)total);
     SAR_CHECK_LAUNCH();
     return SAR_OK;
 }

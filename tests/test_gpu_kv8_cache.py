@@ -55,3 +55,17 @@ def test_a_scale_of_zero_makes_nothing_of_large_scores():
     for n in (1, 50):
         out = cross_attention(torch.full((1, n, 1, 16), 2.0 ** 116, device="cuda"), k, v, scale=0.0)
         assert torch.allclose(out.double(), v.double().mean(1, keepdim=True).expand(1, n, 1, 16), rtol=0, atol=80 * 2.0 ** -23)
+
+
+@pytest.mark.parametrize("Tk", [256, 1100])
+def test_blocks_beyond_all_ratios(Tk):
+    """fp16 queries over V blocks of 2^118 and 2^-38, in turn for every wave: columns that only the small blocks reach come out as 0, the others as infinities, none as NaN."""
+    from aesrc2020_amd.attention import EncoderCache8
+    q, k, v, _ = make(1, 3, Tk, 2, 1, 32, torch.float32, seed=Tk)
+    big = (torch.arange(Tk, device="cuda") // 64 % 3 == 0)[None, :, None, None]
+    v = torch.where(big, 2.0 ** 118, 2.0 ** -38) * (1 + v.abs())
+    v[..., 8:] *= ~big
+    c = EncoderCache8(1, Tk, 1, 32)
+    c.store(k, v)
+    out = c.attend(q.half())
+    assert (out[..., 8:] == 0).all() and torch.isposinf(out[..., :8]).all()
