@@ -178,7 +178,8 @@ class EncoderCache8:
     token reads all of them.
 
     k8, v8 (batch, heads, frames rounded up to 64, dim) float8_e4m3fn; k_scale, v_scale (batch, heads, blocks of 64 frames) fp32 powers of two,
-    value = e4m3 * scale; lens (batch,) int32.  The buffers keep their addresses for the cache's life, so a captured step stays valid over store()."""
+    value = e4m3 * scale; lens (batch,) int32.  The buffers keep their addresses for the cache's life, so a captured step stays valid over store().
+    stored: frames that store() has written, in whole blocks, which the next chunk may start at (to be set where the buffers are filled otherwise)."""
 
     BLOCK = 64
 
@@ -193,6 +194,7 @@ class EncoderCache8:
         self.k_scale, self.v_scale = (torch.empty(batch, heads, n, dtype=torch.float32, device=device) for _ in range(2))
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)                         # (nothing behind a length is ever read)
         self.device = self.k8.device
+        self.stored = 0
 
     def store(self, k, v, k_lens=None, first=0):
         """Write frames [first, first + T) of every utterance from k, v (batch, T, heads, dim) (fp32, bf16 or fp16); `first` is a multiple of 64:
@@ -206,9 +208,12 @@ class EncoderCache8:
         first = int(first)
         if first < 0 or first % self.BLOCK or T < 1 or first + T > self.frames:
             raise ValueError("frames [%d, %d) do not fit: first has to be a multiple of %d, the cache has %d frames" % (first, first + T, self.BLOCK, self.frames))
+        if first > self.stored:
+            raise ValueError("frames [%d, %d) were never stored: a chunk starts where the ones before it end" % (self.stored, first))
         kl = _lens("k_lens", k_lens, B, k.device)
         _launch("sar_kv8_store_" + _SFX[k.dtype], k.device, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], kl, self.k8.data_ptr(), self.k_scale.data_ptr(),
                 self.v8.data_ptr(), self.v_scale.data_ptr(), self.lens.data_ptr(), B, T, H, D, self.k8.shape[2], first)
+        self.stored = -(-(first + T) // self.BLOCK) * self.BLOCK
 
     def attend(self, q, q_lens=None, scale=None, out=None):
         """cross_attention(q, held k, held v, k_lens=lens): q (batch, Tq, Hq, dim) of any of the three types, Hq a multiple of the cache's heads

@@ -69,3 +69,36 @@ def test_blocks_beyond_all_ratios(Tk):
     c.store(k, v)
     out = c.attend(q.half())
     assert (out[..., 8:] == 0).all() and torch.isposinf(out[..., :8]).all()
+
+
+def test_chunks_start_where_the_ones_before_end():
+    """A gap would be attended to, whatever lies there: a new cache's memory, or another utterance's frames."""
+    from aesrc2020_amd.attention import EncoderCache8
+    _, k, v, _ = make(2, 1, 320, 2, 2, 16, torch.float32, seed=1)
+    c = EncoderCache8(2, 320, 2, 16)
+    for first in (64, 256):
+        with pytest.raises(ValueError, match="never stored"):
+            c.store(k[:, :64], v[:, :64], first=first)
+    c.store(k[:, :100], v[:, :100]); c.store(k[:, 128:], v[:, 128:], first=128)
+    assert c.lens.tolist() == [320, 320]
+    c.store(k[:, :70], v[:, :70])                                  # the next utterances: what lies behind is the last ones'
+    with pytest.raises(ValueError, match="never stored"):
+        c.store(k[:, 192:], v[:, 192:], first=192)
+    c.store(k[:, 64:128], v[:, 64:128], first=64)                  # a block again, with its later frames
+    assert c.lens.tolist() == [128, 128] and c.stored == 128
+    c.stored = 256                                                 # filled by other means
+    c.store(k[:, 256:], v[:, 256:], first=256)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_chunks_are_one_store(dt):
+    """Appended chunks of whole blocks hold and answer what one store does, in every type."""
+    from aesrc2020_amd.attention import EncoderCache8
+    q, k, v, _ = make(3, 2, 450, 4, 2, 40, DT[dt], seed=7)
+    c, d = EncoderCache8(3, 450, 2, 40), EncoderCache8(3, 450, 2, 40)
+    d.store(k, v, lens(450, 130, 64))
+    c.store(k[:, :64], v[:, :64]); c.store(k[:, 64:192], v[:, 64:192], lens(128, 66, 0), first=64); c.store(k[:, 192:], v[:, 192:], lens(258, 0, 0), first=192)
+    assert c.lens.tolist() == d.lens.tolist() == [450, 130, 64]
+    for a, b in ((c.k8, d.k8), (c.v8, d.v8)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert torch.equal(c.k_scale, d.k_scale) and torch.equal(c.v_scale, d.v_scale) and torch.equal(c.attend(q), d.attend(q))
