@@ -44,3 +44,26 @@ def test_results_go_into_any_contiguous_buffer(Tq):
         assert cache.attend(q, out=out) is out and torch.equal(out, held)
         got = cross_attention_grad(do, q, k, v, out.copy_(want), lse, dq=make(Tq), dk=make(70), dv=make(70))
         assert all(torch.equal(a, b) for a, b in zip(got, grads))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_the_layer_is_the_calls_in_every_type(dt):
+    """CrossAttention over rows of any of the three types, shared key heads, padded on both sides: bit for bit what the functions give."""
+    from aesrc2020_amd.attention import cross_attention, cross_attention_grad
+    from aesrc2020_amd.engine import ParamStore, store_scope
+    from aesrc2020_amd.layers import CrossAttention
+    B, Lq, Lk, H, heads, kv = 3, 20, 50, 96, 6, 2
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q, dy = (torch.randn(B * Lq, H, generator=g, device="cuda").to(dt) for _ in range(2))
+    k, v = (torch.randn(B * Lk, H // heads * kv, generator=g, device="cuda").to(dt) for _ in range(2))
+    kl, ql = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ((50, 0, 33), (20, 7, 0)))
+    with store_scope(ParamStore(seed=0)):
+        layer = CrossAttention(H, heads, kv, name="att")
+    y = layer.forward(q, k, v, B, Lq, Lk, kl, ql)
+    grads = layer.backward(dy)
+    view = lambda t, n: t.view(B, -1, n, H // heads)  # noqa: E731
+    out, lse = cross_attention(view(q, heads), view(k, kv), view(v, kv), kl, ql, return_lse=True)
+    want = cross_attention_grad(view(dy, heads), view(q, heads), view(k, kv), view(v, kv), out, lse, kl, ql)
+    assert y.dtype == dt and torch.equal(y, out.view(B * Lq, H))
+    for a, b in zip(grads, want):
+        assert a.dtype == dt and torch.equal(a, b.view(a.shape)) and (a != 0).any()

@@ -19,3 +19,20 @@ def test_more_tiles_than_one_row_of_a_launch():
     want, bd = reference(x[rows], w, lab[rows], b, dl[rows])
     check(loss[rows], want[0], bd[0], "loss"); check(lse[rows], want[1], bd[1], "lse")
     assert torch.isfinite(lse).all() and (loss[(lab < 0) | (lab >= V)] == 0).all()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("R,D,V", [(4099, 1000, 4001), (4100, 1024, 4032), (8200, 1224, 16100)])
+def test_large_tiles_of_every_product(R, D, V, dt):
+    """128 x 128 tiles for the logits, dx and dkernel alike: with tails along every axis, copied (4001 wide) and read where they lie (4032), in one piece
+    and in several (16100)."""
+    from aesrc2020_amd.losses import vocab_crossentropy, vocab_crossentropy_grad
+    x, w, lab, b, dl = make(R, D, V, DT[dt], seed=R)
+    want, bd = reference(x, w, lab, b, dl)
+    loss, lse = vocab_crossentropy(x, w, lab, b, return_lse=True)
+    check(loss, want[0], bd[0], "loss"); check(lse, want[1], bd[1], "lse")
+    got = vocab_crossentropy_grad(dl, x, w, lab, lse, b)
+    for g, wv, e, n in zip(got, want[2:], bd[2:], ("dx", "dkernel", "dbias")):
+        check(g, wv, e, n)
+    again = vocab_crossentropy_grad(dl, x, w, lab, lse, b)
+    assert all(torch.equal(g, h) for g, h in zip(got, again))
