@@ -69,17 +69,14 @@ __device__ __forceinline__ float max_of(const float* part) {
     const int l = threadIdx.x & 63;
     return wave_max(fmaxf(fmaxf(part[l], part[l + 64]), fmaxf(part[l + 128], part[l + 192])));
 }
-// exponent e with v 2^e in [2^13, 2^14) (0 for v = 0), kept where 2^e and 2^-e are ordinary numbers
-__device__ __forceinline__ int up_exp(float v) {
+// Scales are exponents, applied by ldexp: 2^e itself may leave fp32's range where the product with it does not.
+__device__ __forceinline__ float times2(float v, int e) { return __builtin_amdgcn_ldexpf(v, e); }
+__device__ __forceinline__ int g_exp(float v) {                   // v 2^-e in [1/2, 1) (0 for v = 0)
     int e = 0;
     (void)frexpf(v, &e);
-    return v == 0.f ? 0 : min(max(14 - e, -110), 110);
+    return v == 0.f ? 0 : e;
 }
-__device__ __forceinline__ int g_exp(float v) {                   // v 2^-e in [1/2, 1)
-    int e = 0;
-    (void)frexpf(v, &e);
-    return v == 0.f ? 0 : min(max(e, -110), 110);
-}
+__device__ __forceinline__ int up_exp(float v) { return v == 0.f ? 0 : DZ_BITS - g_exp(v); }      // v 2^e in [2^13, 2^14)
 
 // labels (R) of 4 or 8 bytes; a row whose label lies outside [0, V) is left out
 struct Labels { const void* p; int bytes, V; };
@@ -139,9 +136,9 @@ __global__ __launch_bounds__(1024) void absmax_kernel(MaxJobs jobs, float* __res
 }
 
 // rows of `cols` elements -> rows of `pitch` operand elements, zeros behind (SCALED: planes hi, lo of fp32), for x and W (blockIdx.y).  The scale comes from
-// `part`'s maxima; or, with row_f, every row has its own, whose inverse is left there, and with `all` the rows go there too under the scale of `part`,
+// `part`'s maxima; or, with row_e, every row has its own, whose exponent is left there, and with `all` the rows go there too under the scale of `part`,
 // those without a label as zeros.
-struct PackJob { const elt* x; void* y; long rows, ld, plane; int cols, pitch; const float* part; float* row_f; void* all; };
+struct PackJob { const elt* x; void* y; long rows, ld, plane; int cols, pitch; const float* part; int* row_e; void* all; };
 struct PackJobs { PackJob j[2]; Labels labels; };
 template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_kernel(PackJobs jobs) {
     const PackJob j = jobs.j[blockIdx.y];
@@ -155,13 +152,13 @@ template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_
             for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? p[k] : (elt)0.f;
         }
     };
-    const auto put = [&](void* to, long r, int c, const elt (&v)[8], float f, bool none) {
+    const auto put = [&](void* to, long r, int c, const elt (&v)[8], int e, bool none) {
         constexpr int PER = Num<OP>::PER;
         OP* y = reinterpret_cast<OP*>(to) + r * j.pitch + c;
         typename Num<OP>::x16 hi[8 / PER], lo[8 / PER];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float s = none ? 0.f : SCALED ? (float)v[k] * f : (float)v[k];
+            const float s = none ? 0.f : SCALED ? times2((float)v[k], e) : (float)v[k];
             hi[k / PER][k % PER] = (OP)s;
             if constexpr (SCALED && NPL == 2) lo[k / PER][k % PER] = (OP)(s - (float)hi[k / PER][k % PER]);
         }
@@ -171,9 +168,9 @@ template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_
             if constexpr (SCALED && NPL == 2) *reinterpret_cast<typename Num<OP>::x16*>(y + j.plane + q * PER) = lo[q];
         }
     };
-    const float f = SCALED && j.part ? ldexpf(1.f, up_exp(max_of(j.part))) : 1.f;
+    const int all = SCALED && j.part ? up_exp(max_of(j.part)) : 0;
     elt v[8];
-    if (SCALED && j.row_f) {                                      // a wave per row, which it reads twice if it is wider than 512
+    if (SCALED && j.row_e) {                                      // a wave per row, which it reads twice if it is wider than 512
         const int lane = threadIdx.x & 63;
         for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < j.rows; r += (long)gridDim.x * 4) {
             float m = 0.f;
@@ -184,11 +181,11 @@ template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_
                 for (int k = 0; k < 8; ++k) { const float a = fabsf((float)v[k]); if (a < INFINITY) m = fmaxf(m, a); }
             }
             const int e = up_exp(wave_max(m));
-            if (lane == 0) j.row_f[r] = ldexpf(1.f, -e);
+            if (lane == 0) j.row_e[r] = e;
             for (int c = lane * 8; c < j.pitch; c += 512) {
                 if (j.pitch > 512) fetch(r, c, v);
-                put(j.y, r, c, v, ldexpf(1.f, e), false);
-                if (j.all) put(j.all, r, c, v, f, !in);
+                put(j.y, r, c, v, e, false);
+                if (j.all) put(j.all, r, c, v, all, !in);
             }
         }
         return;
@@ -200,7 +197,7 @@ template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_
         const int c = ((int)(i - r * across) * 256 + threadIdx.x) * 8;
         if (c >= j.pitch) continue;
         fetch(r, c, v);
-        put(j.y, r, c, v, f, false);
+        put(j.y, r, c, v, all, false);
     }
 }
 
@@ -252,7 +249,7 @@ constexpr int G_FEW = 1024;
 enum { E_LSE, E_DZ, E_GRAD };
 struct Epi {
     const float* parts;                          // maxima: PART_X, PART_W, PART_G
-    const float* row_f;                          // the inverses of x's scales, a row each
+    const int* row_e;                            // exponents of x's scales, a row each
     const elt* bias;
     Labels labels;
     const float *dloss, *lse;
@@ -379,13 +376,16 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
     const int mw = wm * MT * 32, nw = wn * NT * 32;               // the wave's corner of the tile
     // logits in powers of two: y = (acc f + b) log2 e, entries behind the vocabulary -inf
     const auto logits = [&](int v0) {
-        float f[NT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) f[j] = LOG2E;
         if constexpr (SCALED) {
-            const float fw = LOG2E * ldexpf(1.f, -up_exp(max_of(e.parts + PART_W * PARTS)));
+            const int w_exp = up_exp(max_of(e.parts + PART_W * PARTS));
 #pragma unroll
-            for (int j = 0; j < NT; ++j) f[j] = fw * e.row_f[min(n0 + nw + 32 * j + (lane & 31), e.R_all - 1)];
+            for (int j = 0; j < NT; ++j) {
+                const int down = -w_exp - e.row_e[min(n0 + nw + 32 * j + (lane & 31), e.R_all - 1)];
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) acc[i][j][x] = times2(acc[i][j][x], down);
+            }
         }
         const int first = v0 + m0 + mw + 4 * h;
         if (v0 + m0 + BM <= e.V) {
@@ -400,7 +400,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) acc[i][j][4 * a + x] = fmaf(acc[i][j][4 * a + x], f[j], b[x]);
+                        for (int x = 0; x < 4; ++x) acc[i][j][4 * a + x] = fmaf(acc[i][j][4 * a + x], LOG2E, b[x]);
                 }
         } else {
 #pragma unroll
@@ -410,7 +410,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
                     const int v = first + 32 * i + 8 * (x >> 2) + (x & 3);
                     const float b = e.bias && v < e.V ? (float)e.bias[v] * LOG2E : 0.f;
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j][x] = v < e.V ? fmaf(acc[i][j][x], f[j], b) : -INFINITY;
+                    for (int j = 0; j < NT; ++j) acc[i][j][x] = v < e.V ? fmaf(acc[i][j][x], LOG2E, b) : -INFINITY;
                 }
         }
     };
@@ -469,7 +469,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
             } else if (r < e.R) finish_row(e.loss, e.lse_out, r, M, L, fmaxf(own[j], join[2 * BN + nw + 32 * j + lane]), label_of(e.labels, r), e.V);
         }
     } else if constexpr (EPI == E_DZ) {                           // m: vocabulary entries from v0 on, n: rows of x
-        const float gs = ldexpf(1.f, dz_exp(e));
+        const int up = dz_exp(e);
         logits(e.v0);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -477,7 +477,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
             const long lab = r < e.R ? label_of(e.labels, r) : -1;
             const bool has = lab >= 0 && lab < e.V;
             // a row that is left out: p = exp2(-inf) = 0 and g = 0
-            const float g = has ? e.dloss[r] * gs : 0.f, lse = has ? e.lse[r] * LOG2E : INFINITY;
+            const float g = has ? times2(e.dloss[r], up) : 0.f, lse = has ? e.lse[r] * LOG2E : INFINITY;
             // (lse is rounded: where it is large an exponent can come out above 0, which no probability's is; a NaN stays one)
             if (__any(has && fabsf(lse) > 1048576.f))
 #pragma unroll
@@ -535,7 +535,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
                 float v = 0.f;
 #pragma unroll
                 for (int k = 0; k < 256 / CH; ++k) v += red[k * BM + threadIdx.x];
-                v *= 1.f / gs;
+                v = times2(v, -up);
                 const int c = m0 + threadIdx.x;
                 if (!e.db_out) e.db[(long)nt * e.dz_ld + c] = v;
                 else if (e.v0 + c < e.V) e.db_out[c] = (elt)(e.db_accumulate ? (float)e.db_out[c] + v : v);
@@ -544,7 +544,6 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
     } else {
         int ex = -dz_exp(e);
         if constexpr (SCALED) ex -= up_exp(max_of(e.parts + (e.with_w ? PART_W : PART_X) * PARTS));
-        const float f = ldexpf(1.f, ex);
         // every row and column that exists (R, V)
         const auto each = [&](auto&& put) {
 #pragma unroll
@@ -556,7 +555,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
                         const int m = m0 + mw + 32 * i + 8 * (x >> 2) + 4 * h + (x & 3);
-                        if (m < e.R) put(m * e.ldo + n, acc[i][j][x] * f);
+                        if (m < e.R) put(m * e.ldo + n, times2(acc[i][j][x], ex));
                     }
             }
         };
@@ -717,8 +716,10 @@ static Plan plan(const sarVocabCe* a, bool grad) {
 }
 
 // contraction elements per LDS stage: 64, two stages (whole 128-byte lines where an operand is read along the contraction; half the barriers) -- an 8192 x
-// 8192 piece against 1024, us with 64 / with 32: dx 147 / 183, dW 128 / 143, dz 158 / 160, the logits of 8192 x 32000 525 / 548.  fp32 (two planes): 32.
-// Logits of a shorter contraction on 128 x 128 tiles: 32 with three stages, whose blocks start and end beside two others (777 x 512 x 40001: 57 / 53).
+// 8192 piece against 1024, us with 64 / with 32: dx 147 / 183, dW 128 / 143, dz 158 / 160.  fp32 (two planes): 32.
+// Logits of a shorter contraction on 128 x 128 tiles: 32 with three stages, whose blocks start and end beside two others.  bf16, us with 64 / with 32, D =
+// 256, 512, 768, 1024, 2048 (fp16 within 1 % of the same ratios): 777 x 40000 41 / 37, 56 / 53, 71 / 70, 88 / 86, 150 / 157; 4096 x 16000 64 / 56, 93 / 85,
+// 119 / 116, 148 / 149, 258 / 284; 8192 x 32000 220 / 188, 320 / 301, 425 / 425, 532 / 553, 986 / 1081.
 constexpr int step_of(bool planes = NPL == 2) { return planes ? 32 : 64; }
 static int logits_step(const sarVocabCe* a, bool small_tiles) { return small_tiles || a->D > 768 ? step_of() : 32; }
 static unsigned some_blocks(long n) { return (unsigned)(n < 1 ? 1 : n < 4096 ? n : 4096); }
@@ -737,13 +738,13 @@ template <typename OP, bool SCALED> static Operands operands(const sarVocabCe* a
     PackJobs jobs = {{}, max.labels};
     n = 0;
     long blocks = 0;
-    const auto pack = [&](Side& s, size_t to, int rows, int cols, int pitch, const float* part, float* row_f, void* all) {
-        jobs.j[n++] = {reinterpret_cast<const elt*>(s.p), ws + to, rows, s.ld, (long)rows * pitch, cols, pitch, part, row_f, all};
+    const auto pack = [&](Side& s, size_t to, int rows, int cols, int pitch, const float* part, int* row_e, void* all) {
+        jobs.j[n++] = {reinterpret_cast<const elt*>(s.p), ws + to, rows, s.ld, (long)rows * pitch, cols, pitch, part, row_e, all};
         s = {ws + to, (long)rows * pitch, pitch, 0, 0};
-        const long b = row_f ? cdiv(rows, 4) : (long)rows * cdiv(pitch, 2048);
+        const long b = row_e ? cdiv(rows, 4) : (long)rows * cdiv(pitch, 2048);
         blocks = b > blocks ? b : blocks;
     };
-    if (p.pack_x) pack(o.x, p.xo, a->R, a->D, p.Dp, p.own_x ? parts + PART_X * PARTS : nullptr, SCALED ? reinterpret_cast<float*>(ws + p.rows) : nullptr, p.own_x ? ws + p.xg : nullptr);
+    if (p.pack_x) pack(o.x, p.xo, a->R, a->D, p.Dp, p.own_x ? parts + PART_X * PARTS : nullptr, SCALED ? reinterpret_cast<int*>(ws + p.rows) : nullptr, p.own_x ? ws + p.xg : nullptr);
     if (p.pack_w) pack(o.w, p.wo, a->D, a->V, p.Vp, SCALED ? parts + PART_W * PARTS : nullptr, nullptr, nullptr);
     if (n) hipLaunchKernelGGL((pack_kernel<OP, SCALED>), dim3(some_blocks(blocks), n), dim3(256), 0, st, jobs);
     o.xg = o.x;
@@ -783,7 +784,7 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     w.len = p.pack_w ? p.Vp : a->V; w.k = a->D;
     x.len = a->R; x.k = p.pack_x ? p.Dp : a->D;
     Epi e = {};
-    e.parts = reinterpret_cast<float*>(ws + p.parts); e.row_f = reinterpret_cast<float*>(ws + p.rows); e.R_all = a->R;
+    e.parts = reinterpret_cast<float*>(ws + p.parts); e.row_e = reinterpret_cast<int*>(ws + p.rows); e.R_all = a->R;
     e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = {a->labels, a->label_bytes, a->V};
     e.pm = reinterpret_cast<float*>(ws + p.a); e.pl = reinterpret_cast<float*>(ws + p.b); e.zl = reinterpret_cast<float*>(ws + p.zl);
     e.R = a->R; e.V = a->V; e.Rp = p.Rp;
@@ -811,7 +812,7 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         const int v0 = i * p.piece, cols = a->V - v0 < p.piece ? a->V - v0 : p.piece, ld = up64(cols);
         const long plane = (long)p.Rp * ld;
         Epi e = {};
-        e.parts = reinterpret_cast<float*>(ws + p.parts); e.row_f = reinterpret_cast<float*>(ws + p.rows);
+        e.parts = reinterpret_cast<float*>(ws + p.parts); e.row_e = reinterpret_cast<int*>(ws + p.rows);
         e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = {a->labels, a->label_bytes, a->V}; e.dloss = a->dloss; e.lse = a->lse;
         e.dz = dz; e.dz_plane = plane; e.dz_ld = ld;
         if (a->dbias && p.db_slices > 1) e.db = reinterpret_cast<float*>(ws + p.dbp);

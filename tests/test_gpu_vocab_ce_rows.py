@@ -78,3 +78,40 @@ def test_rows_of_many_sizes(R, D, V, dt):
         want, bd = reference(x[s], w, lab[s], b, dl[s])
         check(got[0][s], want[0], bd[0], "loss"); check(got[1][s], want[1], bd[1], "lse")
         check(got[2][s], want[2], bd[2] + 2.0 ** -38 * dl.abs().max().item() * w.double().abs().sum(1), "dx")
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("R,D,V", SIZES)
+def test_powers_of_two_at_the_ends_of_the_range(R, D, V, dt):
+    """x up to the type's largest numbers beside a kernel near its smallest, and the other way: the logits are the same, and so are loss and lse, bit for bit;
+    the gradient that grows is the same times the power, where it stays within the type.  (The one that shrinks sums numbers below 2^-126.  What is below 2^-14 is left out of the inputs: times 2^-110 the rest
+    are normal numbers, with all their bits.)"""
+    x, w, lab, b, dl = make(R, D, V, DT[dt], seed=R)
+    x, w = (torch.where(t.abs() < 2.0 ** -14, torch.zeros_like(t), t) for t in (x, w))
+    base = run(dl, x, w, lab, b)
+    for e in (110, -110):
+        got = run(dl, (x.float() * 2.0 ** e).to(x.dtype), (w.float() * 2.0 ** -e).to(w.dtype), lab, b)
+        assert torch.equal(got[0], base[0]) and torch.equal(got[1], base[1]), e
+        y, z = (g[3 if e > 0 else 2].double() for g in (base, got))
+        y *= 2.0 ** 110
+        fits = y.abs() < 2.0 ** 127
+        assert fits.any() and torch.equal(z[fits], y[fits]) and torch.isfinite(got[2]).all() and (e > 0 or torch.isfinite(got[3]).all()), e
+    assert torch.equal(got[4], base[4]) if b is not None else True
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("R,D,V", SIZES)
+def test_no_row_has_a_label(R, D, V, dt):
+    x, w, lab, b, dl = make(R, D, V, DT[dt], seed=R)
+    got = run(dl, x, w, torch.full_like(lab, V + 3), b)
+    assert (got[0] == 0).all() and torch.equal(got[1], run(dl, x, w, lab, b)[1]) and all((g == 0).all() for g in got[2:] if g is not None)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("R,D,V", SIZES[1:3])
+def test_left_out_rows_at_the_end_of_the_range(R, D, V, dt):
+    x, w, lab, b, dl = make(R, D, V, DT[dt], seed=R)
+    out = (lab < 0) | (lab >= V)
+    want = run(dl, torch.where(out[:, None], torch.zeros_like(x), x), w, lab, b)
+    got = run(dl, torch.where(out[:, None], torch.full_like(x, torch.finfo(x.dtype).max) * torch.sign(x), x), w, lab, b)
+    assert all(torch.equal(g, w_) for i, (g, w_) in enumerate(zip(got, want)) if i != 1)
