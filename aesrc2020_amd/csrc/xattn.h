@@ -58,6 +58,13 @@ __device__ __forceinline__ float backward_exponent(float lse, float up = 0.f) {
     return e == -INFINITY ? 0.f : a > 4194304.f ? fmaf(a, 2.384185791015625e-7f, r) : r;
 }
 
+// The forward's running reference m of a row's exponents follows the maximum `top` only where that is more than LAG ahead (a row starts with its first
+// maximum): most tiles skip the rescaling.  p = 2^(s f - m) is 2^LAG at most, which loses nothing in bf16 and fp32.  fp16 is used in full: m stays BELOW
+// the maximum, so that p reaches up to 2^15 and is a normal number down to 2^-26 .. 2^-29 of the largest (a key that takes nearly all of the weight, and
+// whose v is 0, leaves the result to the others).  (top - m, not m + LAG: the sum rounds by whole units past 2^24.)
+template <typename C> constexpr float lag() { return __is_same(C, _Float16) ? 15.f : 8.f; }
+template <typename C> __device__ __forceinline__ float reference(float top) { return __is_same(C, _Float16) && fabsf(top) < LARGE ? top - 12.f : top; }
+
 struct Row { int t, h; };
 __device__ __forceinline__ Row row_of(const sarXattn& a, int hkv, int r) {
     const int G = a.Hq / a.Hkv, t = r / G;

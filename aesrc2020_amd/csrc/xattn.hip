@@ -189,10 +189,8 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
         top = half_max(top) * sl;
-        // the maximum follows only where it grew by more than 2^8: below that p <= 2^8 loses nothing in any of the types, and most
-        // tiles skip the rescaling
-        if (__any(top > m + 8.f)) {
-            const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
+        if (__any(top - m > lag<T>())) {
+            const float mn = fmaxf(m, reference<T>(top)), f = __builtin_amdgcn_exp2f(m - mn);
             m = mn; l *= f;
             large = __any(fabsf(m) > LARGE && m != NO_MAX);
 #pragma unroll

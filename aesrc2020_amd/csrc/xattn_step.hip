@@ -179,8 +179,8 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
         top = half_max(top) * f;
-        if (__any(top > m + 8.f) || (UNITS && nu != unit)) {
-            const float mn = fmaxf(m, top), e = __builtin_amdgcn_exp2f(m - mn), eo = UNITS ? fminf(e * unit / nu, MOST) : e;     // (in this order: no power of two passes the range before e has taken it back)
+        if (__any(top - m > lag<C>()) || (UNITS && nu != unit)) {
+            const float mn = fmaxf(m, reference<C>(top)), e = __builtin_amdgcn_exp2f(m - mn), eo = UNITS ? fminf(e * unit / nu, MOST) : e;     // (in this order: no power of two passes the range before e has taken it back)
             const bool beyond = UNITS && unit > nu * 1.2089258196146292e24f;     // by 2^80: sums other than 0 are past fp16's range, and stay finite here
             m = mn; l *= e;
             large = __any(fabsf(m) > LARGE && m != NO_MAX);
