@@ -12,10 +12,11 @@
 // fp32 operands are two fp16 planes under a power of two that puts the largest element in [2^13, 2^14): hi + lo hold 22 bits of elements down to 2^-16
 // of that one (below, 2^-38 of it), hi hi + hi lo + lo hi is the product to 2^-22 or so of |a| |b|, at a third of the fp16 rate (the fp32 matrix
 // instructions run at a sixteenth).  For the logits every row of x has its own scale, so that no row reaches another's results; W has one.
-// dz is held in fp16: scaled by the power of two that puts the largest |g| in [1/2, 1), times 2^14, every probability down to 2^-28 is a normal number
-// with 11 bits; for bf16 the backward therefore takes x and W in fp16 too (their 8 bits are exact down to 2^-31 of the largest), which leaves the
-// gradients the accuracy of their own rounding.  dW = x^T dz sums over the rows, so there x is packed a second time, under one scale, of the rows
-// with a label: an element of dW is good to 2^-38 of the largest |x| among them.
+// dz is held in fp16, times 2^14 and a power of two that puts |g| into [1/2, 1): every probability down to 2^-28 is a normal number with 11 bits.  For bf16
+// the backward therefore takes x and W in fp16 too (their 8 bits are exact down to 2^-31 of the largest), which leaves the gradients the accuracy of
+// their own rounding.  Where operands are packed (fp32, bf16) that power is each row's own, which dx takes back by row.  dW = x^T dz sums over the rows, so
+// there x is packed a second time, times the rows' powers, under one scale; rows without a label are zeros.  An element of dW is good to 2^-38 of the
+// largest |x g|.  fp16 x lies where it is, and g's power is one for all rows with a label.
 // Compiled once per element type: SAR_ELT 0 = fp32, 1 = bf16, 2 = fp16.
 #include "attn_tiles.h"
 
@@ -88,9 +89,9 @@ __device__ __forceinline__ bool counts(const Labels& l, long r) {
     return v >= 0 && v < l.V;
 }
 
-enum { MAX_ALL, MAX_ROWS, MAX_G };       // of a whole tensor, of its rows with a label, of dloss
+enum { MAX_ALL, MAX_ROWS, MAX_G };       // of a whole tensor, of its rows with a label times their g's powers of two, of dloss
 struct MaxJob { const void* x; long rows, ld; int cols, kind, part; };
-struct MaxJobs { MaxJob j[3]; Labels labels; };
+struct MaxJobs { MaxJob j[3]; Labels labels; const float* dloss; };
 // partial maxima of the finite |values| of up to three tensors (blockIdx.y): PARTS places each.  What a row that is left out holds must not decide how
 // finely the others' x and dz are held.
 __global__ __launch_bounds__(1024) void absmax_kernel(MaxJobs jobs, float* __restrict__ part) {
@@ -125,7 +126,14 @@ __global__ __launch_bounds__(1024) void absmax_kernel(MaxJobs jobs, float* __res
             if (counts(jobs.labels, c)) see(reinterpret_cast<const float*>(j.x)[c]);
     } else if (j.kind == MAX_ROWS) {                              // a wave per row
         for (long r = blockIdx.x * 16 + (threadIdx.x >> 6); r < j.rows; r += PARTS * 16)
-            if (counts(jobs.labels, r)) row(x + r * j.ld, j.cols, wide, threadIdx.x & 63, 64);
+            if (counts(jobs.labels, r)) {
+                const float before = m;
+                m = 0.f;
+                row(x + r * j.ld, j.cols, wide, threadIdx.x & 63, 64);
+                const float here = times2(m, g_exp(jobs.dloss[r]));
+                m = before;
+                see(here);
+            }
     } else if (j.ld == j.cols) {                                  // no gaps: as one row
         row(x, j.rows * j.cols, aligned && j.rows * j.cols % V == 0, (long)blockIdx.x * 1024 + threadIdx.x, PARTS * 1024);
     } else {
@@ -136,10 +144,12 @@ __global__ __launch_bounds__(1024) void absmax_kernel(MaxJobs jobs, float* __res
 }
 
 // rows of `cols` elements -> rows of `pitch` operand elements, zeros behind (SCALED: planes hi, lo of fp32), for x and W (blockIdx.y).  The scale comes from
-// `part`'s maxima; or, with row_e, every row has its own, whose exponent is left there, and with `all` the rows go there too under the scale of `part`,
-// those without a label as zeros.
+// `part`'s maxima; or, with row_e, every row has its own, whose exponent is left there (row_e[r]; g's in row_e[row_places(rows) + r] if there is a dloss), and with `all`
+// the rows go there too, times g's power and under the scale of `part`, those without a label as zeros.
+// exponents of rows: so many places, that a tile's rows have one each (what those behind the last row hold meets zeros only)
+__device__ __host__ __forceinline__ int row_places(int rows) { return (rows + 63) / 64 * 64 + 64; }
 struct PackJob { const elt* x; void* y; long rows, ld, plane; int cols, pitch; const float* part; int* row_e; void* all; };
-struct PackJobs { PackJob j[2]; Labels labels; };
+struct PackJobs { PackJob j[2]; Labels labels; const float* dloss; };
 template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_kernel(PackJobs jobs) {
     const PackJob j = jobs.j[blockIdx.y];
     const auto fetch = [&](long r, int c, elt (&v)[8]) {
@@ -174,18 +184,22 @@ template <typename OP, bool SCALED> __global__ __launch_bounds__(256) void pack_
         const int lane = threadIdx.x & 63;
         for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < j.rows; r += (long)gridDim.x * 4) {
             float m = 0.f;
-            const bool in = j.all && counts(jobs.labels, r);
+            const bool in = jobs.dloss && counts(jobs.labels, r);
+            const int eg = in ? g_exp(jobs.dloss[r]) : 0;
             for (int c = lane * 8; c < j.pitch; c += 512) {
                 fetch(r, c, v);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) { const float a = fabsf((float)v[k]); if (a < INFINITY) m = fmaxf(m, a); }
             }
             const int e = up_exp(wave_max(m));
-            if (lane == 0) j.row_e[r] = e;
+            if (lane == 0) {
+                j.row_e[r] = e;
+                if (jobs.dloss) j.row_e[row_places((int)j.rows) + r] = eg;
+            }
             for (int c = lane * 8; c < j.pitch; c += 512) {
                 if (j.pitch > 512) fetch(r, c, v);
                 put(j.y, r, c, v, e, false);
-                if (j.all) put(j.all, r, c, v, all, !in);
+                if (j.all) put(j.all, r, c, v, all + eg, !in);
             }
         }
         return;
@@ -242,14 +256,15 @@ template <typename OP, int BK, int ROWS, bool DOWN, bool TAIL> struct Operand {
     }
 };
 
-// where the scale of dz comes from: bf16 planes need none; few rows are looked through by every wave, more by a launch of their own
-enum { G_ONE, G_ROWS, G_PARTS };
+// where the scale of dz comes from: bf16 planes and fp32 need none; packed rows have their own; a few fp16 rows are looked through by every wave, more by a
+// launch of their own
+enum { G_ONE, G_EACH, G_ROWS, G_PARTS };
 constexpr int G_FEW = 1024;
 // what happens to a finished tile: C (m, n), column n = lane % 32 of a 32 x 32 tile
 enum { E_LSE, E_DZ, E_GRAD };
 struct Epi {
     const float* parts;                          // maxima: PART_X, PART_W, PART_G
-    const int* row_e;                            // exponents of x's scales, a row each
+    const int *row_e, *g_e;                      // packed operands: exponents of x's scales, and of dloss, a row each
     const elt* bias;
     Labels labels;
     const float *dloss, *lse;
@@ -268,7 +283,8 @@ __device__ __forceinline__ void finish_row(float* loss, float* lse, int r, float
     if (lse) lse[r] = (m + __builtin_amdgcn_logf(l)) * LN2;
     if (loss) loss[r] = lab >= 0 && lab < V ? (m - own + __builtin_amdgcn_logf(l)) * LN2 : 0.f;
 }
-__device__ __forceinline__ int dz_exp(const Epi& e) {             // dz is held times 2^this
+__device__ __forceinline__ int dz_exp(const Epi& e, int r) { return DZ_BITS - e.g_e[r]; }      // G_EACH: dz is held times 2^this
+__device__ __forceinline__ int dz_exp(const Epi& e) {             // the others'
     if (e.g_from == G_ONE) return 0;                              // (a bf16 has an fp32's range)
     if (e.g_from == G_PARTS) return DZ_BITS - g_exp(max_of(e.parts + PART_G * PARTS));
     float m = 0.f;
@@ -380,7 +396,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
             const int w_exp = up_exp(max_of(e.parts + PART_W * PARTS));
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int down = -w_exp - e.row_e[min(n0 + nw + 32 * j + (lane & 31), e.R_all - 1)];
+                const int down = -w_exp - e.row_e[n0 + nw + 32 * j + (lane & 31)];
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -469,7 +485,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
             } else if (r < e.R) finish_row(e.loss, e.lse_out, r, M, L, fmaxf(own[j], join[2 * BN + nw + 32 * j + lane]), label_of(e.labels, r), e.V);
         }
     } else if constexpr (EPI == E_DZ) {                           // m: vocabulary entries from v0 on, n: rows of x
-        const int up = dz_exp(e);
+        const int up = SCALED ? 0 : dz_exp(e);
         logits(e.v0);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -477,7 +493,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
             const long lab = r < e.R ? label_of(e.labels, r) : -1;
             const bool has = lab >= 0 && lab < e.V;
             // a row that is left out: p = exp2(-inf) = 0 and g = 0
-            const float g = has ? times2(e.dloss[r], up) : 0.f, lse = has ? e.lse[r] * LOG2E : INFINITY;
+            const float g = has ? times2(e.dloss[r], SCALED ? dz_exp(e, r) : up) : 0.f, lse = has ? e.lse[r] * LOG2E : INFINITY;
             // (lse is rounded: where it is large an exponent can come out above 0, which no probability's is; a NaN stays one)
             if (__any(has && fabsf(lse) > 1048576.f))
 #pragma unroll
@@ -497,6 +513,9 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
         float sum[PER];
 #pragma unroll
         for (int k = 0; k < PER; ++k) sum[k] = 0.f;
+        int down[REP];
+#pragma unroll
+        for (int t = 0; t < REP; ++t) down[t] = SCALED && (e.db || e.db_out) ? -dz_exp(e, n0 + (threadIdx.x + 256 * t) / CH) : 0;
 #pragma unroll
         for (int p = 0; p < PZ; ++p) {
             __syncthreads();
@@ -522,7 +541,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
                 const auto q = *reinterpret_cast<const typename Num<OP>::x16*>(lds + chunk_at<BM * E>(row, ch));
                 if (r < e.Rp && c < e.dz_ld) *reinterpret_cast<typename Num<OP>::x16*>(reinterpret_cast<OP*>(e.dz) + p * e.dz_plane + (long)r * e.dz_ld + c) = q;
 #pragma unroll
-                for (int k = 0; k < PER; ++k) sum[k] += (float)q[k];
+                for (int k = 0; k < PER; ++k) sum[k] += SCALED ? times2((float)q[k], down[t]) : (float)q[k];
             }
         }
         if (e.db || e.db_out) {
@@ -535,15 +554,28 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
                 float v = 0.f;
 #pragma unroll
                 for (int k = 0; k < 256 / CH; ++k) v += red[k * BM + threadIdx.x];
-                v = times2(v, -up);
+                if constexpr (!SCALED) v = times2(v, -up);
                 const int c = m0 + threadIdx.x;
                 if (!e.db_out) e.db[(long)nt * e.dz_ld + c] = v;
                 else if (e.v0 + c < e.V) e.db_out[c] = (elt)(e.db_accumulate ? (float)e.db_out[c] + v : v);
             }
         }
     } else {
-        int ex = -dz_exp(e);
-        if constexpr (SCALED) ex -= up_exp(max_of(e.parts + (e.with_w ? PART_W : PART_X) * PARTS));
+        // (packed: dz's powers are the row's for dx, and in x for dW)
+        const int ex = SCALED ? -DZ_BITS - up_exp(max_of(e.parts + (e.with_w ? PART_W : PART_X) * PARTS)) : -dz_exp(e);
+        int down[MT][16];
+        if constexpr (SCALED) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    typedef __attribute__((ext_vector_type(4))) int i32x4;
+                    i32x4 g = {0, 0, 0, 0};
+                    if (e.with_w) g = *reinterpret_cast<const i32x4*>(e.g_e + m0 + mw + 32 * i + 8 * a + 4 * h);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) down[i][4 * a + c] = ex + g[c];
+                }
+        }
         // every row and column that exists (R, V)
         const auto each = [&](auto&& put) {
 #pragma unroll
@@ -555,7 +587,7 @@ __device__ __forceinline__ void Product<OP, BK, MT, NT, AD, BD, EPI, SCALED, PA,
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
                         const int m = m0 + mw + 32 * i + 8 * (x >> 2) + 4 * h + (x & 3);
-                        if (m < e.R) put(m * e.ldo + n, times2(acc[i][j][x], ex));
+                        if (m < e.R) put(m * e.ldo + n, times2(acc[i][j][x], SCALED ? down[i][x] : ex));
                     }
             }
         };
@@ -686,7 +718,7 @@ static Plan plan(const sarVocabCe* a, bool grad) {
         p.dx_parts = p.dx_slices > 1 || p.pieces > 1;
         p.light |= SAR_ELT == 1 && p.small_z && p.small_dx && p.small_dw;
         p.dz_planes = p.light ? 2 : NPL;
-        p.g_from = p.light ? G_ONE : BWD_SCALED || a->R > G_FEW ? G_PARTS : G_ROWS;
+        p.g_from = p.light ? G_ONE : BWD_SCALED ? G_EACH : a->R > G_FEW ? G_PARTS : G_ROWS;
         p.own_x = !p.light && BWD_SCALED && a->dkernel;
     }
     // operands are read where they lie when they have the products' type, their rows start on 4-byte boundaries (what a load into LDS needs) and
@@ -698,7 +730,7 @@ static Plan plan(const sarVocabCe* a, bool grad) {
     size_t at = 0;
     const auto take = [&](size_t n) { const size_t o = at; at += up(n); return o; };
     p.parts = take(3 * PARTS * 4);
-    if (scaled) p.rows = take((size_t)a->R * 4);
+    if (scaled) p.rows = take((size_t)row_places(a->R) * (grad ? 8 : 4));
     if (p.own_x) p.xg = take((size_t)a->R * p.Dp * 2 * NPL);
     if (p.pack_x) p.xo = take((size_t)a->R * p.Dp * 2 * NPL);
     if (p.pack_w) p.wo = take((size_t)a->D * p.Vp * 2 * NPL);
@@ -728,14 +760,15 @@ struct Operands { Side x, w, xg; };
 template <typename OP, bool SCALED> static Operands operands(const sarVocabCe* a, const Plan& p, bool grad, hipStream_t st) {
     char* ws = reinterpret_cast<char*>(a->ws);
     float* parts = reinterpret_cast<float*>(ws + p.parts);
-    MaxJobs max = {{}, {a->labels, a->label_bytes, a->V}};
+    const float* dloss = grad ? a->dloss : nullptr;
+    MaxJobs max = {{}, {a->labels, a->label_bytes, a->V}, dloss};
     int n = 0;
     if (p.own_x) max.j[n++] = {a->x, a->R, a->ldx, a->D, MAX_ROWS, PART_X};
     if (SCALED) max.j[n++] = {a->kernel, a->D, a->ldk, a->V, MAX_ALL, PART_W};
     if (grad && p.g_from == G_PARTS) max.j[n++] = {a->dloss, 1, a->R, a->R, MAX_G, PART_G};
     if (n) hipLaunchKernelGGL(absmax_kernel, dim3(PARTS, n), dim3(1024), 0, st, max, parts);
     Operands o = {{a->x, 0, a->ldx, 0, 0}, {a->kernel, 0, a->ldk, 0, 0}, {}};
-    PackJobs jobs = {{}, max.labels};
+    PackJobs jobs = {{}, max.labels, dloss};
     n = 0;
     long blocks = 0;
     const auto pack = [&](Side& s, size_t to, int rows, int cols, int pitch, const float* part, int* row_e, void* all) {
@@ -784,7 +817,7 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
     w.len = p.pack_w ? p.Vp : a->V; w.k = a->D;
     x.len = a->R; x.k = p.pack_x ? p.Dp : a->D;
     Epi e = {};
-    e.parts = reinterpret_cast<float*>(ws + p.parts); e.row_e = reinterpret_cast<int*>(ws + p.rows); e.R_all = a->R;
+    e.parts = reinterpret_cast<float*>(ws + p.parts); e.row_e = reinterpret_cast<int*>(ws + p.rows);
     e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = {a->labels, a->label_bytes, a->V};
     e.pm = reinterpret_cast<float*>(ws + p.a); e.pl = reinterpret_cast<float*>(ws + p.b); e.zl = reinterpret_cast<float*>(ws + p.zl);
     e.R = a->R; e.V = a->V; e.Rp = p.Rp;
@@ -812,7 +845,7 @@ extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
         const int v0 = i * p.piece, cols = a->V - v0 < p.piece ? a->V - v0 : p.piece, ld = up64(cols);
         const long plane = (long)p.Rp * ld;
         Epi e = {};
-        e.parts = reinterpret_cast<float*>(ws + p.parts); e.row_e = reinterpret_cast<int*>(ws + p.rows);
+        e.parts = reinterpret_cast<float*>(ws + p.parts); e.row_e = reinterpret_cast<int*>(ws + p.rows); e.g_e = e.row_e + row_places(a->R);
         e.bias = reinterpret_cast<const elt*>(a->bias); e.labels = {a->labels, a->label_bytes, a->V}; e.dloss = a->dloss; e.lse = a->lse;
         e.dz = dz; e.dz_plane = plane; e.dz_ld = ld;
         if (a->dbias && p.db_slices > 1) e.db = reinterpret_cast<float*>(ws + p.dbp);

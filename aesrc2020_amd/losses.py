@@ -218,9 +218,9 @@ def vocab_crossentropy(x, kernel, labels, bias=None, return_lse=False, loss=None
 def vocab_crossentropy_grad(dloss, x, kernel, labels, lse, bias=None, dx=None, dkernel=None, dbias=None, accumulate=False, need_dx=True):
     """Gradients of vocab_crossentropy: dloss (R) fp32 -> (dx, dkernel, dbias | None) of the inputs' type, each element rounded once from an fp32
     sum.  accumulate (fp32 only): add to the `dkernel`, `dbias` given, as parameter gradients of this package are.  need_dx=False: dx is None.
-    softmax - onehot is held in 16 bits (fp32: about twice that) relative to the largest |dloss| of a row with a label, so such rows of very different
-    dloss (2^20 and more) belong in different calls.  x has to be finite in rows that are left out too.  A row's
-    dx does not depend on other rows; dkernel, their sum, is good to 2^-38 of the largest |x| of a row with a label (fp32 and bf16, larger calls).
+    softmax - onehot is held in 16 bits (fp32: about twice that).  A row's dx does not depend on other rows, but for fp16, where those bits are relative
+    to the largest |dloss| of a row with a label: such rows of very different dloss (2^20 and more) belong in different calls.  dkernel, the rows' sum, is
+    good to 2^-38 of the largest |x dloss| (fp32 and bf16, larger calls).  x has to be finite in rows that are left out too.
     No atomics: the same inputs give the same bits."""
     x, kernel, R, D, V = _vocab_args(x, kernel, labels, bias)
     if accumulate and (x.dtype != torch.float32 or dkernel is None or (bias is not None and dbias is None)):

@@ -642,9 +642,9 @@ int sar_kv8_attend_f16(const sarXattn* a, const void* k8, const float* k_scale, 
  * x (R, D) with row stride ldx, kernel (D, V) with row stride ldk (elements; the Keras Dense layout), bias (V) or NULL, labels (R) of
  * label_bytes 4 or 8; a label outside [0, V) leaves its row out: loss 0, no gradient (its dloss is not looked at; its x has to be finite all the same: dkernel meets it as 0 x).  loss, lse, dloss (R) fp32 (forward: either may be NULL; backward:
  * lse of the forward).  dx (R, D), dkernel (D, V), dbias (V) contiguous, each may be NULL; accumulate (f32 only): dkernel and dbias are added to.
- * A row's loss, lse and dx do not depend on what other rows of x hold.  Larger calls pack fp32 operands (backward: bf16 ones too) into fp16 under powers of
- * two: elements below 2^-16 (bf16: 2^-31) of the largest of their row of x, or of the whole kernel, are held to 2^-38 of that one; for dkernel the
- * largest of all rows of x with a label counts.
+ * A row's loss, lse and dx do not depend on what other rows of x and dloss hold (f16: dz has one scale, from the largest |dloss| of a row with a label).
+ * Larger calls pack fp32 operands (backward: bf16 ones too) into fp16 under powers of two: elements below 2^-16 (bf16: 2^-31) of the largest of their row
+ * of x, or of the whole kernel, are held to 2^-38 of that one; for dkernel the largest |x dloss| of all rows with a label counts.
  * ws: the matching _workspace_bytes of the same struct, 256-byte aligned; nothing in it has to be initialised, nothing is kept there. */
 typedef struct {
     const void *x, *kernel, *bias, *labels;

@@ -115,3 +115,40 @@ def test_left_out_rows_at_the_end_of_the_range(R, D, V, dt):
     want = run(dl, torch.where(out[:, None], torch.zeros_like(x), x), w, lab, b)
     got = run(dl, torch.where(out[:, None], torch.full_like(x, torch.finfo(x.dtype).max) * torch.sign(x), x), w, lab, b)
     assert all(torch.equal(g, w_) for i, (g, w_) in enumerate(zip(got, want)) if i != 1)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("R,D,V", SIZES)
+def test_the_dloss_of_a_row_leaves_the_other_rows_alone(R, D, V, dt):
+    """A labelled row's dloss up to 1e30 and down to 1e-30: dx of the others does not change by a bit, its own follows.  (fp16 holds dz under one scale.)"""
+    x, w, lab, b, dl = make(R, D, V, DT[dt], seed=R)
+    others = torch.arange(R, device="cuda") != 2
+    want = run(dl, x, w, lab, b)
+    for e in (100, 20, -20, -100):
+        d = dl.clone(); d[2] *= 2.0 ** e
+        got = run(d, x, w, lab, b)
+        assert torch.equal(got[2][others], want[2][others]), e
+        y, z = want[2][2].double() * 2.0 ** e, got[2][2].double()
+        # (in the type's normal numbers; fp32 sums of what lies below them lose bits)
+        assert e < -20 or torch.equal(z, y), e
+        assert all(torch.isfinite(t).all() for t in got[2:] if t is not None)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("R,D,V", SIZES[1:])
+def test_rows_of_many_dlosses(R, D, V, dt):
+    """dloss over twelve orders of magnitude: dx row by row against float64 (each row alone: reference() takes maxima over its rows), dkernel and dbias as a
+    whole, dkernel's packed x adding 2^-37 max |x dloss| for each row's softmax - onehot."""
+    from tests.test_gpu_vocab_ce import check, reference
+    x, w, lab, b, dl = make(R, D, V, DT[dt], seed=R + 2)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    dl = dl * 10.0 ** torch.linspace(-6, 6, R, device="cuda")[torch.randperm(R, generator=g, device="cuda")]
+    got = run(dl, x, w, lab, b)
+    for i in range(0, R, 97):
+        s = slice(i, i + 1)
+        want, bd = reference(x[s], w, lab[s], b, dl[s])
+        check(got[2][s], want[2], bd[2], "dx")
+    want, bd = reference(x, w, lab, b, dl)
+    check(got[3], want[3], bd[3] + 2.0 ** -37 * (x.double().abs().amax(1) * dl.double().abs()).max(), "dkernel")
+    if b is not None:
+        check(got[4], want[4], bd[4], "dbias")
