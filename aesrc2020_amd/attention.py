@@ -10,8 +10,8 @@ import struct
 import torch
 
 from . import _lib
+from ._call import SFX as _SFX, given as _given, launch as _launch, result as _result, with_workspace as _place
 
-_SFX = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}
 _P, _L, _I = ctypes.c_void_p, ctypes.c_long, ctypes.c_int
 
 
@@ -23,7 +23,7 @@ class Xattn(ctypes.Structure):
 
 
 _XATTN = struct.Struct("12Ql15l6ifi")                                  # the same fields: packing bytes costs a fifth of filling the Structure
-_WS, _WS_AT = struct.Struct("Ql"), Xattn.ws.offset
+_WS_AT = Xattn.ws.offset
 _NAMES = {n: {d: "sar_%s_%s" % (n, s) for d, s in _SFX.items()} for n in ("xattn_fwd", "xattn_bwd", "kv8_attend")}
 
 
@@ -61,44 +61,13 @@ def _heads(Hq, Hkv, D):
         raise ValueError("the head width has to be a multiple of 8 from 8 to 128, got %d" % D)
 
 
-def _launch(name, device, *args):
-    """Call an entry point on the current stream of the tensors' device."""
-    fn = _lib.lib().fn[name]
-    index = device.index
-    if torch.cuda.current_device() != index:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
-    else:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))      # (torch.cuda.current_stream().cuda_stream without the Stream object: 2 us less)
-    if rc == -1:
-        raise ValueError("%s does not take these arguments: include/sarnet.h states its limits" % name)
-    if rc != 0:
-        raise RuntimeError("%s failed with status %d" % (name, rc))
-
-
 def _with_workspace(query, device, a):
     """sarXattn as bytes -> the same with a workspace where the call needs one, and the workspace to keep until the launch."""
     n = _lib.lib().fn[query](a)
     if not n:
         return a, None
     ws = torch.empty(n, dtype=torch.uint8, device=device)
-    return a[:_WS_AT] + _WS.pack(ws.data_ptr(), n) + a[_WS_AT + _WS.size:], ws
-
-
-def _result(name, t, shape, dtype, device):
-    if t is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device or not t.is_contiguous() or t.data_ptr() % 16:
-        raise ValueError("%s has to be a contiguous, 16-byte aligned %s tensor of shape %r on %s" % (name, dtype, tuple(shape), device))
-    return t
-
-
-def _given(name, t, shape, dtype, device):
-    """An fp32 vector that a gradient reads as it is: lse, dloss."""
-    if t is None or tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError("%s has to be a contiguous %s tensor of shape %r on %s, got %s" %
-                         (name, dtype, tuple(shape), device, "None" if t is None else "%s %r on %s" % (t.dtype, tuple(t.shape), t.device)))
-    return t
+    return _place(a, _WS_AT, ws), ws
 
 
 def _result_like(name, t, q):

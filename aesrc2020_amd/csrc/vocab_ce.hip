@@ -304,7 +304,8 @@ constexpr unsigned LAUNCH_ROW = 1u << 22;
 // power limit leaves: 0.82 (dz) to 1.07 PFLOP/s (dW) for an 8192 x 8192 piece against 1024.
 // PA, PB: planes of the operands (1, or 2: hi, lo); PZ: planes of the dz that E_DZ writes
 template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED, int PA, int PB, int PZ> struct Product {
-    static constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * (int)sizeof(OP), SB = BN * BK * (int)sizeof(OP), STAGE = PA * SA + PB * SB, ST = 49152 / STAGE < 4 ? (49152 / STAGE > 2 ? 49152 / STAGE : 2) : 4;
+    static constexpr int BM = 64 * MT, BN = 64 * NT, SA = BM * BK * (int)sizeof(OP), SB = BN * BK * (int)sizeof(OP), STAGE = PA * SA + PB * SB,
+                         ST = 49152 / STAGE < 4 ? (49152 / STAGE > 2 ? 49152 / STAGE : 2) : 4;
     static constexpr int LDS = ST * STAGE;
     static __device__ __forceinline__ void run(char* lds, int block, const Job& job);
 };
@@ -834,7 +835,8 @@ extern "C" int SAR_FN(sar_vocab_ce_fwd)(const sarVocabCe* a, hipStream_t st) {
 }
 
 extern "C" int SAR_FN(sar_vocab_ce_bwd)(const sarVocabCe* a, hipStream_t st) {
-    if (bad(a) || !a->x || !a->kernel || !a->labels || !a->dloss || !a->lse || !a->ws || (uintptr_t)a->ws % 256 || (!a->dx && !a->dkernel && !a->dbias) || (a->accumulate && SAR_ELT != 0)) return SAR_EINVAL;
+    if (bad(a) || !a->x || !a->kernel || !a->labels || !a->dloss || !a->lse || !a->ws || (uintptr_t)a->ws % 256 ||
+        (!a->dx && !a->dkernel && !a->dbias) || (a->accumulate && SAR_ELT != 0)) return SAR_EINVAL;
     const Plan p = plan(a, true);
     if (a->ws_bytes < 0 || (size_t)a->ws_bytes < p.bytes) return SAR_EINVAL;
     char* ws = reinterpret_cast<char*>(a->ws);

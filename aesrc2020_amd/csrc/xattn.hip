@@ -247,7 +247,8 @@ template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_wav
 // delta = do . o takes o as the forward rounded it, an error of half a step of |do . o| that is lost among many keys but not among few (bf16, 10
 // keys: the gradients 1.7 times as far from float64 as their own rounding; now 1.4).  SUMMED: a first pass over the keys sums p dp instead, used up to
 // SUMMED_KEYS keys of a 16-bit type (one slice).
-template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dq_kernel(sarXattn a, float2* __restrict__ stats, float* __restrict__ part, int row_tiles, int slices) {
+template <typename T, int DP, int WN, bool SUMMED>
+__global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dq_kernel(sarXattn a, float2* __restrict__ stats, float* __restrict__ part, int row_tiles, int slices) {
     constexpr int KT = step_rows<T, WN>(), P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, WM = 4 / WN, NS = KT / 32 / WM, TILE = KT * P;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
     __shared__ float joined[SUMMED ? WM : 1][WN][64];
@@ -369,7 +370,8 @@ template <typename T, int DP, int WN, bool SUMMED> __global__ __launch_bounds__(
 }
 
 // ---- dK, dV: a wave holds 32 keys as columns n; the rows of one query head after the other stream through LDS
-template <typename T, int DP, int WN> __global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dkv_kernel(sarXattn a, const float2* __restrict__ stats, float* __restrict__ part, int key_tiles, int slices) {
+template <typename T, int DP, int WN>
+__global__ __launch_bounds__(256, (min_waves<T, DP>())) void xattn_dkv_kernel(sarXattn a, const float2* __restrict__ stats, float* __restrict__ part, int key_tiles, int slices) {
     constexpr int WM = 4 / WN, RT = 32 * WM, P = pitch<T, DP>(), NC = DP * (int)sizeof(T) / 32, ND = DP / 32, TILE = RT * P, BUF = 2 * TILE;
     __shared__ __attribute__((aligned(1024))) char lds[2 * BUF];                 // Q, dO; two of each
     __shared__ __attribute__((aligned(16))) float2 row_stats[2][RT];
@@ -783,7 +785,13 @@ template <int DP> static int launch_bwd(const sarXattn& a, hipStream_t st) {
 }
 
 #if SAR_ELT == 0      // the same for every type
-extern "C" size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, few_rows(a) ? step_splits(a, a->elt_bytes == 2 ? (a->D <= 64 ? 8 : 4) : a->D <= 32 ? 8 : a->D <= 64 ? 4 : 2, a->elt_bytes != 2) : fwd_plan(a).splits); }   // (most_waves(); fp32 has the fewest)
+extern "C" size_t sar_xattn_fwd_workspace_bytes(const sarXattn* a) {
+    if (bad_shape(a)) return 0;
+    if (!few_rows(a)) return part_bytes(a, fwd_plan(a).splits);
+    const bool wide = a->elt_bytes != 2;
+    const int waves = wide ? (a->D <= 32 ? 8 : a->D <= 64 ? 4 : 2) : a->D <= 64 ? 8 : 4;         // most_waves(); fp32 has the fewest
+    return part_bytes(a, step_splits(a, waves, wide));
+}
 extern "C" size_t sar_xattn_bwd_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : bwd_plan(a).bytes; }
 #endif
 

@@ -5,8 +5,8 @@
 //
 // The same kernel reads the 8-bit cache (include/sarnet.h: sarKv8): e4m3 values are converted exactly into the 16-bit operand type (bf16 for
 // bf16 and fp32 queries, fp16 for fp16 ones); the scale of a 64-key block multiplies the fp32 scores (K); V's goes into the bf16 values (a bf16 has
-// an fp32's range), and beside fp16 ones into the fp32 sums as a ratio of powers of two.  fp32 queries and probabilities enter as three bf16 planes (8 + 8 + 8 bits hold an fp32 mantissa): products are exact, sums fp32,
-// at a third of the bf16 rate instead of the fp32 MFMA's sixteenth.
+// an fp32's range), and beside fp16 ones into the fp32 sums as a ratio of powers of two.  fp32 queries and probabilities enter as three bf16
+// planes (8 + 8 + 8 bits hold an fp32 mantissa): products are exact, sums fp32, at a third of the bf16 rate instead of the fp32 MFMA's sixteenth.
 // Compiled once per element type: SAR_ELT 0 = fp32, 1 = bf16, 2 = fp16.
 #include "xattn.h"
 
@@ -180,7 +180,8 @@ template <typename T, typename C, bool S8, int DP, int NW> __global__ __launch_b
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
         top = half_max(top) * f;
         if (__any(top - m > lag<C>()) || (UNITS && nu != unit)) {
-            const float mn = fmaxf(m, reference<C>(top)), e = __builtin_amdgcn_exp2f(m - mn), eo = UNITS ? fminf(e * unit / nu, MOST) : e;     // (in this order: no power of two passes the range before e has taken it back)
+            const float mn = fmaxf(m, reference<C>(top)), e = __builtin_amdgcn_exp2f(m - mn);
+            const float eo = UNITS ? fminf(e * unit / nu, MOST) : e;             // (in this order: no power of two passes the range before e has taken it back)
             const bool beyond = UNITS && unit > nu * 1.2089258196146292e24f;     // by 2^80: sums other than 0 are past fp16's range, and stay finite here
             m = mn; l *= e;
             large = __any(fabsf(m) > LARGE && m != NO_MAX);
@@ -397,7 +398,9 @@ int SAR_FN(xattn_step)(const sarXattn* a, hipStream_t stream) { return step<elt,
 // ---- the 8-bit cache
 static bool bad8(const sarXattn* a, long frames) { return bad_shape(a) || frames < a->Tk || frames % KV_BLOCK || frames > (1L << 30); }
 #if SAR_ELT == 0      // the same for every type
-extern "C" size_t sar_kv8_attend_workspace_bytes(const sarXattn* a) { return bad_shape(a) ? 0 : part_bytes(a, step_splits(a, 8, a->elt_bytes != 2)); }   // (its rows are at most 128 bytes: eight waves)
+extern "C" size_t sar_kv8_attend_workspace_bytes(const sarXattn* a) {            // (its rows are at most 128 bytes: eight waves)
+    return bad_shape(a) ? 0 : part_bytes(a, step_splits(a, 8, a->elt_bytes != 2));
+}
 #endif
 extern "C" int SAR_FN(sar_kv8_attend)(const sarXattn* a, const void* k8, const float* k_scale, const void* v8, const float* v_scale, long frames, hipStream_t stream) {
     if (bad8(a, frames) || bad_strides(sizeof(elt), &a->q_sb, 3) || bad_strides(sizeof(elt), &a->o_sb, 3) || !a->q || !a->out || !k8 || !v8 || !k_scale || !v_scale) return SAR_EINVAL;

@@ -10,7 +10,7 @@ import struct
 import torch
 
 from . import _lib
-from .attention import _SFX, _WS, _given, _launch, _result
+from ._call import SFX as _SFX, given as _given, launch as _launch, result as _result, with_workspace
 from .engine import glorot_uniform
 from .layers import Layer
 
@@ -194,7 +194,7 @@ def _vocab_launch(direction, x, kernel, labels, bias, dloss, loss, lse, dx, dker
     a = _VOCAB_CE.pack(*args)
     n = _lib.lib().fn[name + "_workspace_bytes"](a)
     ws = torch.empty(n, dtype=torch.uint8, device=device)                    # (torch's blocks are 512-byte aligned)
-    _launch(name, device, a[:_WS_AT] + _WS.pack(ws.data_ptr(), n) + a[_WS_AT + _WS.size:])
+    _launch(name, device, with_workspace(a, _WS_AT, ws))
 
 
 def _ptr(t):
