@@ -300,7 +300,7 @@ struct Job { Side A, B; Epi e; int mtiles, ntiles, ksteps, slices; };
 constexpr unsigned LAUNCH_ROW = 1u << 22;
 // C = A B^T over k, four waves as 2 x 2, each MT x NT tiles of 32 x 32.  ST stages of LDS, loads ST - 1 steps ahead.
 // What bounds it (16 bits, 128 x 128 tiles): LDS hands out four 16-byte fragments for four matrix instructions of a wave and takes the stages' loads,
-// about as many cycles as the matrix instructions need; with two blocks a CU those are busy 45 (dz) to 68 % (dW) of the time, at the 1.8 GHz that the
+// about as many cycles as the matrix instructions need; with two blocks a CU those are busy 41 (dz) to 63 % (dW) of the time, at the 1.8 GHz that the
 // power limit leaves: 0.82 (dz) to 1.07 PFLOP/s (dW) for an 8192 x 8192 piece against 1024.
 // PA, PB: planes of the operands (1, or 2: hi, lo); PZ: planes of the dz that E_DZ writes
 template <typename OP, int BK, int MT, int NT, bool AD, bool BD, int EPI, bool SCALED, int PA, int PB, int PZ> struct Product {
